@@ -20,13 +20,17 @@
 #include <cstring>
 
 #include "fa_fwd_kernel.h"
+#include "fa_host.h"
 #include "fa_mi355x.h"
 
 namespace {
 
 thread_local char g_last_error[512] = "";
 
-fa_status fail(fa_status s, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+}  // namespace
+
+namespace fa {
+
 fa_status fail(fa_status s, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
@@ -34,6 +38,38 @@ fa_status fail(fa_status s, const char* fmt, ...) {
   va_end(ap);
   return s;
 }
+
+void clear_error() { g_last_error[0] = '\0'; }
+
+namespace {
+constexpr int kMaxDevices = 64;
+std::atomic<int> g_device_cus[kMaxDevices];
+}  // namespace
+
+fa_status current_compute_units(int* cus) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return fail(FA_ERR_HIP, "hipGetDevice failed: %s", hipGetErrorString(e));
+  if (dev >= 0 && dev < kMaxDevices) {
+    const int cached = g_device_cus[dev].load(std::memory_order_relaxed);
+    if (cached > 0) {
+      *cus = cached;
+      return FA_OK;
+    }
+  }
+  e = hipDeviceGetAttribute(cus, hipDeviceAttributeMultiprocessorCount, dev);
+  if (e != hipSuccess)
+    return fail(FA_ERR_HIP, "device query failed: %s", hipGetErrorString(e));
+  if (dev >= 0 && dev < kMaxDevices) g_device_cus[dev].store(*cus, std::memory_order_relaxed);
+  return FA_OK;
+}
+
+}  // namespace fa
+
+namespace {
+
+using fa::current_compute_units;
+using fa::fail;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -103,29 +139,6 @@ void to_kernel_args(const fa_fwd_params* p, fa::KernelArgs* a) {
   a->split.key_groups = 0;
   a->split.head_group = 0;
   a->split.all_rows = 0;
-}
-
-// Compute units of the calling thread's current device (queried once per
-// device; the split plan depends on it).
-constexpr int kMaxDevices = 64;
-std::atomic<int> g_device_cus[kMaxDevices];
-
-fa_status current_compute_units(int* cus) {
-  int dev = 0;
-  hipError_t e = hipGetDevice(&dev);
-  if (e != hipSuccess) return fail(FA_ERR_HIP, "hipGetDevice failed: %s", hipGetErrorString(e));
-  if (dev >= 0 && dev < kMaxDevices) {
-    const int cached = g_device_cus[dev].load(std::memory_order_relaxed);
-    if (cached > 0) {
-      *cus = cached;
-      return FA_OK;
-    }
-  }
-  e = hipDeviceGetAttribute(cus, hipDeviceAttributeMultiprocessorCount, dev);
-  if (e != hipSuccess)
-    return fail(FA_ERR_HIP, "device query failed: %s", hipGetErrorString(e));
-  if (dev >= 0 && dev < kMaxDevices) g_device_cus[dev].store(*cus, std::memory_order_relaxed);
-  return FA_OK;
 }
 
 // Validates p and launches it with the work plan for the current device:
@@ -213,7 +226,7 @@ const char* fa_last_error(void) { return g_last_error; }
 const char* fa_version(void) { return "fa_mi355x 0.1.0 gfx950"; }
 
 fa_status fa_fwd_validate(const fa_fwd_params* p) {
-  g_last_error[0] = '\0';
+  fa::clear_error();
   if (p == nullptr) return fail(FA_ERR_NULL, "params is NULL");
   if (p->q == nullptr) return fail(FA_ERR_NULL, "q is NULL");
   if (p->k == nullptr) return fail(FA_ERR_NULL, "k is NULL");

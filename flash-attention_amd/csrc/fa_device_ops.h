@@ -60,6 +60,18 @@ struct ElemOps<true> {
   }
 };
 
+// v_mfma_f32_16x16x32: c + a b.
+template <bool BF16>
+__device__ __forceinline__ f32x4 mfma16(i16x8 a, i16x8 b, f32x4 c) {
+  if constexpr (BF16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+}
+
 // Two fp32 -> packed pair of the element type, round-to-nearest-even
 // (one v_cvt_pk_f16_f32 / v_cvt_pk_bf16_f32).
 template <bool BF16>

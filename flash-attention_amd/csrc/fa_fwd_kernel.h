@@ -63,6 +63,23 @@ struct FastDiv {
   uint32_t mul, shift;
 };
 
+inline FastDiv make_fast_div(uint32_t d) {
+  if (d < 1) d = 1;  // an unused divisor
+  uint32_t l = 0;    // ceil(log2 d)
+  while ((uint64_t(1) << l) < d) ++l;
+  // mul d = 2^(31 + l) + e with 0 < e <= d <= 2^l, so n mul / 2^(31 + l) =
+  // n / d + n e / (d 2^(31 + l)) is exact for n < 2^31 (the second term is
+  // below 1 / d); mul < 2^32 because d > 2^(l - 1).
+  return FastDiv{(uint32_t)((uint64_t(1) << (31 + l)) / d + 1), l};
+}
+
+#if defined(__HIPCC__)
+// n / d for 0 <= n < 2^31 (make_fast_div).
+__device__ __forceinline__ int fast_div(int n, FastDiv d) {
+  return (int)(__umulhi(2u * (uint32_t)n, d.mul) >> d.shift);
+}
+#endif
+
 // Arguments of the kernels without work items, all a kernel reads before its
 // first load: 216 bytes, where the plan's tables make 2.3 KB.  Every launch
 // copies its arguments to memory the GPU reads, and every workgroup starts by

@@ -167,11 +167,6 @@ constexpr int kKWindow = 3;
 constexpr int kVWindow = 4;
 
 
-// n / d for 0 <= n < 2^31 (make_fast_div).
-__device__ __forceinline__ int fast_div(int n, FastDiv d) {
-  return (int)(__umulhi(2u * (uint32_t)n, d.mul) >> d.shift);
-}
-
 // Head and q-tile of this workgroup in a grid without work items.
 //  * Causal, B * H a multiple of 8: whole heads per XCD, taken in groups of
 //    group_heads (the plan's choice; all of them if it does not divide their
@@ -1166,16 +1161,6 @@ __global__ void __launch_bounds__(256) fa_merge_kernel(const KernelArgs args, in
                                         pack2<BF16>(acc[2] * inv_l, acc[3] * inv_l)};
   if (args.lse != nullptr && d == 0)
     args.lse[(int64_t)bh * args.seq_len + q] = (m == -INFINITY ? 0.0f : m) * args.scale + __logf(l);
-}
-
-FastDiv make_fast_div(uint32_t d) {
-  if (d < 1) d = 1;  // an unused divisor
-  uint32_t l = 0;    // ceil(log2 d)
-  while ((uint64_t(1) << l) < d) ++l;
-  // mul d = 2^(31 + l) + e with 0 < e <= d <= 2^l, so n mul / 2^(31 + l) =
-  // n / d + n e / (d 2^(31 + l)) is exact for n < 2^31 (the second term is
-  // below 1 / d); mul < 2^32 because d > 2^(l - 1).
-  return FastDiv{(uint32_t)((uint64_t(1) << (31 + l)) / d + 1), l};
 }
 
 // The grid order of q-tiles of BM rows (work_item) and its workgroup count.
