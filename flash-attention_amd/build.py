@@ -35,6 +35,8 @@ BUILD_DIR = os.path.join(PKG_ROOT, "_build")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 ARCH = "gfx950"
+# Kernels and C ABI of include/fa_mi355x_cache.h.
+CACHE_SOURCES = ["fa_paged_fwd.hip", "fa_paged_cache.hip", "fa_qk_norm.hip", "fa_cache_api.cpp"]
 # -packed-fp32-ops: keep the compiler from forming v_pk_{add,mul,fma}_f32.
 HIP_FLAGS = [
     f"--offload-arch={ARCH}",
@@ -67,8 +69,9 @@ def _hipcc() -> str:
 
 def build_hip_library(jobs: int) -> list[str]:
     """Compiles csrc/fa_fwd_kernel.hip (kernels and launch), fa_plan.cpp
-    (host work planning) and fa_api.cpp (the C ABI) with hipcc and links the
-    shared library libfa_mi355x.so.  The kernel source is compiled a second
+    (host work planning), fa_api.cpp (the C ABI) and CACHE_SOURCES (the paged
+    cache's operators and the q/k norm) with hipcc and links the shared library
+    libfa_mi355x.so.  The forward's kernel source is compiled a second
     time with -DFA_LDS_POISON into the debug library
     libfa_mi355x_poison.so (same ABI; staged LDS is filled with NaN before
     every staging write), and a third time with -DFA_MFMA32 into
@@ -80,12 +83,13 @@ def build_hip_library(jobs: int) -> list[str]:
     hipcc = _hipcc()
     kernel = os.path.join(CSRC, "fa_fwd_kernel.hip")
     host = [os.path.join(CSRC, "fa_plan.cpp"), os.path.join(CSRC, "fa_api.cpp")]
+    cache = [os.path.join(CSRC, f) for f in CACHE_SOURCES]
 
     def obj_of(src: str, tag: str = "") -> str:
         return os.path.join(BUILD_DIR, os.path.basename(src) + tag + ".o")
 
     cmds = []
-    for src in [kernel, *host]:
+    for src in [kernel, *cache, *host]:
         lang = ["-x", "hip"] if src.endswith(".hip") else []
         cmds.append([hipcc, *HIP_FLAGS, "-I", INCLUDE, "-I", CSRC, *lang, "-c", src,
                      "-o", obj_of(src)])
@@ -100,16 +104,17 @@ def build_hip_library(jobs: int) -> list[str]:
                        ("libfa_mi355x_poison.so", obj_of(kernel, ".poison")),
                        ("libfa_mi355x_mfma32.so", obj_of(kernel, ".mfma32"))):
         lib = os.path.join(OUT_DIR, name)
+        more = [obj_of(c) for c in cache] if kobj == obj_of(kernel) else []
         _run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", kobj,
-              *[obj_of(h) for h in host], "-o", lib + ".tmp"])
+              *[obj_of(h) for h in host], *more, "-o", lib + ".tmp"])
         os.replace(lib + ".tmp", lib)
         libs.append(lib)
     return libs
 
 
 def build_torch_binding() -> str:
-    """Compiles the pybind/torch host binding (fa_torch_ext.cpp) with g++ and
-    links it against libfa_mi355x.so (rpath $ORIGIN)."""
+    """Compiles the pybind/torch host binding (fa_torch_ext.cpp,
+    fa_torch_cache.cpp) with g++ and links it against libfa_mi355x.so (rpath $ORIGIN)."""
     import torch
     from torch.utils import cpp_extension
 
@@ -124,7 +129,7 @@ def build_torch_binding() -> str:
         "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
         *[f"-I{p}" for p in incs],
-        os.path.join(CSRC, "fa_torch_ext.cpp"),
+        os.path.join(CSRC, "fa_torch_ext.cpp"), os.path.join(CSRC, "fa_torch_cache.cpp"),
         f"-L{OUT_DIR}", "-lfa_mi355x",
         f"-L{torch_lib}", "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10_hip",
         "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}",

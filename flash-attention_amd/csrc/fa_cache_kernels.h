@@ -1,0 +1,140 @@
+// Internal interface between the C ABI of the paged cache's operators
+// (fa_cache_api.cpp) and their HIP kernels.  Strides are in bytes here.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "fa_fwd_kernel.h"
+
+namespace fa {
+
+// Sequences over a paged cache (fa_paged_cache): table, lengths and limits.
+struct PageTable {
+  const int32_t* table;
+  const int32_t* cu;
+  const int32_t* lens;
+  int64_t table_stride;  // elements
+  int32_t batch, num_pages, page_shift;
+  int32_t tokens;        // cu's limit
+  int32_t max_kv;        // lens' limit, at most the table's capacity
+};
+
+// Rows of a workgroup: the new tokens of a sequence times the query heads of
+// one kv head, row r = token r / group, head r % group of them, so that every
+// key row read serves the whole group.
+struct PagedFwdArgs {
+  PageTable pt;
+  const char* q;
+  const char* k;
+  const char* v;
+  char* o;
+  float* lse;
+  int64_t q_st, q_sh, o_st, o_sh;  // token, head
+  int64_t k_sp, k_sh, v_sp, v_sh;  // page, head
+  uint32_t k_ss, v_ss;             // key
+  int32_t heads, kv_heads, group;
+  int32_t max_q, causal;
+  float scale_log2;                // softmax scale * log2(e)
+  // Which sequences a launch serves, by their rows, and its grid: slots (row
+  // tiles of all sequences) x kv heads x splits of `chunk` keys.
+  int32_t min_rows, max_rows;
+  int32_t slots, splits, chunk;
+  FastDiv by_group, by_slots, by_kvh, by_splits;
+  float* ws_o;                     // [slot][kv head][split][BM][D] partial o, fp32
+  float* ws_e;                     // the same rows: (log2 of the rounded P's sum, of the plain one's)
+};
+
+// How a call is launched (plan_paged): sequences of at most kDecodeRows rows
+// on the decode kernel, the others on the chunk kernel.
+constexpr int kDecodeRows = 32;
+constexpr int kChunkRows = 128;  // rows of a chunk kernel's workgroup
+
+struct PagedGrid {
+  int32_t rows;  // rows of a slot (BM); 0: not launched
+  int32_t slots, splits, chunk;
+  uint64_t ws_rows;  // rows of partials
+};
+struct PagedPlan {
+  PagedGrid decode, chunk;
+  uint64_t workspace_bytes;
+};
+PagedPlan plan_paged(int tokens, int batch, int kv_heads, int group, int head_dim, int max_q,
+                     int max_kv, int compute_units);
+
+hipError_t launch_paged_fwd(const PagedFwdArgs& args, const PagedPlan& plan, int head_dim, bool bf16,
+                            void* workspace, hipStream_t stream);
+
+struct PagedWeightsArgs {
+  PageTable pt;
+  const char* q;
+  const char* k;
+  const float* lse;
+  float* w;
+  int64_t q_st, q_sh, k_sp, k_sh;
+  int64_t w_sp, w_sh;  // elements
+  uint32_t k_ss;
+  int32_t heads, kv_heads, group, max_q, causal;
+  float scale_log2;
+  int32_t key_tiles, splits;  // grid: sequences x kv heads x key tiles x row splits
+  FastDiv by_group, by_kvh, by_tiles, by_splits;
+  float* ws;           // [splits][batch][kv_heads][key_tiles * 256] partial sums
+};
+constexpr int kWeightKeys = 256;  // keys of a workgroup
+// Row splits of the key weights' grid (1: no workspace).
+int plan_weights(int batch, int kv_heads, int group, int max_q, int max_kv, int compute_units);
+hipError_t launch_paged_weights(const PagedWeightsArgs& args, int head_dim, bool bf16,
+                                hipStream_t stream);
+
+struct PagedEvictArgs {
+  PageTable pt;  // cu unused
+  char* k;
+  char* v;
+  float* w;
+  int64_t k_sp, k_sh, v_sp, v_sh;
+  int64_t w_sp, w_sh;  // elements
+  uint32_t k_ss, v_ss;
+  int32_t kv_heads;
+  const int32_t* new_table;
+  int64_t new_table_stride;
+  int32_t* new_lens;
+  int32_t* kept;
+  int32_t keep, recent;
+};
+hipError_t launch_paged_evict(const PagedEvictArgs& args, int head_dim, hipStream_t stream);
+
+// Rows of q and k (and v, to be copied, when storing) of a grid of tokens;
+// [0] q, [1] k, [2] v.
+struct NormArgs {
+  const char* x[3];
+  char* y[3];                     // outputs; storing: y[1], y[2] are the cache
+  int64_t x_sb[3], x_sh[3], x_st[3];  // batch, head, token
+  int64_t y_sb[3], y_sh[3], y_st[3];  // storing: page, head, key for [1] and [2]
+  const void* weight[2];
+  const float* cos;
+  const float* sin;
+  const int32_t* positions;
+  int64_t pos_stride;             // elements
+  PageTable pt;                   // storing only
+  int64_t capacity;               // storing only: keys that a table row holds
+  int32_t tokens;                 // of all sequences: batch * seq_len
+  int32_t seq_len;                // tokens of one batch entry
+  int32_t heads, kv_heads, head_dim;
+  int32_t rot, table_rows, interleaved, weight_fp32;
+  float eps;
+  FastDiv by_seq;
+  // backward: dx's; the weights' partial sums [blocks][2][D] and results
+  char* dx[2];
+  int64_t dx_sb[2], dx_sh[2], dx_st[2];
+  float* ws;
+  float* dw[2];
+  int32_t blocks_x, head_chunk;   // grid: token blocks x chunks of heads
+};
+hipError_t launch_norm(const NormArgs& args, bool bf16, bool store, int compute_units,
+                       hipStream_t stream);
+// Workgroups of the backward pass, each with 2 * D partial sums.
+int norm_bwd_blocks(int64_t tokens, int heads, int head_dim, int compute_units);
+hipError_t launch_norm_bwd(const NormArgs& args, bool bf16, int compute_units, hipStream_t stream);
+
+}  // namespace fa

@@ -1,0 +1,416 @@
+// Key weights and eviction of a paged key/value cache on gfx950.
+//
+// fa_weights_kernel: add_j = sum over rows i that see key j of
+// exp(scale q_i.k_j - lse_i), one pass over K.  A wave keeps 64 keys in
+// registers as the B operand of v_mfma_f32_16x16x32 and the workgroup's four
+// waves (256 keys) walk over the rows together, 32 at a time through LDS; a
+// lane holds one key of each 16-key block and 4 rows, so its sums stay in
+// registers and meet once at the end.  For one token it is bound by reading K,
+// for chunks by the exponentials (one per row and key, four cycles of a SIMD
+// each per 16 lanes) over half the matrix work of attention.
+//
+// fa_select_kernel: the keep - recent heaviest of a head's keys by a radix
+// search for their least weight, eight bits at a time, and the list of the
+// kept keys in order.  fa_move_kernel copies their rows: bound by memory.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "fa_cache_kernels.h"
+#include "fa_device_ops.h"
+#include "fa_lds_layout.h"
+#include "fa_paged_ops.h"
+
+namespace fa {
+namespace {
+
+using namespace dev;
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) fa_weights_kernel(const PagedWeightsArgs a) {
+  constexpr int ROWB = 2 * D, KST = D / 32, KB = 4, RT = 32;  // 64 keys of a wave, rows of a tile
+  constexpr int TB = RT * ROWB, NI = TB / 4 / 1024;           // bytes of a row tile, DMAs of a wave
+  constexpr int LPR = ROWB / 16;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * TB];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l16 = lane & 15, g4 = lane >> 4;
+  // (sequence, kv head, key tile, row split): the splits slowest
+  const int rest = fast_div(blockIdx.x, a.by_tiles), tile = blockIdx.x - rest * a.key_tiles;
+  const int bk = fast_div(rest, a.by_kvh), kvh = rest - bk * a.kv_heads;
+  const int split = fast_div(bk, a.by_splits), b = bk - split * a.pt.batch;
+  const Seq s = load_seq(a.pt, b, a.max_q);
+  const int key0 = tile * kWeightKeys;
+  if (s.nq <= 0 || key0 >= s.len) return;
+  const int wkey0 = key0 + 64 * wave;
+
+  // This lane's keys wkey0 + 16kb + l16: rows of K past the end re-read the
+  // last key, absent pages page 0; their sums are not used.
+  const int32_t* row = a.pt.table + b * a.pt.table_stride;
+  i16x8 kf[KB][KST];
+  unsigned there = 0;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+    const int r0 = min(wkey0 + 16 * kb, (s.len - 1) & ~15);
+    const int id = page_id(a.pt, row, r0);
+    const bool ok = (uint32_t)id < (uint32_t)a.pt.num_pages;
+    if (ok) there |= 1u << kb;
+    const int in_page = (r0 & ((1 << a.pt.page_shift) - 1)) + min(l16, s.len - 1 - r0);
+    const char* kp = a.k + (int64_t)(ok ? id : 0) * a.k_sp + kvh * a.k_sh + (int64_t)in_page * a.k_ss;
+#pragma unroll
+    for (int st = 0; st < KST; ++st)
+      kf[kb][st] = *reinterpret_cast<const i16x8*>(kp + (32 * st + 8 * g4) * 2);
+  }
+
+  // Rows: those of tokens that see this workgroup's first key, cut into the
+  // grid's splits.
+  const int n_rows = s.nq * a.group;
+  const int i_first = a.causal ? max(0, key0 - s.first) : 0;
+  const int t_begin = min((int)((int64_t)i_first * a.group / RT), n_rows / RT);
+  const int t_all = (n_rows + RT - 1) / RT - t_begin;
+  const int splits = a.ws != nullptr ? a.splits : 1;
+  const int t0 = t_begin + (int)((int64_t)split * t_all / splits);
+  const int t1 = t_begin + (int)((int64_t)(split + 1) * t_all / splits);
+
+  const char* qh = a.q + s.q0 * a.q_st + (int64_t)kvh * a.group * a.q_sh;
+  const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(smem));
+  auto issue = [&](int t, int buf) FA_INLINE {
+    const int i0 = fast_div(min(t * RT, n_rows - 1), a.by_group);  // first token: the DMA's base
+    const char* src = qh + i0 * a.q_st;
+#pragma unroll
+    for (int it = 0; it < NI; ++it) {
+      const int rt = (wave * NI + it) * (1024 / ROWB) + lane / LPR;
+      const int r = min(t * RT + rt, n_rows - 1);
+      const int i = fast_div(r, a.by_group), h = r - i * a.group;
+      const int c = (lane % LPR) ^ lds::Tile16<D>::swz_k(rt);
+      dma_16b((uint32_t)((i - i0) * (int)a.q_st + h * (int)a.q_sh + c * 16), src,
+              base + buf * TB + (wave * NI + it) * 1024);
+    }
+  };
+  // lse (log2) and last visible key of row t * RT + lane % 32, for all lanes;
+  // rows that do not exist or have no weights see nothing.
+  float lse_n = 0.0f;
+  int last_n = -1;
+  auto fetch_row = [&](int t) FA_INLINE {
+    const int r = t * RT + (lane & 31), rc = min(r, n_rows - 1);
+    const int i = fast_div(rc, a.by_group), h = rc - i * a.group;
+    const float l = a.lse[(int64_t)(s.q0 + i) * a.heads + kvh * a.group + h];
+    last_n = r < n_rows && l != -INFINITY ? (a.causal ? min(s.first + i, s.len - 1) : s.len - 1) : -1;
+    lse_n = l * kLog2e;
+  };
+  int k_off[KST];
+#pragma unroll
+  for (int st = 0; st < KST; ++st) k_off[st] = lds::k16_read_offset<D>(0, st, lane);
+
+  float acc[KB] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (t0 < t1) {
+    fetch_row(t0);
+    issue(t0, 0);
+  }
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    const float lse = lse_n;
+    const int last = last_n;
+    const int buf = (t - t0) & 1;
+    if (t + 1 < t1) {
+      issue(t + 1, buf ^ 1);
+      fetch_row(t + 1);
+    }
+    if (__any(last >= wkey0) && wkey0 < s.len) {
+      const bool whole = __all(last >= wkey0 + 63);
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb) {
+        f32x4 sc[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) sc[kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int st = 0; st < KST; ++st) {
+          const i16x8 qa = *reinterpret_cast<const i16x8*>(smem + buf * TB + rb * 16 * ROWB + k_off[st]);
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) sc[kb] = mfma16<BF16>(qa, kf[kb][st], sc[kb]);
+        }
+        // rows 16rb + 4g4 + i, keys wkey0 + 16kb + l16
+        float rl[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rl[i] = __shfl(lse, 16 * rb + 4 * g4 + i);
+        if (whole) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[kb] += fast_exp2(fmaf(sc[kb][i], a.scale_log2, -rl[i]));
+        } else {
+          int rel[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) rel[i] = __shfl(last, 16 * rb + 4 * g4 + i) - wkey0 - l16;
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float p = fast_exp2(fmaf(sc[kb][i], a.scale_log2, -rl[i]));
+              acc[kb] += 16 * kb <= rel[i] ? p : 0.0f;
+            }
+        }
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+  }
+
+  // Lane group g4 finishes key block g4.
+  float mine = 0.0f;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+    float x = acc[kb];
+    x += __shfl_xor(x, 16);
+    x += __shfl_xor(x, 32);
+    if (g4 == kb) mine = x;
+  }
+  const int key = wkey0 + 16 * g4 + l16;
+  if (a.ws != nullptr) {
+    a.ws[((((int64_t)split * a.pt.batch + b) * a.kv_heads + kvh) * a.key_tiles + tile) * kWeightKeys +
+         64 * wave + lane] = mine;
+    return;
+  }
+  if (key < s.len && ((there >> g4) & 1u)) {
+    const int id = row[key >> a.pt.page_shift];
+    float* w = a.w + (int64_t)id * a.w_sp + kvh * a.w_sh + (key & ((1 << a.pt.page_shift) - 1));
+    *w = key >= s.first ? mine : *w + mine;
+  }
+}
+
+// Adds the row splits' sums, in their order, to the weights.
+__global__ void __launch_bounds__(256) fa_weights_sum_kernel(const PagedWeightsArgs a) {
+  const int rest = fast_div(blockIdx.x, a.by_tiles), tile = blockIdx.x - rest * a.key_tiles;
+  const int b = fast_div(rest, a.by_kvh), kvh = rest - b * a.kv_heads;
+  const Seq s = load_seq(a.pt, b, a.max_q);
+  const int key = tile * kWeightKeys + threadIdx.x;
+  if (s.nq <= 0 || key >= s.len) return;
+  const int id = a.pt.table[b * a.pt.table_stride + (key >> a.pt.page_shift)];
+  if ((uint32_t)id >= (uint32_t)a.pt.num_pages) return;
+  float sum = 0.0f;
+  for (int c = 0; c < a.splits; ++c)
+    sum += a.ws[((((int64_t)c * a.pt.batch + b) * a.kv_heads + kvh) * a.key_tiles + tile) * kWeightKeys +
+                threadIdx.x];
+  float* w = a.w + (int64_t)id * a.w_sp + kvh * a.w_sh + (key & ((1 << a.pt.page_shift) - 1));
+  *w = key >= s.first ? sum : *w + sum;
+}
+
+// ---- eviction ----
+
+// Bits of a weight in an order: larger weights, larger numbers; both zeros
+// alike, NaN above all.
+__device__ __forceinline__ uint32_t weight_order(float x) {
+  if (x != x) return ~0u;
+  const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f);  // -0 + 0 = +0
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+constexpr int kSelThreads = 1024;
+constexpr int kSelWaves = kSelThreads / 64;
+constexpr int kSelHold = 16;  // weights a thread keeps in registers
+
+__global__ void __launch_bounds__(kSelThreads) fa_select_kernel(const PagedEvictArgs a) {
+  __shared__ int hist[256];
+  __shared__ int wave_n[2][kSelWaves];
+  __shared__ int pick[2];
+  __shared__ int bad;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = blockIdx.x / a.kv_heads, kvh = blockIdx.x - b * a.kv_heads;
+  const int len = min(max(a.pt.lens[b], 0), a.pt.max_kv);
+  const int n = min(len, a.keep);
+  const int32_t* row = a.pt.table + b * a.pt.table_stride;
+  const int32_t* new_row = a.new_table + b * a.new_table_stride;
+  int32_t* kept = a.kept + ((int64_t)b * a.kv_heads + kvh) * a.keep;
+  const int page = 1 << a.pt.page_shift;
+
+  if (tid == 0) bad = 0;
+  __syncthreads();
+  bool miss = false;
+  for (int i = tid; i * (int64_t)page < len; i += kSelThreads)
+    miss = miss || (uint32_t)row[i] >= (uint32_t)a.pt.num_pages;
+  for (int i = tid; i * (int64_t)page < n; i += kSelThreads)
+    miss = miss || (uint32_t)new_row[i] >= (uint32_t)a.pt.num_pages;
+  if (__any(miss) && lane == 0) bad = 1;
+  __syncthreads();
+  const int count = bad ? 0 : n;
+  if (tid == 0 && kvh == 0) a.new_lens[b] = count;
+  for (int t = count + tid; t < a.keep; t += kSelThreads) kept[t] = -1;
+  if (bad) return;
+  if (len <= a.keep) {
+    for (int t = tid; t < n; t += kSelThreads) kept[t] = t;
+    return;
+  }
+
+  // The want heaviest of the keys before the recent ones.
+  const int old = len - a.recent, want = a.keep - a.recent;
+  auto order_of = [&](int i) FA_INLINE {
+    return weight_order(a.w[(int64_t)row[i >> a.pt.page_shift] * a.w_sp + kvh * a.w_sh + (i & (page - 1))]);
+  };
+  uint32_t held[kSelHold];
+#pragma unroll
+  for (int j = 0; j < kSelHold; ++j) {
+    const int i = j * kSelThreads + tid;
+    held[j] = i < old ? order_of(i) : 0u;
+  }
+  uint32_t prefix = 0;  // the top bits of the want-th largest
+  int left = want;      // its rank among the keys with that prefix
+  for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
+    for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+    __syncthreads();
+    const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
+    auto count_one = [&](uint32_t u) FA_INLINE {
+      if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & 255u], 1);
+    };
+#pragma unroll
+    for (int j = 0; j < kSelHold; ++j)
+      if (j * kSelThreads + tid < old) count_one(held[j]);
+    for (int i = kSelHold * kSelThreads + tid; i < old; i += kSelThreads) count_one(order_of(i));
+    __syncthreads();
+    if (wave == 0) {
+      // counts of the buckets 4 lane .. + 3 and of those above them
+      int c[4], sum = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum += c[j] = hist[4 * lane + j];
+      int above = sum;  // inclusive suffix sum over lanes
+      for (int d = 1; d < 64; d <<= 1) {
+        const int x = __shfl_down(above, d);
+        above += lane + d < 64 ? x : 0;
+      }
+      above -= sum;
+#pragma unroll
+      for (int j = 3; j >= 0; --j) {
+        if (above < left && left <= above + c[j]) {
+          pick[0] = 4 * lane + j;
+          pick[1] = left - above;
+        }
+        above += c[j];
+      }
+    }
+    __syncthreads();
+    prefix |= (uint32_t)pick[0] << shift;
+    left = pick[1];
+  }
+
+  // Kept: keys above the threshold, the first `left` that equal it, and the
+  // recent ones, in order: key i goes to place (larger before i) + (equal
+  // before i, at most left).
+  int gt_before = 0, eq_before = 0;
+  auto place = [&](int i0, bool in, uint32_t u) FA_INLINE {
+    const bool gt = in && want > 0 && u > prefix, eq = in && want > 0 && u == prefix;
+    const uint64_t bg = __ballot(gt), be = __ballot(eq), below = ((uint64_t)1 << lane) - 1;
+    if (lane == 0) {
+      wave_n[0][wave] = __popcll(bg);
+      wave_n[1][wave] = __popcll(be);
+    }
+    __syncthreads();
+    int g = gt_before, e = eq_before, gs = 0, es = 0;
+#pragma unroll
+    for (int w = 0; w < kSelWaves; ++w) {
+      if (w < wave) {
+        g += wave_n[0][w];
+        e += wave_n[1][w];
+      }
+      gs += wave_n[0][w];
+      es += wave_n[1][w];
+    }
+    g += __popcll(bg & below);
+    e += __popcll(be & below);
+    if (gt || (eq && e < left)) kept[g + min(e, left)] = i0 + tid;
+    gt_before += gs;
+    eq_before += es;
+    __syncthreads();
+  };
+#pragma unroll
+  for (int j = 0; j < kSelHold; ++j)
+    if (j * kSelThreads < old) place(j * kSelThreads, j * kSelThreads + tid < old, held[j]);
+  for (int i0 = kSelHold * kSelThreads; i0 < old; i0 += kSelThreads) {
+    const bool in = i0 + tid < old;
+    place(i0, in, in ? order_of(i0 + tid) : 0u);
+  }
+  for (int t = tid; t < a.recent; t += kSelThreads) kept[want + t] = old + t;
+}
+
+// Copies the kept keys' rows of K and V, and their weights.  LPR lanes move a
+// row, kMoveRows rows apart per lane in flight.
+constexpr int kMoveRows = 4;
+template <int D>
+__global__ void __launch_bounds__(256) fa_move_kernel(const PagedEvictArgs a, int blocks) {
+  constexpr int LPR = 2 * D / 16, RPB = 256 / LPR;
+  const int bk = blockIdx.x / blocks, b = bk / a.kv_heads, kvh = bk - b * a.kv_heads;
+  const int n = a.new_lens[b];
+  const int t0 = (blockIdx.x - bk * blocks) * RPB * kMoveRows + (int)threadIdx.x / LPR;
+  const int c = ((int)threadIdx.x % LPR) * 16;
+  const int32_t* row = a.pt.table + b * a.pt.table_stride;
+  const int32_t* new_row = a.new_table + b * a.new_table_stride;
+  const int32_t* kept = a.kept + (int64_t)bk * a.keep;
+  const int shift = a.pt.page_shift, mask = (1 << shift) - 1;
+  int src[kMoveRows];
+  u32x4 k[kMoveRows], v[kMoveRows];
+  float w[kMoveRows];
+#pragma unroll
+  for (int j = 0; j < kMoveRows; ++j) src[j] = t0 + j * RPB < n ? kept[t0 + j * RPB] : -1;
+#pragma unroll
+  for (int j = 0; j < kMoveRows; ++j)
+    if (src[j] >= 0) {
+      const int64_t id = row[src[j] >> shift];
+      const int at = src[j] & mask;
+      k[j] = *reinterpret_cast<const u32x4*>(a.k + id * a.k_sp + kvh * a.k_sh + (int64_t)at * a.k_ss + c);
+      v[j] = *reinterpret_cast<const u32x4*>(a.v + id * a.v_sp + kvh * a.v_sh + (int64_t)at * a.v_ss + c);
+      if (c == 0) w[j] = a.w[id * a.w_sp + kvh * a.w_sh + at];
+    }
+#pragma unroll
+  for (int j = 0; j < kMoveRows; ++j)
+    if (src[j] >= 0) {
+      const int t = t0 + j * RPB, at = t & mask;
+      const int64_t id = new_row[t >> shift];
+      *reinterpret_cast<u32x4*>(a.k + id * a.k_sp + kvh * a.k_sh + (int64_t)at * a.k_ss + c) = k[j];
+      *reinterpret_cast<u32x4*>(a.v + id * a.v_sp + kvh * a.v_sh + (int64_t)at * a.v_ss + c) = v[j];
+      if (c == 0) a.w[id * a.w_sp + kvh * a.w_sh + at] = w[j];
+    }
+}
+
+}  // namespace
+
+hipError_t launch_paged_weights(const PagedWeightsArgs& args, int head_dim, bool bf16,
+                                hipStream_t stream) {
+  PagedWeightsArgs a = args;
+  const int64_t tiles = (int64_t)a.pt.batch * a.kv_heads * a.key_tiles;
+  const int64_t grid = tiles * a.splits;
+  if (grid > 0x7fffffff) return hipErrorInvalidValue;
+  const void* fn;
+  if (head_dim == 128)
+    fn = bf16 ? reinterpret_cast<const void*>(&fa_weights_kernel<128, true>)
+              : reinterpret_cast<const void*>(&fa_weights_kernel<128, false>);
+  else
+    fn = bf16 ? reinterpret_cast<const void*>(&fa_weights_kernel<64, true>)
+              : reinterpret_cast<const void*>(&fa_weights_kernel<64, false>);
+  void* kargs[] = {&a};
+  hipError_t e = hipLaunchKernel(fn, dim3((unsigned)grid), dim3(256), kargs, 0, stream);
+  if (e != hipSuccess || a.ws == nullptr) return e;
+  return hipLaunchKernel(reinterpret_cast<const void*>(&fa_weights_sum_kernel), dim3((unsigned)tiles),
+                         dim3(256), kargs, 0, stream);
+}
+
+hipError_t launch_paged_evict(const PagedEvictArgs& args, int head_dim, hipStream_t stream) {
+  PagedEvictArgs a = args;
+  const int64_t bk = (int64_t)a.pt.batch * a.kv_heads;
+  const int most = std::min(a.keep, a.pt.max_kv);
+  const int per = 256 / (2 * head_dim / 16) * kMoveRows;
+  int blocks = (most + per - 1) / per;
+  if (bk * std::max(blocks, 1) > 0x7fffffff) return hipErrorInvalidValue;
+  void* sargs[] = {&a};
+  hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&fa_select_kernel), dim3((unsigned)bk),
+                                 dim3(kSelThreads), sargs, 0, stream);
+  if (e != hipSuccess || blocks == 0) return e;
+  void* margs[] = {&a, &blocks};
+  const void* fn = head_dim == 128 ? reinterpret_cast<const void*>(&fa_move_kernel<128>)
+                                   : reinterpret_cast<const void*>(&fa_move_kernel<64>);
+  return hipLaunchKernel(fn, dim3((unsigned)(bk * blocks)), dim3(256), margs, 0, stream);
+}
+
+}  // namespace fa

@@ -1,0 +1,132 @@
+// Device building blocks shared by the kernels over a paged cache: sequences
+// and page ids by scalar loads, staging of 16-key groups, LDS reads at
+// addresses, explicit waits.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "fa_cache_kernels.h"
+#include "fa_device_ops.h"
+#include "fa_lds_layout.h"
+
+namespace fa {
+namespace {
+
+using namespace dev;
+
+
+// 16 bytes of LDS at byte address addr + OFF.
+template <int OFF>
+__device__ __forceinline__ i16x8 lds_read16(uint32_t addr) {
+  typedef __attribute__((address_space(3))) const char lds_char_t;
+  return *(__attribute__((address_space(3))) const i16x8*)((lds_char_t*)(uintptr_t)addr + OFF);
+}
+
+// s_waitcnt vmcnt(N), the other counters left alone.
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0f70);
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Ends this wave's LDS reads (lgkmcnt(0)) before what follows, a DMA into the
+// bytes they read: no load moves past it.
+__device__ __forceinline__ void fence_lds_reads() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// A scalar load of p[i]: i is the same in every lane, and no kernel writes p.
+__device__ __forceinline__ int scalar_load(const int32_t* p, int64_t i) {
+  return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)(p + i);
+}
+
+// Sequence b's new tokens and keys, within the limits of the call.
+struct Seq {
+  int q0;     // packed row of its first new token
+  int nq;     // new tokens that are computed (at most max_q)
+  int len;    // keys
+  int first;  // key index of its first new token (negative: more tokens than keys)
+};
+__device__ __forceinline__ Seq load_seq(const PageTable& pt, int b, int max_q) {
+  const int c0 = min(max(scalar_load(pt.cu, b), 0), pt.tokens);
+  const int c1 = min(max(scalar_load(pt.cu, b + 1), c0), pt.tokens);
+  Seq s;
+  s.q0 = c0;
+  s.nq = min(c1 - c0, max_q);
+  s.len = min(max(scalar_load(pt.lens, b), 0), pt.max_kv);
+  s.first = s.len - (c1 - c0);
+  return s;
+}
+
+// Page id of key `key` (wave-uniform) in a sequence's table row.
+__device__ __forceinline__ int page_id(const PageTable& pt, const int32_t* row, int key) {
+  return scalar_load(row, key >> pt.page_shift);
+}
+
+// Sequence b and row tile of a slot: sequence b's tiles of BM rows start at
+// slot f(b) = floor(cu[b] group / BM) + b, which leaves room for the last,
+// partial tile of each sequence.  The sequence is the number of b >= 1 with
+// f(b) <= slot, counted 64 at a time.  False: the slot holds no tile.
+template <int BM>
+__device__ __forceinline__ bool find_slot(const PagedFwdArgs& a, int slot, int& b, int& tile) {
+  const int lane = threadIdx.x & 63;
+  auto start = [&](int i, int cu) FA_INLINE {
+    return (int)((uint32_t)(min(max(cu, 0), a.pt.tokens) * a.group) / BM) + i;
+  };
+  int n = 0;
+  for (int i0 = 1; i0 <= a.pt.batch; i0 += 64) {
+    const int i = i0 + lane;
+    const bool before = i <= a.pt.batch && start(i, a.pt.cu[min(i, a.pt.batch)]) <= slot;
+    n += __popcll(__ballot(before));
+  }
+  b = __builtin_amdgcn_readfirstlane(n);
+  if (b >= a.pt.batch) return false;
+  tile = slot - start(b, scalar_load(a.pt.cu, b));
+  return tile >= 0;
+}
+
+// Staging of 16 consecutive keys of one page: their K rows and V rows to LDS
+// in the layouts of the 16x16x32 kernels (lds::Tile16).  The swizzles go by
+// key % 16, so one set of lane offsets serves every group.
+template <int D>
+struct GroupStage {
+  static constexpr int ROWB = 2 * D, NI = 16 * ROWB / 1024;  // DMA instructions of K or V
+  uint32_t k_src[NI], v_src[NI];
+  int r_lane;  // row of this lane in the first instruction
+  __device__ __forceinline__ void init(int lane, uint32_t k_ss, uint32_t v_ss) {
+    constexpr int LPR = ROWB / 16;  // lanes of a row
+    r_lane = lane / LPR;
+#pragma unroll
+    for (int it = 0; it < NI; ++it) {
+      const int r = it * (64 / LPR) + r_lane, pc = lane % LPR;
+      k_src[it] = r * k_ss + (pc ^ lds::Tile16<D>::swz_k(r)) * 16;
+      v_src[it] = r * v_ss + (pc ^ lds::Tile16<D>::swz_v(r)) * 16;
+    }
+  }
+  // kp, vp: the group's first rows; rows past `lim` re-read row lim.
+  __device__ __forceinline__ void copy(const char* kp, const char* vp, uint32_t k_dst, uint32_t v_dst,
+                                       int lim, uint32_t k_ss, uint32_t v_ss) const {
+    if (lim >= 15) {
+#pragma unroll
+      for (int it = 0; it < NI; ++it) dma_16b(k_src[it], kp, k_dst + it * 1024);
+#pragma unroll
+      for (int it = 0; it < NI; ++it) dma_16b(v_src[it], vp, v_dst + it * 1024);
+    } else {
+#pragma unroll
+      for (int it = 0; it < NI; ++it) {
+        const int over = max(it * (1024 / ROWB) + r_lane - lim, 0);
+        dma_16b(k_src[it] - over * k_ss, kp, k_dst + it * 1024);
+        dma_16b(v_src[it] - over * v_ss, vp, v_dst + it * 1024);
+      }
+    }
+  }
+};
+
+}  // namespace
+}  // namespace fa

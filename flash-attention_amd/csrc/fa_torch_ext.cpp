@@ -154,6 +154,8 @@ pybind11::dict device_info(int device) {
 
 }  // namespace
 
+void bind_cache(pybind11::module_& m);  // fa_torch_cache.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("forward", &fa_forward, pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"),
         pybind11::arg("o") = std::optional<torch::Tensor>{}, pybind11::arg("benchmark") = false,
@@ -164,4 +166,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("device_info", &device_info, pybind11::arg("device") = 0,
         "hipDeviceProp summary and dense fp16/bf16 MFMA peak");
   m.def("version", []() { return std::string(fa_version()); });
+  bind_cache(m);
 }

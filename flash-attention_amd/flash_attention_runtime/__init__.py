@@ -9,7 +9,8 @@ the reference), ``return_lse`` (also return the natural-log logsumexp,
 fp32 [B, H, N]) and ``split_kv`` (default True: problems whose grid would
 leave most CUs idle behind a few long q-tiles split their key ranges across
 workgroups, with an fp32 workspace from torch's allocator; False always runs
-one workgroup per q-tile).
+one workgroup per q-tile).  Beyond the reference, ``cache`` has the operators
+around a paged key/value cache and the q/k norm with rotation.
 
 The reference JIT-compiles its CUDA extension on first use
 (``__init__.py:10-27``); here the HIP library ``libfa_mi355x.so`` and the
@@ -93,4 +94,14 @@ def version() -> str:
     return _EXT.version()
 
 
-__all__ = ["forward", "forward_timed", "device_info", "version"]
+from .cache import (  # noqa: E402  (needs the extension)
+    paged_evict,
+    paged_forward,
+    paged_key_weights,
+    paged_store,
+    qk_norm_rope,
+    qk_norm_rope_backward,
+)
+
+__all__ = ["forward", "forward_timed", "device_info", "version", "paged_forward", "paged_store",
+           "paged_key_weights", "paged_evict", "qk_norm_rope", "qk_norm_rope_backward"]
