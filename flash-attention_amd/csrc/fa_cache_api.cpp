@@ -39,7 +39,7 @@ PagedPlan plan_paged(int tokens, int batch, int kv_heads, int group, int head_di
     g.rows = most <= 16 ? 16 : 32;
     g.slots = batch;
     const int64_t base = (int64_t)batch * kv_heads;
-    cut(g, (4 * (int64_t)compute_units + base - 1) / base, 256);
+    cut(g, (4 * (int64_t)compute_units + base - 1) / base, 512);
   }
   p.workspace_bytes = (p.chunk.ws_rows + p.decode.ws_rows) * (head_dim + 2) * 4;
   return p;

@@ -41,7 +41,11 @@ struct PagedFwdArgs {
   // tiles of all sequences) x kv heads x splits of `chunk` keys.
   int32_t min_rows, max_rows;
   int32_t slots, splits, chunk;
-  FastDiv by_group, by_slots, by_kvh, by_splits;
+  int32_t join;                    // merge: lane groups of a row
+  FastDiv by_group, by_kvh, by_splits;
+  // Order of the chunk kernel's grid (set_order): units are kv heads x splits.
+  int32_t units, per_xcd, unit_group, xcds;
+  FastDiv by_units, by_group_slots, by_unit_group;
   float* ws_o;                     // [slot][kv head][split][BM][D] partial o, fp32
   float* ws_e;                     // the same rows: (log2 of the rounded P's sum, of the plain one's)
 };

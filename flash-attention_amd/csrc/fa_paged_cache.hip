@@ -10,8 +10,8 @@
 // each per 16 lanes) over half the matrix work of attention.
 //
 // fa_select_kernel: the keep - recent heaviest of a head's keys by a radix
-// search for their least weight, eight bits at a time, and the list of the
-// kept keys in order.  fa_move_kernel copies their rows: bound by memory.
+// search for their least weight (digits of 11, 11 and 10 bits), and the list of
+// the kept keys in order.  fa_move_kernel copies their rows: bound by memory.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -212,13 +212,23 @@ __device__ __forceinline__ uint32_t weight_order(float x) {
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / 64;
-constexpr int kSelHold = 16;  // weights a thread keeps in registers
+constexpr int kSelBins = 2048, kSelCopies = 4;
 
+// One workgroup per sequence and kv head.  A thread owns K consecutive keys of
+// a segment of 1024 K, in one page (a page holds whole groups of 16): one page
+// lookup, vector loads, and index order is thread order, so the places of the
+// kept keys are one prefix sum per segment.  Weights of the first segment stay
+// in registers; longer sequences read the others again in each of the three
+// passes.  The histogram has copies by lane, as near weights share their top
+// bits and LDS atomics on one word queue up.  8 sequences x 8 heads of 16384
+// keys: 40 us with one key a thread and eight-bit digits.
+template <int K>
 __global__ void __launch_bounds__(kSelThreads) fa_select_kernel(const PagedEvictArgs a) {
-  __shared__ int hist[256];
-  __shared__ int wave_n[2][kSelWaves];
+  __shared__ int hist[kSelCopies][kSelBins];
+  __shared__ int wave_n[kSelWaves];
   __shared__ int pick[2];
   __shared__ int bad;
+  typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));  // any key weight's address
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.x / a.kv_heads, kvh = blockIdx.x - b * a.kv_heads;
   const int len = min(max(a.pt.lens[b], 0), a.pt.max_kv);
@@ -226,7 +236,7 @@ __global__ void __launch_bounds__(kSelThreads) fa_select_kernel(const PagedEvict
   const int32_t* row = a.pt.table + b * a.pt.table_stride;
   const int32_t* new_row = a.new_table + b * a.new_table_stride;
   int32_t* kept = a.kept + ((int64_t)b * a.kv_heads + kvh) * a.keep;
-  const int page = 1 << a.pt.page_shift;
+  const int shift_p = a.pt.page_shift, page = 1 << shift_p;
 
   if (tid == 0) bad = 0;
   __syncthreads();
@@ -248,89 +258,108 @@ __global__ void __launch_bounds__(kSelThreads) fa_select_kernel(const PagedEvict
 
   // The want heaviest of the keys before the recent ones.
   const int old = len - a.recent, want = a.keep - a.recent;
-  auto order_of = [&](int i) FA_INLINE {
-    return weight_order(a.w[(int64_t)row[i >> a.pt.page_shift] * a.w_sp + kvh * a.w_sh + (i & (page - 1))]);
+  constexpr int kSeg = kSelThreads * K;
+  uint32_t u[K];
+  auto load = [&](int seg) FA_INLINE {
+    const int i0 = seg + tid * K;
+    if (i0 >= old) return;
+    const float* w = a.w + (int64_t)row[i0 >> shift_p] * a.w_sp + kvh * a.w_sh + (i0 & (page - 1));
+#pragma unroll
+    for (int j = 0; j < K; j += 4) {
+      const f32x4_u x = *reinterpret_cast<const f32x4_u*>(w + j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[j + e] = weight_order(x[e]);
+    }
   };
-  uint32_t held[kSelHold];
-#pragma unroll
-  for (int j = 0; j < kSelHold; ++j) {
-    const int i = j * kSelThreads + tid;
-    held[j] = i < old ? order_of(i) : 0u;
-  }
-  uint32_t prefix = 0;  // the top bits of the want-th largest
-  int left = want;      // its rank among the keys with that prefix
-  for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+  load(0);
+  uint32_t prefix = 0, mask = 0;  // the top bits of the want-th largest
+  int left = want;                // its rank among the keys with that prefix
+#pragma unroll 1
+  for (int pass = 0; pass < 3 && want > 0; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t digit = pass == 2 ? 1023u : 2047u;
+    for (int i = tid; i < kSelCopies * kSelBins; i += kSelThreads) (&hist[0][0])[i] = 0;
     __syncthreads();
-    const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
-    auto count_one = [&](uint32_t u) FA_INLINE {
-      if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & 255u], 1);
-    };
+#pragma unroll 1
+    for (int seg = 0; seg < old; seg += kSeg) {
+      if (old > kSeg) load(seg);
 #pragma unroll
-    for (int j = 0; j < kSelHold; ++j)
-      if (j * kSelThreads + tid < old) count_one(held[j]);
-    for (int i = kSelHold * kSelThreads + tid; i < old; i += kSelThreads) count_one(order_of(i));
+      for (int j = 0; j < K; ++j)
+        if (seg + tid * K + j < old && (u[j] & mask) == prefix)
+          atomicAdd(&hist[lane & (kSelCopies - 1)][(u[j] >> shift) & digit], 1);
+    }
     __syncthreads();
-    if (wave == 0) {
-      // counts of the buckets 4 lane .. + 3 and of those above them
-      int c[4], sum = 0;
+    // Two bins a thread; counts of the keys above them by a suffix sum.
+    int c[2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum += c[j] = hist[4 * lane + j];
-      int above = sum;  // inclusive suffix sum over lanes
-      for (int d = 1; d < 64; d <<= 1) {
-        const int x = __shfl_down(above, d);
-        above += lane + d < 64 ? x : 0;
-      }
-      above -= sum;
+    for (int j = 0; j < 2; ++j) {
+      c[j] = 0;
 #pragma unroll
-      for (int j = 3; j >= 0; --j) {
-        if (above < left && left <= above + c[j]) {
-          pick[0] = 4 * lane + j;
-          pick[1] = left - above;
-        }
-        above += c[j];
+      for (int q = 0; q < kSelCopies; ++q) c[j] += hist[q][2 * tid + j];
+    }
+    int above = c[0] + c[1];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int x = __shfl_down(above, d);
+      above += lane + d < 64 ? x : 0;
+    }
+    if (lane == 0) wave_n[wave] = above;
+    __syncthreads();
+    above -= c[0] + c[1];
+#pragma unroll
+    for (int w = 1; w < kSelWaves; ++w) above += w > wave ? wave_n[w] : 0;
+#pragma unroll
+    for (int j = 1; j >= 0; --j) {
+      if (above < left && left <= above + c[j]) {
+        pick[0] = 2 * tid + j;
+        pick[1] = left - above;
       }
+      above += c[j];
     }
     __syncthreads();
     prefix |= (uint32_t)pick[0] << shift;
+    mask |= digit << shift;
     left = pick[1];
   }
 
   // Kept: keys above the threshold, the first `left` that equal it, and the
-  // recent ones, in order: key i goes to place (larger before i) + (equal
-  // before i, at most left).
+  // recent ones: key i goes to place (larger before i) + (equal before i, at
+  // most left).  Both counts in one prefix sum, 16 bits each (a segment has at
+  // most 2^14 keys).
   int gt_before = 0, eq_before = 0;
-  auto place = [&](int i0, bool in, uint32_t u) FA_INLINE {
-    const bool gt = in && want > 0 && u > prefix, eq = in && want > 0 && u == prefix;
-    const uint64_t bg = __ballot(gt), be = __ballot(eq), below = ((uint64_t)1 << lane) - 1;
-    if (lane == 0) {
-      wave_n[0][wave] = __popcll(bg);
-      wave_n[1][wave] = __popcll(be);
+#pragma unroll 1
+  for (int seg = 0; seg < old && want > 0; seg += kSeg) {
+    if (old > kSeg) load(seg);
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+      if (seg + tid * K + j < old) mine += u[j] > prefix ? 1 : u[j] == prefix ? 1 << 16 : 0;
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int x = __shfl_up(sum, d);
+      sum += lane >= d ? x : 0;
     }
+    if (lane == 63) wave_n[wave] = sum;
     __syncthreads();
-    int g = gt_before, e = eq_before, gs = 0, es = 0;
+    int before = sum - mine, all = 0;
 #pragma unroll
     for (int w = 0; w < kSelWaves; ++w) {
-      if (w < wave) {
-        g += wave_n[0][w];
-        e += wave_n[1][w];
-      }
-      gs += wave_n[0][w];
-      es += wave_n[1][w];
+      before += w < wave ? wave_n[w] : 0;
+      all += wave_n[w];
     }
-    g += __popcll(bg & below);
-    e += __popcll(be & below);
-    if (gt || (eq && e < left)) kept[g + min(e, left)] = i0 + tid;
-    gt_before += gs;
-    eq_before += es;
-    __syncthreads();
-  };
+    int g = gt_before + (before & 0xffff), e = eq_before + (before >> 16);
 #pragma unroll
-  for (int j = 0; j < kSelHold; ++j)
-    if (j * kSelThreads < old) place(j * kSelThreads, j * kSelThreads + tid < old, held[j]);
-  for (int i0 = kSelHold * kSelThreads; i0 < old; i0 += kSelThreads) {
-    const bool in = i0 + tid < old;
-    place(i0, in, in ? order_of(i0 + tid) : 0u);
+    for (int j = 0; j < K; ++j) {
+      const int i = seg + tid * K + j;
+      const bool gt = i < old && u[j] > prefix, eq = i < old && u[j] == prefix;
+      if (gt || (eq && e < left)) kept[g + min(e, left)] = i;
+      g += gt;
+      e += eq;
+    }
+    gt_before += all & 0xffff;
+    eq_before += all >> 16;
+    __syncthreads();
   }
   for (int t = tid; t < a.recent; t += kSelThreads) kept[want + t] = old + t;
 }
@@ -404,7 +433,11 @@ hipError_t launch_paged_evict(const PagedEvictArgs& args, int head_dim, hipStrea
   int blocks = (most + per - 1) / per;
   if (bk * std::max(blocks, 1) > 0x7fffffff) return hipErrorInvalidValue;
   void* sargs[] = {&a};
-  hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&fa_select_kernel), dim3((unsigned)bk),
+  // Four keys a thread where they hold all of a sequence: less work in a row.
+  const void* select = a.pt.max_kv <= 4 * kSelThreads
+                           ? reinterpret_cast<const void*>(&fa_select_kernel<4>)
+                           : reinterpret_cast<const void*>(&fa_select_kernel<16>);
+  hipError_t e = hipLaunchKernel(select, dim3((unsigned)bk),
                                  dim3(kSelThreads), sargs, 0, stream);
   if (e != hipSuccess || blocks == 0) return e;
   void* margs[] = {&a, &blocks};

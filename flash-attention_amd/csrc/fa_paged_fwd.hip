@@ -324,16 +324,6 @@ __global__ void __launch_bounds__(256) fa_paged_decode_kernel(const PagedFwdArgs
   W w;
   w.init(wave_lds, wave_lds + 2 * TB, a.scale_log2);
   const int l16 = w.l16, g4 = w.g4;
-  const char* qh = a.q + s.q0 * a.q_st + (int64_t)kvh * a.group * a.q_sh;
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int r = min(16 * rb + l16, n_rows - 1);
-    const int i = fast_div(r, a.by_group), h = r - i * a.group;
-    w.last[rb] = last_key(a, s, i);
-#pragma unroll
-    for (int st = 0; st < W::KST; ++st)
-      w.qf[rb][st] = *reinterpret_cast<const i16x8*>(qh + i * a.q_st + h * a.q_sh + (32 * st + 8 * g4) * 2);
-  }
   const int full_end = max(0, last_key(a, s, 0) + 1);  // every row sees the keys before it
 
   GroupStage<D> stage;
@@ -365,7 +355,23 @@ __global__ void __launch_bounds__(256) fa_paged_decode_kernel(const PagedFwdArgs
     return present;
   };
   unsigned present = 0, present_next = 0;
-  __builtin_amdgcn_s_waitcnt(0);  // q is in registers: only DMA is in flight below
+  if (wave < n_tiles) {
+    fetch(wave);
+    present = issue(wave, 0);
+    if (wave + 4 < n_tiles) fetch(wave + 4);
+  }
+  // q behind the first tile's DMA: loads return in order, so a wait for all but
+  // the next tile's DMA covers q too.
+  const char* qh = a.q + s.q0 * a.q_st + (int64_t)kvh * a.group * a.q_sh;
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const int r = min(16 * rb + l16, n_rows - 1);
+    const int i = fast_div(r, a.by_group), h = r - i * a.group;
+    w.last[rb] = last_key(a, s, i);
+#pragma unroll
+    for (int st = 0; st < W::KST; ++st)
+      w.qf[rb][st] = *reinterpret_cast<const i16x8*>(qh + i * a.q_st + h * a.q_sh + (32 * st + 8 * g4) * 2);
+  }
   auto stage_next = [&](int t, int buf) FA_INLINE {
     if (t + 4 < n_tiles) {
       present_next = issue(t + 4, buf ^ 1);
@@ -379,9 +385,6 @@ __global__ void __launch_bounds__(256) fa_paged_decode_kernel(const PagedFwdArgs
   // tile reaches past it.)
   auto whole = [&](int t) FA_INLINE { return c0 + 32 * t + 32 <= full_end && present == 3u; };
   if (wave < n_tiles) {
-    fetch(wave);
-    present = issue(wave, 0);
-    if (wave + 4 < n_tiles) fetch(wave + 4);
     // Whole tiles, then, from the first tile with a masked key on, the rest:
     // masked tiles are the last ones, or lie on absent pages.
     int t = wave, buf = 0;
@@ -470,6 +473,28 @@ __global__ void __launch_bounds__(256) fa_paged_decode_kernel(const PagedFwdArgs
 
 // ---- many rows: chunks ----
 
+// Unit (kv head and split of its keys) and slot of a workgroup.  Workgroup w
+// runs on XCD w % 8, in order; a unit's slots share its keys through the XCD's
+// L2, and the longest slots of all units should start first:
+//  * a multiple of 8 units: whole units per XCD, up to four of them interleaved;
+//  * 1, 2 or 4: 8 / units XCDs take turns with a unit's slots;
+//  * else all units interleaved over all XCDs.
+__device__ __forceinline__ bool unit_and_slot(const PagedFwdArgs& a, int& unit, int& slot) {
+  const int xcd = blockIdx.x % kNumXcd, i = blockIdx.x / kNumXcd;
+  if (a.per_xcd > 0) {
+    const int grp = fast_div(i, a.by_group_slots), w = i - grp * a.unit_group * a.slots;
+    slot = fast_div(w, a.by_unit_group);
+    unit = xcd * a.per_xcd + grp * a.unit_group + (w - slot * a.unit_group);
+  } else if (a.xcds > 0) {
+    unit = xcd / a.xcds;
+    slot = i * a.xcds + xcd % a.xcds;
+  } else {
+    slot = fast_div(blockIdx.x, a.by_units);
+    unit = blockIdx.x - slot * a.units;
+  }
+  return slot < a.slots;
+}
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
     fa_paged_chunk_kernel(const PagedFwdArgs a) {
@@ -480,12 +505,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Logical order: kv heads, then key splits, then slots, the last (longest
-  // causal) first; xcd_remap gives each XCD a contiguous range of it, whose
-  // workgroups read the same keys.
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int hs = fast_div(id, a.by_slots);
-  const int slot = a.slots - 1 - (id - hs * a.slots);
+  int hs, slot;
+  if (!unit_and_slot(a, hs, slot)) return;
   const int kvh = fast_div(hs, a.by_splits), split = hs - kvh * a.splits;
   int b, tile0;
   if (!find_slot<BM>(a, slot, b, tile0)) return;
@@ -660,13 +681,18 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 }
 
 // Joins the partials of split rows: weights 2^(e - max e) of normalised
-// partials.  BM: rows of a slot; a decode slot is a sequence.
+// partials.  BM: rows of a slot; a decode slot is a sequence.  a.join groups of
+// D / 4 lanes share a row, each with every join-th chunk, four in flight, and
+// meet in LDS: one group per row left 128 chunks to a loop of dependent loads
+// (125 us against 98 for the attention itself at one sequence of 131072 keys).
 template <int D, bool BF16, int BM>
 __global__ void __launch_bounds__(256) fa_paged_merge_kernel(const PagedFwdArgs a) {
-  constexpr int TPR = D / 4, RPB = 256 / TPR;
-  constexpr int PER = (BM + RPB - 1) / RPB;  // workgroups of a slot and kv head
-  const int sk = blockIdx.x / PER, r = (blockIdx.x - sk * PER) * RPB + (int)threadIdx.x / TPR;
-  const int d = ((int)threadIdx.x % TPR) * 4;
+  constexpr int TPR = D / 4, GROUPS = 256 / TPR;
+  __shared__ f32x4 part_o[GROUPS][TPR];
+  __shared__ float part_e[GROUPS][4];  // top, sum of weights; the same of the plain sums
+  const int grp = (int)threadIdx.x / TPR, lane = (int)threadIdx.x % TPR, d = lane * 4;
+  const int rpb = GROUPS / a.join, per = (BM + rpb - 1) / rpb;  // rows, workgroups of a slot
+  const int sk = blockIdx.x / per, r = (blockIdx.x - sk * per) * rpb + grp / a.join;
   const int slot = fast_div(sk, a.by_kvh), kvh = sk - slot * a.kv_heads;
   int b = slot, tile0 = 0;
   if constexpr (BM == kChunkRows) {
@@ -678,31 +704,69 @@ __global__ void __launch_bounds__(256) fa_paged_merge_kernel(const PagedFwdArgs 
   const int last_row = min(row0 + BM, n_rows) - 1;
   const int kv_end = max(0, last_key(a, s, fast_div(last_row, a.by_group)) + 1);
   const int n_act = (kv_end + a.chunk - 1) / a.chunk;
-  if (n_act <= 1 || r >= BM || row0 + r >= n_rows) return;
+  if (n_act <= 1) return;
+  const bool row = r < BM && row0 + r < n_rows;
   const int64_t w0 = (int64_t)sk * a.splits * BM + r;
-  float top = -INFINITY, top_u = -INFINITY;
-  for (int c = 0; c < n_act; ++c) {
-    top = fmaxf(top, a.ws_e[(w0 + (int64_t)c * BM) * 2]);
-    top_u = fmaxf(top_u, a.ws_e[(w0 + (int64_t)c * BM) * 2 + 1]);
-  }
-  float lr = 0.0f, lu = 0.0f;
+  float top = -INFINITY, top_u = -INFINITY, lr = 0.0f, lu = 0.0f;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int c = 0; c < n_act; ++c) {
-    const int64_t wr = w0 + (int64_t)c * BM;
-    const float e = a.ws_e[wr * 2], eu = a.ws_e[wr * 2 + 1];
-    if (e == -INFINITY) continue;  // its keys are all masked for this row
-    const float f = fast_exp2(e - top);
-    lr += f;
-    lu += fast_exp2(eu - top_u);
-    acc += f * *reinterpret_cast<const f32x4*>(a.ws_o + wr * D + d);
+  if (row) {
+    constexpr int BATCH = 4;
+    for (int c = grp & (a.join - 1); c < n_act; c += BATCH * a.join) {
+      float e[BATCH], eu[BATCH];
+      f32x4 o[BATCH];
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        const int64_t wr = w0 + (int64_t)min(c + j * a.join, n_act - 1) * BM;
+        e[j] = a.ws_e[wr * 2];
+        eu[j] = a.ws_e[wr * 2 + 1];
+        o[j] = *reinterpret_cast<const f32x4*>(a.ws_o + wr * D + d);
+      }
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        // (e = -inf: its keys are all masked for this row)
+        if (c + j * a.join >= n_act || e[j] == -INFINITY) continue;
+        const float t = fmaxf(top, e[j]), tu = fmaxf(top_u, eu[j]);
+        const float old = fast_exp2(top - t), f = fast_exp2(e[j] - t);
+        lr = lr * old + f;
+        acc = acc * old + o[j] * f;
+        lu = lu * fast_exp2(top_u - tu) + fast_exp2(eu[j] - tu);
+        top = t;
+        top_u = tu;
+      }
+    }
   }
+  if (a.join > 1) {
+    part_o[grp][lane] = acc;
+    if (lane == 0) {
+      part_e[grp][0] = top;
+      part_e[grp][1] = lr;
+      part_e[grp][2] = top_u;
+      part_e[grp][3] = lu;
+    }
+    __syncthreads();
+    if ((grp & (a.join - 1)) != 0) return;
+    for (int g = 0; g < a.join; ++g) {
+      top = fmaxf(top, part_e[grp + g][0]);
+      top_u = fmaxf(top_u, part_e[grp + g][2]);
+    }
+    lr = lu = 0.0f;
+    acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int g = 0; g < a.join; ++g) {
+      if (part_e[grp + g][1] == 0.0f) continue;  // no chunk with a visible key
+      const float f = fast_exp2(part_e[grp + g][0] - top);
+      lr += f * part_e[grp + g][1];
+      lu += fast_exp2(part_e[grp + g][2] - top_u) * part_e[grp + g][3];
+      acc += part_o[grp + g][lane] * f;
+    }
+  }
+  if (!row) return;
   const bool none = lr == 0.0f;
   const float inv = none ? 0.0f : 1.0f / lr;
   const int i = fast_div(row0 + r, a.by_group), h = kvh * a.group + row0 + r - i * a.group;
   const int64_t t = s.q0 + i;
   *reinterpret_cast<u32x2*>(a.o + t * a.o_st + h * a.o_sh + d * 2) =
       u32x2{pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv)};
-  if (a.lse != nullptr && d == 0)
+  if (a.lse != nullptr && lane == 0)
     a.lse[t * a.heads + h] = none ? -INFINITY : (top_u + __log2f(lu)) * kLn2;
 }
 
@@ -712,6 +776,21 @@ hipError_t launch(F* fn, int64_t grid, const PagedFwdArgs& args, hipStream_t str
   void* kargs[] = {const_cast<PagedFwdArgs*>(&args)};
   return hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)grid), dim3(256), kargs, 0,
                          stream);
+}
+
+// The chunk kernel's grid order (unit_and_slot) and its workgroups.
+int64_t set_order(PagedFwdArgs& a) {
+  a.units = a.kv_heads * a.splits;
+  a.per_xcd = a.units % kNumXcd == 0 ? a.units / kNumXcd : 0;
+  a.unit_group = 1;
+  for (int g = 2; g <= 4; ++g)
+    if (a.per_xcd % g == 0) a.unit_group = g;
+  a.xcds = a.per_xcd == 0 && kNumXcd % a.units == 0 ? kNumXcd / a.units : 0;
+  a.by_units = make_fast_div((uint32_t)a.units);
+  a.by_group_slots = make_fast_div((uint32_t)(a.unit_group * a.slots));
+  a.by_unit_group = make_fast_div((uint32_t)a.unit_group);
+  if (a.xcds > 0) return (int64_t)kNumXcd * ((a.slots + a.xcds - 1) / a.xcds);
+  return (int64_t)a.units * a.slots;
 }
 
 template <int D, bool BF16>
@@ -728,7 +807,6 @@ hipError_t launch_all(const PagedFwdArgs& base, const PagedPlan& plan, void* ws,
     a.slots = g->slots;
     a.splits = g->splits;
     a.chunk = g->chunk;
-    a.by_slots = make_fast_div((uint32_t)g->slots);
     a.by_splits = make_fast_div((uint32_t)(decode ? g->slots * a.kv_heads : g->splits));
     const int64_t sk = (int64_t)g->slots * a.kv_heads;
     a.ws_o = reinterpret_cast<float*>(at);
@@ -736,15 +814,19 @@ hipError_t launch_all(const PagedFwdArgs& base, const PagedPlan& plan, void* ws,
     at += g->ws_rows * (D + 2) * 4;
     hipError_t e;
     if (!decode)
-      e = launch(&fa_paged_chunk_kernel<D, BF16>, sk * g->splits, a, stream);
+      e = launch(&fa_paged_chunk_kernel<D, BF16>, set_order(a), a, stream);
     else if (g->rows == 16)
       e = launch(&fa_paged_decode_kernel<D, BF16, 1>, sk * g->splits, a, stream);
     else
       e = launch(&fa_paged_decode_kernel<D, BF16, 2>, sk * g->splits, a, stream);
     if (e != hipSuccess) return e;
     if (g->splits == 1) continue;
-    constexpr int RPB = 256 / (D / 4);
-    const int64_t per = (g->rows + RPB - 1) / RPB;
+    // As many lane groups a row as it has chunks, a power of two.
+    constexpr int GROUPS = 256 / (D / 4);
+    a.join = 1;
+    while (a.join < g->splits && a.join < GROUPS) a.join *= 2;
+    const int rpb = GROUPS / a.join;
+    const int64_t per = (g->rows + rpb - 1) / rpb;
     if (!decode)
       e = launch(&fa_paged_merge_kernel<D, BF16, kChunkRows>, sk * per, a, stream);
     else if (g->rows == 16)

@@ -69,25 +69,50 @@ __device__ __forceinline__ int page_id(const PageTable& pt, const int32_t* row, 
   return scalar_load(row, key >> pt.page_shift);
 }
 
-// Sequence b and row tile of a slot: sequence b's tiles of BM rows start at
-// slot f(b) = floor(cu[b] group / BM) + b, which leaves room for the last,
-// partial tile of each sequence.  The sequence is the number of b >= 1 with
-// f(b) <= slot, counted 64 at a time.  False: the slot holds no tile.
+// Sequence b and row tile of a slot of the chunk kernel's grid; the slots run
+// from the longest tiles to the shortest.  False: the slot holds no tile.
+//
+// Up to 64 sequences: the ones with more keys first, each lane holding one
+// sequence's tiles and the number of tiles before them.  More: in their order
+// from the last, sequence b's tiles at slot f(b) = floor(cu[b] group / BM) + b,
+// which leaves room for the last, partial tile of each; the sequence is then
+// the number of b >= 1 with f(b) <= slot, counted 64 at a time.
 template <int BM>
 __device__ __forceinline__ bool find_slot(const PagedFwdArgs& a, int slot, int& b, int& tile) {
   const int lane = threadIdx.x & 63;
-  auto start = [&](int i, int cu) FA_INLINE {
+  if (a.pt.batch <= 64) {
+    int tiles = 0, len = -1;
+    if (lane < a.pt.batch) {
+      const int c0 = min(max(a.pt.cu[lane], 0), a.pt.tokens);
+      const int c1 = min(max(a.pt.cu[lane + 1], c0), a.pt.tokens);
+      const int rows = min(c1 - c0, a.max_q) * a.group;
+      tiles = rows >= a.min_rows ? (rows + BM - 1) / BM : 0;
+      len = min(max(a.pt.lens[lane], 0), a.pt.max_kv);
+    }
+    int start = 0;
+    for (int i = 0; i < a.pt.batch; ++i) {
+      const int l = __builtin_amdgcn_readlane(len, i), t = __builtin_amdgcn_readlane(tiles, i);
+      start += l > len || (l == len && i < lane) ? t : 0;
+    }
+    const uint64_t has = __ballot(start <= slot && slot < start + tiles);
+    if (has == 0) return false;
+    b = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(has));
+    tile = __builtin_amdgcn_readlane(start + tiles - 1, b) - slot;
+    return true;
+  }
+  auto begin = [&](int i, int cu) FA_INLINE {
     return (int)((uint32_t)(min(max(cu, 0), a.pt.tokens) * a.group) / BM) + i;
   };
+  slot = a.slots - 1 - slot;
   int n = 0;
   for (int i0 = 1; i0 <= a.pt.batch; i0 += 64) {
     const int i = i0 + lane;
-    const bool before = i <= a.pt.batch && start(i, a.pt.cu[min(i, a.pt.batch)]) <= slot;
+    const bool before = i <= a.pt.batch && begin(i, a.pt.cu[min(i, a.pt.batch)]) <= slot;
     n += __popcll(__ballot(before));
   }
   b = __builtin_amdgcn_readfirstlane(n);
   if (b >= a.pt.batch) return false;
-  tile = slot - start(b, scalar_load(a.pt.cu, b));
+  tile = slot - begin(b, scalar_load(a.pt.cu, b));
   return tile >= 0;
 }
 

@@ -329,20 +329,29 @@ __global__ void __launch_bounds__(256) fa_norm_bwd_kernel(const NormArgs n) {
   }
 }
 
-// Sums the workgroups' parts: 16 columns of a workgroup, 16 threads a column.
+// Sums the workgroups' parts in a fixed order: 8 columns of a workgroup, 32
+// threads a column, eight loads of each in flight.
 template <int D>
 __global__ void __launch_bounds__(256) fa_norm_dw_kernel(const NormArgs n, int blocks) {
-  __shared__ float part[16][17];
-  const int c = threadIdx.x & 15, p = (int)threadIdx.x >> 4;
-  const int col = blockIdx.x * 16 + c;
+  constexpr int P = 32, BATCH = 8;
+  __shared__ float part[P][9];
+  const int c = threadIdx.x & 7, p = (int)threadIdx.x >> 3;
+  const int col = blockIdx.x * 8 + c;
   float sum = 0.0f;
-  for (int i = p; i < blocks; i += 16) sum += n.ws[(int64_t)i * 2 * D + col];
+  for (int i = p; i < blocks; i += P * BATCH) {
+    float x[BATCH];
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j)
+      x[j] = i + j * P < blocks ? n.ws[(int64_t)(i + j * P) * 2 * D + col] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) sum += x[j];
+  }
   part[p][c] = sum;
   __syncthreads();
   if (p == 0) {
     float total = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) total += part[i][c];
+    for (int i = 0; i < P; ++i) total += part[i][c];
     n.dw[col / D][col % D] = total;
   }
 }
@@ -367,7 +376,7 @@ hipError_t launch_bwd_as(const NormArgs& n, int blocks, hipStream_t stream) {
   if (e != hipSuccess) return e;
   int count = blocks;
   void* kargs[] = {const_cast<NormArgs*>(&n), &count};
-  return hipLaunchKernel(reinterpret_cast<const void*>(&fa_norm_dw_kernel<D>), dim3(2 * D / 16), dim3(256),
+  return hipLaunchKernel(reinterpret_cast<const void*>(&fa_norm_dw_kernel<D>), dim3(2 * D / 8), dim3(256),
                          kargs, 0, stream);
 }
 
