@@ -17,29 +17,31 @@ namespace fa {
 PagedPlan plan_paged(int tokens, int batch, int kv_heads, int group, int head_dim, int max_q,
                      int max_kv, int compute_units) {
   PagedPlan p = {};
+  p.compute_units = compute_units;
   const int64_t most = (int64_t)std::min(max_q, tokens) * group;  // rows of a sequence
   const int64_t keys = std::max(max_kv, 1);
-  auto cut = [&](PagedGrid& g, int64_t want, int64_t least) {
-    // `want` splits of at least `least` keys, in whole 64-key tiles
-    want = std::max<int64_t>(1, std::min(want, (keys + least - 1) / least));
-    g.chunk = (int)(((keys + want - 1) / want + 63) / 64 * 64);
-    g.splits = (int)((keys + g.chunk - 1) / g.chunk);
-    g.ws_rows = g.splits > 1 ? (uint64_t)g.slots * kv_heads * g.splits * g.rows : 0;
-  };
   if (most > kDecodeRows) {
     PagedGrid& g = p.chunk;
     g.rows = kChunkRows;
     g.slots = (int)((int64_t)tokens * group / kChunkRows + batch);
-    // Two workgroups per CU; a grid that has them already is not split.
-    const int64_t base = (int64_t)g.slots * kv_heads;
-    cut(g, 2 * (int64_t)compute_units / base, 512);
+    // Two workgroups per CU; the tiles of the last round go in pieces of 512
+    // keys or more, two rounds of them at most.
+    g.conc = std::max(1, 2 * compute_units / kv_heads);
+    g.pieces = keys <= 512 ? 0 : (int)std::min<int64_t>(2 * (int64_t)g.conc, 64 * (int64_t)g.slots);
+    g.ws_rows = (uint64_t)g.pieces * kv_heads * g.rows;
   }
   if (most <= kDecodeRows || batch > 1) {
     PagedGrid& g = p.decode;
     g.rows = most <= 16 ? 16 : 32;
     g.slots = batch;
+    // Four workgroups per CU (one runs at a time at D = 128: lengths are
+    // ragged), of 512 keys or more in whole 64-key tiles.
     const int64_t base = (int64_t)batch * kv_heads;
-    cut(g, (4 * (int64_t)compute_units + base - 1) / base, 512);
+    const int64_t want = std::max<int64_t>(
+        1, std::min((4 * (int64_t)compute_units + base - 1) / base, (keys + 511) / 512));
+    g.chunk = (int)(((keys + want - 1) / want + 63) / 64 * 64);
+    g.splits = (int)((keys + g.chunk - 1) / g.chunk);
+    g.ws_rows = g.splits > 1 ? (uint64_t)base * g.splits * g.rows : 0;
   }
   p.workspace_bytes = (p.chunk.ws_rows + p.decode.ws_rows) * (head_dim + 2) * 4;
   return p;

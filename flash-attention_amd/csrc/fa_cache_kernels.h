@@ -37,16 +37,20 @@ struct PagedFwdArgs {
   int32_t heads, kv_heads, group;
   int32_t max_q, causal;
   float scale_log2;                // softmax scale * log2(e)
-  // Which sequences a launch serves, by their rows, and its grid: slots (row
-  // tiles of all sequences) x kv heads x splits of `chunk` keys.
+  // Which sequences a launch serves, by their rows, and its grid.  Decode
+  // kernel: slots (sequences) x kv heads x splits of `chunk` keys.  Chunk
+  // kernel: at most `slots` row tiles per kv head, and up to 2 conc pieces of
+  // the last ones (LastRound).
   int32_t min_rows, max_rows;
   int32_t slots, splits, chunk;
-  int32_t join;                    // merge: lane groups of a row
-  FastDiv by_group, by_kvh, by_splits;
-  // Order of the chunk kernel's grid (set_order): units are kv heads x splits.
-  int32_t units, per_xcd, unit_group, xcds;
-  FastDiv by_units, by_group_slots, by_unit_group;
-  float* ws_o;                     // [slot][kv head][split][BM][D] partial o, fp32
+  int32_t conc, max_pieces;        // workgroups of a kv head that run at once, its most pieces
+  float piece_cost;
+  int32_t join, merge_rows;        // merge: lane groups of a row, rows of a workgroup
+  FastDiv by_group, by_kvh, by_splits, by_conc;
+  // Order of the chunk kernel's grid (set_order).
+  int32_t places, per_xcd, unit_group, xcds;
+  FastDiv by_group_places, by_unit_group;
+  float* ws_o;                     // [slot or piece][BM][D] partial o, fp32, of each kv head
   float* ws_e;                     // the same rows: (log2 of the rounded P's sum, of the plain one's)
 };
 
@@ -57,11 +61,14 @@ constexpr int kChunkRows = 128;  // rows of a chunk kernel's workgroup
 
 struct PagedGrid {
   int32_t rows;  // rows of a slot (BM); 0: not launched
-  int32_t slots, splits, chunk;
-  uint64_t ws_rows;  // rows of partials
+  int32_t slots;
+  int32_t splits, chunk;  // decode
+  int32_t conc, pieces;   // chunk: at once per kv head, most pieces per kv head
+  uint64_t ws_rows;       // rows of partials
 };
 struct PagedPlan {
   PagedGrid decode, chunk;
+  int32_t compute_units;
   uint64_t workspace_bytes;
 };
 PagedPlan plan_paged(int tokens, int batch, int kv_heads, int group, int head_dim, int max_q,

@@ -19,8 +19,8 @@
 // Long key ranges of few rows are split over workgroups (plan_paged), whose
 // normalised partials fa_paged_merge_kernel joins.
 //
-// Pages are read through their 16-key groups (a page holds whole groups): the
-// page id of a group is wave-uniform and comes by scalar loads one tile ahead.
+// Pages are read through their 16-key groups (a page holds whole groups), whose
+// page ids a wave holds 64 at a time, one a lane (PageIds).
 // Keys past the last visible one re-read that row, absent pages read page 0;
 // the scores of both are masked.
 #include <hip/hip_runtime.h>
@@ -297,13 +297,14 @@ __device__ __forceinline__ int last_key(const PagedFwdArgs& a, const Seq& s, int
 
 // ---- few rows: decode ----
 
-template <int D, bool BF16, int RB>
-__global__ void __launch_bounds__(256) fa_paged_decode_kernel(const PagedFwdArgs a) {
+
+template <int D, bool BF16, int RB, int NW>
+__global__ void __launch_bounds__(64 * NW) fa_paged_decode_kernel(const PagedFwdArgs a) {
   using W = WaveAttn<D, BF16, 2, RB>;
   constexpr int ROWB = 2 * D, TB = 32 * ROWB;   // bytes of a wave's K or V tile
   constexpr int NI = 16 * ROWB / 1024;          // DMA instructions of a 16-key group
   constexpr int BM = 16 * RB;
-  __shared__ __attribute__((aligned(1024))) char smem[4 * 4 * TB];  // per wave K0 K1 V0 V1
+  __shared__ __attribute__((aligned(1024))) char smem[NW * 4 * TB];  // per wave K0 K1 V0 V1
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -311,6 +312,8 @@ __global__ void __launch_bounds__(256) fa_paged_decode_kernel(const PagedFwdArgs
   const int split = fast_div(blockIdx.x, a.by_splits);  // by_splits: by slots * kv heads
   const int bh = blockIdx.x - split * bhs;
   const int b = fast_div(bh, a.by_kvh), kvh = bh - b * a.kv_heads;
+  PageIds ids;
+  ids.start(a.pt, a.pt.table + b * a.pt.table_stride, split * a.chunk);
   const Seq s = load_seq(a.pt, b, a.max_q);
   const int n_rows = s.nq * a.group;
   if (n_rows <= 0 || n_rows > a.max_rows) return;
@@ -328,38 +331,27 @@ __global__ void __launch_bounds__(256) fa_paged_decode_kernel(const PagedFwdArgs
 
   GroupStage<D> stage;
   stage.init(lane, a.k_ss, a.v_ss);
-  const int32_t* row = a.pt.table + b * a.pt.table_stride;
   const char* kbase = a.k + kvh * a.k_sh;
   const char* vbase = a.v + kvh * a.v_sh;
   const int last = c1 - 1;
-  // Page ids of a tile's two groups, fetched one tile ahead.
-  int ids[2];
-  auto fetch = [&](int t) FA_INLINE {
-#pragma unroll
-    for (int g = 0; g < 2; ++g) ids[g] = page_id(a.pt, row, min(c0 + 32 * t + 16 * g, last));
-  };
+  // Stages tile t; returns which of its two groups have a page.
   auto issue = [&](int t, int buf) FA_INLINE -> unsigned {
-    unsigned present = 0;
+    const int key = c0 + 32 * t;
+    ids.reach(key);
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-      const int k0 = c0 + 32 * t + 16 * g, r0 = min(k0, last & ~15);
-      const bool ok = (uint32_t)ids[g] < (uint32_t)a.pt.num_pages;
-      present |= ok ? 1u << g : 0u;
-      const int64_t page = ok ? ids[g] : 0;
+      const int r0 = min(key + 16 * g, last & ~15);
+      const int64_t page = ids.page(r0);
       const int in_page = r0 & ((1 << a.pt.page_shift) - 1);
       const uint32_t dst = wave_lds + buf * TB + g * 16 * ROWB;
       stage.copy(kbase + page * a.k_sp + (int64_t)in_page * a.k_ss,
                  vbase + page * a.v_sp + (int64_t)in_page * a.v_ss, dst, dst + 2 * TB, last - r0,
                  a.k_ss, a.v_ss);
     }
-    return present;
+    return ids.present(key, 3u);
   };
   unsigned present = 0, present_next = 0;
-  if (wave < n_tiles) {
-    fetch(wave);
-    present = issue(wave, 0);
-    if (wave + 4 < n_tiles) fetch(wave + 4);
-  }
+  if (wave < n_tiles) present = issue(wave, 0);
   // q behind the first tile's DMA: loads return in order, so a wait for all but
   // the next tile's DMA covers q too.
   const char* qh = a.q + s.q0 * a.q_st + (int64_t)kvh * a.group * a.q_sh;
@@ -373,9 +365,8 @@ __global__ void __launch_bounds__(256) fa_paged_decode_kernel(const PagedFwdArgs
       w.qf[rb][st] = *reinterpret_cast<const i16x8*>(qh + i * a.q_st + h * a.q_sh + (32 * st + 8 * g4) * 2);
   }
   auto stage_next = [&](int t, int buf) FA_INLINE {
-    if (t + 4 < n_tiles) {
-      present_next = issue(t + 4, buf ^ 1);
-      if (t + 8 < n_tiles) fetch(t + 8);
+    if (t + NW < n_tiles) {
+      present_next = issue(t + NW, buf ^ 1);
       wait_vmcnt<4 * NI>();
     } else {
       wait_vmcnt<0>();
@@ -388,12 +379,12 @@ __global__ void __launch_bounds__(256) fa_paged_decode_kernel(const PagedFwdArgs
     // Whole tiles, then, from the first tile with a masked key on, the rest:
     // masked tiles are the last ones, or lie on absent pages.
     int t = wave, buf = 0;
-    for (; t < n_tiles && whole(t); t += 4) {
+    for (; t < n_tiles && whole(t); t += NW) {
       stage_next(t, 0);
       w.template step<0, false>(c0 + 32 * t, present, 0);
       present = present_next;
       fence_lds_reads();
-      t += 4;
+      t += NW;
       buf = 1;
       if (t >= n_tiles || !whole(t)) break;
       stage_next(t, 1);
@@ -402,7 +393,7 @@ __global__ void __launch_bounds__(256) fa_paged_decode_kernel(const PagedFwdArgs
       fence_lds_reads();
       buf = 0;
     }
-    for (; t < n_tiles; t += 4, buf ^= 1) {
+    for (; t < n_tiles; t += NW, buf ^= 1) {
       stage_next(t, buf);
       w.template step<0, true>(c0 + 32 * t, present, buf * TB);
       present = present_next;
@@ -412,9 +403,9 @@ __global__ void __launch_bounds__(256) fa_paged_decode_kernel(const PagedFwdArgs
 
   // ---- join the four waves: o and sums at the largest offset ----
   constexpr int PITCH = D + 4;  // floats of a row in LDS: rows of 16 lanes on distinct banks
-  float* ow = reinterpret_cast<float*>(smem);                 // [4][BM][PITCH]
-  float* mw = ow + 4 * BM * PITCH;                            // [4][BM][3]
-  static_assert((4 * BM * PITCH + 4 * BM * 3) * 4 <= 4 * 4 * TB, "join area");
+  float* ow = reinterpret_cast<float*>(smem);                 // [NW][BM][PITCH]
+  float* mw = ow + NW * BM * PITCH;                           // [NW][BM][3]
+  static_assert((BM * PITCH + BM * 3) * 4 <= 4 * TB, "join area");
   __syncthreads();
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
@@ -433,16 +424,16 @@ __global__ void __launch_bounds__(256) fa_paged_decode_kernel(const PagedFwdArgs
   constexpr int TPR = D / 4;  // threads of a row
   const int d = ((int)threadIdx.x % TPR) * 4;
 #pragma unroll
-  for (int r = (int)threadIdx.x / TPR; r < BM; r += 256 / TPR) {
+  for (int r = (int)threadIdx.x / TPR; r < BM; r += 64 * NW / TPR) {
     if (r >= n_rows) break;
     float mm = -INFINITY;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) mm = fmaxf(mm, mw[(v * BM + r) * 3]);
+    for (int v = 0; v < NW; ++v) mm = fmaxf(mm, mw[(v * BM + r) * 3]);
     float lr = 0.0f, lu = 0.0f;
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     const float base = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
+    for (int v = 0; v < NW; ++v) {
       const float* p = mw + (v * BM + r) * 3;
       // (a wave that saw no key: factor 0 of sums that are 0, or NaN)
       const float f = fast_exp2((p[0] - base) * a.scale_log2);
@@ -473,26 +464,26 @@ __global__ void __launch_bounds__(256) fa_paged_decode_kernel(const PagedFwdArgs
 
 // ---- many rows: chunks ----
 
-// Unit (kv head and split of its keys) and slot of a workgroup.  Workgroup w
-// runs on XCD w % 8, in order; a unit's slots share its keys through the XCD's
-// L2, and the longest slots of all units should start first:
-//  * a multiple of 8 units: whole units per XCD, up to four of them interleaved;
-//  * 1, 2 or 4: 8 / units XCDs take turns with a unit's slots;
-//  * else all units interleaved over all XCDs.
-__device__ __forceinline__ bool unit_and_slot(const PagedFwdArgs& a, int& unit, int& slot) {
+// Kv head and place (in its list of tiles and pieces) of a workgroup.
+// Workgroup w runs on XCD w % 8, in order; the tiles of a head share its keys
+// through the XCD's L2, and the longest tiles of all heads should start first:
+//  * a multiple of 8 heads: whole heads per XCD, up to four of them interleaved;
+//  * 1, 2 or 4: 8 / heads XCDs take turns with a head's places;
+//  * else all heads interleaved over all XCDs.
+__device__ __forceinline__ bool head_and_place(const PagedFwdArgs& a, int& kvh, int& place) {
   const int xcd = blockIdx.x % kNumXcd, i = blockIdx.x / kNumXcd;
   if (a.per_xcd > 0) {
-    const int grp = fast_div(i, a.by_group_slots), w = i - grp * a.unit_group * a.slots;
-    slot = fast_div(w, a.by_unit_group);
-    unit = xcd * a.per_xcd + grp * a.unit_group + (w - slot * a.unit_group);
+    const int grp = fast_div(i, a.by_group_places), w = i - grp * a.unit_group * a.places;
+    place = fast_div(w, a.by_unit_group);
+    kvh = xcd * a.per_xcd + grp * a.unit_group + (w - place * a.unit_group);
   } else if (a.xcds > 0) {
-    unit = xcd / a.xcds;
-    slot = i * a.xcds + xcd % a.xcds;
+    kvh = xcd / a.xcds;
+    place = i * a.xcds + xcd % a.xcds;
   } else {
-    slot = fast_div(blockIdx.x, a.by_units);
-    unit = blockIdx.x - slot * a.units;
+    place = fast_div(blockIdx.x, a.by_kvh);
+    kvh = blockIdx.x - place * a.kv_heads;
   }
-  return slot < a.slots;
+  return place < a.places;
 }
 
 template <int D, bool BF16>
@@ -505,19 +496,34 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int hs, slot;
-  if (!unit_and_slot(a, hs, slot)) return;
-  const int kvh = fast_div(hs, a.by_splits), split = hs - kvh * a.splits;
-  int b, tile0;
-  if (!find_slot<BM>(a, slot, b, tile0)) return;
+  int kvh, place, b, tile0;
+  if (!head_and_place(a, kvh, place)) return;
+  TileList<BM> list;
+  list.init(a);
+  LastRound end;
+  end.init(a, list.count);
+  int pieces = 1, piece = 0, nth = place;
+  if (place >= end.whole) {
+    pieces = a.ws_o != nullptr ? end.pieces : 1;
+    const int i = place - end.whole;
+    nth = i / pieces;
+    piece = i - nth * pieces;
+    if (nth >= end.rest) return;
+    nth += end.whole;
+  }
+  if (!list.find(a, nth, b, tile0)) return;
   const Seq s = load_seq(a.pt, b, a.max_q);
   const int n_rows = s.nq * a.group, row0 = tile0 * BM;
   if (n_rows < a.min_rows || row0 >= n_rows) return;
   const int last_row = min(row0 + BM, n_rows) - 1;
   const int kv_end = max(0, last_key(a, s, fast_div(last_row, a.by_group)) + 1);
-  const int n_act = max(1, (kv_end + a.chunk - 1) / a.chunk);
-  if (split >= n_act) return;
-  const int c0 = split * a.chunk, c1 = min(kv_end, c0 + a.chunk);
+  int n_act = 1, c0 = 0, c1 = kv_end;
+  if (pieces > 1) {
+    const int keys = piece_keys(kv_end, pieces, n_act);
+    if (piece >= n_act) return;
+    c0 = piece * keys;
+    c1 = min(kv_end, c0 + keys);
+  }
   const int n_tiles = (c1 - c0 + 63) / 64;
 
   const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(smem));
@@ -528,37 +534,28 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 
   GroupStage<D> stage;
   stage.init(lane, a.k_ss, a.v_ss);
-  const int32_t* row = a.pt.table + b * a.pt.table_stride;
   const char* kbase = a.k + kvh * a.k_sh;
   const char* vbase = a.v + kvh * a.v_sh;
   const int last = c1 - 1;
-  // Page ids of the tile's four groups (each wave stages the group of its
-  // number and masks by all four), fetched one tile ahead.
-  int ids[4], own_id = 0;
-  auto fetch = [&](int t) FA_INLINE {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) ids[g] = page_id(a.pt, row, min(c0 + 64 * t + 16 * g, last));
-    own_id = page_id(a.pt, row, min(c0 + 64 * t + 16 * wave, last));
-  };
+  PageIds ids;
+  // Stages this wave's 16-key group of tile t; returns which of the tile's four
+  // groups have a page.
   auto issue = [&](int t, int buf) FA_INLINE -> unsigned {
-    unsigned present = 0;
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-      present |= (uint32_t)ids[g] < (uint32_t)a.pt.num_pages ? 1u << g : 0u;
-    const int r0 = min(c0 + 64 * t + 16 * wave, last & ~15);
-    const int64_t page = (uint32_t)own_id < (uint32_t)a.pt.num_pages ? own_id : 0;
+    const int key = c0 + 64 * t;
+    ids.reach(key);
+    const int r0 = min(key + 16 * wave, last & ~15);
+    const int64_t page = ids.page(r0);
     const int in_page = r0 & ((1 << a.pt.page_shift) - 1);
     const uint32_t dst = base + buf * TB + wave * 16 * ROWB;
     stage.copy(kbase + page * a.k_sp + (int64_t)in_page * a.k_ss,
                vbase + page * a.v_sp + (int64_t)in_page * a.v_ss, dst, dst + 2 * TB, last - r0,
                a.k_ss, a.v_ss);
-    return present;
+    return ids.present(key, 15u);
   };
   unsigned present = 0, present_next = 0;
   if (n_tiles > 0) {
-    fetch(0);
+    ids.start(a.pt, a.pt.table + b * a.pt.table_stride, c0);
     present = issue(0, 0);
-    if (n_tiles > 1) fetch(1);
   }
   const char* qh = a.q + s.q0 * a.q_st + (int64_t)kvh * a.group * a.q_sh;
 #pragma unroll
@@ -579,10 +576,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   __syncthreads();
 
   auto stage_next = [&](int t, int buf) FA_INLINE {
-    if (t + 1 < n_tiles) {
-      present_next = issue(t + 1, buf ^ 1);
-      if (t + 2 < n_tiles) fetch(t + 2);
-    }
+    if (t + 1 < n_tiles) present_next = issue(t + 1, buf ^ 1);
   };
   auto end_tile = [&]() FA_INLINE {
     present = present_next;
@@ -619,7 +613,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     lu[rb] = W::red_sum(w.lu[rb]);
   }
   if (n_act > 1) {  // partials: o normalised, sums as log2
-    const int64_t wr0 = (((int64_t)slot * a.kv_heads + kvh) * a.splits + split) * BM + 32 * wave;
+    const int64_t wr0 = ((int64_t)kvh * a.max_pieces + place - end.whole) * BM + 32 * wave;
 #pragma unroll
     for (int rb = 0; rb < 2; ++rb) {
       const int r = 16 * rb + l16;
@@ -691,148 +685,191 @@ __global__ void __launch_bounds__(256) fa_paged_merge_kernel(const PagedFwdArgs 
   __shared__ f32x4 part_o[GROUPS][TPR];
   __shared__ float part_e[GROUPS][4];  // top, sum of weights; the same of the plain sums
   const int grp = (int)threadIdx.x / TPR, lane = (int)threadIdx.x % TPR, d = lane * 4;
-  const int rpb = GROUPS / a.join, per = (BM + rpb - 1) / rpb;  // rows, workgroups of a slot
-  const int sk = blockIdx.x / per, r = (blockIdx.x - sk * per) * rpb + grp / a.join;
+  constexpr bool kTiles = BM == kChunkRows;
+  // Rows of a workgroup: of a tile (join 1) merge_rows, one after another.
+  const int rpb = kTiles ? a.merge_rows : GROUPS / a.join, per = (BM + rpb - 1) / rpb;
+  const int sk = blockIdx.x / per, r_first = (blockIdx.x - sk * per) * rpb + grp / a.join;
   const int slot = fast_div(sk, a.by_kvh), kvh = sk - slot * a.kv_heads;
-  int b = slot, tile0 = 0;
-  if constexpr (BM == kChunkRows) {
-    if (!find_slot<BM>(a, slot, b, tile0)) return;
+  int b = slot, tile0 = 0, n_act;
+  int64_t w0;  // first partial row
+  Seq s;
+  if constexpr (kTiles) {  // slot: the slot-th tile of the last round
+    TileList<BM> list;
+    list.init(a);
+    LastRound end;
+    end.init(a, list.count);
+    if (end.pieces <= 1 || slot >= end.rest || !list.find(a, end.whole + slot, b, tile0)) return;
+    s = load_seq(a.pt, b, a.max_q);
+    w0 = ((int64_t)kvh * a.max_pieces + slot * end.pieces) * BM;
+    n_act = end.pieces;
+  } else {
+    s = load_seq(a.pt, b, a.max_q);
+    w0 = (int64_t)sk * a.splits * BM;
+    n_act = 0;
   }
-  const Seq s = load_seq(a.pt, b, a.max_q);
   const int n_rows = s.nq * a.group, row0 = tile0 * BM;
   if (n_rows < a.min_rows || n_rows > a.max_rows || row0 >= n_rows) return;
   const int last_row = min(row0 + BM, n_rows) - 1;
   const int kv_end = max(0, last_key(a, s, fast_div(last_row, a.by_group)) + 1);
-  const int n_act = (kv_end + a.chunk - 1) / a.chunk;
+  if constexpr (kTiles)
+    piece_keys(kv_end, n_act, n_act);
+  else
+    n_act = (kv_end + a.chunk - 1) / a.chunk;
   if (n_act <= 1) return;
-  const bool row = r < BM && row0 + r < n_rows;
-  const int64_t w0 = (int64_t)sk * a.splits * BM + r;
-  float top = -INFINITY, top_u = -INFINITY, lr = 0.0f, lu = 0.0f;
-  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (row) {
-    constexpr int BATCH = 4;
-    for (int c = grp & (a.join - 1); c < n_act; c += BATCH * a.join) {
-      float e[BATCH], eu[BATCH];
-      f32x4 o[BATCH];
+  for (int r0 = 0; r0 < (kTiles ? rpb : 1); r0 += GROUPS) {
+    const int r = r_first + r0;
+    const bool row = r < BM && row0 + r < n_rows;
+    float top = -INFINITY, top_u = -INFINITY, lr = 0.0f, lu = 0.0f;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (row) {
+      constexpr int BATCH = 4;
+      for (int c = grp & (a.join - 1); c < n_act; c += BATCH * a.join) {
+        float e[BATCH], eu[BATCH];
+        f32x4 o[BATCH];
 #pragma unroll
-      for (int j = 0; j < BATCH; ++j) {
-        const int64_t wr = w0 + (int64_t)min(c + j * a.join, n_act - 1) * BM;
-        e[j] = a.ws_e[wr * 2];
-        eu[j] = a.ws_e[wr * 2 + 1];
-        o[j] = *reinterpret_cast<const f32x4*>(a.ws_o + wr * D + d);
-      }
+        for (int j = 0; j < BATCH; ++j) {
+          const int64_t wr = w0 + r + (int64_t)min(c + j * a.join, n_act - 1) * BM;
+          e[j] = a.ws_e[wr * 2];
+          eu[j] = a.ws_e[wr * 2 + 1];
+          o[j] = *reinterpret_cast<const f32x4*>(a.ws_o + wr * D + d);
+        }
 #pragma unroll
-      for (int j = 0; j < BATCH; ++j) {
-        // (e = -inf: its keys are all masked for this row)
-        if (c + j * a.join >= n_act || e[j] == -INFINITY) continue;
-        const float t = fmaxf(top, e[j]), tu = fmaxf(top_u, eu[j]);
-        const float old = fast_exp2(top - t), f = fast_exp2(e[j] - t);
-        lr = lr * old + f;
-        acc = acc * old + o[j] * f;
-        lu = lu * fast_exp2(top_u - tu) + fast_exp2(eu[j] - tu);
-        top = t;
-        top_u = tu;
+        for (int j = 0; j < BATCH; ++j) {
+          // (e = -inf: its keys are all masked for this row)
+          if (c + j * a.join >= n_act || e[j] == -INFINITY) continue;
+          const float t = fmaxf(top, e[j]), tu = fmaxf(top_u, eu[j]);
+          const float old = fast_exp2(top - t), f = fast_exp2(e[j] - t);
+          lr = lr * old + f;
+          acc = acc * old + o[j] * f;
+          lu = lu * fast_exp2(top_u - tu) + fast_exp2(eu[j] - tu);
+          top = t;
+          top_u = tu;
+        }
       }
     }
+    if (a.join > 1) {
+      part_o[grp][lane] = acc;
+      if (lane == 0) {
+        part_e[grp][0] = top;
+        part_e[grp][1] = lr;
+        part_e[grp][2] = top_u;
+        part_e[grp][3] = lu;
+      }
+      __syncthreads();
+      if ((grp & (a.join - 1)) != 0) return;
+      for (int g = 0; g < a.join; ++g) {
+        top = fmaxf(top, part_e[grp + g][0]);
+        top_u = fmaxf(top_u, part_e[grp + g][2]);
+      }
+      lr = lu = 0.0f;
+      acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int g = 0; g < a.join; ++g) {
+        if (part_e[grp + g][1] == 0.0f) continue;  // no chunk with a visible key
+        const float f = fast_exp2(part_e[grp + g][0] - top);
+        lr += f * part_e[grp + g][1];
+        lu += fast_exp2(part_e[grp + g][2] - top_u) * part_e[grp + g][3];
+        acc += part_o[grp + g][lane] * f;
+      }
+    }
+    if (!row) continue;
+    const bool none = lr == 0.0f;
+    const float inv = none ? 0.0f : 1.0f / lr;
+    const int i = fast_div(row0 + r, a.by_group), h = kvh * a.group + row0 + r - i * a.group;
+    const int64_t t = s.q0 + i;
+    *reinterpret_cast<u32x2*>(a.o + t * a.o_st + h * a.o_sh + d * 2) =
+        u32x2{pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv)};
+    if (a.lse != nullptr && lane == 0)
+      a.lse[t * a.heads + h] = none ? -INFINITY : (top_u + __log2f(lu)) * kLn2;
   }
-  if (a.join > 1) {
-    part_o[grp][lane] = acc;
-    if (lane == 0) {
-      part_e[grp][0] = top;
-      part_e[grp][1] = lr;
-      part_e[grp][2] = top_u;
-      part_e[grp][3] = lu;
-    }
-    __syncthreads();
-    if ((grp & (a.join - 1)) != 0) return;
-    for (int g = 0; g < a.join; ++g) {
-      top = fmaxf(top, part_e[grp + g][0]);
-      top_u = fmaxf(top_u, part_e[grp + g][2]);
-    }
-    lr = lu = 0.0f;
-    acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int g = 0; g < a.join; ++g) {
-      if (part_e[grp + g][1] == 0.0f) continue;  // no chunk with a visible key
-      const float f = fast_exp2(part_e[grp + g][0] - top);
-      lr += f * part_e[grp + g][1];
-      lu += fast_exp2(part_e[grp + g][2] - top_u) * part_e[grp + g][3];
-      acc += part_o[grp + g][lane] * f;
-    }
-  }
-  if (!row) return;
-  const bool none = lr == 0.0f;
-  const float inv = none ? 0.0f : 1.0f / lr;
-  const int i = fast_div(row0 + r, a.by_group), h = kvh * a.group + row0 + r - i * a.group;
-  const int64_t t = s.q0 + i;
-  *reinterpret_cast<u32x2*>(a.o + t * a.o_st + h * a.o_sh + d * 2) =
-      u32x2{pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv)};
-  if (a.lse != nullptr && lane == 0)
-    a.lse[t * a.heads + h] = none ? -INFINITY : (top_u + __log2f(lu)) * kLn2;
 }
 
 template <class F>
-hipError_t launch(F* fn, int64_t grid, const PagedFwdArgs& args, hipStream_t stream) {
+hipError_t launch(F* fn, int64_t grid, const PagedFwdArgs& args, hipStream_t stream,
+                  int threads = 256) {
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
   void* kargs[] = {const_cast<PagedFwdArgs*>(&args)};
-  return hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)grid), dim3(256), kargs, 0,
-                         stream);
+  return hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)grid), dim3(threads), kargs,
+                         0, stream);
 }
 
-// The chunk kernel's grid order (unit_and_slot) and its workgroups.
+// The chunk kernel's grid order (head_and_place) and its workgroups.
 int64_t set_order(PagedFwdArgs& a) {
-  a.units = a.kv_heads * a.splits;
-  a.per_xcd = a.units % kNumXcd == 0 ? a.units / kNumXcd : 0;
+  a.per_xcd = a.kv_heads % kNumXcd == 0 ? a.kv_heads / kNumXcd : 0;
   a.unit_group = 1;
   for (int g = 2; g <= 4; ++g)
     if (a.per_xcd % g == 0) a.unit_group = g;
-  a.xcds = a.per_xcd == 0 && kNumXcd % a.units == 0 ? kNumXcd / a.units : 0;
-  a.by_units = make_fast_div((uint32_t)a.units);
-  a.by_group_slots = make_fast_div((uint32_t)(a.unit_group * a.slots));
+  a.xcds = a.per_xcd == 0 && kNumXcd % a.kv_heads == 0 ? kNumXcd / a.kv_heads : 0;
+  a.by_group_places = make_fast_div((uint32_t)(a.unit_group * a.places));
   a.by_unit_group = make_fast_div((uint32_t)a.unit_group);
-  if (a.xcds > 0) return (int64_t)kNumXcd * ((a.slots + a.xcds - 1) / a.xcds);
-  return (int64_t)a.units * a.slots;
+  if (a.xcds > 0) return (int64_t)kNumXcd * ((a.places + a.xcds - 1) / a.xcds);
+  return (int64_t)a.kv_heads * a.places;
 }
 
 template <int D, bool BF16>
 hipError_t launch_all(const PagedFwdArgs& base, const PagedPlan& plan, void* ws, hipStream_t stream) {
   char* at = static_cast<char*>(ws);
-  for (const PagedGrid* g : {&plan.chunk, &plan.decode}) {
-    if (g->rows == 0) continue;
+  auto partials = [&](PagedFwdArgs& a, const PagedGrid& g) {
+    a.ws_o = g.ws_rows ? reinterpret_cast<float*>(at) : nullptr;
+    a.ws_e = reinterpret_cast<float*>(at + g.ws_rows * D * 4);
+    at += g.ws_rows * (D + 2) * 4;
+  };
+  constexpr int GROUPS = 256 / (D / 4);  // lane groups of a merge workgroup
+  if (const PagedGrid& g = plan.chunk; g.rows != 0) {
     PagedFwdArgs a = base;
-    const bool decode = g == &plan.decode;
-    // B == 1 and too many rows for the decode kernel: the chunk kernel serves
+    // One sequence with too many rows for the decode kernel: this one serves
     // whatever the sequence holds.
-    a.min_rows = decode || plan.decode.rows == 0 ? 1 : plan.decode.rows + 1;
-    a.max_rows = decode ? g->rows : 0x7fffffff;
-    a.slots = g->slots;
-    a.splits = g->splits;
-    a.chunk = g->chunk;
-    a.by_splits = make_fast_div((uint32_t)(decode ? g->slots * a.kv_heads : g->splits));
-    const int64_t sk = (int64_t)g->slots * a.kv_heads;
-    a.ws_o = reinterpret_cast<float*>(at);
-    a.ws_e = reinterpret_cast<float*>(at + g->ws_rows * D * 4);
-    at += g->ws_rows * (D + 2) * 4;
-    hipError_t e;
-    if (!decode)
-      e = launch(&fa_paged_chunk_kernel<D, BF16>, set_order(a), a, stream);
-    else if (g->rows == 16)
-      e = launch(&fa_paged_decode_kernel<D, BF16, 1>, sk * g->splits, a, stream);
-    else
-      e = launch(&fa_paged_decode_kernel<D, BF16, 2>, sk * g->splits, a, stream);
+    a.min_rows = plan.decode.rows == 0 ? 1 : plan.decode.rows + 1;
+    a.max_rows = 0x7fffffff;
+    a.slots = g.slots;
+    a.conc = g.conc;
+    a.max_pieces = g.pieces;
+    a.by_conc = make_fast_div((uint32_t)g.conc);
+    a.piece_cost = 768.0f / (float)std::max(768, a.pt.max_kv);
+    a.places = g.slots + g.pieces;
+    partials(a, g);
+    hipError_t e = launch(&fa_paged_chunk_kernel<D, BF16>, set_order(a), a, stream);
     if (e != hipSuccess) return e;
-    if (g->splits == 1) continue;
+    if (g.pieces > 0) {
+      a.join = 1;
+      const int64_t tiles = (int64_t)std::min(g.conc - 1, g.slots) * a.kv_heads;
+      // Rows of a workgroup: few, unless that makes thousands of workgroups,
+      // most of which find no tile.
+      a.merge_rows = tiles * (kChunkRows / GROUPS) <= 2048 ? GROUPS : 32;
+      if (tiles > 0)
+        e = launch(&fa_paged_merge_kernel<D, BF16, kChunkRows>, tiles * (kChunkRows / a.merge_rows), a, stream);
+      if (e != hipSuccess) return e;
+    }
+  }
+  if (const PagedGrid& g = plan.decode; g.rows != 0) {
+    PagedFwdArgs a = base;
+    a.min_rows = 1;
+    a.max_rows = g.rows;
+    a.slots = g.slots;
+    a.splits = g.splits;
+    a.chunk = g.chunk;
+    partials(a, g);
+    const int64_t sk = (int64_t)g.slots * a.kv_heads;
+    a.by_splits = make_fast_div((uint32_t)sk);
+    // Two waves a workgroup where two workgroups per CU are there to take
+    // turns at starting and ending (us, 4 waves -> 2: 32 sequences of 4096 keys,
+    // 8 kv heads, D = 128: 105 -> 102; 64 of 1000: 55 -> 50); with fewer, four
+    // waves read sooner (4 sequences of 2000: 17 -> 14).
+    auto decode = [&](auto rb_c) {
+      constexpr int RB = decltype(rb_c)::value;
+      return sk * g.splits >= 2 * plan.compute_units
+                 ? launch(&fa_paged_decode_kernel<D, BF16, RB, 2>, sk * g.splits, a, stream, 128)
+                 : launch(&fa_paged_decode_kernel<D, BF16, RB, 4>, sk * g.splits, a, stream, 256);
+    };
+    hipError_t e = g.rows == 16 ? decode(std::integral_constant<int, 1>{})
+                                : decode(std::integral_constant<int, 2>{});
+    if (e != hipSuccess || g.splits == 1) return e;
     // As many lane groups a row as it has chunks, a power of two.
-    constexpr int GROUPS = 256 / (D / 4);
     a.join = 1;
-    while (a.join < g->splits && a.join < GROUPS) a.join *= 2;
+    while (a.join < g.splits && a.join < GROUPS) a.join *= 2;
     const int rpb = GROUPS / a.join;
-    const int64_t per = (g->rows + rpb - 1) / rpb;
-    if (!decode)
-      e = launch(&fa_paged_merge_kernel<D, BF16, kChunkRows>, sk * per, a, stream);
-    else if (g->rows == 16)
-      e = launch(&fa_paged_merge_kernel<D, BF16, 16>, sk * per, a, stream);
-    else
-      e = launch(&fa_paged_merge_kernel<D, BF16, 32>, sk * per, a, stream);
+    const int64_t per = (g.rows + rpb - 1) / rpb;
+    e = g.rows == 16 ? launch(&fa_paged_merge_kernel<D, BF16, 16>, sk * per, a, stream)
+                     : launch(&fa_paged_merge_kernel<D, BF16, 32>, sk * per, a, stream);
     if (e != hipSuccess) return e;
   }
   return hipSuccess;

@@ -69,19 +69,71 @@ __device__ __forceinline__ int page_id(const PageTable& pt, const int32_t* row, 
   return scalar_load(row, key >> pt.page_shift);
 }
 
-// Sequence b and row tile of a slot of the chunk kernel's grid; the slots run
-// from the longest tiles to the shortest.  False: the slot holds no tile.
+// Page ids of 64 16-key groups, 1024 keys, a lane each, and of the 64 behind
+// them, on their way.  Read lane by lane: scalar loads inside the tile loop
+// would make every LDS wait there a wait for all (they share a counter and
+// return out of order).  The ids of the table's row are loaded as far as the
+// table may be read, whatever the sequence's length, so that their first load
+// need not wait for the length; those past it are not used.
+struct PageIds {
+  const int32_t* row;
+  int limit, shift, base;  // last key of the table; keys base .. base + 1023 are held
+  uint32_t pages;
+  int cur, next;
+  uint64_t there;          // groups with a page
+  __device__ __forceinline__ int load(int key0) const {
+    return row[min(key0 + 16 * (int)(threadIdx.x & 63), limit) >> shift];
+  }
+  // Keys from key0, a multiple of 64 below pt.max_kv.
+  __device__ __forceinline__ void start(const PageTable& pt, const int32_t* r, int key0) {
+    row = r;
+    limit = pt.max_kv - 1;
+    shift = pt.page_shift;
+    base = key0 - 1024;
+    pages = (uint32_t)pt.num_pages;
+    next = load(key0);
+  }
+  __device__ __forceinline__ void advance() {
+    base += 1024;
+    cur = next;
+    there = __ballot((uint32_t)cur < pages);
+    next = load(base + 1024);
+  }
+  // Makes `key` (uniform, ascending) held.
+  __device__ __forceinline__ void reach(int key) {
+    if (key >= base + 1024) advance();
+  }
+  // Page of the group of a held key, page 0 for an absent one.
+  __device__ __forceinline__ int64_t page(int key) const {
+    const int g = (key - base) >> 4;
+    return (there >> g) & 1 ? __builtin_amdgcn_readlane(cur, g) : 0;
+  }
+  // Bit i: whether the i-th group from a held key has a page.
+  __device__ __forceinline__ unsigned present(int key, unsigned mask) const {
+    return (unsigned)(there >> ((key - base) >> 4)) & mask;
+  }
+};
+
+// Row tiles of the chunk kernel, the longest first: sequence and tile of the
+// n-th one, and how many there are.
 //
 // Up to 64 sequences: the ones with more keys first, each lane holding one
 // sequence's tiles and the number of tiles before them.  More: in their order
-// from the last, sequence b's tiles at slot f(b) = floor(cu[b] group / BM) + b,
-// which leaves room for the last, partial tile of each; the sequence is then
-// the number of b >= 1 with f(b) <= slot, counted 64 at a time.
+// from the last, sequence b's tiles at place f(b) = floor(cu[b] group / BM) + b,
+// which leaves room for the last, partial tile of each (places without a tile
+// count as tiles); the sequence is then the number of b >= 1 with f(b) <= place,
+// counted 64 at a time.
 template <int BM>
-__device__ __forceinline__ bool find_slot(const PagedFwdArgs& a, int slot, int& b, int& tile) {
-  const int lane = threadIdx.x & 63;
-  if (a.pt.batch <= 64) {
-    int tiles = 0, len = -1;
+struct TileList {
+  int start, tiles;  // this lane's sequence (up to 64)
+  int count;
+
+  __device__ __forceinline__ void init(const PagedFwdArgs& a) {
+    const int lane = threadIdx.x & 63;
+    count = a.slots;
+    if (a.pt.batch > 64) return;
+    int len = -1;
+    tiles = 0;
     if (lane < a.pt.batch) {
       const int c0 = min(max(a.pt.cu[lane], 0), a.pt.tokens);
       const int c1 = min(max(a.pt.cu[lane + 1], c0), a.pt.tokens);
@@ -89,31 +141,68 @@ __device__ __forceinline__ bool find_slot(const PagedFwdArgs& a, int slot, int& 
       tiles = rows >= a.min_rows ? (rows + BM - 1) / BM : 0;
       len = min(max(a.pt.lens[lane], 0), a.pt.max_kv);
     }
-    int start = 0;
+    start = count = 0;
     for (int i = 0; i < a.pt.batch; ++i) {
       const int l = __builtin_amdgcn_readlane(len, i), t = __builtin_amdgcn_readlane(tiles, i);
       start += l > len || (l == len && i < lane) ? t : 0;
+      count += t;
     }
-    const uint64_t has = __ballot(start <= slot && slot < start + tiles);
-    if (has == 0) return false;
-    b = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(has));
-    tile = __builtin_amdgcn_readlane(start + tiles - 1, b) - slot;
-    return true;
   }
-  auto begin = [&](int i, int cu) FA_INLINE {
-    return (int)((uint32_t)(min(max(cu, 0), a.pt.tokens) * a.group) / BM) + i;
-  };
-  slot = a.slots - 1 - slot;
-  int n = 0;
-  for (int i0 = 1; i0 <= a.pt.batch; i0 += 64) {
-    const int i = i0 + lane;
-    const bool before = i <= a.pt.batch && begin(i, a.pt.cu[min(i, a.pt.batch)]) <= slot;
-    n += __popcll(__ballot(before));
+  __device__ __forceinline__ bool find(const PagedFwdArgs& a, int n, int& b, int& tile) const {
+    if (a.pt.batch <= 64) {
+      const uint64_t has = __ballot(start <= n && n < start + tiles);
+      if (has == 0) return false;
+      b = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(has));
+      tile = __builtin_amdgcn_readlane(start + tiles - 1, b) - n;
+      return true;
+    }
+    const int lane = threadIdx.x & 63, at = a.slots - 1 - n;
+    auto begin = [&](int i, int cu) FA_INLINE {
+      return (int)((uint32_t)(min(max(cu, 0), a.pt.tokens) * a.group) / BM) + i;
+    };
+    int k = 0;
+    for (int i0 = 1; i0 <= a.pt.batch; i0 += 64) {
+      const int i = i0 + lane;
+      const bool before = i <= a.pt.batch && begin(i, a.pt.cu[min(i, a.pt.batch)]) <= at;
+      k += __popcll(__ballot(before));
+    }
+    b = __builtin_amdgcn_readfirstlane(k);
+    if (b >= a.pt.batch) return false;
+    tile = at - begin(b, scalar_load(a.pt.cu, b));
+    return tile >= 0;
   }
-  b = __builtin_amdgcn_readfirstlane(n);
-  if (b >= a.pt.batch) return false;
-  tile = slot - begin(b, scalar_load(a.pt.cu, b));
-  return tile >= 0;
+};
+
+// The chunk kernel's last round.  `conc` workgroups of a kv head run at once;
+// the tiles that are left after whole rounds of them would keep only some of
+// the GPU busy for a whole tile's time, so they are cut into `pieces` of keys:
+// the number that finishes them first, at ceil(rest pieces / conc) rounds of
+// 1 / pieces of a tile plus a piece's own cost (its join, about the time of 768
+// keys).  Lane q weighs q + 1 pieces.
+struct LastRound {
+  int whole, rest, pieces;
+  __device__ __forceinline__ void init(const PagedFwdArgs& a, int count) {
+    const int rounds = fast_div(count, a.by_conc);
+    whole = rounds * a.conc;
+    rest = count - whole;
+    const int q = (int)(threadIdx.x & 63) + 1;
+    const int all = rest * q;
+    float cost = (float)(fast_div(all + a.conc - 1, a.by_conc)) * (1.0f / (float)q + a.piece_cost);
+    if (all > 2 * a.conc && q > 1) cost = INFINITY;
+    float least = cost;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) least = fminf(least, __shfl_xor(least, d));
+    pieces = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(__ballot(cost == least)) + 1);
+  }
+};
+
+// Keys of a piece of a tile that sees keys 0 .. kv_end - 1: whole 64-key
+// tiles, 512 keys at least; and the number of pieces that have keys.
+__device__ __forceinline__ int piece_keys(int kv_end, int pieces, int& used) {
+  const int n = min(pieces, max(1, (kv_end + 511) / 512));
+  const int keys = max(64, ((kv_end + n - 1) / n + 63) / 64 * 64);
+  used = max(1, (kv_end + keys - 1) / keys);
+  return keys;
 }
 
 // Staging of 16 consecutive keys of one page: their K rows and V rows to LDS
