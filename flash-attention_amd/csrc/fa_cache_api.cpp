@@ -47,12 +47,26 @@ PagedPlan plan_paged(int tokens, int batch, int kv_heads, int group, int head_di
   return p;
 }
 
-int plan_weights(int batch, int kv_heads, int group, int max_q, int max_kv, int compute_units) {
-  const int64_t tiles = (int64_t)batch * kv_heads * ((max_kv + kWeightKeys - 1) / kWeightKeys);
-  const int64_t rows = (int64_t)max_q * group;
-  // Two workgroups per CU, each with 128 rows or more.
-  const int64_t want = 2 * (int64_t)compute_units / std::max<int64_t>(tiles, 1);
-  return (int)std::max<int64_t>(1, std::min(want, rows / 128));
+WeightsPlan plan_weights(int tokens, int batch, int kv_heads, int group, int max_q, int max_kv,
+                         int compute_units) {
+  WeightsPlan p = {};
+  const int64_t most = (int64_t)std::min(max_q, tokens) * group;  // rows of a sequence
+  if (most <= kDecodeRows || batch > 1) {
+    p.few_rows = most <= 16 ? 16 : kDecodeRows;
+    // Four workgroups per CU, which run at once, of 256 to 2048 keys in whole
+    // 64-key tiles.
+    const int64_t bk = (int64_t)batch * kv_heads;
+    const int64_t cut = (4 * (int64_t)compute_units + bk - 1) / bk;
+    const int64_t keys = ((max_kv + cut - 1) / cut + 63) / 64 * 64;
+    p.few_keys = (int)std::max<int64_t>(256, std::min<int64_t>(keys, kWeightChunk));
+  }
+  if (most > kDecodeRows) {
+    // Three workgroups per CU, which run at once, each with 128 rows or more.
+    const int64_t tiles = (int64_t)batch * kv_heads * ((max_kv + kWeightKeys - 1) / kWeightKeys);
+    const int64_t want = 3 * (int64_t)compute_units / std::max<int64_t>(tiles, 1);
+    p.splits = (int)std::max<int64_t>(1, std::min(want, most / 128));
+  }
+  return p;
 }
 
 namespace {
@@ -443,11 +457,11 @@ uint64_t weights_bytes(const fa_paged_weights_params& p, int splits) {
   return (uint64_t)splits * p.cache.batch * p.cache.kv_heads * tiles * kWeightKeys * 4;
 }
 
-fa_status weights_splits(const fa_paged_weights_params& p, int* splits) {
+fa_status plan_of(const fa_paged_weights_params& p, WeightsPlan* plan) {
   int cus = 0;
   FA_TRY(current_compute_units(&cus));
-  *splits = plan_weights(p.cache.batch, p.cache.kv_heads, p.heads / p.cache.kv_heads,
-                         std::min(p.max_q, p.tokens), limit_kv(p.cache, p.max_kv), cus);
+  *plan = plan_weights(p.tokens, p.cache.batch, p.cache.kv_heads, p.heads / p.cache.kv_heads, p.max_q,
+                       limit_kv(p.cache, p.max_kv), cus);
   return FA_OK;
 }
 
@@ -513,9 +527,9 @@ fa_status fa_paged_key_weights_workspace_size(const fa_paged_weights_params* p, 
   *bytes = 0;
   FA_TRY(fa_paged_key_weights_validate(p));
   if (idle(*p)) return FA_OK;
-  int splits = 1;
-  FA_TRY(weights_splits(*p, &splits));
-  *bytes = weights_bytes(*p, splits);
+  WeightsPlan plan;
+  FA_TRY(plan_of(*p, &plan));
+  *bytes = weights_bytes(*p, plan.splits);
   return FA_OK;
 }
 
@@ -523,9 +537,9 @@ fa_status fa_paged_key_weights(const fa_paged_weights_params* p, void* workspace
                                uint64_t workspace_bytes, void* stream) {
   FA_TRY(fa_paged_key_weights_validate(p));
   if (idle(*p)) return FA_OK;
-  int splits = 1;
-  FA_TRY(weights_splits(*p, &splits));
-  const uint64_t need = weights_bytes(*p, splits);
+  WeightsPlan plan;
+  FA_TRY(plan_of(*p, &plan));
+  const uint64_t need = weights_bytes(*p, plan.splits);
   FA_TRY(check_workspace(workspace, workspace_bytes, need));
   const fa_paged_cache& c = p->cache;
   PagedWeightsArgs a = {};
@@ -548,13 +562,13 @@ fa_status fa_paged_key_weights(const fa_paged_weights_params* p, void* workspace
   a.causal = p->causal;
   a.scale_log2 = (float)(p->softmax_scale * kLog2e);
   a.key_tiles = (a.pt.max_kv + kWeightKeys - 1) / kWeightKeys;
-  a.splits = splits;
+  a.splits = plan.splits;
   a.by_group = make_fast_div((uint32_t)a.group);
   a.by_kvh = make_fast_div((uint32_t)a.kv_heads);
   a.by_tiles = make_fast_div((uint32_t)a.key_tiles);
   a.by_splits = make_fast_div((uint32_t)c.batch);
   a.ws = need > 0 ? static_cast<float*>(workspace) : nullptr;
-  return launched(launch_paged_weights(a, c.head_dim, c.dtype == FA_DTYPE_BF16,
+  return launched(launch_paged_weights(a, plan, c.head_dim, c.dtype == FA_DTYPE_BF16,
                                        static_cast<hipStream_t>(stream)));
 }
 

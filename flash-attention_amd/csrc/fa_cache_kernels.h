@@ -88,15 +88,27 @@ struct PagedWeightsArgs {
   uint32_t k_ss;
   int32_t heads, kv_heads, group, max_q, causal;
   float scale_log2;
-  int32_t key_tiles, splits;  // grid: sequences x kv heads x key tiles x row splits
+  // Many rows, sequences of min_rows or more; grid: sequences x kv heads x key
+  // tiles x row splits.
+  int32_t min_rows;
+  int32_t key_tiles, splits;
   FastDiv by_group, by_kvh, by_tiles, by_splits;
   float* ws;           // [splits][batch][kv_heads][key_tiles * 256] partial sums
+  // Few rows, at most max_rows; grid: sequences x kv heads x chunks of keys.
+  int32_t max_rows, few_keys, few_chunks;
+  FastDiv by_few;
 };
-constexpr int kWeightKeys = 256;  // keys of a workgroup
-// Row splits of the key weights' grid (1: no workspace).
-int plan_weights(int batch, int kv_heads, int group, int max_q, int max_kv, int compute_units);
-hipError_t launch_paged_weights(const PagedWeightsArgs& args, int head_dim, bool bf16,
-                                hipStream_t stream);
+constexpr int kWeightKeys = 256;    // keys of a workgroup, many rows
+constexpr int kWeightChunk = 2048;  // most keys of a workgroup, few rows
+struct WeightsPlan {
+  int32_t few_rows;  // 16 or 32: sequences of at most so many rows apart; 0: none
+  int32_t few_keys;  // their keys a workgroup
+  int32_t splits;    // row splits of the others (1: no workspace); 0: none
+};
+WeightsPlan plan_weights(int tokens, int batch, int kv_heads, int group, int max_q, int max_kv,
+                         int compute_units);
+hipError_t launch_paged_weights(const PagedWeightsArgs& args, const WeightsPlan& plan, int head_dim,
+                                bool bf16, hipStream_t stream);
 
 struct PagedEvictArgs {
   PageTable pt;  // cu unused

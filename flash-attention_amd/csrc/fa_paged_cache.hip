@@ -1,13 +1,15 @@
 // Key weights and eviction of a paged key/value cache on gfx950.
 //
-// fa_weights_kernel: add_j = sum over rows i that see key j of
-// exp(scale q_i.k_j - lse_i), one pass over K.  A wave keeps 64 keys in
-// registers as the B operand of v_mfma_f32_16x16x32 and the workgroup's four
-// waves (256 keys) walk over the rows together, 32 at a time through LDS; a
-// lane holds one key of each 16-key block and 4 rows, so its sums stay in
-// registers and meet once at the end.  For one token it is bound by reading K,
-// for chunks by the exponentials (one per row and key, four cycles of a SIMD
-// each per 16 lanes) over half the matrix work of attention.
+// Key weights: add_j = sum over rows i that see key j of
+// exp(scale q_i.k_j - lse_i), one pass over K.  fa_weights_few_kernel takes the
+// sequences of at most 32 rows and is bound by reading K.  fa_weights_kernel:
+// a wave keeps 64 keys in registers as the B operand of v_mfma_f32_16x16x32 and
+// the workgroup's four waves (256 keys) walk over the rows together, 64 at a
+// time through LDS; a lane holds one key of each 16-key block and 4 rows, so
+// its sums stay in registers and meet once at the end.  It is bound by the
+// vector unit: per row and key one exponential (a quarter of the rate), one
+// multiply-add and one add, 24 cycles of a SIMD per 64 of them, beside half
+// the matrix work of attention.
 //
 // fa_select_kernel: the keep - recent heaviest of a head's keys by a radix
 // search for their least weight (digits of 11, 11 and 10 bits), and the list of
@@ -30,11 +32,13 @@ using namespace dev;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256) fa_weights_kernel(const PagedWeightsArgs a) {
-  constexpr int ROWB = 2 * D, KST = D / 32, KB = 4, RT = 32;  // 64 keys of a wave, rows of a tile
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3)))
+    fa_weights_kernel(const PagedWeightsArgs a) {
+  constexpr int ROWB = 2 * D, KST = D / 32, KB = 4, RT = 64;  // 64 keys of a wave, rows of a tile
   constexpr int TB = RT * ROWB, NI = TB / 4 / 1024;           // bytes of a row tile, DMAs of a wave
   constexpr int LPR = ROWB / 16;
   __shared__ __attribute__((aligned(1024))) char smem[2 * TB];
+  __shared__ float neg_lse[4][RT];  // of each wave's current row tile
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -45,7 +49,7 @@ __global__ void __launch_bounds__(256) fa_weights_kernel(const PagedWeightsArgs 
   const int split = fast_div(bk, a.by_splits), b = bk - split * a.pt.batch;
   const Seq s = load_seq(a.pt, b, a.max_q);
   const int key0 = tile * kWeightKeys;
-  if (s.nq <= 0 || key0 >= s.len) return;
+  if (s.nq * a.group < a.min_rows || s.nq <= 0 || key0 >= s.len) return;
   const int wkey0 = key0 + 64 * wave;
 
   // This lane's keys wkey0 + 16kb + l16: rows of K past the end re-read the
@@ -91,12 +95,12 @@ __global__ void __launch_bounds__(256) fa_weights_kernel(const PagedWeightsArgs 
               base + buf * TB + (wave * NI + it) * 1024);
     }
   };
-  // lse (log2) and last visible key of row t * RT + lane % 32, for all lanes;
+  // lse (log2) and last visible key of row t * RT + lane, for all lanes;
   // rows that do not exist or have no weights see nothing.
   float lse_n = 0.0f;
   int last_n = -1;
   auto fetch_row = [&](int t) FA_INLINE {
-    const int r = t * RT + (lane & 31), rc = min(r, n_rows - 1);
+    const int r = t * RT + lane, rc = min(r, n_rows - 1);
     const int i = fast_div(rc, a.by_group), h = rc - i * a.group;
     const float l = a.lse[(int64_t)(s.q0 + i) * a.heads + kvh * a.group + h];
     last_n = r < n_rows && l != -INFINITY ? (a.causal ? min(s.first + i, s.len - 1) : s.len - 1) : -1;
@@ -113,53 +117,65 @@ __global__ void __launch_bounds__(256) fa_weights_kernel(const PagedWeightsArgs 
   }
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
-  for (int t = t0; t < t1; ++t) {
+  // One row tile from LDS.  MASKED: some row does not see some of the wave's keys.
+  auto compute = [&](auto masked_c, int buf, float lse, int last) FA_INLINE {
+    constexpr bool MASKED = decltype(masked_c)::value;
+    neg_lse[wave][lane] = -lse;
+    f32x4 sc[2][KB];  // the next 16 rows' products run beside this one's exponentials
+    auto products = [&](int rb) FA_INLINE {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) sc[rb & 1][kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int st = 0; st < KST; ++st) {
+        const i16x8 qa = *reinterpret_cast<const i16x8*>(smem + buf * TB + rb * 16 * ROWB + k_off[st]);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) sc[rb & 1][kb] = mfma16<BF16>(qa, kf[kb][st], sc[rb & 1][kb]);
+      }
+    };
+    products(0);
+#pragma unroll
+    for (int rb = 0; rb < RT / 16; ++rb) {
+      if (rb + 1 < RT / 16) products(rb + 1);
+      // rows 16rb + 4g4 + i, keys wkey0 + 16kb + l16
+      const f32x4 nl = *reinterpret_cast<const f32x4*>(&neg_lse[wave][16 * rb + 4 * g4]);
+      int rel[4];
+      if constexpr (MASKED) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rel[i] = __shfl(last, 16 * rb + 4 * g4 + i) - wkey0 - l16;
+      }
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = fast_exp2(fmaf(sc[rb & 1][kb][i], a.scale_log2, nl[i]));
+          if constexpr (MASKED)
+            acc[kb] += 16 * kb <= rel[i] ? p : 0.0f;
+          else
+            acc[kb] += p;
+        }
+    }
+  };
+  // Rows ascend, and with them the keys they see: masked tiles (or ones that
+  // see none of the wave's keys) first, whole ones, and a last one whose rows
+  // end inside it.  Loops of their own, so that the whole ones carry no masks;
+  // every wave passes one barrier a tile, whichever loop it is in.
+  int t = t0;
+  auto step = [&](auto masked_c) FA_INLINE {
     const float lse = lse_n;
-    const int last = last_n;
-    const int buf = (t - t0) & 1;
+    const int last = last_n, buf = (t - t0) & 1;
     if (t + 1 < t1) {
       issue(t + 1, buf ^ 1);
       fetch_row(t + 1);
     }
-    if (__any(last >= wkey0) && wkey0 < s.len) {
-      const bool whole = __all(last >= wkey0 + 63);
-#pragma unroll
-      for (int rb = 0; rb < 2; ++rb) {
-        f32x4 sc[KB];
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) sc[kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int st = 0; st < KST; ++st) {
-          const i16x8 qa = *reinterpret_cast<const i16x8*>(smem + buf * TB + rb * 16 * ROWB + k_off[st]);
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb) sc[kb] = mfma16<BF16>(qa, kf[kb][st], sc[kb]);
-        }
-        // rows 16rb + 4g4 + i, keys wkey0 + 16kb + l16
-        float rl[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) rl[i] = __shfl(lse, 16 * rb + 4 * g4 + i);
-        if (whole) {
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[kb] += fast_exp2(fmaf(sc[kb][i], a.scale_log2, -rl[i]));
-        } else {
-          int rel[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) rel[i] = __shfl(last, 16 * rb + 4 * g4 + i) - wkey0 - l16;
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float p = fast_exp2(fmaf(sc[kb][i], a.scale_log2, -rl[i]));
-              acc[kb] += 16 * kb <= rel[i] ? p : 0.0f;
-            }
-        }
-      }
-    }
+    if (!decltype(masked_c)::value || (__any(last >= wkey0) && wkey0 < s.len)) compute(masked_c, buf, lse, last);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-  }
+    ++t;
+  };
+  auto whole = [&]() FA_INLINE { return __all(last_n >= wkey0 + 63); };
+  while (t < t1 && !whole()) step(std::true_type{});
+  while (t < t1 && whole()) step(std::false_type{});
+  while (t < t1) step(std::true_type{});
 
   // Lane group g4 finishes key block g4.
   float mine = 0.0f;
@@ -183,13 +199,154 @@ __global__ void __launch_bounds__(256) fa_weights_kernel(const PagedWeightsArgs 
   }
 }
 
+// Few rows (a few tokens): q stays in registers as the A operand, K streams
+// through two LDS tiles of 32 keys that each wave has to itself, and the keys'
+// sums gather in LDS.  Bound by reading K.  32 sequences of up to 8192 keys, 8
+// kv heads, D = 128: 93 us with loads straight to registers, one 256-key tile a
+// workgroup; 78 so, with four workgroups of 2048 keys per CU (5.1 TB/s); 82
+// with four LDS tiles a wave and two workgroups per CU; 88 with 1024 keys.
+template <int D, bool BF16, int RB>
+__global__ void __launch_bounds__(128) fa_weights_few_kernel(const PagedWeightsArgs a) {
+  constexpr int NW = 2, ST = 2, kDepth = ST - 1;             // waves, ring tiles
+  constexpr int ROWB = 2 * D, KST = D / 32, TB = 32 * ROWB, NI = 16 * ROWB / 1024;
+  __shared__ __attribute__((aligned(1024))) char smem[NW * ST * TB];
+  __shared__ float sums[kWeightChunk];  // of a.few_keys keys
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l16 = lane & 15, g4 = lane >> 4;
+  const int rest = fast_div(blockIdx.x, a.by_few), chunk = blockIdx.x - rest * a.few_chunks;
+  const int b = fast_div(rest, a.by_kvh), kvh = rest - b * a.kv_heads;
+  const int c0 = chunk * a.few_keys;
+  const int32_t* row = a.pt.table + b * a.pt.table_stride;
+  PageIds ids;
+  ids.start(a.pt, row, c0);
+  const Seq s = load_seq(a.pt, b, a.max_q);
+  const int n_rows = s.nq * a.group;
+  if (n_rows <= 0 || n_rows > a.max_rows || c0 >= s.len) return;
+  const int c1 = min(s.len, c0 + a.few_keys), last = c1 - 1;
+  const int n_tiles = (c1 - c0 + 31) / 32;
+
+  const uint32_t wave_lds = __builtin_amdgcn_readfirstlane(lds_addr(smem)) + wave * ST * TB;
+  KeyStage<D> stage;
+  stage.init(lane, a.k_ss);
+  const char* kbase = a.k + kvh * a.k_sh;
+  auto issue = [&](int t, int slot) FA_INLINE {
+    const int key = c0 + 32 * t;
+    ids.reach(key);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int r0 = min(key + 16 * g, last & ~15);
+      const int in_page = r0 & ((1 << a.pt.page_shift) - 1);
+      stage.copy(kbase + ids.page(r0) * a.k_sp + (int64_t)in_page * a.k_ss,
+                 wave_lds + slot * TB + g * 16 * ROWB, last - r0, a.k_ss);
+    }
+  };
+  // This wave's tiles: wave, wave + NW, ...
+  const int mine = (n_tiles - wave + NW - 1) / NW;
+#pragma unroll
+  for (int i = 0; i < kDepth; ++i)
+    if (i < mine) issue(wave + i * NW, i);
+
+  // q, and lse (log2) and last visible key of rows 16rb + 4g4 + i.
+  const char* qh = a.q + s.q0 * a.q_st + (int64_t)kvh * a.group * a.q_sh;
+  i16x8 qf[RB][KST];
+  float lse[RB][4];
+  int see[RB][4];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const int r = min(16 * rb + l16, n_rows - 1);
+    const int i = fast_div(r, a.by_group), h = r - i * a.group;
+#pragma unroll
+    for (int st = 0; st < KST; ++st)
+      qf[rb][st] = *reinterpret_cast<const i16x8*>(qh + i * a.q_st + h * a.q_sh + (32 * st + 8 * g4) * 2);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int rr = 16 * rb + 4 * g4 + e, rc = min(rr, n_rows - 1);
+      const int ii = fast_div(rc, a.by_group), hh = rc - ii * a.group;
+      const float l = a.lse[(int64_t)(s.q0 + ii) * a.heads + kvh * a.group + hh];
+      see[rb][e] = rr < n_rows && l != -INFINITY ? (a.causal ? min(s.first + ii, s.len - 1) : s.len - 1) : -1;
+      lse[rb][e] = l * kLog2e;
+    }
+  }
+  uint32_t k_addr[KST];
+#pragma unroll
+  for (int st = 0; st < KST; ++st) k_addr[st] = wave_lds + lds::k16_read_offset<D>(0, st, lane);
+
+  auto tile = [&](auto slot_c, int i) FA_INLINE {
+    constexpr int SLOT = decltype(slot_c)::value;
+    const int t = wave + i * NW;
+    if (i + kDepth < mine) {
+      issue(t + kDepth * NW, (SLOT + kDepth) % ST);
+      wait_vmcnt<2 * NI * kDepth>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    f32x4 sc[2][RB];
+#pragma unroll
+    for (int st = 0; st < KST; ++st)
+      static_for<0, 2>([&](auto kb_c) FA_INLINE {
+        constexpr int kb = decltype(kb_c)::value;
+        const i16x8 kf = lds_read16<SLOT * TB + kb * 16 * ROWB>(k_addr[st]);
+        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) sc[kb][rb] = mfma16<BF16>(qf[rb][st], kf, st == 0 ? zero : sc[kb][rb]);
+      });
+    float x[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const int key = c0 + 32 * t + 16 * kb + l16;
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = fast_exp2(fmaf(sc[kb][rb][e], a.scale_log2, -lse[rb][e]));
+          x[kb] += key <= see[rb][e] ? p : 0.0f;
+        }
+      x[kb] += __shfl_xor(x[kb], 16);
+      x[kb] += __shfl_xor(x[kb], 32);
+    }
+    if (g4 < 2) sums[32 * t + lane] = g4 == 0 ? x[0] : x[1];
+    fence_lds_reads();
+  };
+  for (int i = 0; i < mine; i += ST) {
+    static_for<0, ST>([&](auto slot_c) FA_INLINE {
+      if (i + decltype(slot_c)::value < mine) tile(slot_c, i + decltype(slot_c)::value);
+    });
+  }
+  __syncthreads();
+  // Eight keys a thread in flight: one after another cost as much as the sums.
+  constexpr int PER = 8, STEP = PER * 64 * NW;
+  for (int k0 = c0; k0 < c1; k0 += STEP) {
+    int id[PER];
+    float* w[PER];
+    float old[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int key = k0 + j * 64 * NW + (int)threadIdx.x;
+      id[j] = key < c1 ? row[key >> a.pt.page_shift] : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int key = k0 + j * 64 * NW + (int)threadIdx.x;
+      w[j] = a.w + (int64_t)id[j] * a.w_sp + kvh * a.w_sh + (key & ((1 << a.pt.page_shift) - 1));
+      old[j] = 0.0f;
+      if ((uint32_t)id[j] < (uint32_t)a.pt.num_pages && key < s.first) old[j] = *w[j];
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if ((uint32_t)id[j] < (uint32_t)a.pt.num_pages)
+        *w[j] = old[j] + sums[k0 - c0 + j * 64 * NW + threadIdx.x];
+  }
+}
+
 // Adds the row splits' sums, in their order, to the weights.
 __global__ void __launch_bounds__(256) fa_weights_sum_kernel(const PagedWeightsArgs a) {
   const int rest = fast_div(blockIdx.x, a.by_tiles), tile = blockIdx.x - rest * a.key_tiles;
   const int b = fast_div(rest, a.by_kvh), kvh = rest - b * a.kv_heads;
   const Seq s = load_seq(a.pt, b, a.max_q);
   const int key = tile * kWeightKeys + threadIdx.x;
-  if (s.nq <= 0 || key >= s.len) return;
+  if (s.nq * a.group < a.min_rows || s.nq <= 0 || key >= s.len) return;
   const int id = a.pt.table[b * a.pt.table_stride + (key >> a.pt.page_shift)];
   if ((uint32_t)id >= (uint32_t)a.pt.num_pages) return;
   float sum = 0.0f;
@@ -405,10 +562,34 @@ __global__ void __launch_bounds__(256) fa_move_kernel(const PagedEvictArgs a, in
 
 }  // namespace
 
-hipError_t launch_paged_weights(const PagedWeightsArgs& args, int head_dim, bool bf16,
-                                hipStream_t stream) {
+hipError_t launch_paged_weights(const PagedWeightsArgs& args, const WeightsPlan& plan, int head_dim,
+                                bool bf16, hipStream_t stream) {
   PagedWeightsArgs a = args;
-  const int64_t tiles = (int64_t)a.pt.batch * a.kv_heads * a.key_tiles;
+  a.min_rows = plan.few_rows > 0 ? plan.few_rows + 1 : 1;
+  a.max_rows = plan.few_rows;
+  void* kargs[] = {&a};
+  const int64_t bk = (int64_t)a.pt.batch * a.kv_heads;
+  if (plan.few_rows > 0) {
+    a.few_keys = plan.few_keys;
+    a.few_chunks = (a.pt.max_kv + a.few_keys - 1) / a.few_keys;
+    a.by_few = make_fast_div((uint32_t)a.few_chunks);
+    const int64_t grid = bk * a.few_chunks;
+    if (grid > 0x7fffffff) return hipErrorInvalidValue;
+    auto few = [&](auto rb_c) -> const void* {
+      constexpr int RB = decltype(rb_c)::value;
+      if (head_dim == 128)
+        return bf16 ? reinterpret_cast<const void*>(&fa_weights_few_kernel<128, true, RB>)
+                    : reinterpret_cast<const void*>(&fa_weights_few_kernel<128, false, RB>);
+      return bf16 ? reinterpret_cast<const void*>(&fa_weights_few_kernel<64, true, RB>)
+                  : reinterpret_cast<const void*>(&fa_weights_few_kernel<64, false, RB>);
+    };
+    const void* fn = plan.few_rows <= 16 ? few(std::integral_constant<int, 1>{})
+                                         : few(std::integral_constant<int, 2>{});
+    const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)grid), dim3(128), kargs, 0, stream);
+    if (e != hipSuccess) return e;
+  }
+  if (plan.splits == 0) return hipSuccess;
+  const int64_t tiles = bk * a.key_tiles;
   const int64_t grid = tiles * a.splits;
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
   const void* fn;
@@ -418,8 +599,7 @@ hipError_t launch_paged_weights(const PagedWeightsArgs& args, int head_dim, bool
   else
     fn = bf16 ? reinterpret_cast<const void*>(&fa_weights_kernel<64, true>)
               : reinterpret_cast<const void*>(&fa_weights_kernel<64, false>);
-  void* kargs[] = {&a};
-  hipError_t e = hipLaunchKernel(fn, dim3((unsigned)grid), dim3(256), kargs, 0, stream);
+  const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)grid), dim3(256), kargs, 0, stream);
   if (e != hipSuccess || a.ws == nullptr) return e;
   return hipLaunchKernel(reinterpret_cast<const void*>(&fa_weights_sum_kernel), dim3((unsigned)tiles),
                          dim3(256), kargs, 0, stream);

@@ -242,5 +242,29 @@ struct GroupStage {
   }
 };
 
+// The same for K alone.
+template <int D>
+struct KeyStage {
+  static constexpr int ROWB = 2 * D, NI = 16 * ROWB / 1024;
+  uint32_t src[NI];
+  int r_lane;
+  __device__ __forceinline__ void init(int lane, uint32_t k_ss) {
+    constexpr int LPR = ROWB / 16;
+    r_lane = lane / LPR;
+#pragma unroll
+    for (int it = 0; it < NI; ++it) {
+      const int r = it * (64 / LPR) + r_lane;
+      src[it] = r * k_ss + ((lane % LPR) ^ lds::Tile16<D>::swz_k(r)) * 16;
+    }
+  }
+  __device__ __forceinline__ void copy(const char* kp, uint32_t dst, int lim, uint32_t k_ss) const {
+#pragma unroll
+    for (int it = 0; it < NI; ++it) {
+      const int over = lim >= 15 ? 0 : max(it * (1024 / ROWB) + r_lane - lim, 0);
+      dma_16b(src[it] - over * k_ss, kp, dst + it * 1024);
+    }
+  }
+};
+
 }  // namespace
 }  // namespace fa
