@@ -34,11 +34,16 @@ PagedPlan plan_paged(int tokens, int batch, int kv_heads, int group, int head_di
     PagedGrid& g = p.decode;
     g.rows = most <= 16 ? 16 : 32;
     g.slots = batch;
-    // Four workgroups per CU (one runs at a time at D = 128: lengths are
-    // ragged), of 512 keys or more in whole 64-key tiles.
+    // One workgroup per CU, of 512 to 8192 keys in whole 64-key tiles (the
+    // upper end for batches with one long sequence among short ones).  Ragged
+    // lengths need no finer cut: a CU whose workgroup ended leaves its bandwidth
+    // to the others.  us for 1, 2, 4, 8 workgroups per CU: 32 sequences of up
+    // to 8192 keys, 8 kv heads, D = 128: 144, 147, 151, 157; one of 131072: 99,
+    // 100, 104, 113; 4 of up to 16000: 44, 44, 48, 48.
     const int64_t base = (int64_t)batch * kv_heads;
     const int64_t want = std::max<int64_t>(
-        1, std::min((4 * (int64_t)compute_units + base - 1) / base, (keys + 511) / 512));
+        (keys + 8191) / 8192,
+        std::min((compute_units + base - 1) / base, (keys + 511) / 512));
     g.chunk = (int)(((keys + want - 1) / want + 63) / 64 * 64);
     g.splits = (int)((keys + g.chunk - 1) / g.chunk);
     g.ws_rows = g.splits > 1 ? (uint64_t)base * g.splits * g.rows : 0;

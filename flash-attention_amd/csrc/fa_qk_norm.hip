@@ -140,7 +140,8 @@ struct Lane {
   }
 };
 
-constexpr int kRows = 4;  // rows a lane group has in flight
+constexpr int kRows = 4;      // rows a lane group has in flight
+constexpr int kBwdHeads = 4;  // heads of a block of the backward pass
 
 // Tokens x heads.  STORE: packed new tokens, heads H .. H + KH - 1 are k's and
 // the next KH are v's, both to the cache.
@@ -409,13 +410,13 @@ hipError_t launch_norm(const NormArgs& args, bool bf16, bool store, int compute_
 
 int norm_bwd_blocks(int64_t tokens, int heads, int head_dim, int compute_units) {
   const int per = 256 / (head_dim / 8);
-  const int64_t blocks = (tokens + per - 1) / per * ((heads + 7) / 8);
+  const int64_t blocks = (tokens + per - 1) / per * ((heads + kBwdHeads - 1) / kBwdHeads);
   return (int)std::max<int64_t>(1, std::min<int64_t>(blocks, 4 * (int64_t)compute_units));
 }
 
 hipError_t launch_norm_bwd(const NormArgs& args, bool bf16, int compute_units, hipStream_t stream) {
   NormArgs n = args;
-  n.head_chunk = 8;
+  n.head_chunk = kBwdHeads;
   const int blocks = norm_bwd_blocks(n.tokens, n.heads + n.kv_heads, n.head_dim, compute_units);
   return FA_NORM_PICK(launch_bwd_as, n, blocks, stream);
 }
