@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstdint>
 
@@ -20,6 +21,10 @@ PagedPlan plan_paged(int tokens, int batch, int kv_heads, int group, int head_di
   p.compute_units = compute_units;
   const int64_t most = (int64_t)std::min(max_q, tokens) * group;  // rows of a sequence
   const int64_t keys = std::max(max_kv, 1);
+  // So few keys that the chunk kernel serves every sequence whole: the
+  // launches of a decode kernel and of the joins, about 4.5 us each, cost more
+  // than the tiles that its workgroups would share.
+  constexpr int64_t kShortKeys = 1024;
   if (most > kDecodeRows) {
     PagedGrid& g = p.chunk;
     g.rows = kChunkRows;
@@ -27,15 +32,19 @@ PagedPlan plan_paged(int tokens, int batch, int kv_heads, int group, int head_di
     // Two workgroups per CU; the tiles of the last round go in pieces of 512
     // keys or more, two rounds of them at most.
     g.conc = std::max(1, 2 * compute_units / kv_heads);
-    g.pieces = keys <= 512 ? 0 : (int)std::min<int64_t>(2 * (int64_t)g.conc, 64 * (int64_t)g.slots);
+    g.pieces = keys <= kShortKeys ? 0 : (int)std::min<int64_t>(2 * (int64_t)g.conc, 64 * (int64_t)g.slots);
     g.ws_rows = (uint64_t)g.pieces * kv_heads * g.rows;
   }
-  if (most <= kDecodeRows || batch > 1) {
+  // No sequence can have so few tokens as the decode kernel serves where the
+  // others, at max_q, leave it more.
+  const int64_t least = tokens - (int64_t)(batch - 1) * max_q;
+  if (most <= kDecodeRows || (batch > 1 && keys > kShortKeys && least * group <= kDecodeRows)) {
     PagedGrid& g = p.decode;
     g.rows = most <= 16 ? 16 : 32;
     g.slots = batch;
-    // One workgroup per CU, of 512 to 8192 keys in whole 64-key tiles (the
-    // upper end for batches with one long sequence among short ones).  Ragged
+    // One workgroup per CU, of 128 to 8192 keys in whole 64-key tiles (the
+    // upper end for batches with one long sequence among short ones); up to 512
+    // keys are not split, for the join's launch.  Ragged
     // lengths need no finer cut: a CU whose workgroup ended leaves its bandwidth
     // to the others.  us for 1, 2, 4, 8 workgroups per CU: 32 sequences of up
     // to 8192 keys, 8 kv heads, D = 128: 144, 147, 151, 157; one of 131072: 99,
@@ -43,7 +52,7 @@ PagedPlan plan_paged(int tokens, int batch, int kv_heads, int group, int head_di
     const int64_t base = (int64_t)batch * kv_heads;
     const int64_t want = std::max<int64_t>(
         (keys + 8191) / 8192,
-        std::min((compute_units + base - 1) / base, (keys + 511) / 512));
+        keys <= 512 ? 1 : std::min((compute_units + base - 1) / base, (keys + 127) / 128));
     g.chunk = (int)(((keys + want - 1) / want + 63) / 64 * 64);
     g.splits = (int)((keys + g.chunk - 1) / g.chunk);
     g.ws_rows = g.splits > 1 ? (uint64_t)base * g.splits * g.rows : 0;
@@ -184,8 +193,10 @@ fa_status check_queries(const fa_paged_cache& c, int32_t tokens, int32_t heads, 
   if (max_q < 0 || max_kv < 0)
     return fail(FA_ERR_ARG, "max_q=%d and max_kv=%d must be >= 0", (int)max_q, (int)max_kv);
   FA_TRY(check_flag("causal", causal));
-  if (!std::isfinite(scale) || !(scale > 0.0f))
-    return fail(FA_ERR_ARG, "softmax_scale must be finite and > 0 (got %g)", (double)scale);
+  // (a normal number: the offset's headroom is divided by it)
+  if (!std::isfinite(scale) || !(scale >= FLT_MIN))
+    return fail(FA_ERR_ARG, "softmax_scale must be finite and >= %g (got %g)", (double)FLT_MIN,
+                (double)scale);
   if ((int64_t)tokens * heads > 0x7fffffffLL)
     return fail(FA_ERR_UNSUPPORTED, "tokens*heads = %lld exceeds 2^31-1", (long long)tokens * heads);
   if ((int64_t)c.batch * c.kv_heads > 0x7fffff)

@@ -47,6 +47,8 @@ constexpr float kHeadroom = BF16 ? 4.0f : 1.0f;
 
 constexpr float kLn2 = 0.6931471805599453f;
 
+enum StepMode { kWhole, kMasked, kSafe };
+
 // The state of a wave's RB blocks of 16 rows over tiles of 16 NKB keys, on
 // v_mfma_f32_16x16x32 with the layouts of fa_fwd16_kernel: S^T = K Q^T (lane
 // l: keys 16kb + 4 (l / 16) + i of row 16rb + l % 16), O^T += V^T P^T.
@@ -62,6 +64,7 @@ struct WaveAttn {
   uint32_t k_addr[KST], v_addr[DB];  // LDS operand addresses in tile 0
   float c;
   int lane, l16, g4;
+  bool odd;                 // a masked tile held an infinity or NaN (uniform)
 
   __device__ __forceinline__ void init(uint32_t k_lds, uint32_t v_lds, float scale_log2) {
     lane = threadIdx.x & 63;
@@ -72,6 +75,10 @@ struct WaveAttn {
     for (int st = 0; st < KST; ++st) k_addr[st] = k_lds + lds::k16_read_offset<D>(0, st, lane);
 #pragma unroll
     for (int db = 0; db < DB; ++db) v_addr[db] = v_lds + lds::v16_read_offset<D>(0, 0, db, lane);
+    reset();
+  }
+  __device__ __forceinline__ void reset() {
+    odd = false;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
 #pragma unroll
@@ -93,13 +100,17 @@ struct WaveAttn {
   }
 
   // One tile of keys kt0.. in LDS, OFF + off bytes behind the tile-0 addresses.
-  // MASKED: some row sees only part of it, or a group is absent (bit kb of
-  // `present` clear).
-  template <int OFF, bool MASKED>
-  __device__ __forceinline__ void step(int kt0, unsigned present, uint32_t off) {
+  // MODE kWhole: every row sees all of it.  Else some row sees only part of it,
+  // or a group is absent (bit kb of `present` clear), and 0 times an infinity or
+  // NaN of a masked key must not reach o: kMasked notes such elements in the V
+  // tile (at v_tile) in `odd`, and the caller starts again with kSafe, which
+  // takes care of them.  (One step that does either spilled 32 registers.)
+  template <int OFF, int MODE>
+  __device__ __forceinline__ void step(int kt0, unsigned present, uint32_t off, uint32_t v_tile = 0) {
+    constexpr bool MASKED = MODE != kWhole;
     f32x4 s[NKB][RB];
     {
-      constexpr int NK = NKB * KST, KW = MASKED ? 1 : NK < 3 ? NK : 3;
+      constexpr int NK = NKB * KST, KW = NK < 3 ? NK : 3;
       i16x8 ka[KW];
       static_for<0, KW>([&](auto i_c) FA_INLINE {
         constexpr int i = decltype(i_c)::value;
@@ -202,13 +213,17 @@ struct WaveAttn {
     const short one = BF16 ? (short)0x3F80 : (short)0x3C00;
     const i16x8 ones = {one, one, one, one, one, one, one, one};
 
-    if constexpr (MASKED) {
-      pv_masked(kt0, present, off, pf);
+    if constexpr (MODE == kSafe) {
+      pv_safe(kt0, present, off, pf);
 #pragma unroll
       for (int ch = 0; ch < NCH; ++ch)
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) ls[rb] = mfma16<BF16>(ones, pf[ch][rb], ls[rb]);
       return;
+    }
+    if constexpr (MODE == kMasked) {
+      odd = odd || any_non_finite(v_tile);
+      static_for<0, VD>(read_v);
     }
     __builtin_amdgcn_sched_barrier(0);
     static_for<0, NPV>([&](auto j_c) FA_INLINE {
@@ -224,13 +239,26 @@ struct WaveAttn {
     });
   }
 
-  // O += P V of a masked tile, where 0 * inf of a masked key must not reach o:
+  // Whether the V tile at LDS address v_tile holds an infinity or a NaN.
+  __device__ __forceinline__ bool any_non_finite(uint32_t v_tile) {
+    constexpr uint32_t E = BF16 ? 0x7F807F80u : 0x7C007C00u, L = BF16 ? 0x00800080u : 0x04000400u;
+    uint32_t any = 0;
+#pragma unroll
+    for (int it = 0; it < 16 * NKB * ROWB / 1024; ++it) {
+      const u32x4 w = __builtin_bit_cast(u32x4, lds_read16<0>(v_tile + it * 1024 + lane * 16));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) any |= (w[j] & E) + L;  // an exponent of all ones carries
+    }
+    return __any((any & 0x80008000u) != 0);
+  }
+
+  // O += P V of a masked tile with infinities or NaN in V:
   // the product with infinities and NaN as 0, and per (row, dim) a count of
   // those among the keys that the row sees, on the matrix core with weights 1
   // (+inf), 2^7 (-inf) and 2^14 (NaN), at most 64 of each: sums that fp32
   // holds exactly.
-  __device__ __forceinline__ void pv_masked(int kt0, unsigned present, uint32_t off,
-                                            const i16x8 (&pf)[NCH][RB]) {
+  __device__ __forceinline__ void pv_safe(int kt0, unsigned present, uint32_t off,
+                                          const i16x8 (&pf)[NCH][RB]) {
     constexpr uint32_t E = BF16 ? 0x7F807F80u : 0x7C007C00u, L = BF16 ? 0x00800080u : 0x04000400u;
     constexpr uint32_t M = BF16 ? 0x007F007Fu : 0x03FF03FFu, H = 0x80008000u;
     constexpr uint32_t kOne = BF16 ? 0x3F80u : 0x3C00u;
@@ -259,20 +287,20 @@ struct WaveAttn {
         constexpr int ch = decltype(ch_c)::value, at = ch * 32 * ROWB;
         const u32x4 v =
             __builtin_bit_cast(u32x4, ds_read_tr_pair<at, at + 16 * ROWB>(v_addr[db] + off));
-        u32x4 fin, odd;
+        u32x4 fin, ind;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          auto spread = [](uint32_t x) FA_INLINE { return (x >> 15) * 0xFFFFu; };  // bit 15 -> half
+          auto spread = [](uint32_t x) FA_INLINE { return ((x >> 15) << 16) - (x >> 15); };  // bit 15 -> half
           const uint32_t bad = spread(((v[j] & E) + L) & H);
           const uint32_t nan = bad & spread(((v[j] & M) + 0x7FFF7FFFu) & H);
           const uint32_t neg = spread(v[j] & H);
           fin[j] = v[j] & ~bad;
-          odd[j] = (nan & kNan) | (bad & ~nan & ((neg & kNeg) | (~neg & kPos)));
+          ind[j] = (nan & kNan) | (bad & ~nan & ((neg & kNeg) | (~neg & kPos)));
         }
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
           o[db][rb] = mfma16<BF16>(__builtin_bit_cast(i16x8, fin), pf[ch][rb], o[db][rb]);
-          n[rb] = mfma16<BF16>(__builtin_bit_cast(i16x8, odd), see[ch][rb], n[rb]);
+          n[rb] = mfma16<BF16>(__builtin_bit_cast(i16x8, ind), see[ch][rb], n[rb]);
         }
       });
 #pragma unroll
@@ -381,23 +409,35 @@ __global__ void __launch_bounds__(64 * NW) fa_paged_decode_kernel(const PagedFwd
     int t = wave, buf = 0;
     for (; t < n_tiles && whole(t); t += NW) {
       stage_next(t, 0);
-      w.template step<0, false>(c0 + 32 * t, present, 0);
+      w.template step<0, kWhole>(c0 + 32 * t, present, 0);
       present = present_next;
       fence_lds_reads();
       t += NW;
       buf = 1;
       if (t >= n_tiles || !whole(t)) break;
       stage_next(t, 1);
-      w.template step<TB, false>(c0 + 32 * t, present, 0);
+      w.template step<TB, kWhole>(c0 + 32 * t, present, 0);
       present = present_next;
       fence_lds_reads();
       buf = 0;
     }
     for (; t < n_tiles; t += NW, buf ^= 1) {
       stage_next(t, buf);
-      w.template step<0, true>(c0 + 32 * t, present, buf * TB);
+      w.template step<0, kMasked>(c0 + 32 * t, present, buf * TB, wave_lds + (2 + buf) * TB);
       present = present_next;
       fence_lds_reads();
+    }
+    if (__builtin_expect(w.odd, false)) {
+      w.reset();
+      ids.start(a.pt, a.pt.table + b * a.pt.table_stride, c0);
+      present = issue(wave, 0);
+      buf = 0;
+      for (t = wave; t < n_tiles; t += NW, buf ^= 1) {
+        stage_next(t, buf);
+        w.template step<0, kSafe>(c0 + 32 * t, present, buf * TB);
+        present = present_next;
+        fence_lds_reads();
+      }
     }
   }
 
@@ -493,9 +533,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   constexpr int ROWB = 2 * D, TB = 64 * ROWB, BM = kChunkRows;
   constexpr int DB = D / 16;
   __shared__ __attribute__((aligned(1024))) char smem[4 * TB];  // K0 K1 V0 V1
+  __shared__ int again;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (threadIdx.x == 0) again = 0;  // ordered by the first barrier
   int kvh, place, b, tile0;
   if (!head_and_place(a, kvh, place)) return;
   TileList<BM> list;
@@ -511,8 +553,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     if (nth >= end.rest) return;
     nth += end.whole;
   }
-  if (!list.find(a, nth, b, tile0)) return;
-  const Seq s = load_seq(a.pt, b, a.max_q);
+  Seq s;
+  if (!list.find(a, nth, b, tile0, s)) return;
   const int n_rows = s.nq * a.group, row0 = tile0 * BM;
   if (n_rows < a.min_rows || row0 >= n_rows) return;
   const int last_row = min(row0 + BM, n_rows) - 1;
@@ -590,20 +632,38 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   int t = 0, buf = 0;
   for (; t < n_tiles && whole(t); ++t) {
     stage_next(t, 0);
-    w.template step<0, false>(c0 + 64 * t, present, 0);
+    w.template step<0, kWhole>(c0 + 64 * t, present, 0);
     end_tile();
     ++t;
     buf = 1;
     if (t >= n_tiles || !whole(t)) break;
     stage_next(t, 1);
-    w.template step<TB, false>(c0 + 64 * t, present, 0);
+    w.template step<TB, kWhole>(c0 + 64 * t, present, 0);
     end_tile();
     buf = 0;
   }
   for (; t < n_tiles; ++t, buf ^= 1) {
     stage_next(t, buf);
-    if (c0 + 64 * t < wave_end) w.template step<0, true>(c0 + 64 * t, present, buf * TB);
+    if (c0 + 64 * t < wave_end)
+      w.template step<0, kMasked>(c0 + 64 * t, present, buf * TB, base + (2 + buf) * TB);
     end_tile();
+  }
+  // Infinities or NaN in a masked tile of some wave: all start again (the
+  // staging is shared).
+  if (w.odd && lane == 0) again = 1;
+  __syncthreads();
+  if (__builtin_expect(__builtin_amdgcn_readfirstlane(again) != 0, false)) {
+    w.reset();
+    ids.start(a.pt, a.pt.table + b * a.pt.table_stride, c0);
+    present = issue(0, 0);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    buf = 0;
+    for (t = 0; t < n_tiles; ++t, buf ^= 1) {
+      stage_next(t, buf);
+      if (c0 + 64 * t < wave_end) w.template step<0, kSafe>(c0 + 64 * t, present, buf * TB);
+      end_tile();
+    }
   }
 
   float inv[2], lu[2];
@@ -680,7 +740,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 // meet in LDS: one group per row left 128 chunks to a loop of dependent loads
 // (125 us against 98 for the attention itself at one sequence of 131072 keys).
 template <int D, bool BF16, int BM>
-__global__ void __launch_bounds__(256) fa_paged_merge_kernel(const PagedFwdArgs a) {
+__device__ __forceinline__ void merge_rows(const PagedFwdArgs& a, int block) {
   constexpr int TPR = D / 4, GROUPS = 256 / TPR;
   __shared__ f32x4 part_o[GROUPS][TPR];
   __shared__ float part_e[GROUPS][4];  // top, sum of weights; the same of the plain sums
@@ -688,7 +748,7 @@ __global__ void __launch_bounds__(256) fa_paged_merge_kernel(const PagedFwdArgs 
   constexpr bool kTiles = BM == kChunkRows;
   // Rows of a workgroup: of a tile (join 1) merge_rows, one after another.
   const int rpb = kTiles ? a.merge_rows : GROUPS / a.join, per = (BM + rpb - 1) / rpb;
-  const int sk = blockIdx.x / per, r_first = (blockIdx.x - sk * per) * rpb + grp / a.join;
+  const int sk = block / per, r_first = (block - sk * per) * rpb + grp / a.join;
   const int slot = fast_div(sk, a.by_kvh), kvh = sk - slot * a.kv_heads;
   int b = slot, tile0 = 0, n_act;
   int64_t w0;  // first partial row
@@ -698,8 +758,7 @@ __global__ void __launch_bounds__(256) fa_paged_merge_kernel(const PagedFwdArgs 
     list.init(a);
     LastRound end;
     end.init(a, list.count);
-    if (end.pieces <= 1 || slot >= end.rest || !list.find(a, end.whole + slot, b, tile0)) return;
-    s = load_seq(a.pt, b, a.max_q);
+    if (end.pieces <= 1 || slot >= end.rest || !list.find(a, end.whole + slot, b, tile0, s)) return;
     w0 = ((int64_t)kvh * a.max_pieces + slot * end.pieces) * BM;
     n_act = end.pieces;
   } else {
@@ -783,11 +842,25 @@ __global__ void __launch_bounds__(256) fa_paged_merge_kernel(const PagedFwdArgs 
   }
 }
 
-template <class F>
-hipError_t launch(F* fn, int64_t grid, const PagedFwdArgs& args, hipStream_t stream,
-                  int threads = 256) {
+// The joins of both kernels of a call in one launch.
+struct MergeArgs {
+  PagedFwdArgs chunk, decode;
+  int32_t chunk_blocks, decode_rows;
+};
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) fa_paged_merge_kernel(const MergeArgs m) {
+  if ((int)blockIdx.x < m.chunk_blocks)
+    merge_rows<D, BF16, kChunkRows>(m.chunk, blockIdx.x);
+  else if (m.decode_rows == 16)
+    merge_rows<D, BF16, 16>(m.decode, blockIdx.x - m.chunk_blocks);
+  else
+    merge_rows<D, BF16, 32>(m.decode, blockIdx.x - m.chunk_blocks);
+}
+
+template <class F, class A>
+hipError_t launch(F* fn, int64_t grid, const A& args, hipStream_t stream, int threads = 256) {
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
-  void* kargs[] = {const_cast<PagedFwdArgs*>(&args)};
+  void* kargs[] = {const_cast<A*>(&args)};
   return hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)grid), dim3(threads), kargs,
                          0, stream);
 }
@@ -814,6 +887,8 @@ hipError_t launch_all(const PagedFwdArgs& base, const PagedPlan& plan, void* ws,
     at += g.ws_rows * (D + 2) * 4;
   };
   constexpr int GROUPS = 256 / (D / 4);  // lane groups of a merge workgroup
+  MergeArgs merge = {};
+  int64_t chunk_blocks = 0, decode_blocks = 0;
   if (const PagedGrid& g = plan.chunk; g.rows != 0) {
     PagedFwdArgs a = base;
     // One sequence with too many rows for the decode kernel: this one serves
@@ -835,9 +910,8 @@ hipError_t launch_all(const PagedFwdArgs& base, const PagedPlan& plan, void* ws,
       // Rows of a workgroup: few, unless that makes thousands of workgroups,
       // most of which find no tile.
       a.merge_rows = tiles * (kChunkRows / GROUPS) <= 2048 ? GROUPS : 32;
-      if (tiles > 0)
-        e = launch(&fa_paged_merge_kernel<D, BF16, kChunkRows>, tiles * (kChunkRows / a.merge_rows), a, stream);
-      if (e != hipSuccess) return e;
+      chunk_blocks = tiles * (kChunkRows / a.merge_rows);
+      merge.chunk = a;
     }
   }
   if (const PagedGrid& g = plan.decode; g.rows != 0) {
@@ -862,15 +936,21 @@ hipError_t launch_all(const PagedFwdArgs& base, const PagedPlan& plan, void* ws,
     };
     hipError_t e = g.rows == 16 ? decode(std::integral_constant<int, 1>{})
                                 : decode(std::integral_constant<int, 2>{});
-    if (e != hipSuccess || g.splits == 1) return e;
-    // As many lane groups a row as it has chunks, a power of two.
-    a.join = 1;
-    while (a.join < g.splits && a.join < GROUPS) a.join *= 2;
-    const int rpb = GROUPS / a.join;
-    const int64_t per = (g.rows + rpb - 1) / rpb;
-    e = g.rows == 16 ? launch(&fa_paged_merge_kernel<D, BF16, 16>, sk * per, a, stream)
-                     : launch(&fa_paged_merge_kernel<D, BF16, 32>, sk * per, a, stream);
     if (e != hipSuccess) return e;
+    if (g.splits > 1) {
+      // As many lane groups a row as it has chunks, a power of two.
+      a.join = 1;
+      while (a.join < g.splits && a.join < GROUPS) a.join *= 2;
+      const int rpb = GROUPS / a.join;
+      decode_blocks = sk * ((g.rows + rpb - 1) / rpb);
+      merge.decode = a;
+      merge.decode_rows = g.rows;
+    }
+  }
+  if (chunk_blocks + decode_blocks > 0) {
+    if (chunk_blocks > 0x7fffffff) return hipErrorInvalidValue;
+    merge.chunk_blocks = (int32_t)chunk_blocks;
+    return launch(&fa_paged_merge_kernel<D, BF16>, chunk_blocks + decode_blocks, merge, stream);
   }
   return hipSuccess;
 }

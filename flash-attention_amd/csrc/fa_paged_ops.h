@@ -87,7 +87,7 @@ struct PageIds {
   // Keys from key0, a multiple of 64 below pt.max_kv.
   __device__ __forceinline__ void start(const PageTable& pt, const int32_t* r, int key0) {
     row = r;
-    limit = pt.max_kv - 1;
+    limit = max(pt.max_kv - 1, 0);  // (a table has a page at least)
     shift = pt.page_shift;
     base = key0 - 1024;
     pages = (uint32_t)pt.num_pages;
@@ -125,18 +125,18 @@ struct PageIds {
 // counted 64 at a time.
 template <int BM>
 struct TileList {
-  int start, tiles;  // this lane's sequence (up to 64)
+  int start, tiles, c0, c1, len;  // this lane's sequence (up to 64)
   int count;
 
   __device__ __forceinline__ void init(const PagedFwdArgs& a) {
     const int lane = threadIdx.x & 63;
     count = a.slots;
     if (a.pt.batch > 64) return;
-    int len = -1;
-    tiles = 0;
+    c0 = c1 = tiles = 0;
+    len = -1;
     if (lane < a.pt.batch) {
-      const int c0 = min(max(a.pt.cu[lane], 0), a.pt.tokens);
-      const int c1 = min(max(a.pt.cu[lane + 1], c0), a.pt.tokens);
+      c0 = min(max(a.pt.cu[lane], 0), a.pt.tokens);
+      c1 = min(max(a.pt.cu[lane + 1], c0), a.pt.tokens);
       const int rows = min(c1 - c0, a.max_q) * a.group;
       tiles = rows >= a.min_rows ? (rows + BM - 1) / BM : 0;
       len = min(max(a.pt.lens[lane], 0), a.pt.max_kv);
@@ -148,12 +148,17 @@ struct TileList {
       count += t;
     }
   }
-  __device__ __forceinline__ bool find(const PagedFwdArgs& a, int n, int& b, int& tile) const {
+  __device__ __forceinline__ bool find(const PagedFwdArgs& a, int n, int& b, int& tile, Seq& s) const {
     if (a.pt.batch <= 64) {
       const uint64_t has = __ballot(start <= n && n < start + tiles);
       if (has == 0) return false;
       b = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(has));
       tile = __builtin_amdgcn_readlane(start + tiles - 1, b) - n;
+      const int nq = __builtin_amdgcn_readlane(c1 - c0, b);
+      s.q0 = __builtin_amdgcn_readlane(c0, b);
+      s.nq = min(nq, a.max_q);
+      s.len = __builtin_amdgcn_readlane(len, b);
+      s.first = s.len - nq;
       return true;
     }
     const int lane = threadIdx.x & 63, at = a.slots - 1 - n;
@@ -169,6 +174,7 @@ struct TileList {
     b = __builtin_amdgcn_readfirstlane(k);
     if (b >= a.pt.batch) return false;
     tile = at - begin(b, scalar_load(a.pt.cu, b));
+    s = load_seq(a.pt, b, a.max_q);
     return tile >= 0;
   }
 };

@@ -91,7 +91,8 @@ def paged_key_weights(
     query heads of its kv head and the tokens that see it of
     ``exp(scale q.k - lse)``.  ``q``, ``lse`` and the limits as given to and
     returned by ``paged_forward``.  The new tokens' own keys are set, not added
-    to, so a reused page needs no clearing.  Returns ``key_weights``."""
+    to, so a reused page needs no clearing.  A page must belong to one sequence of
+    the call only (sequences that share a prefix need weights of their own).  Returns ``key_weights``."""
     _no_grad("paged_key_weights", q, lse, k_cache, key_weights)
     _EXT.paged_key_weights(q, lse, k_cache, block_table, cu_seqlens, seq_lens, key_weights, max_q,
                            max_kv, causal, softmax_scale)
@@ -115,7 +116,7 @@ def paged_evict(
     key.  Equal weights: the lower index stays; NaN counts as the largest.
 
     The kept keys, values and weights are copied, in their order, to the pages
-    of ``new_table`` [B, M'], none of which may be read by this call; the old
+    of ``new_table`` [B, M'], each listed once and none read by this call; the old
     pages stay as they are, for the caller to reuse.  Pass the rows of the
     sequences to shorten.  Returns ``(new_lens, kept)``: int32 [B], and int32
     [B, kv_heads, keep] with the former index of the key now at each place (-1

@@ -74,7 +74,7 @@ typedef struct {
   int32_t heads;        /* a multiple of kv_heads */
   int32_t max_q;        /* most new tokens of one sequence; those past it are not computed */
   int32_t max_kv;       /* most keys of one sequence; seq_lens above it are taken as max_kv */
-  float softmax_scale;
+  float softmax_scale;  /* finite, a normal positive number */
   int32_t causal;
 } fa_paged_fwd_params;
 
@@ -84,7 +84,7 @@ typedef struct {
  * A key that is itself one of the new tokens is seen for the first time: its
  * weight is set to the sum, so that the slot of a reused page needs no
  * clearing.  Rows whose lse is -inf add nothing.  Sums run in a fixed order
- * (no atomics). */
+ * (no atomics); a page must belong to one sequence of the call only. */
 typedef struct {
   fa_paged_cache cache;   /* v unused */
   const void* q;          /* [tokens, heads, head_dim] */
@@ -104,8 +104,8 @@ typedef struct {
  * the ones of largest key weight, `keep` keys in all (every key of a sequence
  * that has no more).  Equal weights: the lower index is kept; NaN counts as
  * the largest.  The kept keys, values and weights are copied in their order
- * to the pages of new_table, which no page being read may be among; the old
- * pages are left as they are.  A sequence with an absent page among its keys'
+ * to the pages of new_table, each listed once there and none among the pages
+ * being read; the old pages are left as they are.  A sequence with an absent page among its keys'
  * or its new pages is not copied: its new length is 0 and its kept indices
  * are -1. */
 typedef struct {

@@ -141,7 +141,7 @@ WRITTEN_BAD = [("cache.k_stride[0]", 0, A.FA_ERR_STRIDE), ("cache.v_stride[1]", 
 QUERY_BAD = [
     ("cache.cu_seqlens", None, A.FA_ERR_NULL), ("tokens", -1, A.FA_ERR_SHAPE), ("heads", 0, A.FA_ERR_SHAPE),
     ("heads", 3, A.FA_ERR_SHAPE), ("max_q", -1, A.FA_ERR_ARG), ("max_kv", -1, A.FA_ERR_ARG),
-    ("causal", 2, A.FA_ERR_ARG), ("softmax_scale", 0.0, A.FA_ERR_ARG), ("softmax_scale", math.nan, A.FA_ERR_ARG),
+    ("causal", 2, A.FA_ERR_ARG), ("softmax_scale", 0.0, A.FA_ERR_ARG), ("softmax_scale", 1e-39, A.FA_ERR_ARG), ("softmax_scale", math.nan, A.FA_ERR_ARG),
     ("tokens", 2 ** 30, A.FA_ERR_UNSUPPORTED), ("cache.batch", 2 ** 23, A.FA_ERR_UNSUPPORTED),
     ("q", None, A.FA_ERR_NULL), ("q", PTR + 4, A.FA_ERR_STRIDE), ("q_stride[0]", 100, A.FA_ERR_STRIDE),
     ("lse", PTR + 2, A.FA_ERR_STRIDE),

@@ -88,6 +88,10 @@ SHAPES = {
     "chunks-d64": ([130, 300, 64, 257], [130, 1, 64, 200], 4, 2, 64, 256),
     "prefill": ([193], [193], 3, 3, 128, 64),
     "mixed": ([260, 400, 17, 90], [150, 1, 1, 33], 8, 2, 64, 16),
+    "many-sequences": ([(37 * i) % 150 for i in range(70)], [min((37 * i) % 150, (5 * i) % 47) for i in range(70)],
+                       2, 1, 64, 16),
+    "many-long-sequences": ([1100 + i for i in range(66)], [(i * 7) % 36 for i in range(66)], 2, 1, 64, 64),
+    "last-round-of-one-head": ([1500, 1400], [200, 130], 2, 1, 128, 32),
     "split-decode": ([5000], [1], 4, 2, 128, 64),
     "split-chunk": ([3000], [40], 1, 1, 64, 16),
 }
@@ -354,6 +358,52 @@ def test_agrees_with_the_contiguous_forward(fa, dtype):
     # each within P's and the output's rounding (3 u of values of at most 4.5)
     assert float((o.float() - of[0].transpose(0, 1).float()).abs().max()) <= 6 * R.U[DT[dtype]] * 4.5
     assert float((lse - lf[0].T).abs().max()) <= 1e-3
+
+
+@pytest.mark.parametrize("KH,N", [(1, 9000), (2, 3000), (3, 2500), (4, 2100), (8, 1500), (16, 1300), (24, 1100),
+                                  (32, 1500), (64, 1500), (100, 1200)])
+def test_grid_orders_against_the_contiguous_forward(fa, KH, N):
+    """Head counts that take each order of the grid (whole heads per XCD in
+    groups, heads shared by XCDs, all interleaved), with whole rounds and a last
+    round in pieces, against forward(causal=True): every row written, each within
+    its rounding (3 u of values of at most 5.5)."""
+    print(f"case grid order KH {KH} N {N}", flush=True)
+    D, page = 64, 64
+    g = torch.Generator(device=DEV).manual_seed(KH)
+    q, k, v = (torch.randn(1, KH, N, D, generator=g, device=DEV).half() for _ in range(3))
+    n = -(-N // page)
+    kc, vc = (torch.zeros(n, KH, page, D, dtype=torch.float16, device=DEV) for _ in range(2))
+    for cache, x in ((kc, k), (vc, v)):
+        pad = torch.zeros(KH, n * page, D, dtype=torch.float16, device=DEV)
+        pad[:, :N] = x[0]
+        cache.copy_(pad.view(KH, n, page, D).transpose(0, 1))
+    table = torch.arange(n, dtype=torch.int32, device=DEV)[None]
+    out = torch.full((N, KH, D), math.nan, dtype=torch.float16, device=DEV)
+    o, lse = fa.paged_forward(q[0].transpose(0, 1), kc, vc, table,
+                              torch.tensor([0, N], dtype=torch.int32, device=DEV),
+                              torch.tensor([N], dtype=torch.int32, device=DEV), out, max_q=N, return_lse=True)
+    of, lf = fa.forward(q, k, v, causal=True, return_lse=True)
+    assert float((o.float() - of[0].transpose(0, 1).float()).abs().max()) <= 6 * 2.0 ** -11 * 5.5
+    assert float((lse - lf[0].T).abs().max()) <= 1e-3
+
+
+@pytest.mark.parametrize("name", ["ragged-decode", "chunks"])
+def test_no_keys_allowed(fa, name):
+    """max_kv = 0: every row is empty."""
+    lens, new, H, KH, D, page = SHAPES[name]
+    c = Cache(lens, page, KH, D, torch.float16, 397)
+    q = torch.ones(sum(new), H, D).half()
+    o, lse = run(fa, c, q, cu_of(new), max_q=max(new), max_kv=0)
+    assert not o.any() and bool((lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("scale", [1.2e-38, 1e-20, 100.0])
+@pytest.mark.parametrize("name", ["ragged-decode", "chunks"])
+def test_extreme_scales(fa, name, scale):
+    lens, new, H, KH, D, page = SHAPES[name]
+    c = Cache(lens, page, KH, D, torch.bfloat16, 398)
+    q = torch.randn(sum(new), H, D, generator=torch.Generator().manual_seed(16)).bfloat16()
+    compare(fa, c, q, cu_of(new), max_q=max(new), scale=scale)
 
 
 def test_empty_calls(fa):
