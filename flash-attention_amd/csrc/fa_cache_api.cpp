@@ -65,7 +65,9 @@ WeightsPlan plan_weights(int tokens, int batch, int kv_heads, int group, int max
                          int compute_units) {
   WeightsPlan p = {};
   const int64_t most = (int64_t)std::min(max_q, tokens) * group;  // rows of a sequence
-  if (most <= kDecodeRows || batch > 1) {
+  // (as plan_paged: the launch of the other kernel is spared where it can be)
+  const int64_t least = tokens - (int64_t)(batch - 1) * max_q;
+  if (most <= kDecodeRows || (batch > 1 && max_kv > 1024 && least * group <= kDecodeRows)) {
     p.few_rows = most <= 16 ? 16 : kDecodeRows;
     // Four workgroups per CU, which run at once, of 256 to 2048 keys in whole
     // 64-key tiles.
@@ -75,10 +77,23 @@ WeightsPlan plan_weights(int tokens, int batch, int kv_heads, int group, int max
     p.few_keys = (int)std::max<int64_t>(256, std::min<int64_t>(keys, kWeightChunk));
   }
   if (most > kDecodeRows) {
-    // Three workgroups per CU, which run at once, each with 128 rows or more.
-    const int64_t tiles = (int64_t)batch * kv_heads * ((max_kv + kWeightKeys - 1) / kWeightKeys);
-    const int64_t want = 3 * (int64_t)compute_units / std::max<int64_t>(tiles, 1);
-    p.splits = (int)std::max<int64_t>(1, std::min(want, most / 128));
+    // Three workgroups per CU run at once; row splits fill them, of 128 rows or
+    // more.  Where new tokens are many of the keys, causal masks leave the first
+    // key tile all rows and the last one few: then tiles go in pairs of equal
+    // work if that is long (4 prompts of 4096 tokens, 4 kv heads: 251 -> 151
+    // us), and are cut finer if it is short (28 prompts of up to 1613, one kv
+    // head: 45 -> 33 us; a pair starts twice, 46 us).
+    const int64_t tiles = (max_kv + kWeightKeys - 1) / kWeightKeys;
+    const int64_t bk = (int64_t)batch * kv_heads;
+    auto cut = [&](int64_t places, int per_cu, int rows) {
+      const int64_t want = per_cu * (int64_t)compute_units / std::max<int64_t>(bk * places, 1);
+      return (int)std::max<int64_t>(1, std::min(want, most / rows));
+    };
+    p.splits = cut(tiles, 3, 128);
+    if (4 * (int64_t)max_q >= max_kv) {
+      p.pairs = most / 64 >= 32 * (int64_t)p.splits;
+      p.splits = p.pairs ? cut((tiles + 1) / 2, 3, 128) : cut(tiles, 6, 256);
+    }
   }
   return p;
 }
@@ -582,7 +597,8 @@ fa_status fa_paged_key_weights(const fa_paged_weights_params* p, void* workspace
   a.by_group = make_fast_div((uint32_t)a.group);
   a.by_kvh = make_fast_div((uint32_t)a.kv_heads);
   a.by_tiles = make_fast_div((uint32_t)a.key_tiles);
-  a.by_splits = make_fast_div((uint32_t)c.batch);
+  a.by_batch = make_fast_div((uint32_t)c.batch);
+  a.by_splits = make_fast_div((uint32_t)plan.splits);
   a.ws = need > 0 ? static_cast<float*>(workspace) : nullptr;
   return launched(launch_paged_weights(a, plan, c.head_dim, c.dtype == FA_DTYPE_BF16,
                                        static_cast<hipStream_t>(stream)));

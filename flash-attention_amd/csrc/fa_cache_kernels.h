@@ -88,11 +88,12 @@ struct PagedWeightsArgs {
   uint32_t k_ss;
   int32_t heads, kv_heads, group, max_q, causal;
   float scale_log2;
-  // Many rows, sequences of min_rows or more; grid: sequences x kv heads x key
-  // tiles x row splits.
+  // Many rows, sequences of min_rows or more; grid: sequences x kv heads x
+  // places x row splits, a place being a key tile, or with `pairs` the n-th and
+  // the n-th last.
   int32_t min_rows;
-  int32_t key_tiles, splits;
-  FastDiv by_group, by_kvh, by_tiles, by_splits;
+  int32_t key_tiles, splits, pairs, places;
+  FastDiv by_group, by_kvh, by_tiles, by_places, by_batch, by_splits;
   float* ws;           // [splits][batch][kv_heads][key_tiles * 256] partial sums
   // Few rows, at most max_rows; grid: sequences x kv heads x chunks of keys.
   int32_t max_rows, few_keys, few_chunks;
@@ -104,6 +105,7 @@ struct WeightsPlan {
   int32_t few_rows;  // 16 or 32: sequences of at most so many rows apart; 0: none
   int32_t few_keys;  // their keys a workgroup
   int32_t splits;    // row splits of the others (1: no workspace); 0: none
+  int32_t pairs;     // 1: key tiles in pairs
 };
 WeightsPlan plan_weights(int tokens, int batch, int kv_heads, int group, int max_q, int max_kv,
                          int compute_units);

@@ -43,42 +43,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3)))
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, g4 = lane >> 4;
-  // (sequence, kv head, key tile, row split): the splits slowest
-  const int rest = fast_div(blockIdx.x, a.by_tiles), tile = blockIdx.x - rest * a.key_tiles;
+  // (sequence, kv head, key tile or pair of them, row split): the splits slowest
+  const int rest = fast_div(blockIdx.x, a.by_places), place = blockIdx.x - rest * a.places;
   const int bk = fast_div(rest, a.by_kvh), kvh = rest - bk * a.kv_heads;
-  const int split = fast_div(bk, a.by_splits), b = bk - split * a.pt.batch;
+  const int split = fast_div(bk, a.by_batch), b = bk - split * a.pt.batch;
   const Seq s = load_seq(a.pt, b, a.max_q);
-  const int key0 = tile * kWeightKeys;
-  if (s.nq * a.group < a.min_rows || s.nq <= 0 || key0 >= s.len) return;
-  const int wkey0 = key0 + 64 * wave;
-
-  // This lane's keys wkey0 + 16kb + l16: rows of K past the end re-read the
-  // last key, absent pages page 0; their sums are not used.
-  const int32_t* row = a.pt.table + b * a.pt.table_stride;
-  i16x8 kf[KB][KST];
-  unsigned there = 0;
-#pragma unroll
-  for (int kb = 0; kb < KB; ++kb) {
-    const int r0 = min(wkey0 + 16 * kb, (s.len - 1) & ~15);
-    const int id = page_id(a.pt, row, r0);
-    const bool ok = (uint32_t)id < (uint32_t)a.pt.num_pages;
-    if (ok) there |= 1u << kb;
-    const int in_page = (r0 & ((1 << a.pt.page_shift) - 1)) + min(l16, s.len - 1 - r0);
-    const char* kp = a.k + (int64_t)(ok ? id : 0) * a.k_sp + kvh * a.k_sh + (int64_t)in_page * a.k_ss;
-#pragma unroll
-    for (int st = 0; st < KST; ++st)
-      kf[kb][st] = *reinterpret_cast<const i16x8*>(kp + (32 * st + 8 * g4) * 2);
-  }
-
-  // Rows: those of tokens that see this workgroup's first key, cut into the
-  // grid's splits.
   const int n_rows = s.nq * a.group;
-  const int i_first = a.causal ? max(0, key0 - s.first) : 0;
-  const int t_begin = min((int)((int64_t)i_first * a.group / RT), n_rows / RT);
-  const int t_all = (n_rows + RT - 1) / RT - t_begin;
-  const int splits = a.ws != nullptr ? a.splits : 1;
-  const int t0 = t_begin + (int)((int64_t)split * t_all / splits);
-  const int t1 = t_begin + (int)((int64_t)(split + 1) * t_all / splits);
+  const int n_tiles = (s.len + kWeightKeys - 1) / kWeightKeys;
+  if (n_rows < a.min_rows || n_rows <= 0 || place >= (a.pairs ? (n_tiles + 1) / 2 : n_tiles)) return;
+  const int32_t* row = a.pt.table + b * a.pt.table_stride;
 
   const char* qh = a.q + s.q0 * a.q_st + (int64_t)kvh * a.group * a.q_sh;
   const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(smem));
@@ -110,92 +83,122 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3)))
 #pragma unroll
   for (int st = 0; st < KST; ++st) k_off[st] = lds::k16_read_offset<D>(0, st, lane);
 
-  float acc[KB] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (t0 < t1) {
-    fetch_row(t0);
-    issue(t0, 0);
-  }
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  // One row tile from LDS.  MASKED: some row does not see some of the wave's keys.
-  auto compute = [&](auto masked_c, int buf, float lse, int last) FA_INLINE {
-    constexpr bool MASKED = decltype(masked_c)::value;
-    neg_lse[wave][lane] = -lse;
-    f32x4 sc[2][KB];  // the next 16 rows' products run beside this one's exponentials
-    auto products = [&](int rb) FA_INLINE {
+  for (int sub = 0; sub < 2; ++sub) {
+    const int tile = sub == 0 ? place : n_tiles - 1 - place;
+    if (sub == 1 && (!a.pairs || tile == place)) break;
+    const int key0 = tile * kWeightKeys, wkey0 = key0 + 64 * wave;
+
+    // This lane's keys wkey0 + 16kb + l16: rows of K past the end re-read the
+    // last key, absent pages page 0; their sums are not used.
+    i16x8 kf[KB][KST];
+    unsigned there = 0;
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) sc[rb & 1][kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int kb = 0; kb < KB; ++kb) {
+      const int r0 = min(wkey0 + 16 * kb, (s.len - 1) & ~15);
+      const int id = page_id(a.pt, row, r0);
+      const bool ok = (uint32_t)id < (uint32_t)a.pt.num_pages;
+      if (ok) there |= 1u << kb;
+      const int in_page = (r0 & ((1 << a.pt.page_shift) - 1)) + min(l16, s.len - 1 - r0);
+      const char* kp = a.k + (int64_t)(ok ? id : 0) * a.k_sp + kvh * a.k_sh + (int64_t)in_page * a.k_ss;
 #pragma unroll
-      for (int st = 0; st < KST; ++st) {
-        const i16x8 qa = *reinterpret_cast<const i16x8*>(smem + buf * TB + rb * 16 * ROWB + k_off[st]);
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) sc[rb & 1][kb] = mfma16<BF16>(qa, kf[kb][st], sc[rb & 1][kb]);
-      }
-    };
-    products(0);
-#pragma unroll
-    for (int rb = 0; rb < RT / 16; ++rb) {
-      if (rb + 1 < RT / 16) products(rb + 1);
-      // rows 16rb + 4g4 + i, keys wkey0 + 16kb + l16
-      const f32x4 nl = *reinterpret_cast<const f32x4*>(&neg_lse[wave][16 * rb + 4 * g4]);
-      int rel[4];
-      if constexpr (MASKED) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) rel[i] = __shfl(last, 16 * rb + 4 * g4 + i) - wkey0 - l16;
-      }
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = fast_exp2(fmaf(sc[rb & 1][kb][i], a.scale_log2, nl[i]));
-          if constexpr (MASKED)
-            acc[kb] += 16 * kb <= rel[i] ? p : 0.0f;
-          else
-            acc[kb] += p;
-        }
+      for (int st = 0; st < KST; ++st)
+        kf[kb][st] = *reinterpret_cast<const i16x8*>(kp + (32 * st + 8 * g4) * 2);
     }
-  };
-  // Rows ascend, and with them the keys they see: masked tiles (or ones that
-  // see none of the wave's keys) first, whole ones, and a last one whose rows
-  // end inside it.  Loops of their own, so that the whole ones carry no masks;
-  // every wave passes one barrier a tile, whichever loop it is in.
-  int t = t0;
-  auto step = [&](auto masked_c) FA_INLINE {
-    const float lse = lse_n;
-    const int last = last_n, buf = (t - t0) & 1;
-    if (t + 1 < t1) {
-      issue(t + 1, buf ^ 1);
-      fetch_row(t + 1);
+
+    // Row tiles: from the first token that sees the first key, cut into the
+    // grid's splits.
+    const int i_first = a.causal ? max(0, key0 - s.first) : 0;
+    const int t_begin = (int)min((int64_t)i_first * a.group, (int64_t)n_rows) / RT;
+    const int t_all = (n_rows + RT - 1) / RT - t_begin;
+    const int each = fast_div(t_all, a.by_splits), more = t_all - each * a.splits;
+    const int t0 = t_begin + split * each + min(split, more);
+    const int t1 = t0 + each + (split < more ? 1 : 0);
+
+    float acc[KB] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (t0 < t1) {
+      fetch_row(t0);
+      issue(t0, 0);
     }
-    if (!decltype(masked_c)::value || (__any(last >= wkey0) && wkey0 < s.len)) compute(masked_c, buf, lse, last);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    ++t;
-  };
-  auto whole = [&]() FA_INLINE { return __all(last_n >= wkey0 + 63); };
-  while (t < t1 && !whole()) step(std::true_type{});
-  while (t < t1 && whole()) step(std::false_type{});
-  while (t < t1) step(std::true_type{});
-
-  // Lane group g4 finishes key block g4.
-  float mine = 0.0f;
+    // One row tile from LDS.  MASKED: some row does not see some of the wave's keys.
+    auto compute = [&](auto masked_c, int buf, float lse, int last) FA_INLINE {
+      constexpr bool MASKED = decltype(masked_c)::value;
+      neg_lse[wave][lane] = -lse;
+      f32x4 sc[2][KB];  // the next 16 rows' products run beside this one's exponentials
+      auto products = [&](int rb) FA_INLINE {
 #pragma unroll
-  for (int kb = 0; kb < KB; ++kb) {
-    float x = acc[kb];
-    x += __shfl_xor(x, 16);
-    x += __shfl_xor(x, 32);
-    if (g4 == kb) mine = x;
-  }
-  const int key = wkey0 + 16 * g4 + l16;
-  if (a.ws != nullptr) {
-    a.ws[((((int64_t)split * a.pt.batch + b) * a.kv_heads + kvh) * a.key_tiles + tile) * kWeightKeys +
-         64 * wave + lane] = mine;
-    return;
-  }
-  if (key < s.len && ((there >> g4) & 1u)) {
-    const int id = row[key >> a.pt.page_shift];
-    float* w = a.w + (int64_t)id * a.w_sp + kvh * a.w_sh + (key & ((1 << a.pt.page_shift) - 1));
-    *w = key >= s.first ? mine : *w + mine;
+        for (int kb = 0; kb < KB; ++kb) sc[rb & 1][kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int st = 0; st < KST; ++st) {
+          const i16x8 qa = *reinterpret_cast<const i16x8*>(smem + buf * TB + rb * 16 * ROWB + k_off[st]);
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) sc[rb & 1][kb] = mfma16<BF16>(qa, kf[kb][st], sc[rb & 1][kb]);
+        }
+      };
+      products(0);
+#pragma unroll
+      for (int rb = 0; rb < RT / 16; ++rb) {
+        if (rb + 1 < RT / 16) products(rb + 1);
+        // rows 16rb + 4g4 + i, keys wkey0 + 16kb + l16
+        const f32x4 nl = *reinterpret_cast<const f32x4*>(&neg_lse[wave][16 * rb + 4 * g4]);
+        int rel[4];
+        if constexpr (MASKED) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) rel[i] = __shfl(last, 16 * rb + 4 * g4 + i) - wkey0 - l16;
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p = fast_exp2(fmaf(sc[rb & 1][kb][i], a.scale_log2, nl[i]));
+            if constexpr (MASKED)
+              acc[kb] += 16 * kb <= rel[i] ? p : 0.0f;
+            else
+              acc[kb] += p;
+          }
+      }
+    };
+    // Rows ascend, and with them the keys they see: masked tiles (or ones that
+    // see none of the wave's keys) first, whole ones, and a last one whose rows
+    // end inside it.  Loops of their own, so that the whole ones carry no masks;
+    // every wave passes one barrier a tile, whichever loop it is in.
+    int t = t0;
+    auto step = [&](auto masked_c) FA_INLINE {
+      const float lse = lse_n;
+      const int last = last_n, buf = (t - t0) & 1;
+      if (t + 1 < t1) {
+        issue(t + 1, buf ^ 1);
+        fetch_row(t + 1);
+      }
+      if (!decltype(masked_c)::value || (__any(last >= wkey0) && wkey0 < s.len)) compute(masked_c, buf, lse, last);
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+      ++t;
+    };
+    auto whole = [&]() FA_INLINE { return __all(last_n >= wkey0 + 63); };
+    while (t < t1 && !whole()) step(std::true_type{});
+    while (t < t1 && whole()) step(std::false_type{});
+    while (t < t1) step(std::true_type{});
+
+    // Lane group g4 finishes key block g4.
+    float mine = 0.0f;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      float x = acc[kb];
+      x += __shfl_xor(x, 16);
+      x += __shfl_xor(x, 32);
+      if (g4 == kb) mine = x;
+    }
+    const int key = wkey0 + 16 * g4 + l16;
+    if (a.ws != nullptr) {
+      a.ws[((((int64_t)split * a.pt.batch + b) * a.kv_heads + kvh) * a.key_tiles + tile) * kWeightKeys +
+           64 * wave + lane] = mine;
+    } else if (key < s.len && ((there >> g4) & 1u)) {
+      const int id = row[key >> a.pt.page_shift];
+      float* w = a.w + (int64_t)id * a.w_sp + kvh * a.w_sh + (key & ((1 << a.pt.page_shift) - 1));
+      *w = key >= s.first ? mine : *w + mine;
+    }
   }
 }
 
@@ -348,11 +351,18 @@ __global__ void __launch_bounds__(256) fa_weights_sum_kernel(const PagedWeightsA
   const int key = tile * kWeightKeys + threadIdx.x;
   if (s.nq * a.group < a.min_rows || s.nq <= 0 || key >= s.len) return;
   const int id = a.pt.table[b * a.pt.table_stride + (key >> a.pt.page_shift)];
-  if ((uint32_t)id >= (uint32_t)a.pt.num_pages) return;
+  const float* part = a.ws + (((int64_t)b * a.kv_heads + kvh) * a.key_tiles + tile) * kWeightKeys + threadIdx.x;
+  const int64_t step = (int64_t)a.pt.batch * a.kv_heads * a.key_tiles * kWeightKeys;
+  constexpr int BATCH = 8;  // loads in flight
   float sum = 0.0f;
-  for (int c = 0; c < a.splits; ++c)
-    sum += a.ws[((((int64_t)c * a.pt.batch + b) * a.kv_heads + kvh) * a.key_tiles + tile) * kWeightKeys +
-                threadIdx.x];
+  for (int c = 0; c < a.splits; c += BATCH) {
+    float x[BATCH];
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) x[j] = c + j < a.splits ? part[(c + j) * step] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) sum += x[j];
+  }
+  if ((uint32_t)id >= (uint32_t)a.pt.num_pages) return;
   float* w = a.w + (int64_t)id * a.w_sp + kvh * a.w_sh + (key & ((1 << a.pt.page_shift) - 1));
   *w = key >= s.first ? sum : *w + sum;
 }
@@ -592,7 +602,10 @@ hipError_t launch_paged_weights(const PagedWeightsArgs& args, const WeightsPlan&
   }
   if (plan.splits == 0) return hipSuccess;
   const int64_t tiles = bk * a.key_tiles;
-  const int64_t grid = tiles * a.splits;
+  a.pairs = plan.pairs;
+  a.places = a.pairs ? (a.key_tiles + 1) / 2 : a.key_tiles;
+  a.by_places = make_fast_div((uint32_t)a.places);
+  const int64_t grid = bk * a.places * a.splits;
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
   const void* fn;
   if (head_dim == 128)
