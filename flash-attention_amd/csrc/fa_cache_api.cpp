@@ -85,7 +85,9 @@ WeightsPlan plan_weights(int tokens, int batch, int kv_heads, int group, int max
     // head: 45 -> 33 us; a pair starts twice, 46 us).
     const int64_t tiles = (max_kv + kWeightKeys - 1) / kWeightKeys;
     const int64_t bk = (int64_t)batch * kv_heads;
+    // (Up to 512 rows are not split, for the launch that adds the splits up.)
     auto cut = [&](int64_t places, int per_cu, int rows) {
+      if (most <= 512) return 1;
       const int64_t want = per_cu * (int64_t)compute_units / std::max<int64_t>(bk * places, 1);
       return (int)std::max<int64_t>(1, std::min(want, most / rows));
     };

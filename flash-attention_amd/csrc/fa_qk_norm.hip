@@ -153,14 +153,26 @@ __global__ void __launch_bounds__(256) fa_norm_kernel(const NormArgs n) {
   const int h0 = blockIdx.x / n.blocks_x * n.head_chunk;
   const int heads = n.heads + (STORE ? 2 : 1) * n.kv_heads, h1 = min(heads, h0 + n.head_chunk);
 
+  bool mine = token < n.tokens;
+  const int tok = min(token, n.tokens - 1);
+  const int b = STORE ? 0 : fast_div(tok, n.by_seq), t = STORE ? tok : tok - b * n.seq_len;
+  // What needs no place in the cache is asked for first: the loads below wait
+  // for one another.
+  const int pos = n.positions == nullptr ? t : n.positions[b * n.pos_stride + t];
+  L l;
+  l.place(n);
+  float w[2][8];
+  if (h0 < n.heads) l.weights(n, 0, w[0]);
+  if (h1 > n.heads && h0 < n.heads + n.kv_heads) l.weights(n, 1, w[1]);
+
   // Place in the cache, from the number of sequences that end before the
   // token (counted by the whole wave, 64 sequences at a time).
   int64_t page = -1;
   int at = 0;
-  bool mine = token < n.tokens;
   if constexpr (STORE) {
     const int lane = threadIdx.x & 63;
     const int wave_token = blockIdx.x % n.blocks_x * TPW + ((int)threadIdx.x >> 6) * TPV;
+    const int first = n.pt.cu[0];
     int seq = 0;
     for (int i0 = 1; i0 <= n.pt.batch; i0 += 64) {
       const int i = i0 + lane;
@@ -171,8 +183,8 @@ __global__ void __launch_bounds__(256) fa_norm_kernel(const NormArgs n) {
         if (lane / LPR == g) seq += ended;
       }
     }
-    mine = mine && seq < n.pt.batch && token >= n.pt.cu[0];
-    if (mine) {
+    mine = mine && seq < n.pt.batch && token >= first;
+    if (mine && h1 > n.heads) {
       const int64_t key = (int64_t)n.pt.lens[seq] - n.pt.cu[seq + 1] + token;
       if (key >= 0 && key < n.capacity) {
         const int id = n.pt.table[seq * n.pt.table_stride + (key >> n.pt.page_shift)];
@@ -181,15 +193,8 @@ __global__ void __launch_bounds__(256) fa_norm_kernel(const NormArgs n) {
       }
     }
   }
-  if (!mine) return;
-  const int b = STORE ? 0 : fast_div(token, n.by_seq), t = STORE ? token : token - b * n.seq_len;
-  L l;
-  l.place(n);
-  const int pos = n.positions == nullptr ? t : n.positions[b * n.pos_stride + t];
   l.angles(n, pos);
-  float w[2][8];
-  if (h0 < n.heads) l.weights(n, 0, w[0]);
-  if (h1 > n.heads && h0 < n.heads + n.kv_heads) l.weights(n, 1, w[1]);
+  if (!mine) return;
 
   auto range = [&](auto x_c, int lo, int hi, const float* wt) FA_INLINE {
     constexpr int X = decltype(x_c)::value;

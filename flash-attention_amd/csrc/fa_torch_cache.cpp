@@ -6,12 +6,17 @@
 #include <torch/extension.h>
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <ATen/hip/HIPGraphsUtils.cuh>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
 
+#include <array>
 #include <cmath>
 #include <optional>
+#include <utility>
 
 #include "fa_mi355x_cache.h"
 
@@ -296,9 +301,11 @@ fa_qk_norm_params norm_params(const Tensor& q, const Tensor& k, const Tensor& qw
   return p;
 }
 
-pybind11::tuple qk_norm_rope(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw,
-                             const Tensor& cos, const Tensor& sin, std::optional<Tensor> positions,
-                             double eps, bool interleaved) {
+using Pair = std::pair<Tensor, Tensor>;
+
+Pair norm_forward(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Tensor& cos,
+                  const Tensor& sin, const std::optional<Tensor>& positions, double eps,
+                  bool interleaved) {
   fa_qk_norm_params p = norm_params(q, k, qw, kw, cos, sin, positions, eps, interleaved);
   const c10::OptionalDeviceGuard guard(q.device());
   Tensor qo = torch::empty_like(q), ko = torch::empty_like(k);
@@ -307,7 +314,7 @@ pybind11::tuple qk_norm_rope(const Tensor& q, const Tensor& k, const Tensor& qw,
   set_strides(p.q_out_stride, qo, 3);
   set_strides(p.k_out_stride, ko, 3);
   check_status(fa_qk_norm_rope(&p, stream_of(q)), "qk_norm_rope");
-  return pybind11::make_tuple(qo, ko);
+  return {qo, ko};
 }
 
 // A gradient as the kernel reads it: unit stride, 16-byte rows.
@@ -318,10 +325,11 @@ Tensor readable(const Tensor& g) {
   return ok ? g : g.clone(at::MemoryFormat::Contiguous);
 }
 
-pybind11::tuple qk_norm_rope_backward(const Tensor& dq_out, const Tensor& dk_out, const Tensor& q,
-                                      const Tensor& k, const Tensor& qw, const Tensor& kw,
-                                      const Tensor& cos, const Tensor& sin,
-                                      std::optional<Tensor> positions, double eps, bool interleaved) {
+std::array<Tensor, 4> norm_backward(const Tensor& dq_out, const Tensor& dk_out, const Tensor& q,
+                                    const Tensor& k, const Tensor& qw, const Tensor& kw,
+                                    const Tensor& cos, const Tensor& sin,
+                                    const std::optional<Tensor>& positions, double eps,
+                                    bool interleaved) {
   fa_qk_norm_bwd_params p{};
   p.fwd = norm_params(q, k, qw, kw, cos, sin, positions, eps, interleaved);
   for (const auto& [g, x, name] : {std::make_tuple(&dq_out, &q, "q's gradient"),
@@ -352,7 +360,89 @@ pybind11::tuple qk_norm_rope_backward(const Tensor& dq_out, const Tensor& dk_out
     dqw = dqw.to(qw.dtype());
     dkw = dkw.to(kw.dtype());
   }
-  return pybind11::make_tuple(dq, dk, dqw, dkw);
+  return {dq, dk, dqw, dkw};
+}
+
+// Whether a leaf's gradient accumulator lives on, kept by an autograd graph,
+// on another stream than the current one: a backward pass that is captured
+// here would have to wait for that stream, which ends the capture.
+bool accumulates_elsewhere(const Tensor& t) {
+  if (!t.requires_grad() || !t.is_leaf()) return false;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!node) return false;
+  const auto s = node->stream();
+  return s.has_value() &&
+         *s != at::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).unwrap();
+}
+
+// The norm in autograd, differentiable once.  (A node of its own here: one
+// written in Python costs 60 us more per training step.)
+struct QkNormRope : torch::autograd::Function<QkNormRope> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q,
+                                                const Tensor& k, const Tensor& qw, const Tensor& kw,
+                                                const Tensor& cos, const Tensor& sin,
+                                                const std::optional<Tensor>& positions, double eps,
+                                                bool interleaved) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Pair y = norm_forward(q, k, qw, kw, cos, sin, positions, eps, interleaved);
+    ctx->save_for_backward({q, k, qw, kw, cos, sin, positions.value_or(Tensor())});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    return {y.first, y.second};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list g) {
+    const auto v = ctx->get_saved_variables();
+    std::optional<Tensor> positions;
+    if (v[6].defined()) positions = v[6];
+    std::array<Tensor, 4> d;
+    {
+      at::NoGradGuard no_grad;
+      for (int i = 0; i < 2; ++i)
+        if (!g[i].defined()) g[i] = torch::zeros_like(v[i]);
+      d = norm_backward(g[0], g[1], v[0], v[1], v[2], v[3], v[4], v[5], positions,
+                        ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool());
+    }
+    torch::autograd::variable_list out(d.begin(), d.end());
+    if (at::GradMode::is_enabled()) {  // create_graph: a second derivative is refused when it is asked for
+      for (Tensor& t : out) t.requires_grad_();
+      auto refuse = std::make_shared<torch::autograd::DelayedError>(
+          "trying to differentiate twice qk_norm_rope, which is once_differentiable", 4);
+      out = (*refuse)(std::move(out));
+    }
+    out.resize(9);
+    return out;
+  }
+};
+
+pybind11::tuple qk_norm_rope(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw,
+                             const Tensor& cos, const Tensor& sin, std::optional<Tensor> positions,
+                             double eps, bool interleaved) {
+  if (at::GradMode::is_enabled()) {
+    TORCH_CHECK(!cos.requires_grad() && !sin.requires_grad(),
+                "cos and sin get no gradients: detach them");
+    if (q.requires_grad() || k.requires_grad() || qw.requires_grad() || kw.requires_grad()) {
+      if (at::hip::currentStreamCaptureStatusMayInitCtx() != at::hip::CaptureStatus::None)
+        for (const Tensor* t : {&q, &k, &qw, &kw})
+          TORCH_CHECK(!accumulates_elsewhere(*t),
+                      "qk_norm_rope: an autograd graph made on another stream still holds these leaves, "
+                      "and the backward pass of this capture would have to wait for that stream: release "
+                      "that graph first, or use qk_norm_rope_backward");
+      const auto y = QkNormRope::apply(q, k, qw, kw, cos, sin, positions, eps, interleaved);
+      return pybind11::make_tuple(y[0], y[1]);
+    }
+  }
+  const Pair y = norm_forward(q, k, qw, kw, cos, sin, positions, eps, interleaved);
+  return pybind11::make_tuple(y.first, y.second);
+}
+
+pybind11::tuple qk_norm_rope_backward(const Tensor& dq_out, const Tensor& dk_out, const Tensor& q,
+                                      const Tensor& k, const Tensor& qw, const Tensor& kw,
+                                      const Tensor& cos, const Tensor& sin,
+                                      std::optional<Tensor> positions, double eps, bool interleaved) {
+  at::NoGradGuard no_grad;
+  const auto d = norm_backward(dq_out, dk_out, q, k, qw, kw, cos, sin, positions, eps, interleaved);
+  return pybind11::make_tuple(d[0], d[1], d[2], d[3]);
 }
 
 Tensor paged_store(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& qw, const Tensor& kw,
@@ -393,18 +483,6 @@ Tensor paged_store(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   return o;
 }
 
-// Whether a leaf's gradient accumulator lives on, kept by an autograd graph,
-// on another stream than the current one: a backward pass that is captured
-// here would have to wait for that stream, which ends the capture.
-bool accumulates_elsewhere(const Tensor& t) {
-  if (!t.requires_grad() || !t.is_leaf()) return false;
-  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-  if (!node) return false;
-  const auto s = node->stream();
-  return s.has_value() &&
-         *s != at::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).unwrap();
-}
-
 }  // namespace
 
 void bind_cache(pybind11::module_& m) {
@@ -429,5 +507,4 @@ void bind_cache(pybind11::module_& m) {
         py::arg("k_weight"), py::arg("cos"), py::arg("sin"), py::arg("positions"), py::arg("k_cache"),
         py::arg("v_cache"), py::arg("block_table"), py::arg("cu_seqlens"), py::arg("seq_lens"),
         py::arg("out"), py::arg("eps"), py::arg("interleaved"));
-  m.def("accumulates_elsewhere", &accumulates_elsewhere, py::arg("t"));
 }

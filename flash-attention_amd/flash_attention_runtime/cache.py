@@ -29,7 +29,6 @@ other lengths and tables.  The cache's calls compute no gradients.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _C as _EXT
 
@@ -158,22 +157,6 @@ def paged_store(
                             block_table, cu_seqlens, seq_lens, out, eps, interleaved)
 
 
-class _QkNormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.eps, ctx.interleaved = eps, interleaved
-        return _EXT.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dq_out, dk_out):
-        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-        dq, dk, dqw, dkw = _EXT.qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos,
-                                                      sin, positions, ctx.eps, ctx.interleaved)
-        return dq, dk, dqw, dkw, None, None, None, None, None
-
-
 def qk_norm_rope(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -201,18 +184,6 @@ def qk_norm_rope(
     backward pass through leaves that an older autograd graph still holds is
     refused; ``qk_norm_rope_backward`` can always be captured.
     """
-    if torch.is_grad_enabled():
-        if cos.requires_grad or sin.requires_grad:
-            raise RuntimeError("cos and sin get no gradients: detach them")
-        leaves = (q, k, q_weight, k_weight)
-        if any(t.requires_grad for t in leaves):
-            if torch.cuda.is_current_stream_capturing() and any(
-                    _EXT.accumulates_elsewhere(t) for t in leaves):
-                raise RuntimeError(
-                    "qk_norm_rope: an autograd graph made on another stream still holds these "
-                    "leaves, and the backward pass of this capture would have to wait for that "
-                    "stream: release that graph first, or use qk_norm_rope_backward")
-            return _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
     return _EXT.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
 
 
