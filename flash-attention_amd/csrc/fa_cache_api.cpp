@@ -50,8 +50,10 @@ PagedPlan plan_paged(int tokens, int batch, int kv_heads, int group, int head_di
     // to 8192 keys, 8 kv heads, D = 128: 144, 147, 151, 157; one of 131072: 99,
     // 100, 104, 113; 4 of up to 16000: 44, 44, 48, 48.
     const int64_t base = (int64_t)batch * kv_heads;
+    // (the cut for long sequences as far as its partials stay within 128 MiB)
+    const int64_t part = base * g.rows * (head_dim + 2) * 4;
     const int64_t want = std::max<int64_t>(
-        (keys + 8191) / 8192,
+        std::min((keys + 8191) / 8192, std::max<int64_t>(1, (int64_t(128) << 20) / part)),
         keys <= 512 ? 1 : std::min((compute_units + base - 1) / base, (keys + 127) / 128));
     g.chunk = (int)(((keys + want - 1) / want + 63) / 64 * 64);
     g.splits = (int)((keys + g.chunk - 1) / g.chunk);

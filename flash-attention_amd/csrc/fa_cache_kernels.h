@@ -45,7 +45,8 @@ struct PagedFwdArgs {
   int32_t slots, splits, chunk;
   int32_t conc, max_pieces;        // workgroups of a kv head that run at once, its most pieces
   float piece_cost;
-  int32_t join, merge_rows;        // merge: lane groups of a row, rows of a workgroup
+  // Merge: lane groups of a row; rows of a workgroup (tiles), of a slot (decode).
+  int32_t join, merge_rows, most_rows;
   FastDiv by_group, by_kvh, by_splits, by_conc;
   // Order of the chunk kernel's grid (set_order).
   int32_t places, per_xcd, unit_group, xcds;
