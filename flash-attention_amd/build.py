@@ -72,7 +72,7 @@ def build_hip_library(jobs: int) -> list[str]:
     (host work planning), fa_api.cpp (the C ABI) and CACHE_SOURCES (the paged
     cache's operators and the q/k norm) with hipcc and links the shared library
     libfa_mi355x.so.  The forward's kernel source is compiled a second
-    time with -DFA_LDS_POISON into the debug library
+    time, and the cache's kernels too, with -DFA_LDS_POISON into the debug library
     libfa_mi355x_poison.so (same ABI; staged LDS is filled with NaN before
     every staging write), and a third time with -DFA_MFMA32 into
     libfa_mi355x_mfma32.so (same ABI; fp16 non-causal problems of the
@@ -95,6 +95,9 @@ def build_hip_library(jobs: int) -> list[str]:
                      "-o", obj_of(src)])
     cmds.append([hipcc, *HIP_FLAGS, "-DFA_LDS_POISON", "-I", INCLUDE, "-I", CSRC, "-x", "hip",
                  "-c", kernel, "-o", obj_of(kernel, ".poison")])
+    for src in [c for c in cache if c.endswith(".hip")]:
+        cmds.append([hipcc, *HIP_FLAGS, "-DFA_LDS_POISON", "-I", INCLUDE, "-I", CSRC, "-x", "hip",
+                     "-c", src, "-o", obj_of(src, ".poison")])
     cmds.append([hipcc, *HIP_FLAGS, "-DFA_MFMA32", "-I", INCLUDE, "-I", CSRC, "-x", "hip",
                  "-c", kernel, "-o", obj_of(kernel, ".mfma32")])
     with ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
@@ -104,7 +107,10 @@ def build_hip_library(jobs: int) -> list[str]:
                        ("libfa_mi355x_poison.so", obj_of(kernel, ".poison")),
                        ("libfa_mi355x_mfma32.so", obj_of(kernel, ".mfma32"))):
         lib = os.path.join(OUT_DIR, name)
-        more = [obj_of(c) for c in cache] if kobj == obj_of(kernel) else []
+        # (the cache's operators have no 32x32x16 form: that library leaves them out)
+        poison = ".poison" if "poison" in name else ""
+        more = [obj_of(c, poison if c.endswith(".hip") else "") for c in cache]
+        more = [] if "mfma32" in name else more
         _run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", kobj,
               *[obj_of(h) for h in host], *more, "-o", lib + ".tmp"])
         os.replace(lib + ".tmp", lib)

@@ -64,6 +64,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3)))
       const int r = min(t * RT + rt, n_rows - 1);
       const int i = fast_div(r, a.by_group), h = r - i * a.group;
       const int c = (lane % LPR) ^ lds::Tile16<D>::swz_k(rt);
+      poison_1k(base + buf * TB + (wave * NI + it) * 1024);
       dma_16b((uint32_t)((i - i0) * (int)a.q_st + h * (int)a.q_sh + c * 16), src,
               base + buf * TB + (wave * NI + it) * 1024);
     }

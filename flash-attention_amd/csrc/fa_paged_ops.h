@@ -23,6 +23,23 @@ __device__ __forceinline__ i16x8 lds_read16(uint32_t addr) {
   return *(__attribute__((address_space(3))) const i16x8*)((lds_char_t*)(uintptr_t)addr + OFF);
 }
 
+// The debug build -DFA_LDS_POISON fills LDS bytes with NaN before every DMA into
+// them, as fa_fwd_kernel.hip's: a read ahead of its wait or barrier shows, and
+// with correct synchronisation every result keeps its bits.
+#ifdef FA_LDS_POISON
+constexpr bool kLdsPoison = true;
+#else
+constexpr bool kLdsPoison = false;
+#endif
+__device__ __forceinline__ void poison_1k(uint32_t addr) {
+  if constexpr (kLdsPoison) {
+    typedef __attribute__((address_space(3))) char lds_char_t;
+    *(__attribute__((address_space(3))) u32x4*)((lds_char_t*)(uintptr_t)addr + (threadIdx.x & 63) * 16) =
+        u32x4{~0u, ~0u, ~0u, ~0u};
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+  }
+}
+
 // s_waitcnt vmcnt(N), the other counters left alone.
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
@@ -232,6 +249,11 @@ struct GroupStage {
   // kp, vp: the group's first rows; rows past `lim` re-read row lim.
   __device__ __forceinline__ void copy(const char* kp, const char* vp, uint32_t k_dst, uint32_t v_dst,
                                        int lim, uint32_t k_ss, uint32_t v_ss) const {
+#pragma unroll
+    for (int it = 0; kLdsPoison && it < NI; ++it) {
+      poison_1k(k_dst + it * 1024);
+      poison_1k(v_dst + it * 1024);
+    }
     if (lim >= 15) {
 #pragma unroll
       for (int it = 0; it < NI; ++it) dma_16b(k_src[it], kp, k_dst + it * 1024);
@@ -267,6 +289,7 @@ struct KeyStage {
 #pragma unroll
     for (int it = 0; it < NI; ++it) {
       const int over = lim >= 15 ? 0 : max(it * (1024 / ROWB) + r_lane - lim, 0);
+      poison_1k(dst + it * 1024);
       dma_16b(src[it] - over * k_ss, kp, dst + it * 1024);
     }
   }
