@@ -13,8 +13,8 @@
 //  * fa_paged_chunk_kernel: 128 rows, four waves of 32; K/V tiles of 64 keys
 //    staged through a two-deep LDS ring by global_load_lds DMA, as
 //    fa_fwd16_kernel.  Bound by the matrix cores and the exponentials.
-//    4096 tokens over 16384 keys run at 1140...1160 TFLOP/s (bf16,
-//    D = 128, 8 kv heads; a large matrix product reaches 1200 on the card).
+//    4096 tokens over 16384 keys take 903 us, 1218 TFLOP/s (bf16, D = 128,
+//    8 kv heads; a large matrix product reaches 1200 on the card).
 //  * fa_paged_decode_kernel: 16 or 32 rows (a few tokens), the keys of a chunk
 //    dealt to two or four waves in tiles of 32, each wave with an LDS ring of its
 //    own and no barrier before the end.  Bound by reading the cache: 5.4 TB/s at
@@ -229,6 +229,12 @@ struct WaveAttn {
       odd = odd || any_non_finite(v_tile);
       static_for<0, VD>(read_v);
     }
+    // With two waves on a SIMD unit, the one in its products goes first: the
+    // other's exponentials fill the gaps.  4096 tokens over 16384 keys, bf16,
+    // 8 kv heads: D = 128 949 us without, 903 with; D = 64 543 and 552, so not
+    // there; around Q K^T as well, D = 128 takes 939.
+    constexpr bool FIRST = NKB == 4 && D == 128;
+    if constexpr (FIRST) __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);
     static_for<0, NPV>([&](auto j_c) FA_INLINE {
       constexpr int j = decltype(j_c)::value;
@@ -241,6 +247,7 @@ struct WaveAttn {
       if constexpr (j + VD < NPV) read_v(std::integral_constant<int, j + VD>{});
       __builtin_amdgcn_sched_barrier(0);
     });
+    if constexpr (FIRST) __builtin_amdgcn_s_setprio(0);
   }
 
   // Whether the V tile at LDS address v_tile holds an infinity or a NaN.
