@@ -123,14 +123,20 @@ fa_status check_rows(const char* name, const void* ptr, const int64_t* st, int n
   return FA_OK;
 }
 
-// Rows of a written tensor must not overlap: every stride of a dimension with
-// more than one entry spans a row at least.
-fa_status check_written(const char* name, const int64_t* st, const int64_t* size, int n,
-                        int64_t head_dim) {
-  for (int i = 0; i < n; ++i)
-    if (size[i] > 1 && st[i] < head_dim)
-      return fail(FA_ERR_STRIDE, "%s stride[%d] = %lld is smaller than head_dim %lld (rows overlap)",
-                  name, i, (long long)st[i], (long long)head_dim);
+// Rows of `row` elements of a written tensor must not overlap: each stride, in
+// ascending order, spans what the smaller ones reach.  (n <= 3)
+fa_status check_written(const char* name, const int64_t* st, const int64_t* size, int n, int64_t row) {
+  int order[3] = {0, 1, 2};
+  std::sort(order, order + n, [&](int i, int j) { return st[i] < st[j]; });
+  __int128 reach = row;
+  for (int o = 0; o < n; ++o) {
+    const int i = order[o];
+    if (size[i] <= 1) continue;
+    if (st[i] < reach)
+      return fail(FA_ERR_STRIDE, "%s stride[%d] = %lld is smaller than the %lld elements it must step over"
+                  " (rows overlap)", name, i, (long long)st[i], (long long)reach);
+    reach += (__int128)st[i] * (size[i] - 1);
+  }
   return FA_OK;
 }
 
@@ -212,10 +218,11 @@ fa_status check_queries(const fa_paged_cache& c, int32_t tokens, int32_t heads, 
   if (max_q < 0 || max_kv < 0)
     return fail(FA_ERR_ARG, "max_q=%d and max_kv=%d must be >= 0", (int)max_q, (int)max_kv);
   FA_TRY(check_flag("causal", causal));
-  // (a normal number: the offset's headroom is divided by it)
-  if (!std::isfinite(scale) || !(scale >= FLT_MIN))
-    return fail(FA_ERR_ARG, "softmax_scale must be finite and >= %g (got %g)", (double)FLT_MIN,
-                (double)scale);
+  // (a normal number: the offset's headroom is divided by it; its product with
+  // log2(e) is finite)
+  if (!(scale >= FLT_MIN) || !(scale <= FLT_MAX / 2))
+    return fail(FA_ERR_ARG, "softmax_scale must be from %g to %g (got %g)", (double)FLT_MIN,
+                (double)FLT_MAX / 2, (double)scale);
   if ((int64_t)tokens * heads > 0x7fffffffLL)
     return fail(FA_ERR_UNSUPPORTED, "tokens*heads = %lld exceeds 2^31-1", (long long)tokens * heads);
   if ((int64_t)c.batch * c.kv_heads > 0x7fffff)
@@ -266,8 +273,8 @@ fa_status launched(hipError_t e) {
   return FA_OK;
 }
 
-// Largest byte offset of a tile's rows from its first (32 tokens, one group of
-// heads), which the key weights' staging holds in 32 bits.
+// Largest byte offset of a tile's rows from its first (64 tokens, or fewer of a
+// group of heads), which the key weights' staging holds in 32 bits.
 fa_status check_tile_reach(const int64_t st[2], int32_t group) {
   if (st[0] > kMaxKeyStride || (int64_t)(group - 1) * st[1] > (int64_t(1) << 28))
     return fail(FA_ERR_UNSUPPORTED, "q strides %lld, %lld exceed the kernel's range", (long long)st[0],
@@ -404,6 +411,7 @@ fa_status fa_paged_evict_validate(const fa_paged_evict_params* p) {
   if (p->keep < 1 || p->recent < 0 || p->recent > p->keep)
     return fail(FA_ERR_ARG, "keep=%d must be >= 1 and recent=%d from 0 to keep", (int)p->keep,
                 (int)p->recent);
+  if (p->keep > 1 << 30) return fail(FA_ERR_UNSUPPORTED, "keep=%d exceeds 2^30", (int)p->keep);
   if (p->max_kv < 0) return fail(FA_ERR_ARG, "max_kv=%d must be >= 0", (int)p->max_kv);
   if ((int64_t)c.batch * c.kv_heads > 0x7fffff)
     return fail(FA_ERR_UNSUPPORTED, "batch*kv_heads = %lld exceeds 2^23-1", (long long)c.batch * c.kv_heads);

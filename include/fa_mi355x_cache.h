@@ -74,7 +74,7 @@ typedef struct {
   int32_t heads;        /* a multiple of kv_heads */
   int32_t max_q;        /* most new tokens of one sequence; those past it are not computed */
   int32_t max_kv;       /* most keys of one sequence; seq_lens above it are taken as max_kv */
-  float softmax_scale;  /* finite, a normal positive number */
+  float softmax_scale;  /* a normal positive number, at most FLT_MAX / 2 */
   int32_t causal;
 } fa_paged_fwd_params;
 
@@ -117,7 +117,7 @@ typedef struct {
   int32_t* new_lens;         /* [batch]: min(length, keep) */
   int32_t* kept;             /* [batch, kv_heads, keep] contiguous: index of the key now at t, or -1 */
   int32_t new_pages;         /* new_pages * page_size >= min(keep, max_pages * page_size) */
-  int32_t keep;              /* >= 1 */
+  int32_t keep;              /* 1 to 2^30 */
   int32_t recent;            /* 0 to keep */
   int32_t max_kv;            /* as in fa_paged_fwd_params */
 } fa_paged_evict_params;

@@ -137,11 +137,14 @@ VALUES_BAD = [
     ("cache.v", None, A.FA_ERR_NULL), ("cache.v", PTR + 2, A.FA_ERR_STRIDE),
     ("cache.v_stride[1]", -8, A.FA_ERR_STRIDE), ("cache.v_stride[2]", 2 ** 24 + 8, A.FA_ERR_UNSUPPORTED),
 ]
-WRITTEN_BAD = [("cache.k_stride[0]", 0, A.FA_ERR_STRIDE), ("cache.v_stride[1]", 56, A.FA_ERR_STRIDE)]
+WRITTEN_BAD = [("cache.k_stride[0]", 0, A.FA_ERR_STRIDE), ("cache.v_stride[1]", 56, A.FA_ERR_STRIDE),
+               # heads' last rows overlap the next page's first, though every stride spans a row
+               ("cache.k_stride[0]", 2 * 16 * 64 - 64, A.FA_ERR_STRIDE), ("cache.v_stride[1]", 64, A.FA_ERR_STRIDE)]
 QUERY_BAD = [
     ("cache.cu_seqlens", None, A.FA_ERR_NULL), ("tokens", -1, A.FA_ERR_SHAPE), ("heads", 0, A.FA_ERR_SHAPE),
     ("heads", 3, A.FA_ERR_SHAPE), ("max_q", -1, A.FA_ERR_ARG), ("max_kv", -1, A.FA_ERR_ARG),
-    ("causal", 2, A.FA_ERR_ARG), ("softmax_scale", 0.0, A.FA_ERR_ARG), ("softmax_scale", 1e-39, A.FA_ERR_ARG), ("softmax_scale", math.nan, A.FA_ERR_ARG),
+    ("causal", 2, A.FA_ERR_ARG), ("softmax_scale", 0.0, A.FA_ERR_ARG), ("softmax_scale", 1e-39, A.FA_ERR_ARG),
+    ("softmax_scale", math.nan, A.FA_ERR_ARG), ("softmax_scale", 2e38, A.FA_ERR_ARG),
     ("tokens", 2 ** 30, A.FA_ERR_UNSUPPORTED), ("cache.batch", 2 ** 23, A.FA_ERR_UNSUPPORTED),
     ("q", None, A.FA_ERR_NULL), ("q", PTR + 4, A.FA_ERR_STRIDE), ("q_stride[0]", 100, A.FA_ERR_STRIDE),
     ("lse", PTR + 2, A.FA_ERR_STRIDE),
@@ -162,10 +165,11 @@ BAD = {
     "fa_paged_fwd": CACHE_BAD + VALUES_BAD + QUERY_BAD + [("o", None, A.FA_ERR_NULL), ("o_stride[1]", 0, A.FA_ERR_STRIDE)],
     "fa_paged_key_weights": CACHE_BAD + QUERY_BAD + [
         ("lse", None, A.FA_ERR_NULL), ("key_weights", None, A.FA_ERR_NULL), ("key_weights", PTR + 2, A.FA_ERR_STRIDE),
-        ("w_stride[0]", 8, A.FA_ERR_STRIDE), ("w_stride[1]", 15, A.FA_ERR_STRIDE),
+        ("w_stride[0]", 8, A.FA_ERR_STRIDE), ("w_stride[1]", 15, A.FA_ERR_STRIDE), ("w_stride[0]", 16, A.FA_ERR_STRIDE),
         ("q_stride[0]", 2 ** 24 + 8, A.FA_ERR_UNSUPPORTED), ("q_stride[1]", 2 ** 28 + 8, A.FA_ERR_UNSUPPORTED)],
     "fa_paged_evict": CACHE_BAD + VALUES_BAD + WRITTEN_BAD + [
         ("key_weights", None, A.FA_ERR_NULL), ("w_stride[1]", 8, A.FA_ERR_STRIDE), ("keep", 0, A.FA_ERR_ARG),
+        ("keep", 2 ** 30 + 1, A.FA_ERR_UNSUPPORTED),
         ("recent", 21, A.FA_ERR_ARG), ("recent", -1, A.FA_ERR_ARG), ("max_kv", -1, A.FA_ERR_ARG),
         ("keep", 33, A.FA_ERR_SHAPE), ("new_pages", 0, A.FA_ERR_SHAPE), ("new_table", None, A.FA_ERR_NULL),
         ("new_lens", None, A.FA_ERR_NULL), ("kept", PTR + 2, A.FA_ERR_STRIDE), ("new_table_stride", 1, A.FA_ERR_STRIDE),
