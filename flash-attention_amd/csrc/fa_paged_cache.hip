@@ -184,20 +184,22 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3)))
     while (t < t1 && whole()) step(std::false_type{});
     while (t < t1) step(std::true_type{});
 
-    // Lane group g4 finishes key block g4.
+    // Lane group g4 finishes key block g4, so a lane the key of its number.  (The
+    // lane is asked for again: kept from the start, it was spilled.)
+    const int me = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
     float mine = 0.0f;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       float x = acc[kb];
       x += __shfl_xor(x, 16);
       x += __shfl_xor(x, 32);
-      if (g4 == kb) mine = x;
+      if (me >> 4 == kb) mine = x;
     }
-    const int key = wkey0 + 16 * g4 + l16;
+    const int key = wkey0 + me;
     if (a.ws != nullptr) {
       a.ws[((((int64_t)split * a.pt.batch + b) * a.kv_heads + kvh) * a.key_tiles + tile) * kWeightKeys +
-           64 * wave + lane] = mine;
-    } else if (key < s.len && ((there >> g4) & 1u)) {
+           64 * wave + me] = mine;
+    } else if (key < s.len && ((there >> (me >> 4)) & 1u)) {
       const int id = row[key >> a.pt.page_shift];
       float* w = a.w + (int64_t)id * a.w_sp + kvh * a.w_sh + (key & ((1 << a.pt.page_shift) - 1));
       *w = key >= s.first ? mine : *w + mine;
