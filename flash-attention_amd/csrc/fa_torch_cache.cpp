@@ -6,6 +6,7 @@
 #include <torch/extension.h>
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/HIPGraphsUtils.cuh>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -15,6 +16,7 @@
 
 #include <array>
 #include <cmath>
+#include <initializer_list>
 #include <optional>
 #include <utility>
 
@@ -26,6 +28,13 @@ using torch::Tensor;
 
 void check_status(fa_status s, const char* what) {
   TORCH_CHECK(s == FA_OK, what, " failed: ", fa_status_str(s), ": ", fa_last_error());
+}
+
+void check_no_grad(const char* name, std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : tensors)
+    TORCH_CHECK(!t->requires_grad(), name, " computes no gradients: call it under torch.no_grad() or detach "
+                "its inputs");
 }
 
 void check_half(const Tensor& t, const char* name, int64_t dims, const char* shape) {
@@ -117,9 +126,19 @@ float scale_of(std::optional<double> scale, int64_t d) {
   return static_cast<float>(scale.value_or(1.0 / std::sqrt((double)d)));
 }
 
+// Memory from the caching allocator without the dispatcher, which costs a
+// microsecond a tensor in calls whose kernels take five.
+Tensor new_tensor(c10::IntArrayRef sizes, c10::ScalarType type, const Tensor& ref) {
+  return at::detail::empty_cuda(sizes, type, ref.device(), c10::nullopt);
+}
+Tensor new_like(const Tensor& t) {
+  if (!t.is_non_overlapping_and_dense()) return torch::empty_like(t);
+  return at::detail::empty_strided_cuda(t.sizes(), t.strides(), t.scalar_type(), t.device());
+}
+
 Tensor workspace(uint64_t bytes, const Tensor& ref) {
   Tensor t;
-  if (bytes > 0) t = torch::empty({(int64_t)bytes}, ref.options().dtype(torch::kUInt8));
+  if (bytes > 0) t = new_tensor({(int64_t)bytes}, torch::kUInt8, ref);
   return t;
 }
 
@@ -144,23 +163,25 @@ const float* lse_ptr(const Tensor& lse, const Tensor& q) {
   return lse.data_ptr<float>();
 }
 
-pybind11::tuple paged_forward(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
+pybind11::object paged_forward(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
                               const Tensor& block_table, const Tensor& cu_seqlens,
                               const Tensor& seq_lens, std::optional<Tensor> out, int64_t max_q,
                               std::optional<int64_t> max_kv, bool causal,
                               std::optional<double> softmax_scale, bool return_lse) {
+  check_no_grad("paged_forward", {&q, &k_cache, &v_cache});
   fa_paged_fwd_params p{};
   p.cache = make_cache(k_cache, v_cache, block_table, cu_seqlens, seq_lens);
   check_packed(q, "q", k_cache);
   const c10::OptionalDeviceGuard guard(q.device());
   if (out) {
+    check_no_grad("paged_forward", {&*out});
     check_packed(*out, "out", k_cache, q.size(0), q.size(1));
     TORCH_CHECK(!out->is_alias_of(q) || out->data_ptr() != q.data_ptr() || out->numel() == 0,
                 "out must not be q");
   }
-  Tensor o = out ? *out : torch::empty(q.sizes(), q.options());
+  Tensor o = out ? *out : new_tensor(q.sizes(), q.scalar_type(), q);
   Tensor lse;
-  if (return_lse) lse = torch::empty({q.size(0), q.size(1)}, q.options().dtype(torch::kFloat32));
+  if (return_lse) lse = new_tensor({q.size(0), q.size(1)}, torch::kFloat32, q);
   p.q = q.data_ptr();
   p.o = o.data_ptr();
   p.lse = return_lse ? lse.data_ptr<float>() : nullptr;
@@ -177,13 +198,14 @@ pybind11::tuple paged_forward(const Tensor& q, const Tensor& k_cache, const Tens
   Tensor ws = workspace(bytes, q);
   check_status(fa_paged_fwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)), "paged_forward");
   if (return_lse) return pybind11::make_tuple(o, lse);
-  return pybind11::make_tuple(o);
+  return pybind11::cast(o);
 }
 
 void paged_key_weights(const Tensor& q, const Tensor& lse, const Tensor& k_cache,
                        const Tensor& block_table, const Tensor& cu_seqlens, const Tensor& seq_lens,
                        Tensor key_weights, int64_t max_q, std::optional<int64_t> max_kv, bool causal,
                        std::optional<double> softmax_scale) {
+  check_no_grad("paged_key_weights", {&q, &lse, &k_cache, &key_weights});
   fa_paged_weights_params p{};
   p.cache = make_cache(k_cache, std::nullopt, block_table, cu_seqlens, seq_lens);
   check_packed(q, "q", k_cache);
@@ -208,6 +230,7 @@ void paged_key_weights(const Tensor& q, const Tensor& lse, const Tensor& k_cache
 pybind11::tuple paged_evict(Tensor k_cache, Tensor v_cache, Tensor key_weights,
                             const Tensor& block_table, const Tensor& seq_lens, const Tensor& new_table,
                             int64_t keep, int64_t recent, std::optional<int64_t> max_kv) {
+  check_no_grad("paged_evict", {&k_cache, &v_cache, &key_weights});
   fa_paged_evict_params p{};
   p.cache = make_cache(k_cache, v_cache, block_table, std::nullopt, seq_lens);
   const c10::OptionalDeviceGuard guard(k_cache.device());
@@ -224,9 +247,8 @@ pybind11::tuple paged_evict(Tensor k_cache, Tensor v_cache, Tensor key_weights,
   int32_t none = 0;
   p.new_lens = p.kept = &none;
   check_status(fa_paged_evict_validate(&p), "paged_evict");
-  const auto opt = block_table.options();
-  Tensor new_lens = torch::empty({block_table.size(0)}, opt);
-  Tensor kept = torch::empty({block_table.size(0), k_cache.size(1), keep}, opt);
+  Tensor new_lens = new_tensor({block_table.size(0)}, torch::kInt32, k_cache);
+  Tensor kept = new_tensor({block_table.size(0), k_cache.size(1), keep}, torch::kInt32, k_cache);
   if (block_table.size(0) > 0) {
     p.new_lens = new_lens.data_ptr<int32_t>();
     p.kept = kept.data_ptr<int32_t>();
@@ -308,7 +330,7 @@ Pair norm_forward(const Tensor& q, const Tensor& k, const Tensor& qw, const Tens
                   bool interleaved) {
   fa_qk_norm_params p = norm_params(q, k, qw, kw, cos, sin, positions, eps, interleaved);
   const c10::OptionalDeviceGuard guard(q.device());
-  Tensor qo = torch::empty_like(q), ko = torch::empty_like(k);
+  Tensor qo = new_like(q), ko = new_like(k);
   p.q_out = qo.data_ptr();
   p.k_out = ko.data_ptr();
   set_strides(p.q_out_stride, qo, 3);
@@ -339,9 +361,8 @@ std::array<Tensor, 4> norm_backward(const Tensor& dq_out, const Tensor& dk_out, 
   }
   const c10::OptionalDeviceGuard guard(q.device());
   const Tensor gq = readable(dq_out), gk = readable(dk_out);
-  Tensor dq = torch::empty_like(q), dk = torch::empty_like(k);
-  const auto f32 = q.options().dtype(torch::kFloat32);
-  Tensor dqw = torch::empty({q.size(3)}, f32), dkw = torch::empty({q.size(3)}, f32);
+  Tensor dq = new_like(q), dk = new_like(k);
+  Tensor dqw = new_tensor({q.size(3)}, torch::kFloat32, q), dkw = new_tensor({q.size(3)}, torch::kFloat32, q);
   p.fwd.q_out = gq.data_ptr();
   p.fwd.k_out = gk.data_ptr();
   set_strides(p.fwd.q_out_stride, gq, 3);
@@ -449,14 +470,18 @@ Tensor paged_store(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
                    const Tensor& cos, const Tensor& sin, const Tensor& positions, Tensor k_cache,
                    Tensor v_cache, const Tensor& block_table, const Tensor& cu_seqlens,
                    const Tensor& seq_lens, std::optional<Tensor> out, double eps, bool interleaved) {
+  check_no_grad("paged_store", {&q, &k, &v, &qw, &kw, &k_cache, &v_cache});
   fa_paged_store_params p{};
   p.cache = make_cache(k_cache, v_cache, block_table, cu_seqlens, seq_lens);
   check_packed(q, "q", k_cache);
   check_packed(k, "k", k_cache, q.size(0), k_cache.size(1));
   check_packed(v, "v", k_cache, q.size(0), k_cache.size(1));
   const c10::OptionalDeviceGuard guard(q.device());
-  if (out) check_packed(*out, "out", k_cache, q.size(0), q.size(1));
-  Tensor o = out ? *out : torch::empty(q.sizes(), q.options());
+  if (out) {
+    check_no_grad("paged_store", {&*out});
+    check_packed(*out, "out", k_cache, q.size(0), q.size(1));
+  }
+  Tensor o = out ? *out : new_tensor(q.sizes(), q.scalar_type(), q);
   const NormTables t(q, qw, kw, cos, sin);
   p.q = q.data_ptr();
   p.k = k.data_ptr();

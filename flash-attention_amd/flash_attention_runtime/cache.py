@@ -33,12 +33,6 @@ import torch
 from . import _C as _EXT
 
 
-def _no_grad(name: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} computes no gradients: call it under torch.no_grad() or detach "
-                           "its inputs")
-
-
 def paged_forward(
     q: torch.Tensor,
     k_cache: torch.Tensor,
@@ -65,10 +59,8 @@ def paged_forward(
     Returns ``o`` like q, or ``(o, lse)`` with the natural-log logsumexp, fp32
     [T, H].  A row without visible keys has o = 0 and lse = -inf.
     """
-    _no_grad("paged_forward", q, k_cache, v_cache)
-    res = _EXT.paged_forward(q, k_cache, v_cache, block_table, cu_seqlens, seq_lens, out, max_q,
-                             max_kv, causal, softmax_scale, return_lse)
-    return res if return_lse else res[0]
+    return _EXT.paged_forward(q, k_cache, v_cache, block_table, cu_seqlens, seq_lens, out, max_q,
+                              max_kv, causal, softmax_scale, return_lse)
 
 
 def paged_key_weights(
@@ -92,7 +84,6 @@ def paged_key_weights(
     returned by ``paged_forward``.  The new tokens' own keys are set, not added
     to, so a reused page needs no clearing.  A page must belong to one sequence of
     the call only (sequences that share a prefix need weights of their own).  Returns ``key_weights``."""
-    _no_grad("paged_key_weights", q, lse, k_cache, key_weights)
     _EXT.paged_key_weights(q, lse, k_cache, block_table, cu_seqlens, seq_lens, key_weights, max_q,
                            max_kv, causal, softmax_scale)
     return key_weights
@@ -121,7 +112,6 @@ def paged_evict(
     [B, kv_heads, keep] with the former index of the key now at each place (-1
     behind the last).  A sequence with an absent page is not copied (length 0).
     """
-    _no_grad("paged_evict", k_cache, v_cache, key_weights)
     return _EXT.paged_evict(k_cache, v_cache, key_weights, block_table, seq_lens, new_table, keep,
                             recent, max_kv)
 
@@ -152,7 +142,6 @@ def paged_store(
     must belong to one sequence only; tokens without a place (more tokens than
     keys, absent pages) are not stored.  Returns q's result (``out`` if given,
     which may be q)."""
-    _no_grad("paged_store", q, k, v, q_weight, k_weight, k_cache, v_cache)
     return _EXT.paged_store(q, k, v, q_weight, k_weight, cos, sin, positions, k_cache, v_cache,
                             block_table, cu_seqlens, seq_lens, out, eps, interleaved)
 

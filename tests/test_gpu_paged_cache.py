@@ -396,6 +396,7 @@ def test_refusals(fa):
             (dict(out=q[:4]), "as many tokens"), (dict(out=torch.zeros_like(q)[:, :1].expand(5, 4, 64)), "rows overlap"),
             (dict(q=torch.zeros(5, 4, 65, device=DEV).half()[..., 1:]), "multiple of 8"),
             (dict(q=q.clone().requires_grad_()), "no gradients"),
+            (dict(out=torch.zeros_like(q).requires_grad_()), "no gradients"),
             (dict(cu_seqlens=cu[:2]), "one entry more"),
         ],
         "paged_key_weights": [
@@ -407,15 +408,18 @@ def test_refusals(fa):
             (dict(keep=0), "keep"), (dict(recent=17), "recent"), (dict(recent=-1), "recent"),
             (dict(keep=40), "hold fewer"), (dict(new_table=table), "pages of their own"),
             (dict(new_table=nt[:1]), "as many rows"), (dict(keep=2 ** 40), "32 bits"),
-            (dict(k_cache=k[:, :1].expand_as(k)), "rows overlap"),
+            (dict(k_cache=k[:, :1].expand_as(k)), "rows overlap"), (dict(keep=2 ** 30 + 1), "2\\^30"),
         ],
         "paged_store": [
             (dict(k=q), "number of heads"), (dict(v=kv[:4]), "as many tokens"),
             (dict(positions=pos.long()), "int32"), (dict(positions=pos[:4]), "one entry per token"),
             (dict(q_weight=one[:32]), "head_dim"), (dict(k_cache=k[:1].expand_as(k)), "rows overlap"),
-            (dict(cos=cos.half()), "float32"),
+            (dict(cos=cos.half()), "float32"), (dict(q_weight=one.clone().requires_grad_()), "no gradients"),
+            (dict(out=torch.zeros_like(q).requires_grad_()), "no gradients"),
         ],
     }
+    for name in ("paged_forward", "paged_key_weights", "paged_evict", "paged_store"):
+        more[name].append((dict(k_cache=k.clone().requires_grad_()), "no gradients"))
     for name, changes in more.items():
         for change, text in changes:
             with pytest.raises(RuntimeError, match=text):
