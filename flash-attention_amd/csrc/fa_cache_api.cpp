@@ -15,31 +15,54 @@
 
 namespace fa {
 
+// Whether the chunk kernel may cut the tiles of its last round in pieces
+// (LastRound, of which this is the host's copy), for every number of tiles that
+// sequences of `rows` rows in all can have.  Where it may not, the call is
+// spared the launch that joins them.
+static bool cuts_tiles(int64_t rows, int batch, int conc, int max_pieces, float piece_cost) {
+  if (batch > 8) return true;
+  const int64_t least = (rows + kChunkRows - 1) / kChunkRows;
+  const int64_t most = std::max(least, (rows - batch) / kChunkRows + batch);
+  for (int64_t n = least; n <= most; ++n) {
+    const int64_t rest = n % conc;
+    for (int q = 2; rest > 0 && q <= 64 && rest * q <= max_pieces; ++q)
+      if ((float)((rest * q + conc - 1) / conc) * (1.0f / (float)q + piece_cost) < 1.0f + piece_cost)
+        return true;
+  }
+  return false;
+}
+
 PagedPlan plan_paged(int tokens, int batch, int kv_heads, int group, int head_dim, int max_q,
-                     int max_kv, int compute_units) {
+                     int max_kv, bool causal, int compute_units) {
   PagedPlan p = {};
   p.compute_units = compute_units;
+  PagedGrid& g = p.grid;
   const int64_t most = (int64_t)std::min(max_q, tokens) * group;  // rows of a sequence
   const int64_t keys = std::max(max_kv, 1);
-  // So few keys that the chunk kernel serves every sequence whole: the
-  // launches of a decode kernel and of the joins, about 4.5 us each, cost more
-  // than the tiles that its workgroups would share.
-  constexpr int64_t kShortKeys = 1024;
   if (most > kDecodeRows) {
-    PagedGrid& g = p.chunk;
+    // All sequences of the call, those of few rows too: one launch after the
+    // other for the two kinds was 10 to 30 % slower in every mix (us, two
+    // launches and one: 63 sequences of one token and one of 64, of up to 8000
+    // keys, 32 heads on 8, D = 128: 341, 297; 60 and 4 of 512: 493, 387; 16 of
+    // up to 64 tokens over 3000 keys: 74, 55).
     g.rows = kChunkRows;
-    g.slots = (int)((int64_t)tokens * group / kChunkRows + batch);
+    const int64_t rows = (int64_t)tokens * group;
+    g.slots = (int)(rows / kChunkRows + batch);
     // Two workgroups per CU; the tiles of the last round go in pieces of 512
-    // keys or more, two rounds of them at most.
+    // keys or more, two rounds of them at most.  No pieces, and no launch that
+    // joins them (5 us), for up to 1024 keys; where LastRound would cut none; and
+    // where causal tiles get so much shorter that those of a last round are
+    // short (prompts of 2048, 2800 and 4096 tokens, 32 heads on 8, D = 128: 50, 74
+    // and 130 us without, 55, 82 and 133 with; but fewer tiles than workgroups
+    // hold the longest ones: 2048 tokens, 8 heads on 2: 43 and 34).
     g.conc = std::max(1, 2 * compute_units / kv_heads);
-    g.pieces = keys <= kShortKeys ? 0 : (int)std::min<int64_t>(2 * (int64_t)g.conc, 64 * (int64_t)g.slots);
+    g.pieces = (int)std::min<int64_t>(2 * (int64_t)g.conc, 64 * (int64_t)g.slots);
+    const bool falling = causal && 4 * (int64_t)max_q >= keys;
+    if (keys <= 1024 || (falling && rows / kChunkRows >= g.conc) ||
+        !cuts_tiles(rows, batch, g.conc, g.pieces, piece_cost(keys)))
+      g.pieces = 0;
     g.ws_rows = (uint64_t)g.pieces * kv_heads * g.rows;
-  }
-  // No sequence can have so few tokens as the decode kernel serves where the
-  // others, at max_q, leave it more.
-  const int64_t least = tokens - (int64_t)(batch - 1) * max_q;
-  if (most <= kDecodeRows || (batch > 1 && keys > kShortKeys && least * group <= kDecodeRows)) {
-    PagedGrid& g = p.decode;
+  } else {
     g.rows = most <= 16 ? 16 : 32;
     g.slots = batch;
     // One workgroup per CU, of 128 to 8192 keys in whole 64-key tiles (the
@@ -59,17 +82,22 @@ PagedPlan plan_paged(int tokens, int batch, int kv_heads, int group, int head_di
     g.splits = (int)((keys + g.chunk - 1) / g.chunk);
     g.ws_rows = g.splits > 1 ? (uint64_t)base * g.splits * g.rows : 0;
   }
-  p.workspace_bytes = (p.chunk.ws_rows + p.decode.ws_rows) * (head_dim + 2) * 4;
+  p.workspace_bytes = g.ws_rows * (head_dim + 2) * 4;
   return p;
 }
 
-WeightsPlan plan_weights(int tokens, int batch, int kv_heads, int group, int max_q, int max_kv,
-                         int compute_units) {
+WeightsPlan plan_weights(int tokens, int batch, int kv_heads, int group, int head_dim, int max_q,
+                         int max_kv, int compute_units) {
   WeightsPlan p = {};
   const int64_t most = (int64_t)std::min(max_q, tokens) * group;  // rows of a sequence
-  // (as plan_paged: the launch of the other kernel is spared where it can be)
+  // Beside sequences of many rows, those of few get a kernel of their own where
+  // the cache is large (K of more than 384 MiB; us, two kernels and one: 63
+  // sequences of one token and one of 64, of up to 8000 keys, D = 128: 8 kv heads,
+  // 1 GB, 178 and 212; 2 kv heads, 0.26 GB, 63 and 53), and where there may be any:
+  // no sequence can have so few tokens if the others, at max_q, leave it more.
   const int64_t least = tokens - (int64_t)(batch - 1) * max_q;
-  if (most <= kDecodeRows || (batch > 1 && max_kv > 1024 && least * group <= kDecodeRows)) {
+  const int64_t k_bytes = (int64_t)batch * kv_heads * max_kv * head_dim * 2;
+  if (most <= kDecodeRows || (batch > 1 && k_bytes > (int64_t(384) << 20) && least * group <= kDecodeRows)) {
     p.few_rows = most <= 16 ? 16 : kDecodeRows;
     // Four workgroups per CU, which run at once, of 256 to 2048 keys in whole
     // 64-key tiles.
@@ -490,7 +518,7 @@ fa_status plan_of(const fa_paged_fwd_params& p, PagedPlan* plan) {
   int cus = 0;
   FA_TRY(current_compute_units(&cus));
   *plan = plan_paged(p.tokens, p.cache.batch, p.cache.kv_heads, p.heads / p.cache.kv_heads,
-                     p.cache.head_dim, p.max_q, limit_kv(p.cache, p.max_kv), cus);
+                     p.cache.head_dim, p.max_q, limit_kv(p.cache, p.max_kv), p.causal != 0, cus);
   return FA_OK;
 }
 
@@ -503,8 +531,8 @@ uint64_t weights_bytes(const fa_paged_weights_params& p, int splits) {
 fa_status plan_of(const fa_paged_weights_params& p, WeightsPlan* plan) {
   int cus = 0;
   FA_TRY(current_compute_units(&cus));
-  *plan = plan_weights(p.tokens, p.cache.batch, p.cache.kv_heads, p.heads / p.cache.kv_heads, p.max_q,
-                       limit_kv(p.cache, p.max_kv), cus);
+  *plan = plan_weights(p.tokens, p.cache.batch, p.cache.kv_heads, p.heads / p.cache.kv_heads,
+                       p.cache.head_dim, p.max_q, limit_kv(p.cache, p.max_kv), cus);
   return FA_OK;
 }
 

@@ -37,11 +37,9 @@ struct PagedFwdArgs {
   int32_t heads, kv_heads, group;
   int32_t max_q, causal;
   float scale_log2;                // softmax scale * log2(e)
-  // Which sequences a launch serves, by their rows, and its grid.  Decode
-  // kernel: slots (sequences) x kv heads x splits of `chunk` keys.  Chunk
-  // kernel: at most `slots` row tiles per kv head, and up to 2 conc pieces of
-  // the last ones (LastRound).
-  int32_t min_rows, max_rows;
+  // Grids.  Decode kernel: slots (sequences) x kv heads x splits of `chunk` keys.
+  // Chunk kernel: at most `slots` row tiles per kv head, and up to 2 conc pieces
+  // of the last ones (LastRound).
   int32_t slots, splits, chunk;
   int32_t conc, max_pieces;        // workgroups of a kv head that run at once, its most pieces
   float piece_cost;
@@ -49,31 +47,35 @@ struct PagedFwdArgs {
   int32_t join, merge_rows, most_rows;
   FastDiv by_group, by_kvh, by_splits, by_conc;
   // Order of the chunk kernel's grid (set_order).
-  int32_t places, per_xcd, unit_group, xcds;
+  int32_t places, per_xcd, unit_group, xcds, xcd_cus;
   FastDiv by_group_places, by_unit_group;
   float* ws_o;                     // [slot or piece][BM][D] partial o, fp32, of each kv head
   float* ws_e;                     // the same rows: (log2 of the rounded P's sum, of the plain one's)
 };
 
-// How a call is launched (plan_paged): sequences of at most kDecodeRows rows
-// on the decode kernel, the others on the chunk kernel.
+// Cost of a piece of a tile beside its keys (LastRound): the time of 768 keys,
+// in units of a tile that sees max_kv of them.
+inline float piece_cost(int64_t max_kv) { return 768.0f / (float)(max_kv > 768 ? max_kv : 768); }
+
+// How a call is launched (plan_paged): on the decode kernel where no sequence
+// has more than kDecodeRows rows, else on the chunk kernel.
 constexpr int kDecodeRows = 32;
-constexpr int kChunkRows = 128;  // rows of a chunk kernel's workgroup
+constexpr int kChunkRows = 128;
 
 struct PagedGrid {
-  int32_t rows;  // rows of a slot (BM); 0: not launched
+  int32_t rows;  // rows of a slot (BM): kChunkRows, or 16 or 32
   int32_t slots;
   int32_t splits, chunk;  // decode
   int32_t conc, pieces;   // chunk: at once per kv head, most pieces per kv head
   uint64_t ws_rows;       // rows of partials
 };
 struct PagedPlan {
-  PagedGrid decode, chunk;
+  PagedGrid grid;
   int32_t compute_units;
   uint64_t workspace_bytes;
 };
 PagedPlan plan_paged(int tokens, int batch, int kv_heads, int group, int head_dim, int max_q,
-                     int max_kv, int compute_units);
+                     int max_kv, bool causal, int compute_units);
 
 hipError_t launch_paged_fwd(const PagedFwdArgs& args, const PagedPlan& plan, int head_dim, bool bf16,
                             void* workspace, hipStream_t stream);
@@ -108,8 +110,8 @@ struct WeightsPlan {
   int32_t splits;    // row splits of the others (1: no workspace); 0: none
   int32_t pairs;     // 1: key tiles in pairs
 };
-WeightsPlan plan_weights(int tokens, int batch, int kv_heads, int group, int max_q, int max_kv,
-                         int compute_units);
+WeightsPlan plan_weights(int tokens, int batch, int kv_heads, int group, int head_dim, int max_q,
+                         int max_kv, int compute_units);
 hipError_t launch_paged_weights(const PagedWeightsArgs& args, const WeightsPlan& plan, int head_dim,
                                 bool bf16, hipStream_t stream);
 

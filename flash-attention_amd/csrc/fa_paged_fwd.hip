@@ -15,13 +15,14 @@
 //    fa_fwd16_kernel.  Bound by the matrix cores and the exponentials.
 //    4096 tokens over 16384 keys take 903 us, 1218 TFLOP/s (bf16, D = 128,
 //    8 kv heads; a large matrix product reaches 1200 on the card).
-//  * fa_paged_decode_kernel: 16 or 32 rows (a few tokens), the keys of a chunk
+//  * fa_paged_decode_kernel: at most 16 or 32 rows (a few tokens), the keys of a chunk
 //    dealt to two or four waves in tiles of 32, each wave with an LDS ring of its
 //    own and no barrier before the end.  Bound by reading the cache: 5.4 TB/s at
 //    32 sequences of up to 8192 keys, 8 kv heads, D = 128 (144 us), where a
 //    large copy moves 5.0.
-// Keys are split over workgroups where rows are few (plan_paged, LastRound);
-// fa_paged_merge_kernel joins their normalised partials.
+// One of them serves a call (plan_paged).  Keys are split over workgroups where
+// rows are few (plan_paged, LastRound); fa_paged_merge_kernel joins their
+// normalised partials.
 //
 // Pages are read through their 16-key groups (a page holds whole groups), whose
 // page ids a wave holds 64 at a time, one a lane (PageIds).
@@ -354,7 +355,7 @@ __global__ void __launch_bounds__(64 * NW) fa_paged_decode_kernel(const PagedFwd
   ids.start(a.pt, a.pt.table + b * a.pt.table_stride, split * a.chunk);
   const Seq s = load_seq(a.pt, b, a.max_q);
   const int n_rows = s.nq * a.group;
-  if (n_rows <= 0 || n_rows > a.max_rows) return;
+  if (n_rows <= 0) return;
   const int kv_end = max(0, last_key(a, s, s.nq - 1) + 1);
   const int n_act = max(1, (kv_end + a.chunk - 1) / a.chunk);
   if (split >= n_act) return;
@@ -520,8 +521,14 @@ __global__ void __launch_bounds__(64 * NW) fa_paged_decode_kernel(const PagedFwd
 //  * a multiple of 8 heads: whole heads per XCD, up to four of them interleaved;
 //  * 1, 2 or 4: 8 / heads XCDs take turns with a head's places;
 //  * else all heads interleaved over all XCDs.
-__device__ __forceinline__ bool head_and_place(const PagedFwdArgs& a, int& kvh, int& place) {
-  const int xcd = blockIdx.x % kNumXcd, i = blockIdx.x / kNumXcd;
+// Workgroups k and k + 32 of an XCD, with its 32 CUs, share a CU.  `turn`, where
+// there are so many: the first 32 run backwards, so that the longest of them has
+// the shortest neighbour (us without and with: prompts of 4096 and 8192 tokens, 8
+// heads on 2, D = 128: 62 and 60, 180 and 167; 2048 tokens, 32 on 8: 57 and 55).
+__device__ __forceinline__ bool head_and_place(const PagedFwdArgs& a, bool turn, int& kvh, int& place) {
+  const int xcd = blockIdx.x % kNumXcd;
+  int i = blockIdx.x / kNumXcd;
+  if (turn && i < a.xcd_cus) i = a.xcd_cus - 1 - i;
   if (a.per_xcd > 0) {
     const int grp = fast_div(i, a.by_group_places), w = i - grp * a.unit_group * a.places;
     place = fast_div(w, a.by_unit_group);
@@ -530,8 +537,8 @@ __device__ __forceinline__ bool head_and_place(const PagedFwdArgs& a, int& kvh, 
     kvh = xcd / a.xcds;
     place = i * a.xcds + xcd % a.xcds;
   } else {
-    place = fast_div(blockIdx.x, a.by_kvh);
-    kvh = blockIdx.x - place * a.kv_heads;
+    place = fast_div(i * kNumXcd + xcd, a.by_kvh);
+    kvh = i * kNumXcd + xcd - place * a.kv_heads;
   }
   return place < a.places;
 }
@@ -549,24 +556,28 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (threadIdx.x == 0) again = 0;  // ordered by the first barrier
   int kvh, place, b, tile0;
-  if (!head_and_place(a, kvh, place)) return;
   TileList<BM> list;
   list.init(a);
   LastRound end;
   end.init(a, list.count);
+  const int cut = a.ws_o != nullptr ? end.pieces : 1;
+  // (lists of more than 64 sequences are not by length)
+  const bool turn = a.pt.batch <= 64 && (end.whole + end.rest * cut) * a.kv_heads > kNumXcd * a.xcd_cus;
+  if (!head_and_place(a, turn, kvh, place)) return;
   int pieces = 1, piece = 0, nth = place;
   if (place >= end.whole) {
-    pieces = a.ws_o != nullptr ? end.pieces : 1;
+    pieces = cut;
+    // (First pieces of all tiles, second ones, ...: short tiles have no last ones,
+    // and gaps leave CUs idle.  128 tokens over 2000 keys, 32 heads on 8: 31 -> 27 us.)
     const int i = place - end.whole;
-    nth = i / pieces;
-    piece = i - nth * pieces;
-    if (nth >= end.rest) return;
-    nth += end.whole;
+    if (i >= end.rest * pieces) return;
+    piece = i / end.rest;
+    nth = i - piece * end.rest + end.whole;
   }
   Seq s;
   if (!list.find(a, nth, b, tile0, s)) return;
   const int n_rows = s.nq * a.group, row0 = tile0 * BM;
-  if (n_rows < a.min_rows || row0 >= n_rows) return;
+  if (row0 >= n_rows) return;
   const int last_row = min(row0 + BM, n_rows) - 1;
   const int kv_end = max(0, last_key(a, s, fast_div(last_row, a.by_group)) + 1);
   int n_act = 1, c0 = 0, c1 = kv_end;
@@ -683,7 +694,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     lu[rb] = W::red_sum(w.lu[rb]);
   }
   if (n_act > 1) {  // partials: o normalised, sums as log2
-    const int64_t wr0 = ((int64_t)kvh * a.max_pieces + place - end.whole) * BM + 32 * wave;
+    const int64_t wr0 = ((int64_t)kvh * a.max_pieces + (nth - end.whole) * pieces + piece) * BM + 32 * wave;
 #pragma unroll
     for (int rb = 0; rb < 2; ++rb) {
       const int r = 16 * rb + l16;
@@ -750,7 +761,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 // meet in LDS: one group per row left 128 chunks to a loop of dependent loads
 // (125 us against 98 for the attention itself at one sequence of 131072 keys).
 template <int D, bool BF16, int BM>
-__device__ __forceinline__ void merge_rows(const PagedFwdArgs& a, int block) {
+__global__ void __launch_bounds__(256) fa_paged_merge_kernel(const PagedFwdArgs a) {
+  const int block = blockIdx.x;
   constexpr int TPR = D / 4, GROUPS = 256 / TPR;
   __shared__ f32x4 part_o[GROUPS][TPR];
   __shared__ float part_e[GROUPS][4];  // top, sum of weights; the same of the plain sums
@@ -778,7 +790,7 @@ __device__ __forceinline__ void merge_rows(const PagedFwdArgs& a, int block) {
     n_act = 0;
   }
   const int n_rows = s.nq * a.group, row0 = tile0 * BM;
-  if (n_rows < a.min_rows || n_rows > a.max_rows || row0 >= n_rows) return;
+  if (row0 >= n_rows) return;
   const int last_row = min(row0 + BM, n_rows) - 1;
   const int kv_end = max(0, last_key(a, s, fast_div(last_row, a.by_group)) + 1);
   if constexpr (kTiles)
@@ -853,35 +865,21 @@ __device__ __forceinline__ void merge_rows(const PagedFwdArgs& a, int block) {
   }
 }
 
-// The joins of both kernels of a call in one launch.
-struct MergeArgs {
-  PagedFwdArgs chunk, decode;
-  int32_t chunk_blocks, decode_rows;
-};
-template <int D, bool BF16>
-__global__ void __launch_bounds__(256) fa_paged_merge_kernel(const MergeArgs m) {
-  if ((int)blockIdx.x < m.chunk_blocks)
-    merge_rows<D, BF16, kChunkRows>(m.chunk, blockIdx.x);
-  else if (m.decode_rows == 16)
-    merge_rows<D, BF16, 16>(m.decode, blockIdx.x - m.chunk_blocks);
-  else
-    merge_rows<D, BF16, 32>(m.decode, blockIdx.x - m.chunk_blocks);
-}
-
-template <class F, class A>
-hipError_t launch(F* fn, int64_t grid, const A& args, hipStream_t stream, int threads = 256) {
+template <class F>
+hipError_t launch(F* fn, int64_t grid, const PagedFwdArgs& args, hipStream_t stream, int threads = 256) {
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
-  void* kargs[] = {const_cast<A*>(&args)};
+  void* kargs[] = {const_cast<PagedFwdArgs*>(&args)};
   return hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)grid), dim3(threads), kargs,
                          0, stream);
 }
 
 // The chunk kernel's grid order (head_and_place) and its workgroups.
-int64_t set_order(PagedFwdArgs& a) {
+int64_t set_order(PagedFwdArgs& a, const PagedPlan& plan) {
   a.per_xcd = a.kv_heads % kNumXcd == 0 ? a.kv_heads / kNumXcd : 0;
   a.unit_group = 1;
   for (int g = 2; g <= 4; ++g)
     if (a.per_xcd % g == 0) a.unit_group = g;
+  a.xcd_cus = plan.compute_units / kNumXcd;
   a.xcds = a.per_xcd == 0 && kNumXcd % a.kv_heads == 0 ? kNumXcd / a.kv_heads : 0;
   a.by_group_places = make_fast_div((uint32_t)(a.unit_group * a.places));
   a.by_unit_group = make_fast_div((uint32_t)a.unit_group);
@@ -891,80 +889,52 @@ int64_t set_order(PagedFwdArgs& a) {
 
 template <int D, bool BF16>
 hipError_t launch_all(const PagedFwdArgs& base, const PagedPlan& plan, void* ws, hipStream_t stream) {
-  char* at = static_cast<char*>(ws);
-  auto partials = [&](PagedFwdArgs& a, const PagedGrid& g) {
-    a.ws_o = g.ws_rows ? reinterpret_cast<float*>(at) : nullptr;
-    a.ws_e = reinterpret_cast<float*>(at + g.ws_rows * D * 4);
-    at += g.ws_rows * (D + 2) * 4;
-  };
+  const PagedGrid& g = plan.grid;
+  PagedFwdArgs a = base;
+  a.slots = g.slots;
+  a.ws_o = g.ws_rows ? static_cast<float*>(ws) : nullptr;
+  a.ws_e = g.ws_rows ? a.ws_o + g.ws_rows * D : nullptr;
+  a.join = 1;
   constexpr int GROUPS = 256 / (D / 4);  // lane groups of a merge workgroup
-  MergeArgs merge = {};
-  int64_t chunk_blocks = 0, decode_blocks = 0;
-  if (const PagedGrid& g = plan.chunk; g.rows != 0) {
-    PagedFwdArgs a = base;
-    // One sequence with too many rows for the decode kernel: this one serves
-    // whatever the sequence holds.
-    a.min_rows = plan.decode.rows == 0 ? 1 : plan.decode.rows + 1;
-    a.max_rows = 0x7fffffff;
-    a.slots = g.slots;
+  if (g.rows == kChunkRows) {
     a.conc = g.conc;
     a.max_pieces = g.pieces;
     a.by_conc = make_fast_div((uint32_t)g.conc);
-    a.piece_cost = 768.0f / (float)std::max(768, a.pt.max_kv);
+    a.piece_cost = piece_cost(a.pt.max_kv);
     a.places = g.slots + g.pieces;
-    partials(a, g);
-    hipError_t e = launch(&fa_paged_chunk_kernel<D, BF16>, set_order(a), a, stream);
-    if (e != hipSuccess) return e;
-    if (g.pieces > 0) {
-      a.join = 1;
-      const int64_t tiles = (int64_t)std::min(g.conc - 1, g.slots) * a.kv_heads;
-      // Rows of a workgroup: few, unless that makes thousands of workgroups,
-      // most of which find no tile.
-      a.merge_rows = tiles * (kChunkRows / GROUPS) <= 2048 ? GROUPS : 32;
-      chunk_blocks = tiles * (kChunkRows / a.merge_rows);
-      merge.chunk = a;
-    }
+    const hipError_t e = launch(&fa_paged_chunk_kernel<D, BF16>, set_order(a, plan), a, stream);
+    if (e != hipSuccess || g.pieces == 0) return e;
+    const int64_t tiles = (int64_t)std::min(g.conc - 1, g.slots) * a.kv_heads;
+    // Rows of a workgroup: few, unless that makes thousands of workgroups,
+    // most of which find no tile.
+    a.merge_rows = tiles * (kChunkRows / GROUPS) <= 2048 ? GROUPS : 32;
+    return launch(&fa_paged_merge_kernel<D, BF16, kChunkRows>, tiles * (kChunkRows / a.merge_rows), a,
+                  stream);
   }
-  if (const PagedGrid& g = plan.decode; g.rows != 0) {
-    PagedFwdArgs a = base;
-    a.min_rows = 1;
-    a.max_rows = g.rows;
-    a.slots = g.slots;
-    a.splits = g.splits;
-    a.chunk = g.chunk;
-    partials(a, g);
-    const int64_t sk = (int64_t)g.slots * a.kv_heads;
-    a.by_splits = make_fast_div((uint32_t)sk);
-    // Two waves a workgroup where two workgroups per CU are there to take
-    // turns at starting and ending (us, 4 waves -> 2: 32 sequences of 4096 keys,
-    // 8 kv heads, D = 128: 105 -> 102; 64 of 1000: 55 -> 50); with fewer, four
-    // waves read sooner (4 sequences of 2000: 17 -> 14).
-    auto decode = [&](auto rb_c) {
-      constexpr int RB = decltype(rb_c)::value;
-      return sk * g.splits >= 2 * plan.compute_units
-                 ? launch(&fa_paged_decode_kernel<D, BF16, RB, 2>, sk * g.splits, a, stream, 128)
-                 : launch(&fa_paged_decode_kernel<D, BF16, RB, 4>, sk * g.splits, a, stream, 256);
-    };
-    hipError_t e = g.rows == 16 ? decode(std::integral_constant<int, 1>{})
-                                : decode(std::integral_constant<int, 2>{});
-    if (e != hipSuccess) return e;
-    if (g.splits > 1) {
-      // As many lane groups a row as it has chunks, a power of two.
-      a.join = 1;
-      while (a.join < g.splits && a.join < GROUPS) a.join *= 2;
-      const int rpb = GROUPS / a.join;
-      a.most_rows = std::min<int64_t>(g.rows, (int64_t)a.max_q * a.group);
-      decode_blocks = sk * ((a.most_rows + rpb - 1) / rpb);
-      merge.decode = a;
-      merge.decode_rows = g.rows;
-    }
-  }
-  if (chunk_blocks + decode_blocks > 0) {
-    if (chunk_blocks > 0x7fffffff) return hipErrorInvalidValue;
-    merge.chunk_blocks = (int32_t)chunk_blocks;
-    return launch(&fa_paged_merge_kernel<D, BF16>, chunk_blocks + decode_blocks, merge, stream);
-  }
-  return hipSuccess;
+  a.splits = g.splits;
+  a.chunk = g.chunk;
+  const int64_t sk = (int64_t)g.slots * a.kv_heads;
+  a.by_splits = make_fast_div((uint32_t)sk);
+  // Two waves a workgroup where two workgroups per CU are there to take
+  // turns at starting and ending (us, 4 waves -> 2: 32 sequences of 4096 keys,
+  // 8 kv heads, D = 128: 105 -> 102; 64 of 1000: 55 -> 50); with fewer, four
+  // waves read sooner (4 sequences of 2000: 17 -> 14).
+  auto decode = [&](auto rb_c) {
+    constexpr int RB = decltype(rb_c)::value;
+    return sk * g.splits >= 2 * plan.compute_units
+               ? launch(&fa_paged_decode_kernel<D, BF16, RB, 2>, sk * g.splits, a, stream, 128)
+               : launch(&fa_paged_decode_kernel<D, BF16, RB, 4>, sk * g.splits, a, stream, 256);
+  };
+  const hipError_t e = g.rows == 16 ? decode(std::integral_constant<int, 1>{})
+                                    : decode(std::integral_constant<int, 2>{});
+  if (e != hipSuccess || g.splits == 1) return e;
+  // As many lane groups a row as it has chunks, a power of two.
+  while (a.join < g.splits && a.join < GROUPS) a.join *= 2;
+  const int rpb = GROUPS / a.join;
+  a.most_rows = std::min<int64_t>(g.rows, (int64_t)a.max_q * a.group);
+  const int64_t blocks = sk * ((a.most_rows + rpb - 1) / rpb);
+  return g.rows == 16 ? launch(&fa_paged_merge_kernel<D, BF16, 16>, blocks, a, stream)
+                      : launch(&fa_paged_merge_kernel<D, BF16, 32>, blocks, a, stream);
 }
 
 }  // namespace

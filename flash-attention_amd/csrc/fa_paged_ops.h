@@ -155,7 +155,7 @@ struct TileList {
       c0 = min(max(a.pt.cu[lane], 0), a.pt.tokens);
       c1 = min(max(a.pt.cu[lane + 1], c0), a.pt.tokens);
       const int rows = min(c1 - c0, a.max_q) * a.group;
-      tiles = rows >= a.min_rows ? (rows + BM - 1) / BM : 0;
+      tiles = (rows + BM - 1) / BM;
       len = min(max(a.pt.lens[lane], 0), a.pt.max_kv);
     }
     start = count = 0;
