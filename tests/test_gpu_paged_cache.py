@@ -120,6 +120,26 @@ def test_key_weights(fa, name, dtype):
     R.check("weights", wd, want, tol)
 
 
+@pytest.mark.parametrize("name", ["mixed", "mixed-long", "mixed-long-d128", "group-40-chunk-rows", "empty-sequences"])
+def test_key_weights_of_a_cache_that_may_be_large(fa, name):
+    """Limits of more than 384 MiB of K, by a wide table: sequences of few rows
+    get a kernel of their own beside the others."""
+    print(f"case weights large limits {name}", flush=True)
+    lens, new, H, KH, D, page = SHAPES[name]
+    keys = 384 * 2 ** 20 // (len(lens) * KH * D * 2) + 1
+    c = Cache(lens, page, KH, D, torch.float16, 525, wide=-(-keys // page))
+    T = sum(new)
+    q = torch.randn(T, H, D, generator=torch.Generator().manual_seed(26)).half()
+    lse = 6 + torch.randn(T, H, generator=torch.Generator().manual_seed(27))
+    k, _, table = c.dev()
+    cu = cu_of(new)
+    w = weights_of(c, 28)
+    wd = fa.paged_key_weights(q.to(DEV), lse.to(DEV), k, table, cu.to(DEV), c.lens.to(DEV), w.to(DEV),
+                              max_q=max(new))
+    want, tol = R.key_weights(q, lse, c.k, c.table, cu, c.lens, w, scale=D ** -0.5)
+    R.check("weights", wd, want, tol)
+
+
 @pytest.mark.parametrize("name", ["ragged-decode", "mixed", "few-tokens"])
 def test_key_weights_with_limits_no_mask_and_absent_pages(fa, name):
     print(f"case weights limits {name}", flush=True)

@@ -92,6 +92,8 @@ SHAPES = {
                        2, 1, 64, 16),
     "many-long-sequences": ([1100 + i for i in range(66)], [(i * 7) % 36 for i in range(66)], 2, 1, 64, 64),
     "last-round-of-one-head": ([1500, 1400], [200, 130], 2, 1, 128, 32),
+    "mixed-long": ([2500, 3000, 1100, 40, 2049], [1, 90, 2, 3, 1], 8, 2, 64, 64),
+    "mixed-long-d128": ([1700, 2300, 1], [130, 1, 1], 4, 2, 128, 16),
     "split-decode": ([5000], [1], 4, 2, 128, 64),
     "split-chunk": ([3000], [40], 1, 1, 64, 16),
 }
