@@ -107,24 +107,28 @@ WeightsPlan plan_weights(int tokens, int batch, int kv_heads, int group, int hea
     p.few_keys = (int)std::max<int64_t>(256, std::min<int64_t>(keys, kWeightChunk));
   }
   if (most > kDecodeRows) {
-    // Three workgroups per CU run at once; row splits fill them, of 128 rows or
+    // Three workgroups per CU run at once; row splits fill them, of a row tile or
     // more.  Where new tokens are many of the keys, causal masks leave the first
     // key tile all rows and the last one few: then tiles go in pairs of equal
     // work if that is long (4 prompts of 4096 tokens, 4 kv heads: 251 -> 151
-    // us), and are cut finer if it is short (28 prompts of up to 1613, one kv
-    // head: 45 -> 33 us; a pair starts twice, 46 us).
+    // us), and are cut finer if it is short, twice over for splits of four row
+    // tiles (28 prompts of up to 1613, one kv head: 45 -> 33 us; a pair starts
+    // twice, 46 us), else up to two workgroups per CU (prompts of 256, 512 and
+    // 1000 tokens, 8 kv heads, group 4: 9.6, 12 and 21 us; 15, 16 and 23 with four
+    // row tiles at least, 9.6, 12 and 27 with one at any number).
     const int64_t tiles = (max_kv + kWeightKeys - 1) / kWeightKeys;
     const int64_t bk = (int64_t)batch * kv_heads;
-    // (Up to 512 rows are not split, for the launch that adds the splits up.)
+    // (Up to 256 rows are not split, for the launch that adds the splits up; 512
+    // over 2000 keys, 8 kv heads: 21 us without, 12 with.)
     auto cut = [&](int64_t places, int per_cu, int rows) {
-      if (most <= 512) return 1;
+      if (most <= 256) return 1;
       const int64_t want = per_cu * (int64_t)compute_units / std::max<int64_t>(bk * places, 1);
       return (int)std::max<int64_t>(1, std::min(want, most / rows));
     };
-    p.splits = cut(tiles, 3, 128);
+    p.splits = cut(tiles, 3, 64);
     if (4 * (int64_t)max_q >= max_kv) {
       p.pairs = most / 64 >= 32 * (int64_t)p.splits;
-      p.splits = p.pairs ? cut((tiles + 1) / 2, 3, 128) : cut(tiles, 6, 256);
+      p.splits = p.pairs ? cut((tiles + 1) / 2, 3, 64) : std::max(cut(tiles, 6, 256), cut(tiles, 2, 64));
     }
   }
   return p;
