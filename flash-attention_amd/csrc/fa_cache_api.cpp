@@ -16,18 +16,19 @@
 namespace fa {
 
 // Whether the chunk kernel may cut the tiles of its last round in pieces
-// (LastRound, of which this is the host's copy), for every number of tiles that
-// sequences of `rows` rows in all can have.  Where it may not, the call is
-// spared the launch that joins them.
+// (LastRound), for every number of tiles that sequences of `rows` rows in all
+// can have.  Where it may not, the call is spared the launch that joins them.
 static bool cuts_tiles(int64_t rows, int batch, int conc, int max_pieces, float piece_cost) {
   if (batch > 8) return true;
   const int64_t least = (rows + kChunkRows - 1) / kChunkRows;
   const int64_t most = std::max(least, (rows - batch) / kChunkRows + batch);
   for (int64_t n = least; n <= most; ++n) {
     const int64_t rest = n % conc;
-    for (int q = 2; rest > 0 && q <= 64 && rest * q <= max_pieces; ++q)
-      if ((float)((rest * q + conc - 1) / conc) * (1.0f / (float)q + piece_cost) < 1.0f + piece_cost)
+    for (int q = 2; rest > 0 && q <= 64; ++q) {
+      const int64_t all = rest * q;
+      if (cut_cost((int)all, (int)((all + conc - 1) / conc), q, max_pieces, piece_cost) < 1.0f + piece_cost)
         return true;
+    }
   }
   return false;
 }

@@ -6,7 +6,16 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <math.h>
+
 #include "fa_fwd_kernel.h"
+
+// Arithmetic that the host's plans and the kernels share.
+#if defined(__HIPCC__)
+#define FA_PLAN_FN __host__ __device__ __forceinline__
+#else
+#define FA_PLAN_FN inline
+#endif
 
 namespace fa {
 
@@ -38,8 +47,8 @@ struct PagedFwdArgs {
   int32_t max_q, causal;
   float scale_log2;                // softmax scale * log2(e)
   // Grids.  Decode kernel: slots (sequences) x kv heads x splits of `chunk` keys.
-  // Chunk kernel: at most `slots` row tiles per kv head, and up to 2 conc pieces
-  // of the last ones (LastRound).
+  // Chunk kernel: at most `slots` row tiles per kv head, and up to max_pieces
+  // pieces of the last ones (LastRound; 0: none is cut).
   int32_t slots, splits, chunk;
   int32_t conc, max_pieces;        // workgroups of a kv head that run at once, its most pieces
   float piece_cost;
@@ -56,6 +65,23 @@ struct PagedFwdArgs {
 // Cost of a piece of a tile beside its keys (LastRound): the time of 768 keys,
 // in units of a tile that sees max_kv of them.
 inline float piece_cost(int64_t max_kv) { return 768.0f / (float)(max_kv > 768 ? max_kv : 768); }
+
+// Tiles of the chunk kernel's list, of `found` that the offsets make: offsets
+// that ascend make at most `slots`, others may make more, which are left out.
+FA_PLAN_FN int listed_tiles(int found, int slots) { return found < slots ? found : slots; }
+
+// Time of the last round's tiles cut into q pieces each, `all` in all, in units
+// of a tile: rounds of pieces, each 1 / q of a tile and a piece's own cost.  The
+// workspace holds max_pieces of them, so more are never cut.
+FA_PLAN_FN float cut_cost(int all, int rounds, int q, int max_pieces, float piece_cost) {
+  return q > 1 && all > max_pieces ? INFINITY : (float)rounds * (1.0f / (float)q + piece_cost);
+}
+
+// Place in the workspace, in tiles, of a piece of the tile-th tile of the last
+// round: below max_pieces for each kv head (tile * pieces + piece < all).
+FA_PLAN_FN int64_t partial_tile(int kvh, int max_pieces, int tile, int pieces, int piece) {
+  return (int64_t)kvh * max_pieces + tile * pieces + piece;
+}
 
 // How a call is launched (plan_paged): on the decode kernel where no sequence
 // has more than kDecodeRows rows, else on the chunk kernel.

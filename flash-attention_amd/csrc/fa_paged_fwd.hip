@@ -560,13 +560,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   list.init(a);
   LastRound end;
   end.init(a, list.count);
-  const int cut = a.ws_o != nullptr ? end.pieces : 1;
   // (lists of more than 64 sequences are not by length)
-  const bool turn = a.pt.batch <= 64 && (end.whole + end.rest * cut) * a.kv_heads > kNumXcd * a.xcd_cus;
+  const bool turn = a.pt.batch <= 64 && (end.whole + end.rest * end.pieces) * a.kv_heads > kNumXcd * a.xcd_cus;
   if (!head_and_place(a, turn, kvh, place)) return;
   int pieces = 1, piece = 0, nth = place;
   if (place >= end.whole) {
-    pieces = cut;
+    pieces = end.pieces;
     // (First pieces of all tiles, second ones, ...: short tiles have no last ones,
     // and gaps leave CUs idle.  128 tokens over 2000 keys, 32 heads on 8: 31 -> 27 us.)
     const int i = place - end.whole;
@@ -694,7 +693,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     lu[rb] = W::red_sum(w.lu[rb]);
   }
   if (n_act > 1) {  // partials: o normalised, sums as log2
-    const int64_t wr0 = ((int64_t)kvh * a.max_pieces + (nth - end.whole) * pieces + piece) * BM + 32 * wave;
+    const int64_t wr0 = partial_tile(kvh, a.max_pieces, nth - end.whole, pieces, piece) * BM + 32 * wave;
 #pragma unroll
     for (int rb = 0; rb < 2; ++rb) {
       const int r = 16 * rb + l16;
@@ -782,7 +781,7 @@ __global__ void __launch_bounds__(256) fa_paged_merge_kernel(const PagedFwdArgs 
     LastRound end;
     end.init(a, list.count);
     if (end.pieces <= 1 || slot >= end.rest || !list.find(a, end.whole + slot, b, tile0, s)) return;
-    w0 = ((int64_t)kvh * a.max_pieces + slot * end.pieces) * BM;
+    w0 = partial_tile(kvh, a.max_pieces, slot, end.pieces, 0) * BM;
     n_act = end.pieces;
   } else {
     s = load_seq(a.pt, b, a.max_q);

@@ -164,6 +164,7 @@ struct TileList {
       start += l > len || (l == len && i < lane) ? t : 0;
       count += t;
     }
+    count = listed_tiles(count, a.slots);
   }
   __device__ __forceinline__ bool find(const PagedFwdArgs& a, int n, int& b, int& tile, Seq& s) const {
     if (a.pt.batch <= 64) {
@@ -201,7 +202,7 @@ struct TileList {
 // the GPU busy for a whole tile's time, so they are cut into `pieces` of keys:
 // the number that finishes them first, at ceil(rest pieces / conc) rounds of
 // 1 / pieces of a tile plus a piece's own cost (its join, about the time of 768
-// keys).  Lane q weighs q + 1 pieces.
+// keys), as far as the workspace holds them.  Lane q weighs q + 1 pieces.
 struct LastRound {
   int whole, rest, pieces;
   __device__ __forceinline__ void init(const PagedFwdArgs& a, int count) {
@@ -210,8 +211,7 @@ struct LastRound {
     rest = count - whole;
     const int q = (int)(threadIdx.x & 63) + 1;
     const int all = rest * q;
-    float cost = (float)(fast_div(all + a.conc - 1, a.by_conc)) * (1.0f / (float)q + a.piece_cost);
-    if (all > 2 * a.conc && q > 1) cost = INFINITY;
+    const float cost = cut_cost(all, fast_div(all + a.conc - 1, a.by_conc), q, a.max_pieces, a.piece_cost);
     float least = cost;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) least = fminf(least, __shfl_xor(least, d));

@@ -25,7 +25,9 @@
  * id outside [0, num_pages) is an absent page (its keys are masked, read as
  * weight 0 and never written), seq_lens is limited to [0, max_kv] and to the
  * table's max_pages pages, cu_seqlens to [0, tokens].  Rows of q that belong
- * to no sequence are not written to in o and lse.
+ * to no sequence are not written to in o and lse.  cu_seqlens must not
+ * descend: the rows and keys of sequences that do get unspecified values, and
+ * nothing else is written.
  */
 #ifndef FA_MI355X_CACHE_H
 #define FA_MI355X_CACHE_H
