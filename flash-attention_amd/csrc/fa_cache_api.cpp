@@ -745,8 +745,7 @@ fa_status fa_paged_store(const fa_paged_store_params* p, void* stream) {
   n.cos = p->cos;
   n.sin = p->sin;
   n.positions = p->positions;
-  n.pt = page_table(c, p->tokens, 0);
-  n.capacity = (int64_t)c.max_pages * c.page_size;
+  n.pt = page_table(c, p->tokens, c.max_pages * c.page_size);
   n.tokens = p->tokens;
   n.seq_len = p->tokens;
   n.heads = p->heads;

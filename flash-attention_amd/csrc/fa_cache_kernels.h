@@ -171,7 +171,6 @@ struct NormArgs {
   const int32_t* positions;
   int64_t pos_stride;             // elements
   PageTable pt;                   // storing only
-  int64_t capacity;               // storing only: keys that a table row holds
   int32_t tokens;                 // of all sequences: batch * seq_len
   int32_t seq_len;                // tokens of one batch entry
   int32_t heads, kv_heads, head_dim;

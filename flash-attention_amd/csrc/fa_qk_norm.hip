@@ -188,11 +188,14 @@ __global__ void __launch_bounds__(256) fa_norm_kernel(const NormArgs n) {
     }
     mine = mine && seq < n.pt.batch && token >= first;
     if (mine && h1 > n.heads) {
-      const int64_t key = (int64_t)n.pt.lens[seq] - n.pt.cu[seq + 1] + token;
-      if (key >= 0 && key < n.capacity) {
+      // (the limits of load_seq: the token's key is the one its query ends at)
+      const int c0 = min(max(n.pt.cu[seq], 0), n.tokens);
+      const int c1 = min(max(n.pt.cu[seq + 1], c0), n.tokens);
+      const int key = min(max(n.pt.lens[seq], 0), n.pt.max_kv) - c1 + token;
+      if (key >= 0 && token >= c0 && token < c1) {
         const int id = n.pt.table[seq * n.pt.table_stride + (key >> n.pt.page_shift)];
         if ((uint32_t)id < (uint32_t)n.pt.num_pages) page = id;
-        at = (int)(key & ((1 << n.pt.page_shift) - 1));
+        at = key & ((1 << n.pt.page_shift) - 1);
       }
     }
   }

@@ -174,7 +174,8 @@ typedef struct {
  * head_dim]), k's result and v go to the tokens' places in the cache.  The
  * pages that receive new tokens must belong to one sequence only.  Tokens past
  * a sequence's keys (more new tokens than keys: the first ones) or on absent
- * pages are not stored. */
+ * pages are not stored.  seq_lens is limited by the table alone: a length that
+ * fa_paged_fwd cuts at a smaller max_kv has its tokens at other keys there. */
 typedef struct {
   fa_paged_cache cache;
   const void* q;        /* [tokens, heads, head_dim] */

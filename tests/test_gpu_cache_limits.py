@@ -9,6 +9,9 @@ import torch
 
 import abi_ctypes as A
 import cache_ctypes as C
+import cache_reference as R
+from test_gpu_paged_forward import Cache
+from test_gpu_qk_norm import tables
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -55,3 +58,70 @@ def test_nothing_behind_the_workspace_is_written(cu):
     assert rc == A.FA_OK, L.fa_last_error()
     torch.cuda.synchronize()
     assert bool((ws[need.value:] == 0x5A).all())
+
+
+def store_and_compare(fa, c, lens, cu, T):
+    """paged_store of T tokens against the 64-bit form, whose lengths are limited to
+    the table and whose offsets to the rows, as in every other call."""
+    H, KH, D, page = 2, c.k.shape[1], c.k.shape[3], c.page
+    g = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn(T, h, D, generator=g).to(c.k.dtype) for h in (H, KH, KH))
+    w = 1 + 0.2 * torch.randn(D, generator=g)
+    cos, sin = tables(100, D)
+    pos = torch.randint(0, 100, (T,), generator=g, dtype=torch.int32)
+    kc, vc, table = c.dev()
+    out = torch.full((T, H, D), 9.0, dtype=q.dtype, device=DEV)
+    fa.paged_store(q.to(DEV), k.to(DEV), v.to(DEV), w.to(DEV), w.to(DEV), cos.to(DEV), sin.to(DEV),
+                   pos.to(DEV), kc, vc, table, torch.tensor(cu, dtype=torch.int32, device=DEV),
+                   torch.tensor(lens, dtype=torch.int32, device=DEV), out)
+    wq, tq = R.norm_rope(q, w, cos, sin, pos[:, None].expand(T, H), eps=1e-6, interleaved=False)
+    wk, tk = R.norm_rope(k, w, cos, sin, pos[:, None].expand(T, KH), eps=1e-6, interleaved=False)
+    want_k, want_v, tol = c.k.double(), c.v.double(), torch.zeros(c.k.shape, dtype=torch.float64)
+    rows = torch.zeros(T, dtype=torch.bool)
+    for b, c0, nq, n, first in R.sequences(cu, lens, T, capacity=c.table.shape[1] * page):
+        rows[c0:c0 + nq] = True
+        for i in range(max(0, -first), nq):
+            at = (int(c.table[b, (first + i) // page]), slice(None), (first + i) % page)
+            want_k[at], tol[at], want_v[at] = wk[c0 + i], tk[c0 + i], v[c0 + i].double()
+    R.check("q", out[rows.to(DEV)], wq[rows], tq[rows])
+    assert bool((out.cpu()[~rows] == 9).all())
+    R.check("k_cache", kc, want_k, tol)
+    R.check("v_cache", vc, want_v, torch.zeros_like(tol))
+
+
+@pytest.mark.parametrize("name,lens,cu", [
+    ("length above the table", [70, 40], [0, 10, 15]),
+    ("far above it", [2 ** 31 - 1, 64], [0, 10, 15]),
+    ("more tokens than the table has keys", [200, 40], [0, 100, 110]),
+    ("no keys", [-5, 0], [0, 10, 15]),
+    ("last offset above the rows", [64, 40], [0, 10, 40]),
+    ("every offset above the rows", [64, 40], [50, 60, 70]),
+    ("offsets to both sides of the rows", [64, 40], [-7, 3, 2 ** 31 - 1]),
+    ("rows before the first and behind the last", [64, 40], [2, 9, 11]),
+])
+def test_store_limits_lengths_and_offsets_as_the_other_calls(fa, name, lens, cu):
+    print("case store limits", name, flush=True)
+    c = Cache([64, 64], 16, 2, 64, torch.bfloat16, 700)
+    store_and_compare(fa, c, lens, cu, 110 if cu[-1] == 110 else 15)
+
+
+def test_store_then_forward_agree_on_a_length_above_the_table(fa):
+    """Each token's own key is where its query looks for it: with values that name
+    the token and a score that only its own key reaches, every row gets its token."""
+    D, T, n = 64, 10, 64
+    c = Cache([n], 16, 1, D, torch.float16, 701)
+    kc, vc, table = c.dev()
+    kc.zero_(), vc.zero_()
+    # q and k of token i along axis i: a score of D against 0 for every other key
+    q = torch.zeros(T, 1, D, device=DEV).half()
+    q[torch.arange(T), 0, torch.arange(T)] = 1.0
+    v = torch.arange(1, T + 1, device=DEV).half()[:, None, None].expand(T, 1, D).contiguous()
+    w = torch.ones(D, device=DEV)
+    cos, sin = torch.ones(1, D // 2, device=DEV), torch.zeros(1, D // 2, device=DEV)
+    cu = torch.tensor([0, T], dtype=torch.int32, device=DEV)
+    ln = torch.tensor([n + 6], dtype=torch.int32, device=DEV)
+    pos = torch.zeros(T, dtype=torch.int32, device=DEV)
+    qn = fa.paged_store(q, q, v, w, w, cos, sin, pos, kc, vc, table, cu, ln)
+    o = fa.paged_forward(qn, kc, vc, table, cu, ln, max_q=T, softmax_scale=1.0)
+    # weight of each other key: exp(-64), so that the row is its own value but for fp16's steps
+    assert float((o[:, 0, 0].float() - torch.arange(1, T + 1, device=DEV)).abs().max()) <= T * 2.0 ** -10
