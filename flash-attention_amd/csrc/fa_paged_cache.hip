@@ -15,7 +15,8 @@
 //
 // fa_select_kernel: the keep - recent heaviest of a head's keys by a radix
 // search for their least weight (digits of 11, 11 and 10 bits), and the list of
-// the kept keys in order.  fa_move_kernel copies their rows: bound by memory.
+// the kept keys in order.  fa_move_kernel copies their rows, and counts them
+// for the new lengths: bound by memory.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -421,8 +422,9 @@ __global__ void __launch_bounds__(kSelThreads) fa_select_kernel(const PagedEvict
     miss = miss || (uint32_t)new_row[i] >= (uint32_t)a.pt.num_pages;
   if (__any(miss) && lane == 0) bad = 1;
   __syncthreads();
+  // (The new length is not written here: it may be the old one's place, which
+  // the other heads still read.)
   const int count = bad ? 0 : n;
-  if (tid == 0 && kvh == 0) a.new_lens[b] = count;
   for (int t = count + tid; t < a.keep; t += kSelThreads) kept[t] = -1;
   if (bad) return;
   if (len <= a.keep) {
@@ -541,13 +543,13 @@ __global__ void __launch_bounds__(kSelThreads) fa_select_kernel(const PagedEvict
 }
 
 // Copies the kept keys' rows of K and V, and their weights.  LPR lanes move a
-// row, kMoveRows rows apart per lane in flight.
+// row, kMoveRows rows apart per lane in flight.  The number of kept keys, the
+// same for every head of a sequence, ends at the first place that holds -1.
 constexpr int kMoveRows = 2;  // (of 64 heads of 4096 keys, D = 128, 55 us: 4 rows 2 us more, 8 rows 7)
 template <int D>
-__global__ void __launch_bounds__(256) fa_move_kernel(const PagedEvictArgs a, int blocks) {
+__global__ void __launch_bounds__(256) fa_move_kernel(const PagedEvictArgs a, int blocks, int most) {
   constexpr int LPR = 2 * D / 16, RPB = 256 / LPR;
   const int bk = blockIdx.x / blocks, b = bk / a.kv_heads, kvh = bk - b * a.kv_heads;
-  const int n = a.new_lens[b];
   const int t0 = (blockIdx.x - bk * blocks) * RPB * kMoveRows + (int)threadIdx.x / LPR;
   const int c = ((int)threadIdx.x % LPR) * 16;
   const int32_t* row = a.pt.table + b * a.pt.table_stride;
@@ -558,7 +560,15 @@ __global__ void __launch_bounds__(256) fa_move_kernel(const PagedEvictArgs a, in
   u32x4 k[kMoveRows], v[kMoveRows];
   float w[kMoveRows];
 #pragma unroll
-  for (int j = 0; j < kMoveRows; ++j) src[j] = t0 + j * RPB < n ? kept[t0 + j * RPB] : -1;
+  for (int j = 0; j < kMoveRows; ++j) src[j] = t0 + j * RPB < most ? kept[t0 + j * RPB] : -1;
+  if (kvh == 0 && c == 0) {
+#pragma unroll
+    for (int j = 0; j < kMoveRows; ++j) {
+      const int t = t0 + j * RPB;
+      if (src[j] >= 0 && (t + 1 == most || kept[t + 1] < 0)) a.new_lens[b] = t + 1;
+      if (t == 0 && src[j] < 0) a.new_lens[b] = 0;
+    }
+  }
 #pragma unroll
   for (int j = 0; j < kMoveRows; ++j)
     if (src[j] >= 0) {
@@ -630,10 +640,10 @@ hipError_t launch_paged_weights(const PagedWeightsArgs& args, const WeightsPlan&
 hipError_t launch_paged_evict(const PagedEvictArgs& args, int head_dim, hipStream_t stream) {
   PagedEvictArgs a = args;
   const int64_t bk = (int64_t)a.pt.batch * a.kv_heads;
-  const int most = std::min(a.keep, a.pt.max_kv);
+  int most = std::min(a.keep, a.pt.max_kv);
   const int per = 256 / (2 * head_dim / 16) * kMoveRows;
-  int blocks = (most + per - 1) / per;
-  if (bk * std::max(blocks, 1) > 0x7fffffff) return hipErrorInvalidValue;
+  int blocks = std::max(1, (most + per - 1) / per);  // (no keys: the new lengths)
+  if (bk * blocks > 0x7fffffff) return hipErrorInvalidValue;
   void* sargs[] = {&a};
   // Four keys a thread where they hold all of a sequence: less work in a row.
   const void* select = a.pt.max_kv <= 4 * kSelThreads
@@ -641,8 +651,8 @@ hipError_t launch_paged_evict(const PagedEvictArgs& args, int head_dim, hipStrea
                            : reinterpret_cast<const void*>(&fa_select_kernel<16>);
   hipError_t e = hipLaunchKernel(select, dim3((unsigned)bk),
                                  dim3(kSelThreads), sargs, 0, stream);
-  if (e != hipSuccess || blocks == 0) return e;
-  void* margs[] = {&a, &blocks};
+  if (e != hipSuccess) return e;
+  void* margs[] = {&a, &blocks, &most};
   const void* fn = head_dim == 128 ? reinterpret_cast<const void*>(&fa_move_kernel<128>)
                                    : reinterpret_cast<const void*>(&fa_move_kernel<64>);
   return hipLaunchKernel(fn, dim3((unsigned)(bk * blocks)), dim3(256), margs, 0, stream);

@@ -116,7 +116,7 @@ typedef struct {
   int64_t w_stride[2];       /* page, kv head */
   const int32_t* new_table;  /* [batch][new_pages], row stride new_table_stride */
   int64_t new_table_stride;
-  int32_t* new_lens;         /* [batch]: min(length, keep) */
+  int32_t* new_lens;         /* [batch]: min(length, keep); may be cache.seq_lens itself */
   int32_t* kept;             /* [batch, kv_heads, keep] contiguous: index of the key now at t, or -1 */
   int32_t new_pages;         /* new_pages * page_size >= min(keep, max_pages * page_size) */
   int32_t keep;              /* 1 to 2^30 */

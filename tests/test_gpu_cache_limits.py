@@ -10,6 +10,7 @@ import torch
 import abi_ctypes as A
 import cache_ctypes as C
 import cache_reference as R
+from test_gpu_paged_cache import evict_compare, evict_setup
 from test_gpu_paged_forward import Cache
 from test_gpu_qk_norm import tables
 
@@ -125,3 +126,49 @@ def test_store_then_forward_agree_on_a_length_above_the_table(fa):
     o = fa.paged_forward(qn, kc, vc, table, cu, ln, max_q=T, softmax_scale=1.0)
     # weight of each other key: exp(-64), so that the row is its own value but for fp16's steps
     assert float((o[:, 0, 0].float() - torch.arange(1, T + 1, device=DEV)).abs().max()) <= T * 2.0 ** -10
+
+
+def test_evict_may_update_the_lengths_in_place():
+    """new_lens is seq_lens: no head may see the new length in place of the old one.
+    Thousands of heads with the same keys and weights, beside a large product on
+    another stream, so that many of them start after others have ended."""
+    print("case evict in place", flush=True)
+    kh, keep, recent, page, D, lens = 8192, 64, 8, 16, 64, [600, 500]
+    c, new_table, w = evict_setup(lens, page, 1, D, torch.float16, keep, 710)
+    want = R.evict(c.k, c.v, w, c.table, c.lens, new_table, keep=keep, recent=recent)
+    table, nt = c.table.to(DEV), new_table.to(DEV)
+    start = [t.to(DEV).expand(-1, kh, *t.shape[2:]) for t in (c.k, c.v, w)]
+    k, v, wd = (t.contiguous() for t in start)
+    big, side = torch.randn(8192, 8192, device=DEV).half(), torch.cuda.Stream()
+    L = C.load()
+    for trial in range(3):
+        for t, x in zip((k, v, wd), start):
+            t.copy_(x)
+        ln = c.lens.to(DEV)
+        kept = torch.full((2, kh, keep), -7, dtype=torch.int32, device=DEV)
+        p = C.PagedEvict()
+        p.cache = cache_of(k, v, table, None, ln)
+        p.key_weights, p.w_stride[0], p.w_stride[1] = wd.data_ptr(), wd.stride(0), wd.stride(1)
+        p.new_table, p.new_table_stride, p.new_pages = nt.data_ptr(), nt.stride(0), nt.shape[1]
+        p.new_lens, p.kept, p.keep, p.recent, p.max_kv = ln.data_ptr(), kept.data_ptr(), keep, recent, max(lens)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.mm(big, big)
+        rc = L.fa_paged_evict(ctypes.byref(p), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        assert rc == A.FA_OK, L.fa_last_error()
+        torch.cuda.synchronize()
+        assert torch.equal(ln.cpu(), want[0])
+        assert bool((kept == want[1].to(DEV)).all()), trial  # (of one head: the same for all)
+        for got, ref in ((k, want[2]), (v, want[3]), (wd, want[4])):
+            kind = torch.int16 if got.dtype == torch.float16 else torch.int32
+            assert bool((got.view(kind) == ref.to(DEV).view(kind)).all()), trial
+
+
+@pytest.mark.parametrize("keep", [1, 16, 17, 5000])
+def test_evict_lengths_at_the_edges_of_what_is_kept(fa, keep):
+    """Lengths of zero, below, at and above keep; an absent page; a table of no keys."""
+    lens = [0, 1, keep - 1, keep, keep + 1, 3 * keep, 40]
+    c, new_table, w = evict_setup(lens, 16, 2, 64, torch.float16, keep, 711)
+    c.table[6, 0] = -1
+    evict_compare(fa, c, new_table, w, keep=keep, recent=min(keep, 3))
+    evict_compare(fa, c, new_table, w, keep=keep, recent=0, max_kv=0)
