@@ -19,6 +19,7 @@ namespace fa {
 // (LastRound), for every number of tiles that sequences of `rows` rows in all
 // can have.  Where it may not, the call is spared the launch that joins them.
 static bool cuts_tiles(int64_t rows, int batch, int conc, int max_pieces, float piece_cost) {
+  if (conc == 1) return false;  // whole rounds only
   if (batch > 8) return true;
   const int64_t least = (rows + kChunkRows - 1) / kChunkRows;
   const int64_t most = std::max(least, (rows - batch) / kChunkRows + batch);

@@ -11,7 +11,7 @@ import abi_ctypes as A
 import cache_ctypes as C
 import cache_reference as R
 from test_gpu_paged_cache import evict_compare, evict_setup
-from test_gpu_paged_forward import Cache
+from test_gpu_paged_forward import Cache, compare, cu_of
 from test_gpu_qk_norm import tables
 
 pytestmark = pytest.mark.gpu
@@ -172,3 +172,14 @@ def test_evict_lengths_at_the_edges_of_what_is_kept(fa, keep):
     c.table[6, 0] = -1
     evict_compare(fa, c, new_table, w, keep=keep, recent=min(keep, 3))
     evict_compare(fa, c, new_table, w, keep=keep, recent=0, max_kv=0)
+
+
+@pytest.mark.parametrize("new", [[40, 3, 1, 0, 1, 2, 1, 1, 33], [35, 1]])
+def test_more_kv_heads_than_compute_units(fa, new):
+    """One workgroup of a kv head at a time: no rounds to cut, no join."""
+    print("case many heads", new, flush=True)
+    KH = torch.cuda.get_device_properties(0).multi_processor_count + 1
+    lens = [n + 5 * i for i, n in enumerate(new)]
+    c = Cache(lens, 16, KH, 64, torch.bfloat16, 720, wide=100)
+    q = torch.randn(sum(new), KH, 64, generator=torch.Generator().manual_seed(5)).bfloat16()
+    compare(fa, c, q, cu_of(new), max_q=max(new))

@@ -92,3 +92,22 @@ def test_any_offsets_stay_in_the_workspace(plans, kind):
                     rng.choice([1, 700, 1025, 9000, 131072]), rng.random() < 0.8)
         cut += got is not None and got[2] > 1
     assert cut > 200
+
+
+@pytest.mark.parametrize("kv_heads,cus", [(257, 256), (512, 256), (513, 256), (1000, 256), (64, 32), (33, 32), (5, 2)])
+@pytest.mark.parametrize("batch", [1, 9, 70])
+def test_as_many_heads_as_compute_units_cut_nothing(plans, kv_heads, cus, batch):
+    """Where a kv head has one workgroup at a time, every round is a whole one: no
+    pieces, no workspace and no launch that joins them (its grid would be empty)."""
+    p = plan(plans, 400, batch, kv_heads, 1, 64, 100, 4096, cus=cus)
+    assert p["rows"] == CHUNK_ROWS and (p["conc"] == 1) == (kv_heads > cus)
+    if p["conc"] == 1:
+        assert p["pieces"] == 0 and p["ws_rows"] == 0 and p["bytes"] == 0
+
+
+def test_a_call_that_may_cut_has_tiles_to_join(plans):
+    rng = random.Random(8)
+    for _ in range(3000):
+        p = plan(plans, rng.choice([40, 400, 5000]), rng.choice([1, 4, 9, 64, 200]), rng.randint(1, 600), 1, 64,
+                 rng.choice([33, 400, 5000]), rng.choice([64, 1025, 100000]), rng.random() < 0.5, rng.choice([8, 32, 256]))
+        assert p["pieces"] == 0 or min(p["conc"] - 1, p["slots"]) > 0, p
