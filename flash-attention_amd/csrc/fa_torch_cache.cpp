@@ -37,6 +37,19 @@ void check_no_grad(const char* name, std::initializer_list<const Tensor*> tensor
                 "its inputs");
 }
 
+// No call carries tangents on: none may be dropped.  (no_grad does not stop them.)
+void check_no_tangent(const char* name, std::initializer_list<const Tensor*> tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : tensors)
+    TORCH_CHECK(!t->_fw_grad(0).defined(), name, " has no forward-mode derivative: an input has a tangent");
+}
+
+// Both, for a call without derivatives.
+void check_no_derivative(const char* name, std::initializer_list<const Tensor*> tensors) {
+  check_no_grad(name, tensors);
+  check_no_tangent(name, tensors);
+}
+
 void check_half(const Tensor& t, const char* name, int64_t dims, const char* shape) {
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
   TORCH_CHECK(t.dim() == dims, name, " must be a ", dims, "D tensor with shape ", shape);
@@ -168,13 +181,13 @@ pybind11::object paged_forward(const Tensor& q, const Tensor& k_cache, const Ten
                               const Tensor& seq_lens, std::optional<Tensor> out, int64_t max_q,
                               std::optional<int64_t> max_kv, bool causal,
                               std::optional<double> softmax_scale, bool return_lse) {
-  check_no_grad("paged_forward", {&q, &k_cache, &v_cache});
+  check_no_derivative("paged_forward", {&q, &k_cache, &v_cache});
+  if (out) check_no_derivative("paged_forward", {&*out});
   fa_paged_fwd_params p{};
   p.cache = make_cache(k_cache, v_cache, block_table, cu_seqlens, seq_lens);
   check_packed(q, "q", k_cache);
   const c10::OptionalDeviceGuard guard(q.device());
   if (out) {
-    check_no_grad("paged_forward", {&*out});
     check_packed(*out, "out", k_cache, q.size(0), q.size(1));
     TORCH_CHECK(!out->is_alias_of(q) || out->data_ptr() != q.data_ptr() || out->numel() == 0,
                 "out must not be q");
@@ -205,7 +218,7 @@ void paged_key_weights(const Tensor& q, const Tensor& lse, const Tensor& k_cache
                        const Tensor& block_table, const Tensor& cu_seqlens, const Tensor& seq_lens,
                        Tensor key_weights, int64_t max_q, std::optional<int64_t> max_kv, bool causal,
                        std::optional<double> softmax_scale) {
-  check_no_grad("paged_key_weights", {&q, &lse, &k_cache, &key_weights});
+  check_no_derivative("paged_key_weights", {&q, &lse, &k_cache, &key_weights});
   fa_paged_weights_params p{};
   p.cache = make_cache(k_cache, std::nullopt, block_table, cu_seqlens, seq_lens);
   check_packed(q, "q", k_cache);
@@ -230,7 +243,7 @@ void paged_key_weights(const Tensor& q, const Tensor& lse, const Tensor& k_cache
 pybind11::tuple paged_evict(Tensor k_cache, Tensor v_cache, Tensor key_weights,
                             const Tensor& block_table, const Tensor& seq_lens, const Tensor& new_table,
                             int64_t keep, int64_t recent, std::optional<int64_t> max_kv) {
-  check_no_grad("paged_evict", {&k_cache, &v_cache, &key_weights});
+  check_no_derivative("paged_evict", {&k_cache, &v_cache, &key_weights});
   fa_paged_evict_params p{};
   p.cache = make_cache(k_cache, v_cache, block_table, std::nullopt, seq_lens);
   const c10::OptionalDeviceGuard guard(k_cache.device());
@@ -439,6 +452,7 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
 pybind11::tuple qk_norm_rope(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw,
                              const Tensor& cos, const Tensor& sin, std::optional<Tensor> positions,
                              double eps, bool interleaved) {
+  check_no_tangent("qk_norm_rope", {&q, &k, &qw, &kw, &cos, &sin});
   if (at::GradMode::is_enabled()) {
     TORCH_CHECK(!cos.requires_grad() && !sin.requires_grad(),
                 "cos and sin get no gradients: detach them");
@@ -461,6 +475,7 @@ pybind11::tuple qk_norm_rope_backward(const Tensor& dq_out, const Tensor& dk_out
                                       const Tensor& k, const Tensor& qw, const Tensor& kw,
                                       const Tensor& cos, const Tensor& sin,
                                       std::optional<Tensor> positions, double eps, bool interleaved) {
+  check_no_tangent("qk_norm_rope_backward", {&dq_out, &dk_out, &q, &k, &qw, &kw, &cos, &sin});
   at::NoGradGuard no_grad;
   const auto d = norm_backward(dq_out, dk_out, q, k, qw, kw, cos, sin, positions, eps, interleaved);
   return pybind11::make_tuple(d[0], d[1], d[2], d[3]);
@@ -470,7 +485,9 @@ Tensor paged_store(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
                    const Tensor& cos, const Tensor& sin, const Tensor& positions, Tensor k_cache,
                    Tensor v_cache, const Tensor& block_table, const Tensor& cu_seqlens,
                    const Tensor& seq_lens, std::optional<Tensor> out, double eps, bool interleaved) {
-  check_no_grad("paged_store", {&q, &k, &v, &qw, &kw, &k_cache, &v_cache});
+  check_no_derivative("paged_store", {&q, &k, &v, &qw, &kw, &k_cache, &v_cache});
+  check_no_tangent("paged_store", {&cos, &sin});
+  if (out) check_no_derivative("paged_store", {&*out});
   fa_paged_store_params p{};
   p.cache = make_cache(k_cache, v_cache, block_table, cu_seqlens, seq_lens);
   check_packed(q, "q", k_cache);
@@ -478,7 +495,6 @@ Tensor paged_store(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   check_packed(v, "v", k_cache, q.size(0), k_cache.size(1));
   const c10::OptionalDeviceGuard guard(q.device());
   if (out) {
-    check_no_grad("paged_store", {&*out});
     check_packed(*out, "out", k_cache, q.size(0), q.size(1));
   }
   Tensor o = out ? *out : new_tensor(q.sizes(), q.scalar_type(), q);

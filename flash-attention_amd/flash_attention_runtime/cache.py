@@ -24,7 +24,8 @@ A step of a server with a bounded cache::
     lens, kept = fa.paged_evict(kc, vc, weights, table, lens, new_table, keep=4096, recent=256)
 
 No call waits for the GPU; each may be captured into a graph and replayed with
-other lengths and tables.  The cache's calls compute no gradients.
+other lengths and tables.  The cache's calls compute no gradients, and no call
+carries forward-mode tangents on: inputs that ask for them are refused.
 """
 from __future__ import annotations
 
