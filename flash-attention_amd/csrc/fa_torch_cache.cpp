@@ -485,8 +485,7 @@ Tensor paged_store(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
                    const Tensor& cos, const Tensor& sin, const Tensor& positions, Tensor k_cache,
                    Tensor v_cache, const Tensor& block_table, const Tensor& cu_seqlens,
                    const Tensor& seq_lens, std::optional<Tensor> out, double eps, bool interleaved) {
-  check_no_derivative("paged_store", {&q, &k, &v, &qw, &kw, &k_cache, &v_cache});
-  check_no_tangent("paged_store", {&cos, &sin});
+  check_no_derivative("paged_store", {&q, &k, &v, &qw, &kw, &cos, &sin, &k_cache, &v_cache});
   if (out) check_no_derivative("paged_store", {&*out});
   fa_paged_store_params p{};
   p.cache = make_cache(k_cache, v_cache, block_table, cu_seqlens, seq_lens);

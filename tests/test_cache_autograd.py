@@ -46,3 +46,13 @@ def test_forward_mode_tangents_are_refused(fa, name, arg):
         args[arg] = fwd.unpack_dual(args[arg]).primal
         with pytest.raises(RuntimeError, match="CUDA tensor"):
             getattr(fa, name)(**args)
+
+
+@pytest.mark.parametrize("name,arg", [(n, a) for n, a in CASES if n.startswith("paged")])
+def test_gradients_that_a_call_would_drop_are_refused(fa, name, arg):
+    args = arguments()[name]
+    args[arg].requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        getattr(fa, name)(**args)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensor"):
+        getattr(fa, name)(**args)
