@@ -50,6 +50,13 @@ void check_no_derivative(const char* name, std::initializer_list<const Tensor*> 
   check_no_tangent(name, tensors);
 }
 
+// Tensors that a call has written: a new version of each, so that an autograd
+// graph that had saved one notices.  (Inference tensors have no versions.)
+void wrote(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    if (!t->is_inference()) torch::autograd::impl::bump_version(*t);
+}
+
 void check_half(const Tensor& t, const char* name, int64_t dims, const char* shape) {
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
   TORCH_CHECK(t.dim() == dims, name, " must be a ", dims, "D tensor with shape ", shape);
@@ -210,6 +217,7 @@ pybind11::object paged_forward(const Tensor& q, const Tensor& k_cache, const Ten
   check_status(fa_paged_fwd_workspace_size(&p, &bytes), "paged_forward");
   Tensor ws = workspace(bytes, q);
   check_status(fa_paged_fwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)), "paged_forward");
+  if (out) wrote({&o});
   if (return_lse) return pybind11::make_tuple(o, lse);
   return pybind11::cast(o);
 }
@@ -238,6 +246,7 @@ void paged_key_weights(const Tensor& q, const Tensor& lse, const Tensor& k_cache
   Tensor ws = workspace(bytes, q);
   check_status(fa_paged_key_weights(&p, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
                "paged_key_weights");
+  wrote({&key_weights});
 }
 
 pybind11::tuple paged_evict(Tensor k_cache, Tensor v_cache, Tensor key_weights,
@@ -267,6 +276,7 @@ pybind11::tuple paged_evict(Tensor k_cache, Tensor v_cache, Tensor key_weights,
     p.kept = kept.data_ptr<int32_t>();
   }
   check_status(fa_paged_evict(&p, stream_of(k_cache)), "paged_evict");
+  wrote({&k_cache, &v_cache, &key_weights});
   return pybind11::make_tuple(new_lens, kept);
 }
 
@@ -520,6 +530,8 @@ Tensor paged_store(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   p.weight_fp32 = t.fp32;
   p.eps = static_cast<float>(eps);
   check_status(fa_paged_store(&p, stream_of(q)), "paged_store");
+  wrote({&k_cache, &v_cache});
+  if (out) wrote({&o});
   return o;
 }
 
