@@ -138,6 +138,79 @@ WeightsPlan plan_weights(int tokens, int batch, int kv_heads, int group, int hea
 
 namespace {
 
+using Wide = __int128;  // strides times sizes
+
+Wide floor_div(Wide a, Wide b) { return a / b - (a % b < 0 ? 1 : 0); }
+
+// Whether some i[d] of lo[d]..hi[d] make -row_a < delta + sum i[d] stride[d] < row_b,
+// strides descending.  A stride that spans what the smaller ones reach leaves two
+// or three values to look at; overlapping rows, more, count as a meeting.
+bool meets(Wide delta, const int64_t* stride, const int64_t* lo, const int64_t* hi, int n, int64_t row_a,
+           int64_t row_b) {
+  if (n == 0) return -row_a < delta && delta < row_b;
+  Wide least = 0, most = 0;  // of the smaller strides' sum
+  for (int d = 1; d < n; ++d) {
+    least += (Wide)lo[d] * stride[d];
+    most += (Wide)hi[d] * stride[d];
+  }
+  const Wide s = stride[0];
+  const Wide first = std::max<Wide>(lo[0], -floor_div(-(-row_a + 1 - delta - most), s));
+  const Wide last = std::min<Wide>(hi[0], floor_div(row_b - 1 - delta - least, s));
+  if (last - first > 3) return true;
+  for (Wide i = first; i <= last; ++i)
+    if (meets(delta + i * s, stride + 1, lo + 1, hi + 1, n - 1, row_a, row_b)) return true;
+  return false;
+}
+
+int64_t gcd(int64_t a, int64_t b) { return b == 0 ? a : gcd(b, a % b); }
+
+}  // namespace
+
+bool may_overlap(const RowSet& a, const RowSet& b) {
+  Wide reach[2];
+  const RowSet* sets[2] = {&a, &b};
+  for (int x = 0; x < 2; ++x) {
+    reach[x] = sets[x]->row;
+    for (int d = 0; d < sets[x]->n; ++d) {
+      if (sets[x]->size[d] == 0) return false;
+      if (sets[x]->size[d] == 1) continue;
+      reach[x] += (Wide)sets[x]->stride[d] * (sets[x]->size[d] - 1);
+    }
+  }
+  const Wide bytes = (Wide)(intptr_t)b.base - (Wide)(intptr_t)a.base;
+  if (bytes >= 2 * reach[0] || -bytes >= 2 * reach[1]) return false;
+  if (bytes % 2 != 0) return true;
+  const Wide delta = bytes / 2;  // of b's first row behind a's
+  int64_t stride[3], lo[3], hi[3];
+  int n = 0;
+  bool same = a.n == b.n;
+  for (int d = 0; same && d < a.n; ++d) {
+    same = a.size[d] == 1 || b.size[d] == 1 || a.stride[d] == b.stride[d];
+    const int64_t s = a.size[d] > 1 ? a.stride[d] : b.stride[d];
+    if (s == 0 || (a.size[d] == 1 && b.size[d] == 1)) continue;
+    int at = n++;
+    for (; at > 0 && stride[at - 1] < s; --at) {
+      stride[at] = stride[at - 1];
+      lo[at] = lo[at - 1];
+      hi[at] = hi[at - 1];
+    }
+    stride[at] = s;
+    lo[at] = -(a.size[d] - 1);
+    hi[at] = b.size[d] - 1;
+  }
+  // b's rows start at delta + sum i_b stride, a's at sum i_a stride
+  if (same) return meets(delta, stride, lo, hi, n, b.row, a.row);
+  int64_t common = 0;
+  for (const RowSet* r : sets)
+    for (int d = 0; d < r->n; ++d)
+      if (r->size[d] > 1) common = gcd(common, r->stride[d]);
+  if (common == 0) return true;
+  const Wide at = ((delta % common) + common) % common;
+  return at < a.row || at + b.row > common;
+}
+
+namespace {
+
 constexpr int64_t kMaxKeyStride = int64_t(1) << 24;  // as the forward's seq stride
 
 bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }

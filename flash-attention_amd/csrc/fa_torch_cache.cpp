@@ -20,6 +20,7 @@
 #include <optional>
 #include <utility>
 
+#include "fa_host.h"
 #include "fa_mi355x_cache.h"
 
 namespace {
@@ -41,7 +42,8 @@ void check_no_grad(const char* name, std::initializer_list<const Tensor*> tensor
 void check_no_tangent(const char* name, std::initializer_list<const Tensor*> tensors) {
   if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
   for (const Tensor* t : tensors)
-    TORCH_CHECK(!t->_fw_grad(0).defined(), name, " has no forward-mode derivative: an input has a tangent");
+    TORCH_CHECK(t->unsafeGetTensorImpl()->autograd_meta() == nullptr || !t->_fw_grad(0).defined(), name,
+                " has no forward-mode derivative: an input has a tangent");
 }
 
 // Both, for a call without derivatives.
@@ -142,6 +144,37 @@ void check_packed(const Tensor& t, const char* name, const Tensor& k, int64_t to
   TORCH_CHECK(heads < 0 || t.size(1) == heads, name, " has the wrong number of heads");
 }
 
+// The rows of a tensor of 2-byte elements with unit stride along its last
+// dimension (check_half), and the end of their memory.
+struct Rows : fa::RowSet {
+  const char* end;
+  explicit Rows(const Tensor& t) : RowSet{t.data_ptr(), {}, {}, (int)t.dim() - 1, t.sizes().back()} {
+    const auto sizes = t.sizes(), strides = t.strides();
+    int64_t reach = row;
+    for (int d = 0; d < n; ++d) {
+      stride[d] = strides[d];
+      size[d] = sizes[d];
+      reach += stride[d] * (size[d] - 1);
+    }
+    end = static_cast<const char*>(base) + 2 * reach;
+  }
+};
+
+// `out` is written while the call still reads `in`.  (Nearly always their memory
+// is apart as a whole, which is seen here.)
+void check_apart(const Rows& out, const char* out_name, const Rows& in, const char* in_name) {
+  if (out.end <= in.base || in.end <= out.base) return;
+  TORCH_CHECK(!fa::may_overlap(out, in), out_name, " must not overlap ", in_name);
+}
+
+// A result in the place of its input, row for row.
+bool same_rows(const Tensor& a, const Tensor& b) {
+  if (a.data_ptr() != b.data_ptr() || a.sizes() != b.sizes()) return false;
+  for (int d = 0; d < a.dim(); ++d)
+    if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
+}
+
 float scale_of(std::optional<double> scale, int64_t d) {
   return static_cast<float>(scale.value_or(1.0 / std::sqrt((double)d)));
 }
@@ -198,6 +231,10 @@ pybind11::object paged_forward(const Tensor& q, const Tensor& k_cache, const Ten
     check_packed(*out, "out", k_cache, q.size(0), q.size(1));
     TORCH_CHECK(!out->is_alias_of(q) || out->data_ptr() != q.data_ptr() || out->numel() == 0,
                 "out must not be q");
+    const Rows rows(*out);
+    check_apart(rows, "out", Rows(q), "q");
+    check_apart(rows, "out", Rows(k_cache), "k_cache");
+    check_apart(rows, "out", Rows(v_cache), "v_cache");
   }
   Tensor o = out ? *out : new_tensor(q.sizes(), q.scalar_type(), q);
   Tensor lse;
@@ -255,6 +292,7 @@ pybind11::tuple paged_evict(Tensor k_cache, Tensor v_cache, Tensor key_weights,
   check_no_derivative("paged_evict", {&k_cache, &v_cache, &key_weights});
   fa_paged_evict_params p{};
   p.cache = make_cache(k_cache, v_cache, block_table, std::nullopt, seq_lens);
+  check_apart(Rows(k_cache), "k_cache", Rows(v_cache), "v_cache");
   const c10::OptionalDeviceGuard guard(k_cache.device());
   p.key_weights = key_weight_ptr(key_weights, k_cache, p.w_stride);
   p.new_table = index_ptr(new_table, "new_table", 2, k_cache);
@@ -502,9 +540,19 @@ Tensor paged_store(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   check_packed(q, "q", k_cache);
   check_packed(k, "k", k_cache, q.size(0), k_cache.size(1));
   check_packed(v, "v", k_cache, q.size(0), k_cache.size(1));
+  const Rows pools[2] = {Rows(k_cache), Rows(v_cache)};
+  const Rows rows[3] = {Rows(q), Rows(k), Rows(v)};
+  const char* const pool_names[2] = {"k_cache", "v_cache"};
+  const char* const names[3] = {"q, unless it is q", "k", "v"};
+  check_apart(pools[0], "k_cache", pools[1], "v_cache");
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 3; ++j) check_apart(pools[i], pool_names[i], rows[j], j == 0 ? "q" : names[j]);
   const c10::OptionalDeviceGuard guard(q.device());
   if (out) {
     check_packed(*out, "out", k_cache, q.size(0), q.size(1));
+    const Rows result(*out);
+    for (int j = same_rows(*out, q) ? 1 : 0; j < 3; ++j) check_apart(result, "out", rows[j], names[j]);
+    for (int i = 0; i < 2; ++i) check_apart(result, "out", pools[i], pool_names[i]);
   }
   Tensor o = out ? *out : new_tensor(q.sizes(), q.scalar_type(), q);
   const NormTables t(q, qw, kw, cos, sin);

@@ -142,7 +142,7 @@ def paged_store(
     an eviction they run ahead of the places).  The pages that receive tokens
     must belong to one sequence only; tokens without a place (more tokens than
     keys, absent pages) are not stored.  Returns q's result (``out`` if given,
-    which may be q)."""
+    which may be q itself, row for row)."""
     return _EXT.paged_store(q, k, v, q_weight, k_weight, cos, sin, positions, k_cache, v_cache,
                             block_table, cu_seqlens, seq_lens, out, eps, interleaved)
 

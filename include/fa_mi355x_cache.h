@@ -28,6 +28,9 @@
  * to no sequence are not written to in o and lse.  cu_seqlens must not
  * descend: the rows and keys of sequences that do get unspecified values, and
  * nothing else is written.
+ *
+ * What a call writes shares no element with what it reads, nor k's pool with
+ * v's where both are written, unless a field says that it may.
  */
 #ifndef FA_MI355X_CACHE_H
 #define FA_MI355X_CACHE_H
