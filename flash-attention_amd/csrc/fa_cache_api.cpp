@@ -212,6 +212,9 @@ bool may_overlap(const RowSet& a, const RowSet& b) {
 namespace {
 
 constexpr int64_t kMaxKeyStride = int64_t(1) << 24;  // as the forward's seq stride
+// Rows of a call: the kernels number the rows of whole tiles, up to 128 past the
+// last one, in 31 bits.
+constexpr int64_t kMaxRows = (int64_t(1) << 31) - 256;
 
 bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
@@ -330,8 +333,8 @@ fa_status check_queries(const fa_paged_cache& c, int32_t tokens, int32_t heads, 
   if (!(scale >= FLT_MIN) || !(scale <= FLT_MAX / 2))
     return fail(FA_ERR_ARG, "softmax_scale must be from %g to %g (got %g)", (double)FLT_MIN,
                 (double)FLT_MAX / 2, (double)scale);
-  if ((int64_t)tokens * heads > 0x7fffffffLL)
-    return fail(FA_ERR_UNSUPPORTED, "tokens*heads = %lld exceeds 2^31-1", (long long)tokens * heads);
+  if ((int64_t)tokens * heads > kMaxRows)
+    return fail(FA_ERR_UNSUPPORTED, "tokens*heads = %lld exceeds 2^31-256", (long long)tokens * heads);
   if ((int64_t)c.batch * c.kv_heads > 0x7fffff)
     return fail(FA_ERR_UNSUPPORTED, "batch*kv_heads = %lld exceeds 2^23-1",
                 (long long)c.batch * c.kv_heads);
@@ -448,7 +451,7 @@ fa_status check_norm_params(const fa_qk_norm_params* p, bool backward) {
   if (p->batch < 1 || p->heads < 1 || p->kv_heads < 1 || p->seq_len < 1)
     return fail(FA_ERR_SHAPE, "batch=%d heads=%d kv_heads=%d seq_len=%d must all be >= 1", (int)p->batch,
                 (int)p->heads, (int)p->kv_heads, (int)p->seq_len);
-  if ((int64_t)p->batch * p->seq_len > 0x7fffffffLL ||
+  if ((int64_t)p->batch * p->seq_len > kMaxRows ||
       (int64_t)p->batch * p->seq_len * ((int64_t)p->heads + p->kv_heads) > (int64_t(1) << 36))
     return fail(FA_ERR_UNSUPPORTED, "batch*seq_len and its heads exceed the kernel's range");
   const int64_t qs[3] = {p->batch, p->heads, p->seq_len}, ks[3] = {p->batch, p->kv_heads, p->seq_len};
@@ -568,7 +571,8 @@ fa_status fa_paged_store_validate(const fa_paged_store_params* p) {
   FA_TRY(check_cache(c, true, true, true));
   if (p->tokens < 0 || p->heads < 1)
     return fail(FA_ERR_SHAPE, "tokens=%d must be >= 0 and heads=%d >= 1", (int)p->tokens, (int)p->heads);
-  if ((int64_t)p->tokens * ((int64_t)p->heads + 2 * c.kv_heads) > (int64_t(1) << 36))
+  if (p->tokens > kMaxRows ||
+      (int64_t)p->tokens * ((int64_t)p->heads + 2 * c.kv_heads) > (int64_t(1) << 36))
     return fail(FA_ERR_UNSUPPORTED, "tokens and heads exceed the kernel's range");
   FA_TRY(check_norm(p->q_weight, p->k_weight, p->cos, p->sin, p->rot, p->table_rows, p->interleaved,
                     p->weight_fp32, p->eps, c.head_dim));
