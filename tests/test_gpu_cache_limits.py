@@ -183,3 +183,43 @@ def test_more_kv_heads_than_compute_units(fa, new):
     c = Cache(lens, 16, KH, 64, torch.bfloat16, 720, wide=100)
     q = torch.randn(sum(new), KH, 64, generator=torch.Generator().manual_seed(5)).bfloat16()
     compare(fa, c, q, cu_of(new), max_q=max(new))
+
+
+# cu, T: offsets past the rows, before them, and descending ones that leave no row
+# to two sequences
+SENSELESS = [([0, 200, 100, 150], 100), ([-5, 3, 1000, 2000], 100), ([0, 0, 0, 0], 100), ([90, 60, 30, 0], 100),
+             ([40, 70, 2 ** 31 - 1, -2 ** 31], 100)]
+
+
+@pytest.mark.parametrize("more", [0, 70])
+@pytest.mark.parametrize("max_q", [50, 7])
+@pytest.mark.parametrize("cu,T", SENSELESS)
+def test_offsets_and_lengths_that_make_no_sense(fa, cu, T, max_q, more):
+    """Each call against its 64-bit form under the same limits, rows and weights of
+    no sequence untouched: decode and chunk kernels, lists of up to 64 sequences and
+    of more (sequences without rows behind the others)."""
+    print("case senseless", cu, max_q, more, flush=True)
+    H, KH, D, page = 4, 2, 64, 16
+    c = Cache([100, 30, 64], page, KH, D, torch.float16, 730)
+    lens = torch.tensor([2 ** 31 - 1, -7, 64] + [20] * more, dtype=torch.int32)
+    cu = torch.tensor(cu + [cu[-1]] * more, dtype=torch.int32)
+    c.table = torch.cat([c.table, torch.full((more, c.table.shape[1]), -1, dtype=torch.int32)])
+    g = torch.Generator().manual_seed(6)
+    q = torch.randn(T, H, D, generator=g).half()
+    k, v, table = c.dev()
+    out = torch.full_like(q, 5.0).to(DEV)
+    o, lse = fa.paged_forward(q.to(DEV), k, v, table, cu.to(DEV), lens.to(DEV), out, max_q=max_q, return_lse=True)
+    want, want_l, tol, tol_l = R.attend(q, c.k, c.v, c.table, cu, lens, scale=D ** -0.5, max_q=max_q)
+    # (the first sequence's length is the table's 112 keys: its rows see the NaN of keys 100 on)
+    rows = torch.zeros(T, dtype=torch.bool)
+    for _, c0, nq, _, _ in R.sequences(cu, lens, T, max_q):
+        rows[c0:c0 + nq] = True
+    R.check("o", o.cpu()[rows], want[rows], tol[rows])
+    R.check("lse", lse.cpu()[rows], want_l[rows], tol_l[rows])
+    assert bool((out.cpu()[~rows] == 5).all())
+    w = torch.rand(c.k.shape[:3], generator=g)
+    # (rows of no sequence: a logsumexp that would show)
+    given = torch.where(rows[:, None], want_l.float(), torch.tensor(-20.0))
+    wd = fa.paged_key_weights(q.to(DEV), given.to(DEV), k, table, cu.to(DEV), lens.to(DEV), w.to(DEV), max_q=max_q)
+    want_w, tol_w = R.key_weights(q, given, c.k, c.table, cu, lens, w, scale=D ** -0.5, max_q=max_q)
+    R.check("weights", wd, want_w, tol_w)
