@@ -43,10 +43,13 @@ PagedPlan plan_paged(int tokens, int batch, int kv_heads, int group, int head_di
   const int64_t keys = std::max(max_kv, 1);
   if (most > kDecodeRows) {
     // All sequences of the call, those of few rows too: one launch after the
-    // other for the two kinds was 10 to 30 % slower in every mix (us, two
-    // launches and one: 63 sequences of one token and one of 64, of up to 8000
+    // other for the two kinds was 10 to 30 % slower in mixes of like lengths (us,
+    // two launches and one: 63 sequences of one token and one of 64, of up to 8000
     // keys, 32 heads on 8, D = 128: 341, 297; 60 and 4 of 512: 493, 387; 16 of
-    // up to 64 tokens over 3000 keys: 74, 55).
+    // up to 64 tokens over 3000 keys: 74, 55).  It is not where a sequence of few
+    // rows is far longer than the others, whose tile is a whole one here: one
+    // token over 131072 keys and a prompt of 2048, 102 and 49 in two calls, 2336
+    // in one.
     g.rows = kChunkRows;
     const int64_t rows = (int64_t)tokens * group;
     g.slots = (int)(rows / kChunkRows + batch);

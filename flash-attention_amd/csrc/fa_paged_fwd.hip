@@ -13,8 +13,9 @@
 //  * fa_paged_chunk_kernel: 128 rows, four waves of 32; K/V tiles of 64 keys
 //    staged through a two-deep LDS ring by global_load_lds DMA, as
 //    fa_fwd16_kernel.  Bound by the matrix cores and the exponentials.
-//    4096 tokens over 16384 keys take 903 us, 1218 TFLOP/s (bf16, D = 128,
-//    8 kv heads; a large matrix product reaches 1200 on the card).
+//    4096 tokens over 16384 keys, 32 heads on 8, D = 128, bf16: causal 798 us,
+//    1205 TFLOP/s of visible pairs; without the mask 903 us, 1218.  (A matrix
+//    product of 8192^3 reaches 1370.)
 //  * fa_paged_decode_kernel: at most 16 or 32 rows (a few tokens), the keys of a chunk
 //    dealt to two or four waves in tiles of 32, each wave with an LDS ring of its
 //    own and no barrier before the end.  Bound by reading the cache: 5.4 TB/s at
@@ -231,9 +232,10 @@ struct WaveAttn {
       static_for<0, VD>(read_v);
     }
     // With two waves on a SIMD unit, the one in its products goes first: the
-    // other's exponentials fill the gaps.  4096 tokens over 16384 keys, bf16,
-    // 8 kv heads: D = 128 949 us without, 903 with; D = 64 543 and 552, so not
-    // there; around Q K^T as well, D = 128 takes 939.
+    // other's exponentials fill the gaps.  4096 tokens over 16384 keys, bf16, 32
+    // heads on 8, us without and with: D = 128 causal 827 and 798, without the
+    // mask 948 and 903, there 939 with Q K^T as well; D = 64 530 and 527, and 603
+    // and 601, so not there.
     constexpr bool FIRST = NKB == 4 && D == 128;
     if constexpr (FIRST) __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);

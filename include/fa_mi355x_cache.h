@@ -131,8 +131,9 @@ typedef struct {
  * of q and k.  R turns the pairs (i, i + rot/2), or with interleaved (2i,
  * 2i + 1), of the first rot dims by the angle whose cosine and sine are row
  * pos of the tables: (a, b) -> (a cos - b sin, b cos + a sin); the other dims
- * keep their value.  All in fp32, rounded once.  A position outside the tables
- * gives rows of NaN. */
+ * keep their value.  All in fp32, rounded once; the mean square overflows for
+ * rows of values above about 1e18, which become 0.  A position outside the
+ * tables gives rows of NaN. */
 typedef struct {
   const void* q;         /* [batch, heads, seq_len, head_dim], unit stride along head_dim */
   const void* k;         /* [batch, kv_heads, seq_len, head_dim] */
