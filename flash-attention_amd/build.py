@@ -35,8 +35,9 @@ BUILD_DIR = os.path.join(PKG_ROOT, "_build")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 ARCH = "gfx950"
-# Kernels and C ABI of include/fa_mi355x_cache.h.
-CACHE_SOURCES = ["fa_paged_fwd.hip", "fa_paged_cache.hip", "fa_qk_norm.hip", "fa_cache_api.cpp"]
+# Kernels and C ABI of include/fa_mi355x_cache.h and include/fa_mi355x_attention.h.
+CACHE_SOURCES = ["fa_paged_fwd.hip", "fa_paged_scored.hip", "fa_paged_cache.hip", "fa_qk_norm.hip",
+                 "fa_attention_fwd.hip", "fa_attention_bwd.hip", "fa_cache_api.cpp", "fa_attention_api.cpp"]
 # -packed-fp32-ops: keep the compiler from forming v_pk_{add,mul,fma}_f32.
 HIP_FLAGS = [
     f"--offload-arch={ARCH}",
@@ -70,7 +71,7 @@ def _hipcc() -> str:
 def build_hip_library(jobs: int) -> list[str]:
     """Compiles csrc/fa_fwd_kernel.hip (kernels and launch), fa_plan.cpp
     (host work planning), fa_api.cpp (the C ABI) and CACHE_SOURCES (the paged
-    cache's operators and the q/k norm) with hipcc and links the shared library
+    cache's operators, the q/k norm and attention with gradients) with hipcc and links the shared library
     libfa_mi355x.so.  The forward's kernel source is compiled a second
     time, and the cache's kernels too, with -DFA_LDS_POISON into the debug library
     libfa_mi355x_poison.so (same ABI; staged LDS is filled with NaN before
@@ -120,7 +121,7 @@ def build_hip_library(jobs: int) -> list[str]:
 
 def build_torch_binding() -> str:
     """Compiles the pybind/torch host binding (fa_torch_ext.cpp,
-    fa_torch_cache.cpp) with g++ and links it against libfa_mi355x.so (rpath $ORIGIN)."""
+    fa_torch_cache.cpp, fa_torch_attention.cpp) with g++ and links it against libfa_mi355x.so (rpath $ORIGIN)."""
     import torch
     from torch.utils import cpp_extension
 
@@ -135,7 +136,7 @@ def build_torch_binding() -> str:
         "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
         *[f"-I{p}" for p in incs],
-        os.path.join(CSRC, "fa_torch_ext.cpp"), os.path.join(CSRC, "fa_torch_cache.cpp"),
+        *[os.path.join(CSRC, f) for f in ("fa_torch_ext.cpp", "fa_torch_cache.cpp", "fa_torch_attention.cpp")],
         f"-L{OUT_DIR}", "-lfa_mi355x",
         f"-L{torch_lib}", "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10_hip",
         "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}",

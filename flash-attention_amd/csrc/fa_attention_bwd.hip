@@ -1,0 +1,777 @@
+// Gradients of attention with capped, biased and masked scores, on gfx950.
+//
+//   delta_i = go_i.o_i - glse_i;  dS = P (go_i.v_j - delta_i) (1 - (c / cap)^2)
+//   gv_j = sum_i P go_i;  gk_j = scale sum_i dS q_i;  gq_i = scale sum_j dS k_j
+//
+// P is computed again from the logsumexp.  Three kernels, no atomics: sums run in
+// a fixed order, at the price of computing scores and go.v twice (7 products of
+// the size of q.k in place of 5):
+//  * fa_attn_rows_kernel: delta, the keys that each row sees, and, for every span
+//    of 32 rows, their limits.
+//  * fa_attn_dkv_kernel: 256 keys of a kv head, 64 to a pair of waves; passes over
+//    the spans of 32 rows that see any of them, of all query heads of the group,
+//    staged through a ring.  One wave of a pair holds K and gv, does S = Q K^T, P and
+//    gv^T += go^T P and leaves P in LDS; the other holds V and gk and does
+//    go V^T, dS and gk^T += Q^T dS a span later.  (One wave cannot hold both
+//    accumulators of D = 128 for as many keys, and an LDS read of rows has to feed four
+//    products: with two, reading at full rate takes as long as they do.)  S and go V^T
+//    come out with lanes along the keys, as P and dS have to go in.
+//  * fa_attn_dq_kernel: 128 rows of a head, as the forward pass.
+//
+// Rounding: P and dS are rounded to the input type for the matrix cores (as P of
+// the forward pass); all sums are fp32.  fp16 has few exponents: P is scaled by
+// 2^12, so that it keeps its 11 bits down to 2^-26, and dS by a power of two that brings
+// the largest |go| (of the rows of a dk, dv workgroup; of a dq row) to 2^-12 .. 2^-11.
+//
+// Masked keys and rows contribute nothing whatever they hold: their P and dS are
+// 0, and infinities and NaN among the staged rows of a tile that is not seen
+// whole are cleared (clean_rows); rows and keys that do see one get NaN.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "fa_attention_ops.h"
+#include "fa_wave_attn.h"
+
+namespace fa {
+namespace {
+
+using namespace dev;
+
+template <bool BF16>
+constexpr float kShift = BF16 ? 0.0f : 12.0f;  // log2 of P's factor
+
+// The record of a span, [2][4 fields][16 rows] floats: for each 16 rows
+enum RecordField { kLse, kDelta, kLo, kHi };  // (lse in log2, less kShift)
+constexpr int kRecord = kSpan * 4;
+
+// 2^-(e + 12) for a largest |go| in [2^e, 2^(e + 1)): dS's factor.  1 for bf16.
+template <bool BF16>
+__device__ __forceinline__ float grad_factor(float top) {
+  if constexpr (BF16) return 1.0f;
+  const int e = (int)((__builtin_bit_cast(uint32_t, top) >> 23) & 255) - 127;
+  if (e < -24 || e > 15) return 1.0f;  // 0, or no number
+  return __builtin_bit_cast(float, (uint32_t)(127 - 12 - e) << 23);
+}
+
+template <bool BF16>
+__device__ __forceinline__ void unpack2(uint32_t u, float* f) {
+  if constexpr (BF16) {
+    f[0] = __builtin_bit_cast(float, u << 16);
+    f[1] = __builtin_bit_cast(float, u & 0xffff0000u);
+  } else {
+    const f16x2 x = __builtin_bit_cast(f16x2, u);
+    f[0] = (float)x[0];
+    f[1] = (float)x[1];
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ void unpack8(u32x4 w, float* f) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) unpack2<BF16>(w[j], f + 2 * j);
+}
+
+// ---- rows ----
+
+// 64 rows of one head a workgroup, D / 8 lanes a row.  Bound by reading go and o.
+constexpr int kRowsBlock = 64;
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) fa_attn_rows_kernel(const AttnArgs a) {
+  constexpr int LPR = D / 8, RPP = 256 / LPR;  // rows of a pass
+  __shared__ float delta[kRowsBlock], top[kRowsBlock];
+  const int blocks = (a.n + kRowsBlock - 1) / kRowsBlock;
+  const int bh = blockIdx.x / blocks, block = blockIdx.x - bh * blocks;
+  const int b = bh / a.heads, h = bh - b * a.heads;
+  const char* gh = a.go.p + b * a.go.sb + h * a.go.sh;
+  const char* oh = a.o.p + b * a.o.sb + h * a.o.sh;
+#pragma unroll
+  for (int r0 = 0; r0 < kRowsBlock; r0 += RPP) {
+    const int r = r0 + (int)threadIdx.x / LPR;
+    const int64_t i = min(block * kRowsBlock + r, a.n - 1);
+    const int at = (int)threadIdx.x % LPR * 16;
+    float g[8], o[8], sum = 0.0f, most = 0.0f;
+    unpack8<BF16>(*reinterpret_cast<const u32x4*>(gh + i * a.go.st + at), g);
+    unpack8<BF16>(*reinterpret_cast<const u32x4*>(oh + i * a.o.st + at), o);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      sum = fmaf(g[j], o[j], sum);
+      most = fmaxf(most, fabsf(g[j]));
+    }
+#pragma unroll
+    for (int d = 1; d < LPR; d <<= 1) {
+      sum += __shfl_xor(sum, d);
+      most = fmaxf(most, __shfl_xor(most, d));
+    }
+    if (threadIdx.x % LPR == 0) {
+      delta[r] = sum;
+      top[r] = most;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x >= kRowsBlock) return;
+  const int r = threadIdx.x, i = block * kRowsBlock + r, span = i / kSpan;
+  RowKeys k = {kNoKey, 0};
+  float lse = INFINITY, d = 0.0f, most = 0.0f;  // P = 0
+  if (i < a.n) {
+    k = row_keys(a, b, i);
+    if (k.hi > 0) {
+      const int64_t at = (int64_t)bh * a.n + i;
+      lse = a.lse[at] * kLog2e - kShift<BF16>;
+      d = delta[r] - (a.glse != nullptr ? a.glse[at] : 0.0f);
+      most = top[r];
+    }
+  }
+  TileKeys t;
+  t.start(k);
+  t.reduce<kSpan>();
+  if constexpr (!BF16) {
+#pragma unroll
+    for (int w = 1; w < kSpan; w <<= 1) most = fmaxf(most, __shfl_xor(most, w));
+  }
+  if (span >= a.spans) return;
+  const int64_t bhs = (int64_t)bh * a.spans + span;
+  float* rec = a.records + bhs * kRecord + (r % kSpan >> 4) * 64 + (r & 15);
+  rec[16 * kLse] = lse;
+  rec[16 * kDelta] = d;
+  rec[16 * kLo] = __builtin_bit_cast(float, k.lo);
+  rec[16 * kHi] = __builtin_bit_cast(float, k.hi);
+  if (r % kSpan != 0) return;
+  if (h == 0)
+    reinterpret_cast<int4*>(a.bounds)[(int64_t)b * a.spans + span] = int4{t.lo, t.hi, t.all_lo, t.all_hi};
+  if constexpr (!BF16) a.tops[bhs] = most;
+}
+
+// ---- scores and their gradients, four at a time ----
+
+// A value that is the same in every lane, in a scalar register.
+__device__ __forceinline__ float uniform(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
+// The compiler takes x as new here: it is computed before, and what is computed from
+// it after, not kept in registers from outside of a loop.
+template <class T>
+__device__ __forceinline__ T fresh(T x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+template <bool CAP>
+struct Grads {
+  Score score;
+  float slope, unit;  // unit: of the score that the exponent takes
+  __device__ __forceinline__ void init(const AttnArgs& a, int h) {
+    score.init(a.score);
+    slope = uniform(score.biased ? a.score.slopes[h] * kLog2e : 0.0f);
+    unit = uniform(CAP || score.biased ? 1.0f : a.scale_log2);
+  }
+  // (scores q.k, capped and biased); away: from a score's row to its key.
+  __device__ __forceinline__ float capped(float x) const { return CAP ? score.cap(x) : x; }
+  __device__ __forceinline__ float biased(float x, float away) const {
+    return fmaf(-slope, fabsf(away), CAP ? x : x * score.unit);
+  }
+  // P's factor 1 - tanh^2 from its exponent, plus lse, less the bias: the capped
+  // score.  A masked one's, -inf, and a NaN have 0.
+  __device__ __forceinline__ float slope_of(float x) const {
+    const float t = x * score.inverse;
+    return fmaxf(fmaf(-t, t, 1.0f), 0.0f);
+  }
+};
+
+template <bool BF16>
+__device__ __forceinline__ i16x8 pack8(const f32x4& x, const f32x4& y) {
+  return __builtin_bit_cast(i16x8, u32x4{pack2<BF16>(x[0], x[1]), pack2<BF16>(x[2], x[3]),
+                                         pack2<BF16>(y[0], y[1]), pack2<BF16>(y[2], y[3])});
+}
+
+__device__ __forceinline__ f32x4 lds_quad(uint32_t addr) {
+  return __builtin_bit_cast(f32x4, lds_read16<0>(addr));
+}
+
+// c[cb] = sum over D of the 16 rows at LDS address `at` (a lane's offset in it)
+// times the 16 NCB columns held in f.
+template <int D, bool BF16, int NCB>
+__device__ __forceinline__ void row_product(uint32_t at, const i16x8 (&f)[NCB][D / 32], f32x4 (&c)[NCB]) {
+  constexpr int KST = D / 32, AHEAD = NCB > 2 ? 2 : KST < 3 ? KST : 3;
+  const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+  i16x8 x[AHEAD];
+  auto read = [&](auto i_c) FA_INLINE {
+    constexpr int st = decltype(i_c)::value;
+    x[st % AHEAD] = lds_read16<0>(at ^ lds::TileBoth<D>::row_step(st));
+  };
+  static_for<0, AHEAD>(read);
+  __builtin_amdgcn_sched_barrier(0);
+  static_for<0, KST>([&](auto i_c) FA_INLINE {
+    constexpr int st = decltype(i_c)::value;
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) c[cb] = mfma16<BF16>(x[st % AHEAD], f[cb][st], st == 0 ? zero : c[cb]);
+    if constexpr (st + AHEAD < KST) read(std::integral_constant<int, st + AHEAD>{});
+    __builtin_amdgcn_sched_barrier(0);
+  });
+}
+
+// acc[db][cb] += the 32 rows at LDS address `at`, turned, times f[cb].
+template <int D, bool BF16, int NCB>
+__device__ __forceinline__ void turned_product(uint32_t at, const i16x8 (&f)[NCB], f32x4 (&acc)[D / 16][NCB]) {
+  constexpr int DB = D / 16, AHEAD = NCB > 2 ? 2 : 4, ROWB = 2 * D;
+  i16x8 x[AHEAD];
+  auto read = [&](auto i_c) FA_INLINE {
+    constexpr int db = decltype(i_c)::value;
+    x[db % AHEAD] = ds_read_tr_pair<0, 16 * ROWB>(at ^ lds::TileBoth<D>::turned_block(db));
+  };
+  static_for<0, AHEAD>(read);
+  __builtin_amdgcn_sched_barrier(0);
+  static_for<0, DB>([&](auto i_c) FA_INLINE {
+    constexpr int db = decltype(i_c)::value;
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) acc[db][cb] = mfma16<BF16>(x[db % AHEAD], f[cb], acc[db][cb]);
+    if constexpr (db + AHEAD < DB) read(std::integral_constant<int, db + AHEAD>{});
+    __builtin_amdgcn_sched_barrier(0);
+  });
+}
+
+// ---- gradients of k and v ----
+
+template <int D, bool BF16, bool CAP>
+struct DkvWave {
+  static constexpr int ROWB = 2 * D, KST = D / 32, DB = D / 16, NCB = kAttnKeys / 64;
+  static constexpr int TB = kSpan * ROWB, SLOT = 2 * TB + 1024, SLOTS = 4;  // bytes: Q, go, record
+  static constexpr int PB = NCB * 1024;                                     // of a pair's P
+  static constexpr int WPT = D / 32;  // waves that stage a tensor's rows
+  static constexpr int NI = kSpan / WPT * ROWB / 1024, LPR = ROWB / 16;
+  static_assert(NI == 2, "two copies a wave");
+  struct Shared {
+    char ring[SLOTS * SLOT];
+    char p[8 * PB];
+    float spoiled[SLOTS][2][kSpan];  // NaN for rows of Q, of go with an infinity or NaN, else 0
+    float top[8];
+  };
+  struct Item {  // a span of rows
+    int head, span;          // head < 0: none
+    bool seen, whole, all;   // the pair's keys by some row, by all; the workgroup's by all
+  };
+
+  // SECOND: the half that does go V^T, dS and gk.
+  template <bool SECOND>
+  static __device__ __forceinline__ void run(const AttnArgs& a, Shared& sh) {
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pair = wave & 3;
+    // As the forward pass, the first keys first: a causal mask's longest.
+    const int unit_blocks = a.key_tiles * a.splits;
+    const int at = xcd_remap(blockIdx.x, gridDim.x);
+    const int unit = fast_div(at, a.by_keys), within = at - unit * unit_blocks;
+    const int tile = fast_div(within, a.by_splits), split = within - tile * a.splits;
+    const int b = fast_div(unit, a.by_kvh), kvh = unit - b * a.kv_heads, h0 = kvh * a.group;
+    const int j0 = tile * kAttnKeys, w0 = j0 + 16 * NCB * pair;
+
+    i16x8 f[NCB][KST];
+    {
+      const Rows3& x = SECOND ? a.v : a.k;
+      const char* xp = x.p + b * x.sb + kvh * x.sh + 16 * g4;
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        const int64_t j = min(w0 + 16 * cb + l16, a.m - 1);
+#pragma unroll
+        for (int st = 0; st < KST; ++st) f[cb][st] = *reinterpret_cast<const i16x8*>(xp + j * x.st + 64 * st);
+      }
+    }
+    float factor = 1.0f;
+    if constexpr (!BF16) {
+      float top = 0.0f;
+      const float* tops = a.tops + ((int64_t)b * a.heads + h0) * a.spans;
+      for (int64_t i = threadIdx.x; i < (int64_t)a.group * a.spans; i += 512) top = fmaxf(top, tops[i]);
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+      if (lane == 0) sh.top[wave] = top;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, sh.top[i]);
+      factor = uniform(grad_factor<BF16>(uniform(top)));
+    }
+    f32x4 acc[DB][NCB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) acc[db][cb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    // The spans with a row that sees a key of the workgroup, of the split's (every
+    // splits-th, so that the splits of a causal mask are alike), head after head:
+    // bit i of `hit` is span at0 + i.
+    const int4* bounds = reinterpret_cast<const int4*>(a.bounds) + (int64_t)b * a.spans;
+    uint64_t hit = 0, seen = 0, whole = 0, all = 0;
+    int h = 0, at0 = -64;
+    auto next = [&]() FA_INLINE -> Item {
+      while (hit == 0) {
+        at0 += 64;
+        if (at0 >= a.spans) {
+          at0 = 0;
+          if (++h >= a.group) return Item{-1, 0, false, false, false};
+        }
+        const int s = at0 + lane;
+        int4 k = {kNoKey, 0, kNoKey, 0};
+        if (s < a.spans) k = bounds[s];
+        const bool mine = s - fast_div(s, a.by_splits) * a.splits == split;
+        hit = __ballot(mine && k.x < j0 + kAttnKeys && k.y > j0);
+        seen = __ballot(k.x < w0 + 16 * NCB && k.y > w0);
+        whole = __ballot(k.z <= w0 && k.w >= w0 + 16 * NCB);
+        all = __ballot(k.z <= j0 && k.w >= j0 + kAttnKeys);
+      }
+      const int i = __builtin_ctzll(hit);
+      hit &= hit - 1;
+      return Item{h, at0 + i, (bool)((seen >> i) & 1), (bool)((whole >> i) & 1), (bool)((all >> i) & 1)};
+    };
+
+    // Staging: at D = 128 all waves copy 8 rows each, the first ones of Q, the others
+    // of go; at D = 64 four waves copy 16 rows.  Wave 0 brings the record.
+    const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(&sh));
+    const int sr = wave % WPT * (kSpan / WPT);  // this wave's first row
+    const bool stages = wave < 2 * WPT, of_go = wave >= WPT;
+    const Rows3& sx = of_go ? a.go : a.q;
+    const char* sp = sx.p + b * sx.sb + h0 * sx.sh;
+    const uint32_t sst = (uint32_t)sx.st, sto = (of_go ? TB : 0) + sr * ROWB;
+    const char* records = reinterpret_cast<const char*>(a.records + ((int64_t)b * a.heads + h0) * a.spans * kRecord);
+    auto issue = [&](const Item& x, int slot) FA_INLINE {
+      if (!stages) return;
+      const int r0 = min(x.span * kSpan + sr, a.n - 1), lim = a.n - 1 - r0;
+      const char* p = sp + x.head * sx.sh + r0 * sx.st;
+      const uint32_t dst = base + slot * SLOT + sto;
+      const int l = fresh(lane);
+#pragma unroll
+      for (int it = 0; it < NI; ++it) {
+        poison_1k(dst + it * 1024);
+        const int r = it * (64 / LPR) + l / LPR, c = (l % LPR) ^ lds::TileBoth<D>::swz(sr + r);
+        dma_16b(min(r, lim) * sst + c * 16, p, dst + it * 1024);
+      }
+      if (wave == 0) {  // (1 KiB: the next record too, or what is behind the last one)
+        poison_1k(base + slot * SLOT + 2 * TB);
+        dma_16b(l * 16, records + ((int64_t)x.head * a.spans + x.span) * kRecord * 4, base + slot * SLOT + 2 * TB);
+      }
+    };
+    // The copies of a span are there, `later`: but for those of one issued after it.
+    // If the span is not seen whole, this wave cleans the rows that it has copied.
+    const uint32_t spoiled_at = base + offsetof(Shared, spoiled);
+    auto finish = [&](const Item& x, int slot, bool later) FA_INLINE {
+      if (later && stages) {
+        if (wave == 0)
+          wait_vmcnt<NI + 1>();
+        else
+          wait_vmcnt<NI>();
+      } else {
+        wait_vmcnt<0>();
+      }
+      if (stages && x.head >= 0 && !x.all) {
+        const unsigned bad = clean_rows<D, BF16, kSpan / WPT>(base + slot * SLOT + sto);
+        if (lane < kSpan / WPT)
+          lds_write4(spoiled_at + (slot * 2 + (of_go ? 1 : 0)) * kSpan * 4 + (sr + lane) * 4,
+                     (bad >> lane) & 1 ? NAN : 0.0f);
+      }
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+      __syncthreads();
+    };
+
+    Grads<CAP> grads;
+    const uint32_t row_at = base + (SECOND ? TB : 0), turned_at = base + (SECOND ? 0 : TB);
+    const uint32_t p_at = base + offsetof(Shared, p) + pair * 2 * PB;
+
+    // A span in `slot`, P in buffer pb.  (Scores become P in place: the accumulators
+    // leave few registers.)
+    auto step = [&](int row0, int slot, int pb, bool masked) FA_INLINE {
+      const int l = fresh(lane);  // (nothing below is worth a register across spans)
+      const int key0 = w0 + (l & 15);
+      u32x4 w[NCB];  // P or dS as packed pairs: words 0, 1 of rows 4 g4 .., 2, 3 of those 16 on
+      static_for<0, 2>([&](auto rb_c) FA_INLINE {
+        constexpr int rb = decltype(rb_c)::value;
+        f32x4 c[NCB];
+        row_product<D, BF16, NCB>(row_at + slot * SLOT + rb * 16 * ROWB + lds::TileBoth<D>::row_offset(l), f, c);
+        const uint32_t quad = base + slot * SLOT + 2 * TB + rb * 256 + (l >> 4) * 16;
+        const uint32_t p_quad = p_at + pb * PB + rb * 512 + l * 8;
+        f32x4 stat = lds_quad(quad + (SECOND ? 64 * kDelta : 64 * kLse));
+        // (two blocks at a time: all at once would take more registers than there are)
+        auto each = [&](auto&& fn) FA_INLINE {
+#pragma unroll
+          for (int cb = 0; cb < NCB; ++cb) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[cb][i] = fn(c[cb][i], cb, i);
+            if (cb % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+          }
+        };
+        const int away = row0 + 16 * rb + 4 * (l >> 4) + a.m - a.n - key0;  // of key block 0
+        auto away_of = [&](int cb, int i) FA_INLINE { return (float)(away - 16 * cb) + (float)i; };
+        if constexpr (!SECOND) {
+          if (masked) {
+            const uint32_t bad = spoiled_at + slot * 2 * kSpan * 4 + rb * 64 + (l >> 4) * 16;
+            stat += lds_quad(bad) + lds_quad(bad + kSpan * 4);
+          }
+          if constexpr (CAP) each([&](float x, int, int) FA_INLINE { return grads.capped(x); });
+          if (grads.score.biased)
+            each([&](float x, int cb, int i) FA_INLINE { return grads.biased(x, away_of(cb, i)); });
+          each([&](float x, int, int i) FA_INLINE { return fmaf(x, grads.unit, -stat[i]); });
+        } else {
+          each([&](float x, int, int i) FA_INLINE { return x - stat[i]; });
+        }
+        if (masked) {  // P = 2^-inf; dS = P 0
+          const float none = SECOND ? 0.0f : -INFINITY;
+          const i32x4 lo = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kLo)) - key0;
+          each([&](float x, int cb, int i) FA_INLINE { return fresh(16 * cb >= lo[i] ? x : none); });
+          const i32x4 hi = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kHi)) - key0;
+          each([&](float x, int cb, int i) FA_INLINE { return 16 * cb < hi[i] ? x : none; });
+        }
+        static_for<0, NCB>([&](auto cb_c) FA_INLINE {
+          constexpr int cb = decltype(cb_c)::value;
+          f32x4 x;
+          if constexpr (SECOND) {
+            const u32x2 pw = lds_read8<cb * 1024>(p_quad);
+            float p[4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) unpack2<BF16>(pw[j], p + 2 * j);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = (BF16 ? p[i] : p[i] * factor) * c[cb][i];
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = fast_exp2(c[cb][i]);
+          }
+          const u32x2 out = {pack2<BF16>(x[0], x[1]), pack2<BF16>(x[2], x[3])};
+          w[cb][2 * rb] = fresh((uint32_t)out[0]);
+          w[cb][2 * rb + 1] = fresh((uint32_t)out[1]);
+          if constexpr (!SECOND) {
+            u32x2 mate = out;
+            if constexpr (CAP) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                float u = c[cb][i] + stat[i];
+                if (grads.score.biased) u = fmaf(grads.slope, fabsf(away_of(cb, i)), u);
+                x[i] *= grads.slope_of(u);
+              }
+              mate = u32x2{pack2<BF16>(x[0], x[1]), pack2<BF16>(x[2], x[3])};
+            }
+            lds_write8<cb * 1024>(p_quad, mate);
+          }
+          if constexpr (CAP || cb % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+        });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      i16x8 wf[NCB];
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) wf[cb] = __builtin_bit_cast(i16x8, w[cb]);
+      turned_product<D, BF16, NCB>(turned_at + slot * SLOT + lds::TileBoth<D>::turned_offset(fresh(lane)), wf, acc);
+    };
+
+    // Spans t + 1 and t + 2 are on their way while the first waves have t and the
+    // second ones t - 1.
+    Item before = {-1, 0, false, false, false}, now = next(), then = before;
+    int slot = 0, pb = 0, head = -1;
+    wait_vmcnt<0>();  // (what was loaded so far: no wait for it later, which would be one for copies too)
+    if (now.head >= 0) {
+      issue(now, 0);
+      then = next();
+      if (then.head >= 0) issue(then, 1);
+      finish(now, 0, then.head >= 0);
+    }
+    while (now.head >= 0 || before.head >= 0) {
+      Item last = {-1, 0, false, false, false};
+      if (then.head >= 0) last = next();
+      if (last.head >= 0) issue(last, (slot + 2) % SLOTS);
+      const Item mine = SECOND ? before : now;
+      if (mine.head >= 0 && mine.seen) {
+        if (mine.head != head) {
+          head = mine.head;
+          grads.init(a, h0 + head);
+        }
+        step(mine.span * kSpan, SECOND ? (slot + SLOTS - 1) % SLOTS : slot, SECOND ? pb ^ 1 : pb, !mine.whole);
+      }
+      finish(then, (slot + 1) % SLOTS, last.head >= 0);
+      before = now;
+      now = then;
+      then = last;
+      slot = (slot + 1) % SLOTS;
+      pb ^= 1;
+    }
+
+    // (powers of two but for the scale)
+    const float out = SECOND ? a.scale * fast_exp2(-kShift<BF16>) / factor : fast_exp2(-kShift<BF16>);
+    const int l = fresh(lane);
+    if (a.parts != nullptr) {
+      const int64_t rows = (int64_t)a.batch * a.kv_heads * a.m;
+      float* to = a.parts + ((int64_t)split * rows + (int64_t)unit * a.m) * 2 * D + (SECOND ? 0 : D) + 4 * (l >> 4);
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        const int j = w0 + 16 * cb + (l & 15);
+        if (j >= a.m) continue;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          *reinterpret_cast<f32x4*>(to + (int64_t)j * 2 * D + 16 * db) = acc[db][cb] * out;
+      }
+      return;
+    }
+    const Rows3& y = SECOND ? a.gk : a.gv;
+    char* yp = y.p + b * y.sb + kvh * y.sh;
+    const float outs[2] = {out, out};
+    static_for<0, NCB / 2>([&](auto i_c) FA_INLINE {
+      constexpr int i = decltype(i_c)::value;
+      f32x4 part[DB][2];
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb) part[db][cb] = acc[db][2 * i + cb];
+      write_rows<D, BF16>(sh.ring + wave * 32 * ROWB, part, outs, l, [&](int r) FA_INLINE -> char* {
+        const int j = w0 + 32 * i + r;
+        return j < a.m ? yp + j * y.st : nullptr;
+      });
+    });
+  }
+};
+
+template <int D, bool BF16, bool CAP>
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+    fa_attn_dkv_kernel(const AttnArgs a) {
+  using W = DkvWave<D, BF16, CAP>;
+  static_assert(4 * 32 * 2 * D * 2 <= sizeof(typename W::Shared), "rows on their way out");
+  __shared__ __attribute__((aligned(1024))) typename W::Shared sh;
+  // Waves 0..3 and 4..7: the two of a pair share a SIMD unit, one's exponentials
+  // beside the other's products.  Both halves pass the same barriers.
+  if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 8) == 0)
+    W::template run<false>(a, sh);
+  else
+    W::template run<true>(a, sh);
+}
+
+// Adds the splits' parts in their order: 8 elements a thread.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) fa_attn_join_kernel(const AttnArgs a) {
+  constexpr int TPR = 2 * D / 8;  // threads of a key
+  const int64_t rows = (int64_t)a.batch * a.kv_heads * a.m;
+  const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  if (row >= rows) return;
+  const int d = (int)threadIdx.x % TPR * 8;
+  f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = x;
+  for (int s = 0; s < a.splits; ++s) {
+    const float* from = a.parts + (s * rows + row) * 2 * D + d;
+    x += *reinterpret_cast<const f32x4*>(from);
+    y += *reinterpret_cast<const f32x4*>(from + 4);
+  }
+  const int64_t unit = row / a.m, j = row - unit * a.m;
+  const int64_t b = unit / a.kv_heads, kvh = unit - b * a.kv_heads;
+  const Rows3& to = d < D ? a.gk : a.gv;
+  *reinterpret_cast<i16x8*>(to.p + b * to.sb + kvh * to.sh + j * to.st + (d % D) * 2) = pack8<BF16>(x, y);
+}
+
+// ---- gradients of q ----
+
+template <int D, bool BF16, bool CAP>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+    fa_attn_dq_kernel(const AttnArgs a) {
+  constexpr int ROWB = 2 * D, TB = 64 * ROWB, KST = D / 32, DB = D / 16;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * TB];  // K0 V0 K1 V1
+  __shared__ TileKeys part[4];
+
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int unit_blocks = a.tiles * a.group;
+  const int at = xcd_remap(blockIdx.x, gridDim.x);
+  const int unit = fast_div(at, a.by_unit), within = at - unit * unit_blocks;
+  const int back = fast_div(within, a.by_group);
+  const int b = fast_div(unit, a.by_kvh), kvh = unit - b * a.kv_heads;
+  const int h = kvh * a.group + within - back * a.group;
+  const int row0 = (a.tiles - 1 - back) * kAttnRows, wrow0 = row0 + 32 * wave;
+
+  i16x8 qf[2][KST], gf[2][KST];
+  float lse[2], delta[2], factor[2];
+  RowKeys see[2];
+  TileKeys keys;
+#pragma unroll
+  for (int rb = 0; rb < 2; ++rb) {
+    const int r = min(wrow0 + 16 * rb + l16, a.n - 1);
+    const int64_t i = r;
+    const char* qp = a.q.p + b * a.q.sb + h * a.q.sh + i * a.q.st + 16 * g4;
+    const char* gp = a.go.p + b * a.go.sb + h * a.go.sh + i * a.go.st + 16 * g4;
+#pragma unroll
+    for (int st = 0; st < KST; ++st) {
+      qf[rb][st] = *reinterpret_cast<const i16x8*>(qp + 64 * st);
+      gf[rb][st] = *reinterpret_cast<const i16x8*>(gp + 64 * st);
+    }
+    const float* rec = a.records + (((int64_t)b * a.heads + h) * a.spans + r / kSpan) * kRecord +
+                       r % kSpan / 16 * 64 + r % 16;
+    lse[rb] = rec[16 * kLse];
+    delta[rb] = rec[16 * kDelta];
+    see[rb].lo = __builtin_bit_cast(int, rec[16 * kLo]);
+    see[rb].hi = __builtin_bit_cast(int, rec[16 * kHi]);
+    TileKeys t;
+    t.start(see[rb]);
+    if (rb == 0)
+      keys = t;
+    else
+      keys.add(t);
+    factor[rb] = 1.0f;
+    if constexpr (!BF16) {
+      float top = 0.0f;
+#pragma unroll
+      for (int st = 0; st < KST; ++st) {
+        float f[8];
+        unpack8<BF16>(__builtin_bit_cast(u32x4, gf[rb][st]), f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(f[j]));
+      }
+      factor[rb] = grad_factor<BF16>(WaveAttn<D, BF16, 4, 2>::red_max(top));
+    }
+  }
+  keys.reduce<16>();
+  if (lane == 0) part[wave] = keys;
+  __syncthreads();
+  TileKeys all = part[0];
+#pragma unroll
+  for (int i = 1; i < 4; ++i) all.add(part[i]);
+  keys.uniform();
+  all.uniform();
+
+  const int c0 = all.lo, c1 = all.hi;
+  const int n_tiles = c0 < c1 ? (c1 - c0 + 63) / 64 : 0;
+  const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(smem));
+  const char* kh = a.k.p + b * a.k.sb + kvh * a.k.sh;
+  const char* vh = a.v.p + b * a.v.sb + kvh * a.v.sh;
+  RowStage<D> stage_k;
+  RowStage<D> stage_v;
+  stage_k.init(lane, (uint32_t)a.k.st);
+  stage_v.init(lane, (uint32_t)a.v.st);
+  auto issue = [&](int t, int buf) FA_INLINE {
+    const int r0 = min(c0 + 64 * t + 16 * wave, c1 - 1);
+    const uint32_t dst = base + buf * 2 * TB + wave * 16 * ROWB;
+    stage_k.copy(kh + r0 * a.k.st, dst, c1 - 1 - r0, (uint32_t)a.k.st);
+    stage_v.copy(vh + r0 * a.v.st, dst + TB, c1 - 1 - r0, (uint32_t)a.v.st);
+  };
+  // The staged keys of tile t are there: cleaned if some row does not see all of
+  // them, with V's rows set to NaN for the ones that do.
+  auto finish = [&](int t, int buf) FA_INLINE {
+    __builtin_amdgcn_s_waitcnt(0);
+    const int k0 = c0 + 64 * t;
+    if (t < n_tiles && !(k0 >= all.all_lo && k0 + 64 <= all.all_hi)) {
+      const uint32_t rows = base + buf * 2 * TB + wave * 16 * ROWB;
+      const unsigned bad = clean_rows<D, BF16, 16>(rows);
+      if (__builtin_expect(bad != 0, false)) {
+        constexpr int LPR = ROWB / 16;
+        for (int r = lane / LPR; r < 16; r += 64 / LPR)
+          if ((bad >> r) & 1) lds_write16(rows + TB + r * ROWB + lane % LPR * 16, u32x4{~0u, ~0u, ~0u, ~0u});
+      }
+      __builtin_amdgcn_s_waitcnt(0);
+    }
+    __syncthreads();
+  };
+
+  f32x4 gq[DB][2];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) gq[db][rb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const uint32_t row_at = base + lds::TileBoth<D>::row_offset(lane);
+  const uint32_t turned_at = base + lds::TileBoth<D>::turned_offset(lane);
+  Grads<CAP> grads;
+  grads.init(a, h);
+  const int ahead = a.m - a.n;
+
+  // 32 keys from k0, in half `half` of the tile.
+  auto step = [&](int k0, int off, int half, bool masked) FA_INLINE {
+    const uint32_t rows = row_at + off + half * 32 * ROWB;
+    f32x4 s[2][2], dp[2][2];
+    static_for<0, 2>([&](auto kb_c) FA_INLINE {
+      constexpr int kb = decltype(kb_c)::value;
+      row_product<D, BF16, 2>(rows + kb * 16 * ROWB, qf, s[kb]);
+      row_product<D, BF16, 2>(rows + TB + kb * 16 * ROWB, gf, dp[kb]);
+    });
+    i16x8 df[2];
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) {
+      const int key0 = k0 + 4 * g4;
+      const int pos = min(wrow0 + 16 * rb + l16, a.n - 1) + ahead;
+      auto away_of = [&](int kb, int i) FA_INLINE { return (float)(key0 + 16 * kb - pos) + (float)i; };
+      auto each = [&](auto&& fn) FA_INLINE {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[kb][rb][i] = fn(s[kb][rb][i], kb, i);
+      };
+      if constexpr (CAP) each([&](float x, int, int) FA_INLINE { return grads.capped(x); });
+      if (grads.score.biased)
+        each([&](float x, int kb, int i) FA_INLINE { return grads.biased(x, away_of(kb, i)); });
+      each([&](float x, int kb, int i) FA_INLINE {
+        const float e = fmaf(x, grads.unit, -lse[rb]);
+        float p = fast_exp2(e);
+        if constexpr (CAP) {
+          float u = e + lse[rb];
+          if (grads.score.biased) u = fmaf(grads.slope, fabsf(away_of(kb, i)), u);
+          p *= grads.slope_of(u);
+        }
+        if constexpr (!BF16) p *= factor[rb];
+        return p * (dp[kb][rb][i] - delta[rb]);
+      });
+      if (masked)
+        each([&](float x, int kb, int i) FA_INLINE {
+          const int key = key0 + 16 * kb + i;
+          return key >= see[rb].lo && key < see[rb].hi ? x : 0.0f;
+        });
+      df[rb] = pack8<BF16>(s[0][rb], s[1][rb]);
+    }
+    turned_product<D, BF16, 2>(turned_at + off + half * 32 * ROWB, df, gq);
+  };
+
+  if (n_tiles > 0) {
+    issue(0, 0);
+    finish(0, 0);
+  }
+  int buf = 0;
+  for (int t = 0; t < n_tiles; ++t, buf ^= 1) {
+    const int k0 = c0 + 64 * t;
+    if (t + 1 < n_tiles) issue(t + 1, buf ^ 1);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int k = k0 + 32 * half;
+      if (k >= keys.all_lo && k + 32 <= keys.all_hi)
+        step(k, buf * 2 * TB, half, false);
+      else if (k < keys.hi && k + 32 > keys.lo)
+        step(k, buf * 2 * TB, half, true);
+    }
+    finish(t + 1, buf ^ 1);
+  }
+
+  float f[2];
+#pragma unroll
+  for (int rb = 0; rb < 2; ++rb) f[rb] = a.scale * fast_exp2(-kShift<BF16>) / factor[rb];
+  char* qh = a.gq.p + b * a.gq.sb + h * a.gq.sh;
+  write_rows<D, BF16>(smem + wave * 32 * ROWB, gq, f, lane, [&](int r) FA_INLINE -> char* {
+    return wrow0 + r < a.n ? qh + (wrow0 + r) * a.gq.st : nullptr;
+  });
+}
+
+template <class F>
+hipError_t launch(F* fn, int64_t grid, const AttnArgs& a, hipStream_t stream, int threads = 256) {
+  if (grid > 0x7fffffff) return hipErrorInvalidValue;
+  void* kargs[] = {const_cast<AttnArgs*>(&a)};
+  return hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)grid), dim3(threads), kargs, 0, stream);
+}
+
+template <int D, bool BF16>
+hipError_t launch_as(const AttnArgs& a, hipStream_t stream) {
+  hipError_t e = launch(&fa_attn_rows_kernel<D, BF16>, (int64_t)a.batch * a.heads * ((a.n + kRowsBlock - 1) / kRowsBlock),
+                        a, stream);
+  if (e != hipSuccess) return e;
+  const bool cap = a.score.cap > 0.0f;
+  const int64_t dkv = (int64_t)a.batch * a.kv_heads * a.key_tiles * a.splits;
+  e = cap ? launch(&fa_attn_dkv_kernel<D, BF16, true>, dkv, a, stream, 512)
+          : launch(&fa_attn_dkv_kernel<D, BF16, false>, dkv, a, stream, 512);
+  if (e != hipSuccess) return e;
+  if (a.parts != nullptr) {
+    const int64_t rows = (int64_t)a.batch * a.kv_heads * a.m;
+    e = launch(&fa_attn_join_kernel<D, BF16>, (rows * (2 * D / 8) + 255) / 256, a, stream);
+    if (e != hipSuccess) return e;
+  }
+  const int64_t dq = (int64_t)a.batch * a.heads * a.tiles;
+  return cap ? launch(&fa_attn_dq_kernel<D, BF16, true>, dq, a, stream)
+             : launch(&fa_attn_dq_kernel<D, BF16, false>, dq, a, stream);
+}
+
+}  // namespace
+
+hipError_t launch_attn_bwd(const AttnArgs& a, int head_dim, bool bf16, hipStream_t stream) {
+  if (head_dim == 128) return bf16 ? launch_as<128, true>(a, stream) : launch_as<128, false>(a, stream);
+  return bf16 ? launch_as<64, true>(a, stream) : launch_as<64, false>(a, stream);
+}
+
+}  // namespace fa

@@ -1,0 +1,169 @@
+// Attention of whole tensors with capped, biased and masked scores, on gfx950.
+//
+//   z = scale q_i.k_j;  c = cap tanh(z / cap);  x = c - slope |p_i - j|
+//   o_i = sum_j P v_j, P = exp(x - lse_i), over the keys lo_i <= j < hi_i
+//
+// A workgroup has 128 rows of a head, four waves of 32, and passes once over the
+// keys that any of them sees, 64 at a time through a two-deep LDS ring
+// (WaveAttn).  Its keys start at the first one that a row sees, so that the tiles of a
+// document begin with it.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "fa_attention_ops.h"
+#include "fa_wave_attn.h"
+
+namespace fa {
+namespace {
+
+using namespace dev;
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+    fa_attn_fwd_kernel(const AttnArgs a) {
+  using W = WaveAttn<D, BF16, 4, 2, true>;
+  constexpr int ROWB = 2 * D, TB = 64 * ROWB;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * TB];  // K0 K1 V0 V1
+  __shared__ TileKeys part[4];
+  __shared__ int again;
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (threadIdx.x == 0) again = 0;  // ordered by the first barrier
+  // XCD x has the kv heads x, ... in a row, so that their keys stay in its L2; of
+  // each the last tiles first, which are the longest of a causal mask.
+  const int unit_blocks = a.tiles * a.group;
+  const int at = xcd_remap(blockIdx.x, gridDim.x);
+  const int unit = fast_div(at, a.by_unit), within = at - unit * unit_blocks;
+  const int back = fast_div(within, a.by_group);
+  const int b = fast_div(unit, a.by_kvh), kvh = unit - b * a.kv_heads;
+  const int h = kvh * a.group + within - back * a.group;
+  const int row0 = (a.tiles - 1 - back) * kAttnRows, wrow0 = row0 + 32 * wave;
+
+  const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(smem));
+  W w;
+  w.init(base, base + 2 * TB, a.scale_log2);
+  w.init_score(a.score);
+  const int l16 = w.l16, g4 = w.g4;
+  const float slope = w.score.biased ? a.score.slopes[h] * kLog2e : 0.0f;
+  const char* qh = a.q.p + b * a.q.sb + h * a.q.sh;
+  TileKeys keys;
+#pragma unroll
+  for (int rb = 0; rb < 2; ++rb) {
+    const int i = min(wrow0 + 16 * rb + l16, a.n - 1);
+    const RowKeys k = row_keys(a, b, i);
+    w.first[rb] = k.lo;
+    w.last[rb] = k.hi - 1;
+    w.pos[rb] = i + a.m - a.n;
+    w.slope[rb] = slope;
+    TileKeys t;
+    t.start(k);
+    if (rb == 0)
+      keys = t;
+    else
+      keys.add(t);
+#pragma unroll
+    for (int st = 0; st < W::KST; ++st)
+      w.qf[rb][st] = *reinterpret_cast<const i16x8*>(qh + i * a.q.st + (32 * st + 8 * g4) * 2);
+  }
+  keys.reduce<16>();
+  if (lane == 0) part[wave] = keys;
+  __syncthreads();
+  TileKeys all = part[0];
+#pragma unroll
+  for (int i = 1; i < 4; ++i) all.add(part[i]);
+  keys.uniform();
+  all.uniform();
+
+  const int c0 = all.lo, c1 = all.hi;  // (no key: kNoKey and 0)
+  const int n_tiles = c0 < c1 ? (c1 - c0 + 63) / 64 : 0;
+  const char* kh = a.k.p + b * a.k.sb + kvh * a.k.sh;
+  const char* vh = a.v.p + b * a.v.sb + kvh * a.v.sh;
+  GroupStage<D> stage;
+  stage.init(lane, (uint32_t)a.k.st, (uint32_t)a.v.st);
+  auto issue = [&](int t, int buf) FA_INLINE {
+    const int r0 = min(c0 + 64 * t + 16 * wave, c1 - 1);
+    const uint32_t dst = base + buf * TB + wave * 16 * ROWB;
+    stage.copy(kh + r0 * a.k.st, vh + r0 * a.v.st, dst, dst + 2 * TB, c1 - 1 - r0, (uint32_t)a.k.st,
+               (uint32_t)a.v.st);
+  };
+  auto end_tile = [&]() FA_INLINE {
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+  };
+  if (n_tiles > 0) issue(0, 0);
+  end_tile();
+  // Tiles with a masked key, those that every row of the wave sees whole, and the
+  // rest.  Every wave passes one barrier a tile, whichever loop it is in.
+  int t = 0, buf = 0;
+  auto masked = [&](int end) FA_INLINE {
+    for (; t < end; ++t, buf ^= 1) {
+      const int k0 = c0 + 64 * t;
+      if (t + 1 < n_tiles) issue(t + 1, buf ^ 1);
+      if (k0 < keys.hi && k0 + 64 > keys.lo)
+        w.template step<0, kMasked>(k0, 15u, buf * TB, base + (2 + buf) * TB);
+      end_tile();
+    }
+  };
+  const int whole0 = keys.all_lo <= c0 ? 0 : (int)min((uint32_t)n_tiles, ((uint32_t)(keys.all_lo - c0) + 63) / 64);
+  const int whole1 = min(n_tiles, max(keys.all_hi - c0, 0) / 64);
+  masked(whole0);
+  for (; t < whole1; ++t, buf ^= 1) {
+    if (t + 1 < n_tiles) issue(t + 1, buf ^ 1);
+    w.template step<0, kWhole>(c0 + 64 * t, 15u, buf * TB);
+    end_tile();
+  }
+  masked(n_tiles);
+  // Infinities or NaN in a masked tile of some wave: all start again (the
+  // staging is shared).
+  if (w.odd && lane == 0) again = 1;
+  __syncthreads();
+  if (__builtin_expect(__builtin_amdgcn_readfirstlane(again) != 0, false)) {
+    w.reset();
+    issue(0, 0);
+    end_tile();
+    buf = 0;
+    for (t = 0; t < n_tiles; ++t, buf ^= 1) {
+      const int k0 = c0 + 64 * t;
+      if (t + 1 < n_tiles) issue(t + 1, buf ^ 1);
+      if (k0 < keys.hi && k0 + 64 > keys.lo) w.template step<0, kSafe>(k0, 15u, buf * TB);
+      end_tile();
+    }
+  }
+
+  float inv[2], lu[2];
+#pragma unroll
+  for (int rb = 0; rb < 2; ++rb) {
+    inv[rb] = w.ls[rb][0] == 0.0f ? 0.0f : 1.0f / w.ls[rb][0];
+    lu[rb] = W::red_sum(w.lu[rb]);
+  }
+  char* oh = a.o.p + b * a.o.sb + h * a.o.sh;
+  write_rows<D, BF16>(smem + wave * 32 * ROWB, w.o, inv, lane, [&](int r) FA_INLINE -> char* {
+    return wrow0 + r < a.n ? oh + (wrow0 + r) * a.o.st : nullptr;
+  });
+  if (a.lse != nullptr && g4 < 2) {
+    const int r = wrow0 + 16 * g4 + l16;
+    const float m = g4 == 0 ? w.m[0] : w.m[1], sum = g4 == 0 ? w.ls[0][0] : w.ls[1][0];
+    const float l = g4 == 0 ? lu[0] : lu[1];
+    if (r < a.n)
+      a.lse[((int64_t)b * a.heads + h) * a.n + r] = sum == 0.0f ? -INFINITY : (m * w.c + __log2f(l)) * kLn2;
+  }
+}
+
+template <int D, bool BF16>
+hipError_t launch_as(const AttnArgs& a, hipStream_t stream) {
+  const int64_t grid = (int64_t)a.batch * a.heads * a.tiles;
+  if (grid > 0x7fffffff) return hipErrorInvalidValue;
+  void* kargs[] = {const_cast<AttnArgs*>(&a)};
+  return hipLaunchKernel(reinterpret_cast<const void*>(&fa_attn_fwd_kernel<D, BF16>), dim3((unsigned)grid),
+                         dim3(256), kargs, 0, stream);
+}
+
+}  // namespace
+
+hipError_t launch_attn_fwd(const AttnArgs& a, int head_dim, bool bf16, hipStream_t stream) {
+  if (head_dim == 128) return bf16 ? launch_as<128, true>(a, stream) : launch_as<128, false>(a, stream);
+  return bf16 ? launch_as<64, true>(a, stream) : launch_as<64, false>(a, stream);
+}
+
+}  // namespace fa

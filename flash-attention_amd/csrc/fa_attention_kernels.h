@@ -1,0 +1,56 @@
+// Internal interface between the C ABI of attention with gradients
+// (fa_attention_api.cpp) and its HIP kernels.  Strides are in bytes here.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "fa_fwd_kernel.h"
+#include "fa_score.h"
+
+namespace fa {
+
+// Rows of whole tensors [batch, heads, rows, head_dim].
+struct Rows3 {
+  char* p;
+  int64_t sb, sh, st;  // batch, head, row
+};
+
+struct AttnArgs {
+  Rows3 q, k, v, o;
+  float* lse;               // [batch, heads, n] contiguous
+  const int32_t* ranges;    // pairs (first key, end) of each row; NULL: all keys
+  int64_t range_sb;         // elements
+  int32_t batch, heads, kv_heads, group;
+  int32_t n, m;             // rows, keys
+  int32_t causal;
+  float scale, scale_log2;
+  ScoreArgs score;
+  int32_t tiles;            // row tiles of a head (kAttnRows)
+  FastDiv by_unit, by_group, by_kvh;  // by_unit: tiles * group workgroups of a kv head
+  // backward
+  Rows3 go, gq, gk, gv;     // gradients of o, q, k, v
+  const float* glse;        // of lse; may be NULL
+  float* records;           // [batch, heads, spans][2][4][16], see fa_attention_bwd.hip
+  int32_t* bounds;          // [batch, spans][4]: limits of a span's rows
+  float* tops;              // [batch, heads, spans]: largest |go|
+  int32_t spans;            // spans of kSpan rows
+  int32_t key_tiles, splits;
+  FastDiv by_keys, by_splits;  // by_keys: key tiles * splits workgroups of a kv head
+  float* parts;             // [splits][batch, kv_heads, m][2][D] gradients of k and v; NULL: one split
+};
+
+constexpr int kAttnRows = 128;  // rows of a forward or dq workgroup
+constexpr int kAttnKeys = 256;  // keys of a dk, dv workgroup
+constexpr int kSpan = 32;       // rows that it stages at a time
+
+struct AttnBwdPlan {
+  int32_t splits;
+  uint64_t records, bounds, tops, parts;  // bytes, each a multiple of 16
+};
+AttnBwdPlan plan_attn_bwd(const AttnArgs& a, int head_dim, int compute_units);
+
+hipError_t launch_attn_fwd(const AttnArgs& args, int head_dim, bool bf16, hipStream_t stream);
+hipError_t launch_attn_bwd(const AttnArgs& args, int head_dim, bool bf16, hipStream_t stream);
+
+}  // namespace fa

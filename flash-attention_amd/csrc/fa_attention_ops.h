@@ -1,0 +1,137 @@
+// Device building blocks shared by the kernels of attention on whole tensors:
+// the keys that a row sees, staging of rows, cleaning of masked rows.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "fa_attention_kernels.h"
+#include "fa_device_ops.h"
+#include "fa_lds_layout.h"
+#include "fa_paged_ops.h"
+
+namespace fa {
+namespace {
+
+using namespace dev;
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// Keys lo .. hi - 1; a row that sees none has lo = kNoKey, hi = 0.
+constexpr int kNoKey = 0x7fffffff;
+struct RowKeys {
+  int lo, hi;
+};
+__device__ __forceinline__ RowKeys row_keys(const AttnArgs& a, int b, int i) {
+  const int p = i + a.m - a.n;
+  RowKeys k = {0, a.m};
+  if (a.ranges != nullptr) {
+    const int2 r = *reinterpret_cast<const int2*>(a.ranges + b * a.range_sb + 2 * (int64_t)i);
+    k.lo = max(r.x, 0);
+    k.hi = min(r.y, a.m);
+  }
+  if (a.causal) k.hi = min(k.hi, p + 1);
+  if (a.score.window > 0) {
+    k.lo = max(k.lo, p - (a.score.window - 1));
+    if (!a.causal) k.hi = min(k.hi, p + a.score.window);
+  }
+  if (k.lo >= k.hi) k = {kNoKey, 0};
+  return k;
+}
+
+// Keys that some row sees, and that every row sees.
+struct TileKeys {
+  int lo, hi, all_lo, all_hi;
+  __device__ __forceinline__ void start(const RowKeys& k) { *this = {k.lo, k.hi, k.lo, k.hi}; }
+  __device__ __forceinline__ void add(const TileKeys& o) {
+    lo = min(lo, o.lo);
+    hi = max(hi, o.hi);
+    all_lo = max(all_lo, o.all_lo);
+    all_hi = min(all_hi, o.all_hi);
+  }
+  template <int WIDTH>
+  __device__ __forceinline__ void reduce() {  // over aligned groups of WIDTH lanes
+#pragma unroll
+    for (int d = 1; d < WIDTH; d <<= 1)
+      add({__shfl_xor(lo, d), __shfl_xor(hi, d), __shfl_xor(all_lo, d), __shfl_xor(all_hi, d)});
+  }
+  __device__ __forceinline__ void uniform() {
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+    all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+  }
+};
+
+// Staging of 16 rows of a tensor into LDS in the layout of lds::TileBoth.
+template <int D>
+struct RowStage {
+  static constexpr int ROWB = 2 * D, NI = 16 * ROWB / 1024, LPR = ROWB / 16;
+  uint32_t src[NI];
+  __device__ __forceinline__ void init(int lane, uint32_t st) {
+#pragma unroll
+    for (int it = 0; it < NI; ++it) {
+      const int r = it * (64 / LPR) + lane / LPR;
+      src[it] = r * st + ((lane % LPR) ^ lds::TileBoth<D>::swz(r)) * 16;
+    }
+  }
+  // p: the first row; rows past `lim` re-read row lim.
+  __device__ __forceinline__ void copy(const char* p, uint32_t dst, int lim, uint32_t st) const {
+#pragma unroll
+    for (int it = 0; it < NI; ++it) {
+      poison_1k(dst + it * 1024);
+      const int r = it * (64 / LPR) + (int)(threadIdx.x & 63) / LPR;
+      const uint32_t over = lim >= 15 ? 0u : (uint32_t)max(r - lim, 0);
+      dma_16b(src[it] - over * st, p, dst + it * 1024);
+    }
+  }
+};
+
+template <int OFF>
+__device__ __forceinline__ u32x2 lds_read8(uint32_t addr) {
+  return *(__attribute__((address_space(3))) const u32x2*)(uintptr_t)(addr + OFF);
+}
+template <int OFF>
+__device__ __forceinline__ void lds_write8(uint32_t addr, u32x2 w) {
+  *(__attribute__((address_space(3))) u32x2*)(uintptr_t)(addr + OFF) = w;
+}
+__device__ __forceinline__ void lds_write4(uint32_t addr, float x) {
+  *(__attribute__((address_space(3))) float*)(uintptr_t)addr = x;
+}
+__device__ __forceinline__ void lds_write16(uint32_t addr, u32x4 w) {
+  *(__attribute__((address_space(3))) u32x4*)(uintptr_t)addr = w;
+}
+
+// A tile that some row or key does not see whole: 0 times an infinity or NaN of a
+// masked row would be NaN in the products that sum over these rows.  Clears the
+// infinities and NaN among the ROWS rows at LDS address `at`, which this wave has
+// staged, and returns the rows (bit r) that held any.
+template <int D, bool BF16, int ROWS>
+__device__ __forceinline__ unsigned clean_rows(uint32_t at) {
+  constexpr int ROWB = 2 * D, NI = ROWS * ROWB / 1024, LPR = ROWB / 16;
+  constexpr uint32_t E = BF16 ? 0x7F807F80u : 0x7C007C00u, L = BF16 ? 0x00800080u : 0x04000400u;
+  const int lane = threadIdx.x & 63;
+  unsigned rows = 0;
+#pragma unroll
+  for (int it = 0; it < NI; ++it) {
+    const uint32_t addr = at + it * 1024 + lane * 16;
+    u32x4 w = __builtin_bit_cast(u32x4, lds_read16<0>(addr));
+    uint32_t any = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) any |= (w[j] & E) + L;  // an exponent of all ones carries
+    uint64_t bad = __ballot((any & 0x80008000u) != 0);
+    if (__builtin_expect(bad == 0, true)) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t half = ((w[j] & E) + L) & 0x80008000u;
+      w[j] &= ~(((half >> 15) << 16) - (half >> 15));
+    }
+    lds_write16(addr, w);
+    for (int r = 0; r < 64 / LPR; ++r)
+      if ((bad >> (r * LPR)) & ((1ull << LPR) - 1)) rows |= 1u << (it * (64 / LPR) + r);
+  }
+  return rows;
+}
+
+}  // namespace
+}  // namespace fa

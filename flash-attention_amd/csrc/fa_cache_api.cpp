@@ -10,7 +10,9 @@
 #include <cstdint>
 
 #include "fa_cache_kernels.h"
+#include "fa_checks.h"
 #include "fa_host.h"
+#include "fa_mi355x_attention.h"
 #include "fa_mi355x_cache.h"
 
 namespace fa {
@@ -35,12 +37,19 @@ static bool cuts_tiles(int64_t rows, int batch, int conc, int max_pieces, float 
 }
 
 PagedPlan plan_paged(int tokens, int batch, int kv_heads, int group, int head_dim, int max_q,
-                     int max_kv, bool causal, int compute_units) {
+                     int max_kv, bool causal, int compute_units, int window) {
   PagedPlan p = {};
   p.compute_units = compute_units;
   PagedGrid& g = p.grid;
   const int64_t most = (int64_t)std::min(max_q, tokens) * group;  // rows of a sequence
-  const int64_t keys = std::max(max_kv, 1);
+  int64_t keys = std::max(max_kv, 1);
+  if (window > 0) {
+    // What the tokens of a tile see in a window, from a tile of keys on.
+    const int64_t tokens_of = most > kDecodeRows ? std::min<int64_t>(max_q, (kChunkRows + group - 1) / group + 1) : max_q;
+    keys = std::min<int64_t>(keys, (causal ? 1 : 2) * (int64_t)window + tokens_of + 63);
+    causal = false;  // (tiles of a window are of one length)
+  }
+  g.keys = (int)keys;
   if (most > kDecodeRows) {
     // All sequences of the call, those of few rows too: one launch after the
     // other for the two kinds was 10 to 30 % slower in mixes of like lengths (us,
@@ -214,74 +223,6 @@ bool may_overlap(const RowSet& a, const RowSet& b) {
 
 namespace {
 
-constexpr int64_t kMaxKeyStride = int64_t(1) << 24;  // as the forward's seq stride
-// Rows of a call: the kernels number the rows of whole tiles, up to 128 past the
-// last one, in 31 bits.
-constexpr int64_t kMaxRows = (int64_t(1) << 31) - 256;
-
-bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-
-// Strides of a 2-byte tensor whose rows are read in 16-byte pieces.
-fa_status check_rows(const char* name, const void* ptr, const int64_t* st, int n) {
-  if (ptr == nullptr) return fail(FA_ERR_NULL, "%s is NULL", name);
-  for (int i = 0; i < n; ++i) {
-    if (st[i] < 0)
-      return fail(FA_ERR_STRIDE, "%s stride[%d] = %lld is negative", name, i, (long long)st[i]);
-    if (st[i] % 8 != 0)
-      return fail(FA_ERR_STRIDE,
-                  "%s stride[%d] = %lld is not a multiple of 8 elements (16-byte rows required)",
-                  name, i, (long long)st[i]);
-  }
-  if (!aligned(ptr, 16)) return fail(FA_ERR_STRIDE, "%s pointer is not 16-byte aligned", name);
-  return FA_OK;
-}
-
-// Rows of `row` elements of a written tensor must not overlap: each stride, in
-// ascending order, spans what the smaller ones reach.  (n <= 3)
-fa_status check_written(const char* name, const int64_t* st, const int64_t* size, int n, int64_t row) {
-  int order[3] = {0, 1, 2};
-  std::sort(order, order + n, [&](int i, int j) { return st[i] < st[j]; });
-  __int128 reach = row;
-  for (int o = 0; o < n; ++o) {
-    const int i = order[o];
-    if (size[i] <= 1) continue;
-    if (st[i] < reach)
-      return fail(FA_ERR_STRIDE, "%s stride[%d] = %lld is smaller than the %lld elements it must step over"
-                  " (rows overlap)", name, i, (long long)st[i], (long long)reach);
-    reach += (__int128)st[i] * (size[i] - 1);
-  }
-  return FA_OK;
-}
-
-fa_status check_dtype(int32_t dtype) {
-  if (dtype != FA_DTYPE_F16 && dtype != FA_DTYPE_BF16)
-    return fail(FA_ERR_DTYPE, "dtype %d is not fp16 (0) or bf16 (1)", (int)dtype);
-  return FA_OK;
-}
-
-fa_status check_head_dim(int32_t d) {
-  if (d != 64 && d != 128)
-    return fail(FA_ERR_HEADDIM, "Only head_dim 64 and 128 are supported (got %d)", (int)d);
-  return FA_OK;
-}
-
-fa_status check_flag(const char* name, int32_t v) {
-  if (v != 0 && v != 1) return fail(FA_ERR_ARG, "%s must be 0 or 1 (got %d)", name, (int)v);
-  return FA_OK;
-}
-
-#define FA_TRY(expr)                     \
-  do {                                   \
-    const fa_status s_ = (expr);         \
-    if (s_ != FA_OK) return s_;          \
-  } while (0)
-
-fa_status check_int32(const char* name, const void* p, bool required = true) {
-  if (p == nullptr) return required ? fail(FA_ERR_NULL, "%s is NULL", name) : FA_OK;
-  if (!aligned(p, 4)) return fail(FA_ERR_STRIDE, "%s pointer is not 4-byte aligned", name);
-  return FA_OK;
-}
-
 // written: the call writes k and v.  v may be absent where with_v is false.
 fa_status check_cache(const fa_paged_cache& c, bool with_v, bool with_cu, bool written) {
   FA_TRY(check_dtype(c.dtype));
@@ -331,11 +272,7 @@ fa_status check_queries(const fa_paged_cache& c, int32_t tokens, int32_t heads, 
   if (max_q < 0 || max_kv < 0)
     return fail(FA_ERR_ARG, "max_q=%d and max_kv=%d must be >= 0", (int)max_q, (int)max_kv);
   FA_TRY(check_flag("causal", causal));
-  // (a normal number: the offset's headroom is divided by it; its product with
-  // log2(e) is finite)
-  if (!(scale >= FLT_MIN) || !(scale <= FLT_MAX / 2))
-    return fail(FA_ERR_ARG, "softmax_scale must be from %g to %g (got %g)", (double)FLT_MIN,
-                (double)FLT_MAX / 2, (double)scale);
+  FA_TRY(check_scale(scale));
   if ((int64_t)tokens * heads > kMaxRows)
     return fail(FA_ERR_UNSUPPORTED, "tokens*heads = %lld exceeds 2^31-256", (long long)tokens * heads);
   if ((int64_t)c.batch * c.kv_heads > 0x7fffff)
@@ -366,24 +303,6 @@ PageTable page_table(const fa_paged_cache& c, int32_t tokens, int32_t max_kv) {
   t.tokens = tokens;
   t.max_kv = max_kv;
   return t;
-}
-
-constexpr double kLog2e = 1.4426950408889634;
-
-fa_status check_workspace(void* ws, uint64_t have, uint64_t need) {
-  if (need == 0) return FA_OK;
-  if (ws == nullptr)
-    return fail(FA_ERR_NULL, "workspace is NULL but %llu bytes are needed", (unsigned long long)need);
-  if (have < need)
-    return fail(FA_ERR_ARG, "workspace of %llu bytes is smaller than the %llu bytes needed",
-                (unsigned long long)have, (unsigned long long)need);
-  if (!aligned(ws, 16)) return fail(FA_ERR_STRIDE, "workspace pointer is not 16-byte aligned");
-  return FA_OK;
-}
-
-fa_status launched(hipError_t e) {
-  if (e != hipSuccess) return fail(FA_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(e));
-  return FA_OK;
 }
 
 // Largest byte offset of a tile's rows from its first (64 tokens, or fewer of a
@@ -446,6 +365,25 @@ NormArgs norm_args(const fa_qk_norm_params& p) {
   n.eps = p.eps;
   n.by_seq = make_fast_div((uint32_t)p.seq_len);
   return n;
+}
+
+// The axes of a rotation by `pairs` pairs at `positions`.
+fa_status check_axes(const fa_rotary_axes* axes, int pairs, const int32_t* positions) {
+  if (axes == nullptr) return fail(FA_ERR_NULL, "axes is NULL");
+  if (axes->axes < 1 || axes->axes > 4) return fail(FA_ERR_ARG, "axes must be 1 to 4 (got %d)", (int)axes->axes);
+  for (int i = 0; i < pairs; ++i)
+    if (axes->axis[i] >= axes->axes)
+      return fail(FA_ERR_ARG, "pair %d turns by axis %d of %d", i, (int)axes->axis[i], (int)axes->axes);
+  if (axes->axis_stride < 0) return fail(FA_ERR_STRIDE, "axis_stride is negative");
+  if (positions == nullptr) return fail(FA_ERR_NULL, "positions is NULL, but a token has several");
+  return FA_OK;
+}
+
+void set_axes(NormArgs& n, const fa_rotary_axes& axes) {
+  n.axes = axes.axes;
+  n.axis_stride = axes.axis_stride;
+  n.axis_bits[0] = n.axis_bits[1] = 0;
+  for (int i = 0; i < n.rot / 2; ++i) n.axis_bits[i / 32] |= (uint64_t)axes.axis[i] << (2 * (i % 32));
 }
 
 fa_status check_norm_params(const fa_qk_norm_params* p, bool backward) {
@@ -600,11 +538,11 @@ bool idle(const fa_paged_weights_params& p) {
   return p.tokens == 0 || p.cache.batch == 0 || p.max_q == 0 || p.max_kv == 0;
 }
 
-fa_status plan_of(const fa_paged_fwd_params& p, PagedPlan* plan) {
+fa_status plan_of(const fa_paged_fwd_params& p, int window, PagedPlan* plan) {
   int cus = 0;
   FA_TRY(current_compute_units(&cus));
   *plan = plan_paged(p.tokens, p.cache.batch, p.cache.kv_heads, p.heads / p.cache.kv_heads,
-                     p.cache.head_dim, p.max_q, limit_kv(p.cache, p.max_kv), p.causal != 0, cus);
+                     p.cache.head_dim, p.max_q, limit_kv(p.cache, p.max_kv), p.causal != 0, cus, window);
   return FA_OK;
 }
 
@@ -629,26 +567,9 @@ uint64_t norm_bwd_bytes(const fa_qk_norm_params& f, int cus) {
 
 }  // namespace
 
-extern "C" {
+namespace {
 
-fa_status fa_paged_fwd_workspace_size(const fa_paged_fwd_params* p, uint64_t* bytes) {
-  if (bytes == nullptr) return fail(FA_ERR_NULL, "bytes is NULL");
-  *bytes = 0;
-  FA_TRY(fa_paged_fwd_validate(p));
-  if (idle(*p)) return FA_OK;
-  PagedPlan plan;
-  FA_TRY(plan_of(*p, &plan));
-  *bytes = plan.workspace_bytes;
-  return FA_OK;
-}
-
-fa_status fa_paged_fwd(const fa_paged_fwd_params* p, void* workspace, uint64_t workspace_bytes,
-                       void* stream) {
-  FA_TRY(fa_paged_fwd_validate(p));
-  if (idle(*p)) return FA_OK;
-  PagedPlan plan;
-  FA_TRY(plan_of(*p, &plan));
-  FA_TRY(check_workspace(workspace, workspace_bytes, plan.workspace_bytes));
+PagedFwdArgs paged_args(const fa_paged_fwd_params* p) {
   const fa_paged_cache& c = p->cache;
   PagedFwdArgs a = {};
   a.pt = page_table(c, p->tokens, limit_kv(c, p->max_kv));
@@ -675,8 +596,66 @@ fa_status fa_paged_fwd(const fa_paged_fwd_params* p, void* workspace, uint64_t w
   a.scale_log2 = (float)(p->softmax_scale * kLog2e);
   a.by_group = make_fast_div((uint32_t)a.group);
   a.by_kvh = make_fast_div((uint32_t)a.kv_heads);
-  return launched(launch_paged_fwd(a, plan, c.head_dim, c.dtype == FA_DTYPE_BF16, workspace,
-                                   static_cast<hipStream_t>(stream)));
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+fa_status fa_paged_fwd_workspace_size(const fa_paged_fwd_params* p, uint64_t* bytes) {
+  if (bytes == nullptr) return fail(FA_ERR_NULL, "bytes is NULL");
+  *bytes = 0;
+  FA_TRY(fa_paged_fwd_validate(p));
+  if (idle(*p)) return FA_OK;
+  PagedPlan plan;
+  FA_TRY(plan_of(*p, 0, &plan));
+  *bytes = plan.workspace_bytes;
+  return FA_OK;
+}
+
+fa_status fa_paged_fwd(const fa_paged_fwd_params* p, void* workspace, uint64_t workspace_bytes,
+                       void* stream) {
+  FA_TRY(fa_paged_fwd_validate(p));
+  if (idle(*p)) return FA_OK;
+  PagedPlan plan;
+  FA_TRY(plan_of(*p, 0, &plan));
+  FA_TRY(check_workspace(workspace, workspace_bytes, plan.workspace_bytes));
+  return launched(launch_paged_fwd(paged_args(p), plan, p->cache.head_dim, p->cache.dtype == FA_DTYPE_BF16,
+                                   workspace, static_cast<hipStream_t>(stream)));
+}
+
+fa_status fa_paged_fwd_scored_validate(const fa_paged_fwd_params* p, const fa_score_params* score) {
+  FA_TRY(fa_paged_fwd_validate(p));
+  if (score == nullptr) return fail(FA_ERR_NULL, "score is NULL");
+  return check_score(*score, p->softmax_scale);
+}
+
+fa_status fa_paged_fwd_scored_workspace_size(const fa_paged_fwd_params* p, const fa_score_params* score,
+                                             uint64_t* bytes) {
+  if (bytes == nullptr) return fail(FA_ERR_NULL, "bytes is NULL");
+  *bytes = 0;
+  FA_TRY(fa_paged_fwd_scored_validate(p, score));
+  if (idle(*p)) return FA_OK;
+  PagedPlan plan;
+  FA_TRY(plan_of(*p, score_args(*score, p->softmax_scale).window, &plan));
+  *bytes = plan.workspace_bytes;
+  return FA_OK;
+}
+
+fa_status fa_paged_fwd_scored(const fa_paged_fwd_params* p, const fa_score_params* score, void* workspace,
+                              uint64_t workspace_bytes, void* stream) {
+  FA_TRY(fa_paged_fwd_scored_validate(p, score));
+  if (score->softcap == 0.0f && score->slopes == nullptr && score->window == 0)
+    return fa_paged_fwd(p, workspace, workspace_bytes, stream);
+  if (idle(*p)) return FA_OK;
+  PagedFwdArgs a = paged_args(p);
+  a.score = score_args(*score, p->softmax_scale);
+  PagedPlan plan;
+  FA_TRY(plan_of(*p, a.score.window, &plan));
+  FA_TRY(check_workspace(workspace, workspace_bytes, plan.workspace_bytes));
+  return launched(launch_paged_scored(a, plan, p->cache.head_dim, p->cache.dtype == FA_DTYPE_BF16, workspace,
+                                      static_cast<hipStream_t>(stream)));
 }
 
 fa_status fa_paged_key_weights_workspace_size(const fa_paged_weights_params* p, uint64_t* bytes) {
@@ -757,31 +736,25 @@ fa_status fa_paged_evict(const fa_paged_evict_params* p, void* stream) {
   return launched(launch_paged_evict(a, c.head_dim, static_cast<hipStream_t>(stream)));
 }
 
-fa_status fa_qk_norm_rope(const fa_qk_norm_params* p, void* stream) {
-  FA_TRY(fa_qk_norm_rope_validate(p));
+}  // extern "C"
+
+namespace {
+
+fa_status norm_forward(const fa_qk_norm_params& p, const fa_rotary_axes* axes, void* stream) {
   int cus = 0;
   FA_TRY(current_compute_units(&cus));
-  return launched(launch_norm(norm_args(*p), p->dtype == FA_DTYPE_BF16, false, cus,
-                              static_cast<hipStream_t>(stream)));
+  NormArgs n = norm_args(p);
+  if (axes != nullptr) set_axes(n, *axes);
+  return launched(launch_norm(n, p.dtype == FA_DTYPE_BF16, false, cus, static_cast<hipStream_t>(stream)));
 }
 
-fa_status fa_qk_norm_rope_bwd_workspace_size(const fa_qk_norm_bwd_params* p, uint64_t* bytes) {
-  if (bytes == nullptr) return fail(FA_ERR_NULL, "bytes is NULL");
-  *bytes = 0;
-  FA_TRY(fa_qk_norm_rope_bwd_validate(p));
-  int cus = 0;
-  FA_TRY(current_compute_units(&cus));
-  *bytes = norm_bwd_bytes(p->fwd, cus);
-  return FA_OK;
-}
-
-fa_status fa_qk_norm_rope_bwd(const fa_qk_norm_bwd_params* p, void* workspace, uint64_t workspace_bytes,
-                              void* stream) {
-  FA_TRY(fa_qk_norm_rope_bwd_validate(p));
+fa_status norm_backward(const fa_qk_norm_bwd_params* p, const fa_rotary_axes* axes, void* workspace,
+                        uint64_t workspace_bytes, void* stream) {
   int cus = 0;
   FA_TRY(current_compute_units(&cus));
   FA_TRY(check_workspace(workspace, workspace_bytes, norm_bwd_bytes(p->fwd, cus)));
   NormArgs n = norm_args(p->fwd);
+  if (axes != nullptr) set_axes(n, *axes);
   void* dx[2] = {p->dq, p->dk};
   const int64_t* ds[2] = {p->dq_stride, p->dk_stride};
   for (int i = 0; i < 2; ++i) {
@@ -796,8 +769,7 @@ fa_status fa_qk_norm_rope_bwd(const fa_qk_norm_bwd_params* p, void* workspace, u
   return launched(launch_norm_bwd(n, p->fwd.dtype == FA_DTYPE_BF16, cus, static_cast<hipStream_t>(stream)));
 }
 
-fa_status fa_paged_store(const fa_paged_store_params* p, void* stream) {
-  FA_TRY(fa_paged_store_validate(p));
+fa_status norm_store(const fa_paged_store_params* p, const fa_rotary_axes* axes, void* stream) {
   const fa_paged_cache& c = p->cache;
   if (p->tokens == 0 || c.batch == 0) return FA_OK;
   int cus = 0;
@@ -837,8 +809,70 @@ fa_status fa_paged_store(const fa_paged_store_params* p, void* stream) {
   n.interleaved = p->interleaved;
   n.weight_fp32 = p->weight_fp32;
   n.eps = p->eps;
+  if (axes != nullptr) set_axes(n, *axes);
   n.by_seq = make_fast_div((uint32_t)p->tokens);
   return launched(launch_norm(n, c.dtype == FA_DTYPE_BF16, true, cus, static_cast<hipStream_t>(stream)));
+}
+
+}  // namespace
+
+extern "C" {
+
+fa_status fa_qk_norm_rope(const fa_qk_norm_params* p, void* stream) {
+  FA_TRY(fa_qk_norm_rope_validate(p));
+  return norm_forward(*p, nullptr, stream);
+}
+
+fa_status fa_qk_norm_rope_axes_validate(const fa_qk_norm_params* p, const fa_rotary_axes* axes) {
+  FA_TRY(fa_qk_norm_rope_validate(p));
+  return check_axes(axes, p->rot / 2, p->positions);
+}
+
+fa_status fa_qk_norm_rope_axes(const fa_qk_norm_params* p, const fa_rotary_axes* axes, void* stream) {
+  FA_TRY(fa_qk_norm_rope_axes_validate(p, axes));
+  return norm_forward(*p, axes, stream);
+}
+
+fa_status fa_qk_norm_rope_bwd_workspace_size(const fa_qk_norm_bwd_params* p, uint64_t* bytes) {
+  if (bytes == nullptr) return fail(FA_ERR_NULL, "bytes is NULL");
+  *bytes = 0;
+  FA_TRY(fa_qk_norm_rope_bwd_validate(p));
+  int cus = 0;
+  FA_TRY(current_compute_units(&cus));
+  *bytes = norm_bwd_bytes(p->fwd, cus);
+  return FA_OK;
+}
+
+fa_status fa_qk_norm_rope_bwd(const fa_qk_norm_bwd_params* p, void* workspace, uint64_t workspace_bytes,
+                              void* stream) {
+  FA_TRY(fa_qk_norm_rope_bwd_validate(p));
+  return norm_backward(p, nullptr, workspace, workspace_bytes, stream);
+}
+
+fa_status fa_qk_norm_rope_bwd_axes_validate(const fa_qk_norm_bwd_params* p, const fa_rotary_axes* axes) {
+  FA_TRY(fa_qk_norm_rope_bwd_validate(p));
+  return check_axes(axes, p->fwd.rot / 2, p->fwd.positions);
+}
+
+fa_status fa_qk_norm_rope_bwd_axes(const fa_qk_norm_bwd_params* p, const fa_rotary_axes* axes,
+                                   void* workspace, uint64_t workspace_bytes, void* stream) {
+  FA_TRY(fa_qk_norm_rope_bwd_axes_validate(p, axes));
+  return norm_backward(p, axes, workspace, workspace_bytes, stream);
+}
+
+fa_status fa_paged_store(const fa_paged_store_params* p, void* stream) {
+  FA_TRY(fa_paged_store_validate(p));
+  return norm_store(p, nullptr, stream);
+}
+
+fa_status fa_paged_store_axes_validate(const fa_paged_store_params* p, const fa_rotary_axes* axes) {
+  FA_TRY(fa_paged_store_validate(p));
+  return p->tokens == 0 ? FA_OK : check_axes(axes, p->rot / 2, p->positions);
+}
+
+fa_status fa_paged_store_axes(const fa_paged_store_params* p, const fa_rotary_axes* axes, void* stream) {
+  FA_TRY(fa_paged_store_axes_validate(p, axes));
+  return norm_store(p, axes, stream);
 }
 
 }  // extern "C"

@@ -9,6 +9,7 @@
 #include <math.h>
 
 #include "fa_fwd_kernel.h"
+#include "fa_score.h"
 
 // Arithmetic that the host's plans and the kernels share.
 #if defined(__HIPCC__)
@@ -60,6 +61,7 @@ struct PagedFwdArgs {
   FastDiv by_group_places, by_unit_group;
   float* ws_o;                     // [slot or piece][BM][D] partial o, fp32, of each kv head
   float* ws_e;                     // the same rows: (log2 of the rounded P's sum, of the plain one's)
+  ScoreArgs score;                 // read by the scored kernels only
 };
 
 // Cost of a piece of a tile beside its keys (LastRound): the time of 768 keys,
@@ -93,6 +95,7 @@ struct PagedGrid {
   int32_t slots;
   int32_t splits, chunk;  // decode
   int32_t conc, pieces;   // chunk: at once per kv head, most pieces per kv head
+  int32_t keys;           // most keys that a tile sees
   uint64_t ws_rows;       // rows of partials
 };
 struct PagedPlan {
@@ -101,10 +104,13 @@ struct PagedPlan {
   uint64_t workspace_bytes;
 };
 PagedPlan plan_paged(int tokens, int batch, int kv_heads, int group, int head_dim, int max_q,
-                     int max_kv, bool causal, int compute_units);
+                     int max_kv, bool causal, int compute_units, int window = 0);
 
 hipError_t launch_paged_fwd(const PagedFwdArgs& args, const PagedPlan& plan, int head_dim, bool bf16,
                             void* workspace, hipStream_t stream);
+// The same with args.score.
+hipError_t launch_paged_scored(const PagedFwdArgs& args, const PagedPlan& plan, int head_dim, bool bf16,
+                               void* workspace, hipStream_t stream);
 
 struct PagedWeightsArgs {
   PageTable pt;
@@ -170,6 +176,9 @@ struct NormArgs {
   const float* sin;
   const int32_t* positions;
   int64_t pos_stride;             // elements
+  int32_t axes;                   // positions of a token; 0: one for all pairs of dims
+  int64_t axis_stride;            // elements from one axis's positions to the next's
+  uint64_t axis_bits[2];          // two bits a pair: its axis
   PageTable pt;                   // storing only
   int32_t tokens;                 // of all sequences: batch * seq_len
   int32_t seq_len;                // tokens of one batch entry

@@ -153,6 +153,33 @@ FA_LAYOUT_FN int v16_read_offset(int ch, int h, int db, int lane) {
   return key * T::ROWB + (((col >> 3) ^ Tile16<D>::swz_v(key)) << 4) + (col & 7) * 2;
 }
 
+// ---- Tiles read both by rows and transposed (attention's backward pass) ----
+// One swizzle for the 16-byte row reads of k16_read_offset, whose 16 rows need
+// distinct positions, and for the transposing reads of v16_read_offset, whose 8
+// rows need distinct pairs of positions: the pair goes by row % 8 (or its half,
+// at two rows to the banks), the place within it by the next bit.  Both offsets
+// are a lane's own for step or block 0 with one exclusive or: chunks 4 st and
+// 2 db only set bits above those of the lane's chunk.
+template <int D>
+struct TileBoth {
+  static constexpr int ROWB = 2 * D;
+  static FA_LAYOUT_FN int swz(int r) {
+    return D == 128 ? ((r & 7) << 1) | ((r >> 3) & 1) : (((r >> 1) & 3) << 1) | ((r >> 3) & 1);
+  }
+  // 16 bytes: row lane % 16, elements 32 st + 8 (lane / 16) .. + 7.
+  static FA_LAYOUT_FN int row_offset(int lane) {
+    const int r = lane & 15;
+    return r * ROWB + (((lane >> 4) ^ swz(r)) << 4);
+  }
+  static FA_LAYOUT_FN int row_step(int st) { return st << 6; }
+  // 8 bytes: row 4 (lane / 16) + (lane % 16) / 4, columns 16 db + 4 (lane % 4) .. + 3.
+  static FA_LAYOUT_FN int turned_offset(int lane) {
+    const int l16 = lane & 15, r = 4 * (lane >> 4) + (l16 >> 2);
+    return r * ROWB + ((((l16 & 3) >> 1) ^ swz(r)) << 4) + (l16 & 1) * 8;
+  }
+  static FA_LAYOUT_FN int turned_block(int db) { return db << 5; }
+};
+
 // Row tiles: 32 rows of `rowb` bytes (rowb = 128, 256 or 512) that a wave
 // stages on its own, Q for its MFMA operands (4-wave workgroups) and O or
 // the fp32 split partials on their way out.  Row r's 16-byte chunk c sits at

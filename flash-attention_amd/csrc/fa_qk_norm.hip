@@ -105,6 +105,35 @@ struct Lane {
     a = 2 * ea;
     b = INTER || !turned ? a + 8 : 2 * (n.rot / 2 + 4 * j);
   }
+  // The positions of the lane's pairs, each on its own axis (n.axes > 0).
+  __device__ __forceinline__ void positions(const NormArgs& n, int64_t at, int* pos) const {
+    const int j = threadIdx.x % LPR;
+    const uint32_t bits = (uint32_t)(n.axis_bits[j >> 3] >> (8 * (j & 7)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pos[i] = n.positions[((bits >> (2 * i)) & 3) * n.axis_stride + at];
+  }
+  // Their cosines and sines: 1 and 0 past the rotation, NaN for a position outside
+  // the tables.  (Where an axis has whole lanes they are one load.)
+  __device__ __forceinline__ void angles(const NormArgs& n, const int* pos) {
+    const int j = threadIdx.x % LPR, half = n.rot / 2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[i] = 1.0f;
+      s[i] = 0.0f;
+    }
+    if (8 * j >= n.rot) return;
+    if (pos[0] == pos[1] && pos[0] == pos[2] && pos[0] == pos[3]) {
+      angles(n, pos[0]);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool known = (uint32_t)pos[i] < (uint32_t)n.table_rows;
+      const int64_t at = known ? (int64_t)pos[i] * half + 4 * j + i : 0;
+      c[i] = known ? n.cos[at] : NAN;
+      s[i] = known ? n.sin[at] : NAN;
+    }
+  }
   // The token's cosines and sines: 1 and 0 past the rotation, NaN for a
   // position outside the tables.
   __device__ __forceinline__ void angles(const NormArgs& n, int pos) {
@@ -161,8 +190,12 @@ __global__ void __launch_bounds__(256) fa_norm_kernel(const NormArgs n) {
   const int b = STORE ? 0 : fast_div(tok, n.by_seq), t = STORE ? tok : tok - b * n.seq_len;
   // What needs no place in the cache is asked for first: the loads below wait
   // for one another.
-  const int pos = n.positions == nullptr ? t : n.positions[b * n.pos_stride + t];
   L l;
+  int pos[4] = {t, t, t, t};
+  if (n.axes > 0)
+    l.positions(n, b * n.pos_stride + t, pos);
+  else if (n.positions != nullptr)
+    pos[0] = n.positions[b * n.pos_stride + t];
   l.place(n);
   float w[2][8];
   if (h0 < n.heads) l.weights(n, 0, w[0]);
@@ -199,7 +232,10 @@ __global__ void __launch_bounds__(256) fa_norm_kernel(const NormArgs n) {
       }
     }
   }
-  l.angles(n, pos);
+  if (n.axes > 0)
+    l.angles(n, pos);
+  else
+    l.angles(n, pos[0]);
   if (!mine) return;
 
   auto range = [&](auto x_c, int lo, int hi, const float* wt) FA_INLINE {
@@ -277,8 +313,13 @@ __global__ void __launch_bounds__(256) fa_norm_bwd_kernel(const NormArgs n) {
     const int token = tb * TPW + (int)threadIdx.x / LPR;
     if (token >= n.tokens) continue;
     const int b = fast_div(token, n.by_seq), t = token - b * n.seq_len;
-    const int pos = n.positions == nullptr ? t : n.positions[b * n.pos_stride + t];
-    l.angles(n, pos);
+    if (n.axes > 0) {
+      int pos[4];
+      l.positions(n, b * n.pos_stride + t, pos);
+      l.angles(n, pos);
+    } else {
+      l.angles(n, n.positions == nullptr ? t : n.positions[b * n.pos_stride + t]);
+    }
     auto range = [&](auto x_c, int lo, int hi) FA_INLINE {
       constexpr int X = decltype(x_c)::value;
       const char* xs = n.x[X] + b * n.x_sb[X] + t * n.x_st[X];

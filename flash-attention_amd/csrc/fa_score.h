@@ -1,0 +1,56 @@
+// Scores of attention beside the plain scale q.k: the cap, the bias by distance
+// and the window, as the host passes them and as the kernels apply them.
+#pragma once
+
+#include <stdint.h>
+
+#if defined(__HIPCC__)
+#include <hip/hip_runtime.h>
+
+#include "fa_device_ops.h"
+#endif
+
+namespace fa {
+
+struct ScoreArgs {
+  float cap;            // softcap * log2(e); 0: none
+  float cap_twice, cap_inverse;  // twice that, and its inverse
+  float cap_in;         // 2 softmax_scale log2(e) / softcap
+  float unit;           // log2(e) softmax_scale, or 1 for capped scores: what the bias is added to
+  const float* slopes;  // of each query head; NULL: no bias
+  int32_t window;       // keys at a distance below it are seen; 0: all
+};
+
+#if defined(__HIPCC__)
+namespace {
+
+// The scores of a wave, in units of log2 so that exp2 takes them as they are.
+struct Score {
+  bool capped, biased;
+  float in, out, twice, inverse;  // capped
+  float unit;            // factor of the scores that the bias is added to
+  __device__ __forceinline__ void init(const ScoreArgs& a) {
+    capped = a.cap > 0.0f;
+    biased = a.slopes != nullptr;
+    in = a.cap_in;
+    out = a.cap;
+    twice = a.cap_twice;
+    inverse = a.cap_inverse;
+    unit = a.unit;
+  }
+  // out tanh(x) with e^2x = 2^(in x): out - 2 out / (1 + e^2x).  Its error, about
+  // 1.2e-7 out, is that of 1 + e^2x: of no weight for scores up to some hundreds.
+  // Three instructions beside two of a quarter of the rate.
+  __device__ __forceinline__ float cap(float x) const {
+    return fmaf(-twice, half_tail(x), out);
+  }
+  // (1 - tanh(x)) / 2
+  __device__ __forceinline__ float half_tail(float x) const {
+    return __builtin_amdgcn_rcpf(1.0f + dev::fast_exp2(x * in));
+  }
+};
+
+}  // namespace
+#endif
+
+}  // namespace fa

@@ -3,100 +3,15 @@
 // fa_torch_ext.cpp it holds no kernels: tensors become parameter blocks,
 // workspaces come from torch's caching allocator on the current stream of the
 // tensors' device.
-#include <torch/extension.h>
-
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <ATen/hip/EmptyTensor.h>
-#include <ATen/hip/HIPGraphsUtils.cuh>
-#include <c10/core/DeviceGuard.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/variable.h>
-
 #include <array>
-#include <cmath>
-#include <initializer_list>
-#include <optional>
+#include <cstring>
+#include <string>
 #include <utility>
 
 #include "fa_host.h"
-#include "fa_mi355x_cache.h"
+#include "fa_torch_common.h"
 
 namespace {
-
-using torch::Tensor;
-
-void check_status(fa_status s, const char* what) {
-  TORCH_CHECK(s == FA_OK, what, " failed: ", fa_status_str(s), ": ", fa_last_error());
-}
-
-void check_no_grad(const char* name, std::initializer_list<const Tensor*> tensors) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const Tensor* t : tensors)
-    TORCH_CHECK(!t->requires_grad(), name, " computes no gradients: call it under torch.no_grad() or detach "
-                "its inputs");
-}
-
-// No call carries tangents on: none may be dropped.  (no_grad does not stop them.)
-void check_no_tangent(const char* name, std::initializer_list<const Tensor*> tensors) {
-  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
-  for (const Tensor* t : tensors)
-    TORCH_CHECK(t->unsafeGetTensorImpl()->autograd_meta() == nullptr || !t->_fw_grad(0).defined(), name,
-                " has no forward-mode derivative: an input has a tangent");
-}
-
-// Both, for a call without derivatives.
-void check_no_derivative(const char* name, std::initializer_list<const Tensor*> tensors) {
-  check_no_grad(name, tensors);
-  check_no_tangent(name, tensors);
-}
-
-// Tensors that a call has written: a new version of each, so that an autograd
-// graph that had saved one notices.  (Inference tensors have no versions.)
-void wrote(std::initializer_list<const Tensor*> tensors) {
-  for (const Tensor* t : tensors)
-    if (!t->is_inference()) torch::autograd::impl::bump_version(*t);
-}
-
-void check_half(const Tensor& t, const char* name, int64_t dims, const char* shape) {
-  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
-  TORCH_CHECK(t.dim() == dims, name, " must be a ", dims, "D tensor with shape ", shape);
-  TORCH_CHECK(t.dtype() == torch::kFloat16 || t.dtype() == torch::kBFloat16, name,
-              " must be float16 or bfloat16");
-  TORCH_CHECK(t.size(dims - 1) <= 1 || t.stride(dims - 1) == 1, name,
-              " must have unit stride in the last dimension");
-}
-
-void check_like(const Tensor& t, const char* name, const Tensor& ref) {
-  TORCH_CHECK(t.device() == ref.device(), name, " must be on the same device as the others");
-  TORCH_CHECK(t.dtype() == ref.dtype(), name, " must have the same dtype as the others");
-}
-
-// An int32 index tensor in rows of unit stride.
-const int32_t* index_ptr(const Tensor& t, const char* name, int64_t dims, const Tensor& ref) {
-  TORCH_CHECK(t.is_cuda() && t.device() == ref.device(), name,
-              " must be a CUDA tensor on the same device as the others");
-  TORCH_CHECK(t.dtype() == torch::kInt32, name, " must be int32");
-  TORCH_CHECK(t.dim() == dims, name, " must have ", dims, " dimension(s)");
-  TORCH_CHECK(t.size(dims - 1) <= 1 || t.stride(dims - 1) == 1, name,
-              " must have unit stride in the last dimension");
-  return t.numel() == 0 ? nullptr : t.data_ptr<int32_t>();
-}
-
-int32_t int32_of(int64_t v, const char* name) {
-  TORCH_CHECK(v >= INT32_MIN && v <= INT32_MAX, name, " does not fit 32 bits");
-  return static_cast<int32_t>(v);
-}
-
-void set_strides(int64_t* out, const Tensor& t, int n) {
-  for (int i = 0; i < n; ++i) out[i] = t.size(i) > 1 ? t.stride(i) : 0;
-  // (the stride of a dimension of one entry means nothing, and may be anything)
-}
-
-void* stream_of(const Tensor& t) {
-  return at::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
-}
 
 fa_paged_cache make_cache(const Tensor& k, const std::optional<Tensor>& v, const Tensor& table,
                           const std::optional<Tensor>& cu, const Tensor& lens) {
@@ -175,26 +90,6 @@ bool same_rows(const Tensor& a, const Tensor& b) {
   return true;
 }
 
-float scale_of(std::optional<double> scale, int64_t d) {
-  return static_cast<float>(scale.value_or(1.0 / std::sqrt((double)d)));
-}
-
-// Memory from the caching allocator without the dispatcher, which costs a
-// microsecond a tensor in calls whose kernels take five.
-Tensor new_tensor(c10::IntArrayRef sizes, c10::ScalarType type, const Tensor& ref) {
-  return at::detail::empty_cuda(sizes, type, ref.device(), c10::nullopt);
-}
-Tensor new_like(const Tensor& t) {
-  if (!t.is_non_overlapping_and_dense()) return torch::empty_like(t);
-  return at::detail::empty_strided_cuda(t.sizes(), t.strides(), t.scalar_type(), t.device());
-}
-
-Tensor workspace(uint64_t bytes, const Tensor& ref) {
-  Tensor t;
-  if (bytes > 0) t = new_tensor({(int64_t)bytes}, torch::kUInt8, ref);
-  return t;
-}
-
 float* key_weight_ptr(const Tensor& w, const Tensor& k, int64_t stride[2]) {
   TORCH_CHECK(w.is_cuda() && w.device() == k.device(),
               "key_weights must be a CUDA tensor on the same device as the others");
@@ -220,8 +115,11 @@ pybind11::object paged_forward(const Tensor& q, const Tensor& k_cache, const Ten
                               const Tensor& block_table, const Tensor& cu_seqlens,
                               const Tensor& seq_lens, std::optional<Tensor> out, int64_t max_q,
                               std::optional<int64_t> max_kv, bool causal,
-                              std::optional<double> softmax_scale, bool return_lse) {
+                              std::optional<double> softmax_scale, bool return_lse,
+                              std::optional<double> softcap, std::optional<int64_t> window,
+                              std::optional<Tensor> slopes) {
   check_no_derivative("paged_forward", {&q, &k_cache, &v_cache});
+  if (slopes) check_no_derivative("paged_forward", {&*slopes});
   if (out) check_no_derivative("paged_forward", {&*out});
   fa_paged_fwd_params p{};
   p.cache = make_cache(k_cache, v_cache, block_table, cu_seqlens, seq_lens);
@@ -250,10 +148,12 @@ pybind11::object paged_forward(const Tensor& q, const Tensor& k_cache, const Ten
   p.max_kv = kv_limit(p.cache, max_kv);
   p.softmax_scale = scale_of(softmax_scale, q.size(2));
   p.causal = causal;
+  const fa_score_params score = score_params(softcap, window, slopes, q.size(1), q);
   uint64_t bytes = 0;
-  check_status(fa_paged_fwd_workspace_size(&p, &bytes), "paged_forward");
+  check_status(fa_paged_fwd_scored_workspace_size(&p, &score, &bytes), "paged_forward");
   Tensor ws = workspace(bytes, q);
-  check_status(fa_paged_fwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)), "paged_forward");
+  check_status(fa_paged_fwd_scored(&p, &score, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
+               "paged_forward");
   if (out) wrote({&o});
   if (return_lse) return pybind11::make_tuple(o, lse);
   return pybind11::cast(o);
@@ -345,9 +245,24 @@ struct NormTables {
   }
 };
 
+// Axes of the pairs of rotated dims, a byte each; none: one position a token.
+using Axes = std::optional<std::string>;
+
+// Their number is that of the positions' first dimension.
+fa_rotary_axes rotary_axes(const std::string& axes, int32_t rot, const Tensor& positions) {
+  TORCH_CHECK((int64_t)axes.size() == rot / 2 && axes.size() <= 64,
+              "axes must have one entry per pair of rotated dims");
+  fa_rotary_axes a{};
+  std::memcpy(a.axis, axes.data(), axes.size());
+  a.axes = int32_of(positions.size(0), "the number of axes");
+  a.axis_stride = positions.size(0) > 1 ? positions.stride(0) : 0;
+  return a;
+}
+
+// With axes, a is filled in.
 fa_qk_norm_params norm_params(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw,
                               const Tensor& cos, const Tensor& sin, const std::optional<Tensor>& positions,
-                              double eps, bool interleaved) {
+                              double eps, bool interleaved, const Axes& axes, fa_rotary_axes& a) {
   check_half(q, "q", 4, "[B, H, N, D]");
   check_half(k, "k", 4, "[B, H, N, D]");
   check_like(k, "k", q);
@@ -363,7 +278,15 @@ fa_qk_norm_params norm_params(const Tensor& q, const Tensor& k, const Tensor& qw
   p.k_weight = kw.data_ptr();
   p.cos = cos.data_ptr<float>();
   p.sin = sin.data_ptr<float>();
-  if (positions) {
+  if (axes) {
+    TORCH_CHECK(positions, "axes need positions");
+    const int64_t dims = positions->dim();
+    p.positions = index_ptr(*positions, "positions", dims == 3 ? 3 : 2, q);
+    TORCH_CHECK(positions->size(-1) == q.size(2) && (dims == 2 || positions->size(1) == q.size(0)),
+                "with axes, positions must have shape [axes, N] or [axes, B, N]");
+    p.pos_stride = dims == 3 && positions->size(1) > 1 ? positions->stride(1) : 0;
+    a = rotary_axes(*axes, t.rot, *positions);
+  } else if (positions) {
     p.positions = index_ptr(*positions, "positions", positions->dim() == 2 ? 2 : 1, q);
     TORCH_CHECK(positions->size(-1) == q.size(2) &&
                     (positions->dim() == 1 || positions->size(0) == q.size(0)),
@@ -388,33 +311,28 @@ using Pair = std::pair<Tensor, Tensor>;
 
 Pair norm_forward(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Tensor& cos,
                   const Tensor& sin, const std::optional<Tensor>& positions, double eps,
-                  bool interleaved) {
-  fa_qk_norm_params p = norm_params(q, k, qw, kw, cos, sin, positions, eps, interleaved);
+                  bool interleaved, const Axes& axes) {
+  fa_rotary_axes a{};
+  fa_qk_norm_params p = norm_params(q, k, qw, kw, cos, sin, positions, eps, interleaved, axes, a);
   const c10::OptionalDeviceGuard guard(q.device());
   Tensor qo = new_like(q), ko = new_like(k);
   p.q_out = qo.data_ptr();
   p.k_out = ko.data_ptr();
   set_strides(p.q_out_stride, qo, 3);
   set_strides(p.k_out_stride, ko, 3);
-  check_status(fa_qk_norm_rope(&p, stream_of(q)), "qk_norm_rope");
+  check_status(axes ? fa_qk_norm_rope_axes(&p, &a, stream_of(q)) : fa_qk_norm_rope(&p, stream_of(q)),
+               "qk_norm_rope");
   return {qo, ko};
-}
-
-// A gradient as the kernel reads it: unit stride, 16-byte rows.
-Tensor readable(const Tensor& g) {
-  bool ok = g.size(3) <= 1 || g.stride(3) == 1;
-  for (int i = 0; i < 3; ++i) ok = ok && (g.size(i) <= 1 || (g.stride(i) >= 0 && g.stride(i) % 8 == 0));
-  ok = ok && (reinterpret_cast<uintptr_t>(g.data_ptr()) & 15u) == 0;
-  return ok ? g : g.clone(at::MemoryFormat::Contiguous);
 }
 
 std::array<Tensor, 4> norm_backward(const Tensor& dq_out, const Tensor& dk_out, const Tensor& q,
                                     const Tensor& k, const Tensor& qw, const Tensor& kw,
                                     const Tensor& cos, const Tensor& sin,
                                     const std::optional<Tensor>& positions, double eps,
-                                    bool interleaved) {
+                                    bool interleaved, const Axes& axes) {
   fa_qk_norm_bwd_params p{};
-  p.fwd = norm_params(q, k, qw, kw, cos, sin, positions, eps, interleaved);
+  fa_rotary_axes a{};
+  p.fwd = norm_params(q, k, qw, kw, cos, sin, positions, eps, interleaved, axes, a);
   for (const auto& [g, x, name] : {std::make_tuple(&dq_out, &q, "q's gradient"),
                                    std::make_tuple(&dk_out, &k, "k's gradient")}) {
     TORCH_CHECK(g->is_cuda() && g->sizes() == x->sizes(), name, " must have its tensor's shape");
@@ -437,24 +355,14 @@ std::array<Tensor, 4> norm_backward(const Tensor& dq_out, const Tensor& dk_out, 
   uint64_t bytes = 0;
   check_status(fa_qk_norm_rope_bwd_workspace_size(&p, &bytes), "qk_norm_rope_backward");
   Tensor ws = workspace(bytes, q);
-  check_status(fa_qk_norm_rope_bwd(&p, ws.data_ptr(), bytes, stream_of(q)), "qk_norm_rope_backward");
+  check_status(axes ? fa_qk_norm_rope_bwd_axes(&p, &a, ws.data_ptr(), bytes, stream_of(q))
+                    : fa_qk_norm_rope_bwd(&p, ws.data_ptr(), bytes, stream_of(q)),
+               "qk_norm_rope_backward");
   if (qw.dtype() != torch::kFloat32) {
     dqw = dqw.to(qw.dtype());
     dkw = dkw.to(kw.dtype());
   }
   return {dq, dk, dqw, dkw};
-}
-
-// Whether a leaf's gradient accumulator lives on, kept by an autograd graph,
-// on another stream than the current one: a backward pass that is captured
-// here would have to wait for that stream, which ends the capture.
-bool accumulates_elsewhere(const Tensor& t) {
-  if (!t.requires_grad() || !t.is_leaf()) return false;
-  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-  if (!node) return false;
-  const auto s = node->stream();
-  return s.has_value() &&
-         *s != at::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).unwrap();
 }
 
 // The norm in autograd, differentiable once.  (A node of its own here: one
@@ -464,12 +372,13 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
                                                 const Tensor& k, const Tensor& qw, const Tensor& kw,
                                                 const Tensor& cos, const Tensor& sin,
                                                 const std::optional<Tensor>& positions, double eps,
-                                                bool interleaved) {
+                                                bool interleaved, const Axes& axes) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const Pair y = norm_forward(q, k, qw, kw, cos, sin, positions, eps, interleaved);
+    const Pair y = norm_forward(q, k, qw, kw, cos, sin, positions, eps, interleaved, axes);
     ctx->save_for_backward({q, k, qw, kw, cos, sin, positions.value_or(Tensor())});
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["axes"] = axes;
     return {y.first, y.second};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
@@ -483,56 +392,48 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
       for (int i = 0; i < 2; ++i)
         if (!g[i].defined()) g[i] = torch::zeros_like(v[i]);
       d = norm_backward(g[0], g[1], v[0], v[1], v[2], v[3], v[4], v[5], positions,
-                        ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool());
+                        ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool(),
+                        ctx->saved_data["axes"].toOptional<std::string>());
     }
-    torch::autograd::variable_list out(d.begin(), d.end());
-    if (at::GradMode::is_enabled()) {  // create_graph: a second derivative is refused when it is asked for
-      for (Tensor& t : out) t.requires_grad_();
-      auto refuse = std::make_shared<torch::autograd::DelayedError>(
-          "trying to differentiate twice qk_norm_rope, which is once_differentiable", 4);
-      out = (*refuse)(std::move(out));
-    }
-    out.resize(9);
+    torch::autograd::variable_list out = once({d.begin(), d.end()}, "qk_norm_rope");
+    out.resize(10);
     return out;
   }
 };
 
 pybind11::tuple qk_norm_rope(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw,
                              const Tensor& cos, const Tensor& sin, std::optional<Tensor> positions,
-                             double eps, bool interleaved) {
+                             double eps, bool interleaved, Axes axes) {
   check_no_tangent("qk_norm_rope", {&q, &k, &qw, &kw, &cos, &sin});
   if (at::GradMode::is_enabled()) {
     TORCH_CHECK(!cos.requires_grad() && !sin.requires_grad(),
                 "cos and sin get no gradients: detach them");
     if (q.requires_grad() || k.requires_grad() || qw.requires_grad() || kw.requires_grad()) {
-      if (at::hip::currentStreamCaptureStatusMayInitCtx() != at::hip::CaptureStatus::None)
-        for (const Tensor* t : {&q, &k, &qw, &kw})
-          TORCH_CHECK(!accumulates_elsewhere(*t),
-                      "qk_norm_rope: an autograd graph made on another stream still holds these leaves, "
-                      "and the backward pass of this capture would have to wait for that stream: release "
-                      "that graph first, or use qk_norm_rope_backward");
-      const auto y = QkNormRope::apply(q, k, qw, kw, cos, sin, positions, eps, interleaved);
+      check_capture("qk_norm_rope", "qk_norm_rope_backward", {&q, &k, &qw, &kw});
+      const auto y = QkNormRope::apply(q, k, qw, kw, cos, sin, positions, eps, interleaved, axes);
       return pybind11::make_tuple(y[0], y[1]);
     }
   }
-  const Pair y = norm_forward(q, k, qw, kw, cos, sin, positions, eps, interleaved);
+  const Pair y = norm_forward(q, k, qw, kw, cos, sin, positions, eps, interleaved, axes);
   return pybind11::make_tuple(y.first, y.second);
 }
 
 pybind11::tuple qk_norm_rope_backward(const Tensor& dq_out, const Tensor& dk_out, const Tensor& q,
                                       const Tensor& k, const Tensor& qw, const Tensor& kw,
                                       const Tensor& cos, const Tensor& sin,
-                                      std::optional<Tensor> positions, double eps, bool interleaved) {
+                                      std::optional<Tensor> positions, double eps, bool interleaved,
+                                      Axes axes) {
   check_no_tangent("qk_norm_rope_backward", {&dq_out, &dk_out, &q, &k, &qw, &kw, &cos, &sin});
   at::NoGradGuard no_grad;
-  const auto d = norm_backward(dq_out, dk_out, q, k, qw, kw, cos, sin, positions, eps, interleaved);
+  const auto d = norm_backward(dq_out, dk_out, q, k, qw, kw, cos, sin, positions, eps, interleaved, axes);
   return pybind11::make_tuple(d[0], d[1], d[2], d[3]);
 }
 
 Tensor paged_store(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& qw, const Tensor& kw,
                    const Tensor& cos, const Tensor& sin, const Tensor& positions, Tensor k_cache,
                    Tensor v_cache, const Tensor& block_table, const Tensor& cu_seqlens,
-                   const Tensor& seq_lens, std::optional<Tensor> out, double eps, bool interleaved) {
+                   const Tensor& seq_lens, std::optional<Tensor> out, double eps, bool interleaved,
+                   Axes axes) {
   check_no_derivative("paged_store", {&q, &k, &v, &qw, &kw, &cos, &sin, &k_cache, &v_cache});
   if (out) check_no_derivative("paged_store", {&*out});
   fa_paged_store_params p{};
@@ -568,8 +469,9 @@ Tensor paged_store(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   p.k_weight = kw.data_ptr();
   p.cos = cos.data_ptr<float>();
   p.sin = sin.data_ptr<float>();
-  p.positions = index_ptr(positions, "positions", 1, q);
-  TORCH_CHECK(positions.size(0) == q.size(0), "positions must have one entry per token");
+  p.positions = index_ptr(positions, "positions", axes ? 2 : 1, q);
+  TORCH_CHECK(positions.size(-1) == q.size(0), axes ? "with axes, positions must have shape [axes, tokens]"
+                                                    : "positions must have one entry per token");
   p.tokens = int32_of(q.size(0), "tokens");
   p.heads = int32_of(q.size(1), "heads");
   p.rot = t.rot;
@@ -577,7 +479,12 @@ Tensor paged_store(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   p.interleaved = interleaved;
   p.weight_fp32 = t.fp32;
   p.eps = static_cast<float>(eps);
-  check_status(fa_paged_store(&p, stream_of(q)), "paged_store");
+  if (axes) {
+    const fa_rotary_axes a = rotary_axes(*axes, t.rot, positions);
+    check_status(fa_paged_store_axes(&p, &a, stream_of(q)), "paged_store");
+  } else {
+    check_status(fa_paged_store(&p, stream_of(q)), "paged_store");
+  }
   wrote({&k_cache, &v_cache});
   if (out) wrote({&o});
   return o;
@@ -590,7 +497,8 @@ void bind_cache(pybind11::module_& m) {
   m.def("paged_forward", &paged_forward, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
         py::arg("block_table"), py::arg("cu_seqlens"), py::arg("seq_lens"), py::arg("out"),
         py::arg("max_q"), py::arg("max_kv"), py::arg("causal"), py::arg("softmax_scale"),
-        py::arg("return_lse"));
+        py::arg("return_lse"), py::arg("softcap") = std::optional<double>{},
+        py::arg("window") = std::optional<int64_t>{}, py::arg("slopes") = std::optional<Tensor>{});
   m.def("paged_key_weights", &paged_key_weights, py::arg("q"), py::arg("lse"), py::arg("k_cache"),
         py::arg("block_table"), py::arg("cu_seqlens"), py::arg("seq_lens"), py::arg("key_weights"),
         py::arg("max_q"), py::arg("max_kv"), py::arg("causal"), py::arg("softmax_scale"));
@@ -599,12 +507,13 @@ void bind_cache(pybind11::module_& m) {
         py::arg("recent"), py::arg("max_kv"));
   m.def("qk_norm_rope", &qk_norm_rope, py::arg("q"), py::arg("k"), py::arg("q_weight"),
         py::arg("k_weight"), py::arg("cos"), py::arg("sin"), py::arg("positions"), py::arg("eps"),
-        py::arg("interleaved"));
+        py::arg("interleaved"), py::arg("axes") = Axes{});
   m.def("qk_norm_rope_backward", &qk_norm_rope_backward, py::arg("dq_out"), py::arg("dk_out"),
         py::arg("q"), py::arg("k"), py::arg("q_weight"), py::arg("k_weight"), py::arg("cos"),
-        py::arg("sin"), py::arg("positions"), py::arg("eps"), py::arg("interleaved"));
+        py::arg("sin"), py::arg("positions"), py::arg("eps"), py::arg("interleaved"),
+        py::arg("axes") = Axes{});
   m.def("paged_store", &paged_store, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("q_weight"),
         py::arg("k_weight"), py::arg("cos"), py::arg("sin"), py::arg("positions"), py::arg("k_cache"),
         py::arg("v_cache"), py::arg("block_table"), py::arg("cu_seqlens"), py::arg("seq_lens"),
-        py::arg("out"), py::arg("eps"), py::arg("interleaved"));
+        py::arg("out"), py::arg("eps"), py::arg("interleaved"), py::arg("axes") = Axes{});
 }

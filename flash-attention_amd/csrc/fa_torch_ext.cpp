@@ -154,7 +154,8 @@ pybind11::dict device_info(int device) {
 
 }  // namespace
 
-void bind_cache(pybind11::module_& m);  // fa_torch_cache.cpp
+void bind_cache(pybind11::module_& m);      // fa_torch_cache.cpp
+void bind_attention(pybind11::module_& m);  // fa_torch_attention.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("forward", &fa_forward, pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"),
@@ -167,4 +168,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "hipDeviceProp summary and dense fp16/bf16 MFMA peak");
   m.def("version", []() { return std::string(fa_version()); });
   bind_cache(m);
+  bind_attention(m);
 }

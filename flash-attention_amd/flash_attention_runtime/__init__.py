@@ -10,7 +10,8 @@ fp32 [B, H, N]) and ``split_kv`` (default True: problems whose grid would
 leave most CUs idle behind a few long q-tiles split their key ranges across
 workgroups, with an fp32 workspace from torch's allocator; False always runs
 one workgroup per q-tile).  Beyond the reference, ``cache`` has the operators
-around a paged key/value cache and the q/k norm with rotation.
+around a paged key/value cache and the q/k norm with rotation, and ``attention``
+has attention with gradients and with capped, biased and masked scores.
 
 The reference JIT-compiles its CUDA extension on first use
 (``__init__.py:10-27``); here the HIP library ``libfa_mi355x.so`` and the
@@ -94,7 +95,8 @@ def version() -> str:
     return _EXT.version()
 
 
-from .cache import (  # noqa: E402  (needs the extension)
+from .attention import attention, attention_backward, document_ranges  # noqa: E402  (needs the extension)
+from .cache import (  # noqa: E402
     paged_evict,
     paged_forward,
     paged_key_weights,
@@ -104,4 +106,5 @@ from .cache import (  # noqa: E402  (needs the extension)
 )
 
 __all__ = ["forward", "forward_timed", "device_info", "version", "paged_forward", "paged_store",
-           "paged_key_weights", "paged_evict", "qk_norm_rope", "qk_norm_rope_backward"]
+           "paged_key_weights", "paged_evict", "qk_norm_rope", "qk_norm_rope_backward", "attention",
+           "attention_backward", "document_ranges"]

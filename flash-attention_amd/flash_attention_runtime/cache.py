@@ -30,6 +30,8 @@ carries forward-mode tangents on: inputs that ask for them are refused.
 """
 from __future__ import annotations
 
+from collections.abc import Sequence
+
 import torch
 
 from . import _C as _EXT
@@ -49,6 +51,9 @@ def paged_forward(
     causal: bool = True,
     softmax_scale: float | None = None,
     return_lse: bool = False,
+    softcap: float | None = None,
+    window: int | None = None,
+    slopes: torch.Tensor | None = None,
 ):
     """Attention of the new tokens ``q`` [T, H, D] over their sequences' keys.
 
@@ -61,11 +66,15 @@ def paged_forward(
     keys than the others is not split where another has more than 32 rows (new
     tokens times heads per kv head): pass it in a call of its own.
 
+    ``softcap``, ``window`` and ``slopes`` as in ``attention``, p being the token's key: scores
+    become ``softcap * tanh(z / softcap)``, keys at a distance of ``window`` or more are neither
+    seen nor read, and ``slopes`` (fp32 [H] on the GPU) times the distance is taken off.
+
     Returns ``o`` like q, or ``(o, lse)`` with the natural-log logsumexp, fp32
     [T, H].  A row without visible keys has o = 0 and lse = -inf.
     """
     return _EXT.paged_forward(q, k_cache, v_cache, block_table, cu_seqlens, seq_lens, out, max_q,
-                              max_kv, causal, softmax_scale, return_lse)
+                              max_kv, causal, softmax_scale, return_lse, softcap, window, slopes)
 
 
 def paged_key_weights(
@@ -122,6 +131,10 @@ def paged_evict(
                             recent, max_kv)
 
 
+def _axes(axes) -> bytes | None:
+    return axes if axes is None or isinstance(axes, bytes) else bytes(axes)
+
+
 def paged_store(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -140,16 +153,18 @@ def paged_store(
     *,
     eps: float = 1e-6,
     interleaved: bool = False,
+    axes: bytes | Sequence[int] | None = None,
 ) -> torch.Tensor:
     """``qk_norm_rope`` of packed new tokens, ``q`` [T, H, D], ``k`` and ``v``
     [T, kv_heads, D], with k's result and v written to the tokens' places in the
     cache.  ``positions`` int32 [T] are the rows of the rotation's tables (after
     an eviction they run ahead of the places).  The pages that receive tokens
     must belong to one sequence only; tokens without a place (more tokens than
-    keys, absent pages) are not stored.  Returns q's result (``out`` if given,
-    which may be q itself, row for row)."""
+    keys, absent pages) are not stored.  ``axes`` as in ``qk_norm_rope``, with
+    ``positions`` [A, T].  Returns q's result (``out`` if given, which may be q
+    itself, row for row)."""
     return _EXT.paged_store(q, k, v, q_weight, k_weight, cos, sin, positions, k_cache, v_cache,
-                            block_table, cu_seqlens, seq_lens, out, eps, interleaved)
+                            block_table, cu_seqlens, seq_lens, out, eps, interleaved, _axes(axes))
 
 
 def qk_norm_rope(
@@ -163,6 +178,7 @@ def qk_norm_rope(
     *,
     eps: float = 1e-6,
     interleaved: bool = False,
+    axes: bytes | Sequence[int] | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """RMS norm of each head's row of ``q`` [B, H, N, D] and ``k`` [B, H', N, D]
     with the weights [D] (fp32 or q's dtype), then the position rotation, in one
@@ -174,13 +190,19 @@ def qk_norm_rope(
     ``positions`` (int32 [N] or [B, N]; default 0, 1, ...).  A position outside
     the tables gives NaN.
 
+    ``axes``: a token has a position on each of A <= 4 axes (time, height, width),
+    ``positions`` [A, N] or [A, B, N], and pair i turns by the position on axis
+    ``axes[i]`` (r / 2 small integers; ``bytes`` are taken as they are).  It still
+    uses column i of the tables: axes in blocks, in turn, or with frequencies of their
+    own are a matter of ``axes`` and the tables.
+
     Returns new q and k in the layout of the inputs.  Differentiable once in q,
     k and the weights; cos and sin get no gradients.  (``forward`` computes none:
-    a training step needs an attention with a backward pass behind this.)  In a graph capture a
+    a training step has ``attention`` behind this.)  In a graph capture a
     backward pass through leaves that an older autograd graph still holds is
     refused; ``qk_norm_rope_backward`` can always be captured.
     """
-    return _EXT.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    return _EXT.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, _axes(axes))
 
 
 def qk_norm_rope_backward(
@@ -196,9 +218,10 @@ def qk_norm_rope_backward(
     *,
     eps: float = 1e-6,
     interleaved: bool = False,
+    axes: bytes | Sequence[int] | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """The gradients of ``qk_norm_rope`` for the gradients of its results, without
     autograd: ``(dq, dk, dq_weight, dk_weight)``.  The weights' gradients are
     summed in fp32 in a fixed order and have the weights' dtype."""
     return _EXT.qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, positions,
-                                      eps, interleaved)
+                                      eps, interleaved, _axes(axes))
