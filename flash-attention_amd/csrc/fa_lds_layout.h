@@ -154,17 +154,22 @@ FA_LAYOUT_FN int v16_read_offset(int ch, int h, int db, int lane) {
 }
 
 // ---- Tiles read both by rows and transposed (attention's backward pass) ----
-// One swizzle for the 16-byte row reads of k16_read_offset, whose 16 rows need
-// distinct positions, and for the transposing reads of v16_read_offset, whose 8
-// rows need distinct pairs of positions: the pair goes by row % 8 (or its half,
-// at two rows to the banks), the place within it by the next bit.  Both offsets
-// are a lane's own for step or block 0 with one exclusive or: chunks 4 st and
-// 2 db only set bits above those of the lane's chunk.
+// One swizzle for the row reads of k16_read_offset and the transposing reads of
+// v16_read_offset.  A cycle of the latter serves lanes 0 .. 31: 8 rows, which need
+// distinct pairs of positions, so the pair goes by row % 8 (or its half, at two rows to
+// the banks).  A cycle of the 16-byte reads serves lanes 0 .. 3, 12 .. 15 and 20 .. 27 (or
+// their complement): rows 0 .. 3 and 12 .. 15 of one chunk, 4 .. 11 of its
+// neighbour.  So rows that share a pair (their last bit tells them apart) are of the same
+// eight: row r and 12 .. 15 for r < 4, 8 .. 11 for r = 4 .. 7.  (Measured: no conflict;
+// with pairs of r and r + 8 every row read takes 8 cycles in place of 4.)  Both offsets are
+// a lane's own for step or block 0 with one exclusive or: chunks 4 st and 2 db only
+// set bits above those of the lane's chunk.
 template <int D>
 struct TileBoth {
   static constexpr int ROWB = 2 * D;
   static FA_LAYOUT_FN int swz(int r) {
-    return D == 128 ? ((r & 7) << 1) | ((r >> 3) & 1) : (((r >> 1) & 3) << 1) | ((r >> 3) & 1);
+    const int high = (r >> 3) & 1;
+    return D == 128 ? (((r & 7) ^ (high << 2)) << 1) | high : ((((r >> 1) & 3) ^ (high << 1)) << 1) | high;
   }
   // 16 bytes: row lane % 16, elements 32 st + 8 (lane / 16) .. + 7.
   static FA_LAYOUT_FN int row_offset(int lane) {

@@ -1,6 +1,7 @@
 """The LDS layout of tiles that are read both by rows and transposed (lds::TileBoth), on a host build of the
-kernels' own functions: every read finds what was staged for it, and neither kind has a bank conflict under the model of
-test_lds_layout.py (64 banks of 4 bytes; 16 lanes a cycle for 16-byte reads, 32 for the transposing ones)."""
+kernels' own functions: every read finds what was staged for it, and neither kind has a bank conflict: 64 banks of
+4 bytes; a cycle of the transposing reads serves 32 lanes, one of the 16-byte reads 16, lanes 0 to 3, 12 to 15 and 20
+to 27 or the others (of each 32), as SQ_LDS_BANK_CONFLICT shows for swizzles that tell such groups apart."""
 from __future__ import annotations
 
 import ctypes
@@ -43,8 +44,10 @@ def test_row_reads(at, d):
     for step in range(d // 32):
         got = [at(d, 1, lane, step) for lane in range(64)]
         assert got == [place(at, d, lane % 16, 32 * step + 8 * (lane // 16)) for lane in range(64)]
-        for group in range(4):
-            assert conflict_free(got[16 * group:16 * group + 16], 16), (step, group)
+        first = [*range(4), *range(12, 16), *range(20, 28)]
+        for lanes in (first, [i for i in range(32) if i not in first]):
+            for half in (0, 32):
+                assert conflict_free([got[half + i] for i in lanes], 16), (step, lanes[0], half)
 
 
 @pytest.mark.parametrize("d", [64, 128])
