@@ -41,7 +41,7 @@ fa_status check_attn(const fa_attn_params& p, bool backward) {
     return fail(FA_ERR_SHAPE, "heads=%d must be a multiple of kv_heads=%d", (int)p.heads, (int)p.kv_heads);
   if (p.seq_len > kMaxLength || p.keys > kMaxLength)
     return fail(FA_ERR_UNSUPPORTED, "seq_len=%d and keys=%d must be at most 2^28", (int)p.seq_len, (int)p.keys);
-  // (workgroups of 64 rows, and of 256 keys in parts of 4 spans of rows)
+  // (workgroups of 64 rows, and of 128 keys in parts of 4 spans of rows)
   const int64_t rows = ((int64_t)p.seq_len + 63) / 64, keys = ((int64_t)p.keys + kAttnKeys - 1) / kAttnKeys;
   if ((__int128)p.batch * p.heads * (rows + keys) > (int64_t(1) << 30))
     return fail(FA_ERR_UNSUPPORTED, "batch*heads and the lengths exceed the kernel's range");

@@ -8,14 +8,11 @@
 // the size of q.k in place of 5):
 //  * fa_attn_rows_kernel: delta, the keys that each row sees, and, for every span
 //    of 32 rows, their limits.
-//  * fa_attn_dkv_kernel: 256 keys of a kv head, 64 to a pair of waves; passes over
-//    the spans of 32 rows that see any of them, of all query heads of the group,
-//    staged through a ring.  One wave of a pair holds K and gv, does S = Q K^T, P and
-//    gv^T += go^T P and leaves P in LDS; the other holds V and gk and does
-//    go V^T, dS and gk^T += Q^T dS a span later.  (One wave cannot hold both
-//    accumulators of D = 128 for as many keys, and an LDS read of rows has to feed four
-//    products: with two, reading at full rate takes as long as they do.)  S and go V^T
-//    come out with lanes along the keys, as P and dS have to go in.
+//  * fa_attn_dkv_kernel: 128 keys of a kv head, four waves of 32, whose K and V
+//    stay in registers; passes over the spans of 32 rows that see any of them, of all query
+//    heads of the group, staged through a ring.  S = Q K^T and go V^T come out with
+//    lanes along the keys, as P and dS have to go into gv^T += go^T P and
+//    gk^T += Q^T dS.
 //  * fa_attn_dq_kernel: 128 rows of a head, as the forward pass.
 //
 // Rounding: P and dS are rounded to the input type for the matrix cores (as P of
@@ -43,7 +40,7 @@ template <bool BF16>
 constexpr float kShift = BF16 ? 0.0f : 12.0f;  // log2 of P's factor
 
 // The record of a span, [2][4 fields][16 rows] floats: for each 16 rows
-enum RecordField { kLse, kDelta, kLo, kHi };  // (lse in log2, less kShift)
+enum RecordField { kLse, kDelta, kLo, kHi };  // (lse in log2, less kShift; minus delta)
 constexpr int kRecord = kSpan * 4;
 
 // 2^-(e + 12) for a largest |go| in [2^e, 2^(e + 1)): dS's factor.  1 for bf16.
@@ -118,7 +115,7 @@ __global__ void __launch_bounds__(256) fa_attn_rows_kernel(const AttnArgs a) {
     if (k.hi > 0) {
       const int64_t at = (int64_t)bh * a.n + i;
       lse = a.lse[at] * kLog2e - kShift<BF16>;
-      d = delta[r] - (a.glse != nullptr ? a.glse[at] : 0.0f);
+      d = (a.glse != nullptr ? a.glse[at] : 0.0f) - delta[r];
       most = top[r];
     }
   }
@@ -188,12 +185,12 @@ __device__ __forceinline__ f32x4 lds_quad(uint32_t addr) {
   return __builtin_bit_cast(f32x4, lds_read16<0>(addr));
 }
 
-// c[cb] = sum over D of the 16 rows at LDS address `at` (a lane's offset in it)
-// times the 16 NCB columns held in f.
+// c[cb] = init + sum over D of the 16 rows at LDS address `at` (a lane's offset in
+// it) times the 16 NCB columns held in f.
 template <int D, bool BF16, int NCB>
-__device__ __forceinline__ void row_product(uint32_t at, const i16x8 (&f)[NCB][D / 32], f32x4 (&c)[NCB]) {
-  constexpr int KST = D / 32, AHEAD = NCB > 2 ? 2 : KST < 3 ? KST : 3;
-  const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+__device__ __forceinline__ void row_product(uint32_t at, const i16x8 (&f)[NCB][D / 32], const f32x4& init,
+                                            f32x4 (&c)[NCB]) {
+  constexpr int KST = D / 32, AHEAD = KST < 3 ? KST : 3;
   i16x8 x[AHEAD];
   auto read = [&](auto i_c) FA_INLINE {
     constexpr int st = decltype(i_c)::value;
@@ -204,7 +201,7 @@ __device__ __forceinline__ void row_product(uint32_t at, const i16x8 (&f)[NCB][D
   static_for<0, KST>([&](auto i_c) FA_INLINE {
     constexpr int st = decltype(i_c)::value;
 #pragma unroll
-    for (int cb = 0; cb < NCB; ++cb) c[cb] = mfma16<BF16>(x[st % AHEAD], f[cb][st], st == 0 ? zero : c[cb]);
+    for (int cb = 0; cb < NCB; ++cb) c[cb] = mfma16<BF16>(x[st % AHEAD], f[cb][st], st == 0 ? init : c[cb]);
     if constexpr (st + AHEAD < KST) read(std::integral_constant<int, st + AHEAD>{});
     __builtin_amdgcn_sched_barrier(0);
   });
@@ -213,7 +210,7 @@ __device__ __forceinline__ void row_product(uint32_t at, const i16x8 (&f)[NCB][D
 // acc[db][cb] += the 32 rows at LDS address `at`, turned, times f[cb].
 template <int D, bool BF16, int NCB>
 __device__ __forceinline__ void turned_product(uint32_t at, const i16x8 (&f)[NCB], f32x4 (&acc)[D / 16][NCB]) {
-  constexpr int DB = D / 16, AHEAD = NCB > 2 ? 2 : 4, ROWB = 2 * D;
+  constexpr int DB = D / 16, AHEAD = 3, ROWB = 2 * D;
   i16x8 x[AHEAD];
   auto read = [&](auto i_c) FA_INLINE {
     constexpr int db = decltype(i_c)::value;
@@ -232,307 +229,297 @@ __device__ __forceinline__ void turned_product(uint32_t at, const i16x8 (&f)[NCB
 
 // ---- gradients of k and v ----
 
+// A span of rows of a head, below 0: none; `code`: the span, and whether the wave's
+// keys are seen by some row, by all, and the workgroup's by all.
+struct Span {
+  int head;
+  uint32_t code;
+  __device__ __forceinline__ bool is() const { return head >= 0; }
+  __device__ __forceinline__ int at() const { return (int)(code & 0x1fffffffu); }
+  __device__ __forceinline__ bool seen() const { return (code >> 29) & 1; }
+  __device__ __forceinline__ bool whole() const { return (code >> 30) & 1; }
+  __device__ __forceinline__ bool all() const { return code >> 31; }
+};
+
+// The kernel's arguments, read where they are used: what only the ends of a loop need
+// would take scalar registers all along it.
+__device__ __forceinline__ const __attribute__((address_space(4))) AttnArgs& late_args() {
+  auto* p = (const __attribute__((address_space(4))) AttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *p;
+}
+
 template <int D, bool BF16, bool CAP>
-struct DkvWave {
-  static constexpr int ROWB = 2 * D, KST = D / 32, DB = D / 16, NCB = kAttnKeys / 64;
-  static constexpr int TB = kSpan * ROWB, SLOT = 2 * TB + 1024, SLOTS = 4;  // bytes: Q, go, record
-  static constexpr int PB = NCB * 1024;                                     // of a pair's P
-  static constexpr int WPT = D / 32;  // waves that stage a tensor's rows
-  static constexpr int NI = kSpan / WPT * ROWB / 1024, LPR = ROWB / 16;
-  static_assert(NI == 2, "two copies a wave");
-  struct Shared {
-    char ring[SLOTS * SLOT];
-    char p[8 * PB];
-    float spoiled[SLOTS][2][kSpan];  // NaN for rows of Q, of go with an infinity or NaN, else 0
-    float top[8];
-  };
-  struct Item {  // a span of rows
-    int head, span;          // head < 0: none
-    bool seen, whole, all;   // the pair's keys by some row, by all; the workgroup's by all
-  };
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 128 ? 2 : 3, D == 128 ? 2 : 3)))
+    fa_attn_dkv_kernel(const AttnArgs a) {
+  constexpr int ROWB = 2 * D, KST = D / 32, DB = D / 16;
+  constexpr int TB = kSpan * ROWB, SLOT = 2 * TB + 1024, SLOTS = 4;  // bytes: Q, go, record
+  constexpr int NI = 16 * ROWB / 1024, LPR = ROWB / 16, RPI = 64 / LPR;  // copies of 16 rows
+  __shared__ __attribute__((aligned(1024))) char smem[SLOTS * SLOT];
+  __shared__ float spoiled[SLOTS][2][kSpan];  // NaN for rows of Q, of go with an infinity or NaN, else 0
+  __shared__ float top_part[4];
 
-  // SECOND: the half that does go V^T, dS and gk.
-  template <bool SECOND>
-  static __device__ __forceinline__ void run(const AttnArgs& a, Shared& sh) {
-    const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pair = wave & 3;
-    // As the forward pass, the first keys first: a causal mask's longest.
-    const int unit_blocks = a.key_tiles * a.splits;
-    const int at = xcd_remap(blockIdx.x, gridDim.x);
-    const int unit = fast_div(at, a.by_keys), within = at - unit * unit_blocks;
-    const int tile = fast_div(within, a.by_splits), split = within - tile * a.splits;
-    const int b = fast_div(unit, a.by_kvh), kvh = unit - b * a.kv_heads, h0 = kvh * a.group;
-    const int j0 = tile * kAttnKeys, w0 = j0 + 16 * NCB * pair;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // As the forward pass, the first keys first: a causal mask's longest.
+  const int unit_blocks = a.key_tiles * a.splits;
+  const int at = xcd_remap(blockIdx.x, gridDim.x);
+  const int unit = fast_div(at, a.by_keys), within = at - unit * unit_blocks;
+  const int tile = fast_div(within, a.by_splits), split = within - tile * a.splits;
+  const int b = fast_div(unit, a.by_kvh), kvh = unit - b * a.kv_heads, h0 = kvh * a.group;
+  const int j0 = tile * kAttnKeys, w0 = j0 + 32 * wave;
 
-    i16x8 f[NCB][KST];
-    {
-      const Rows3& x = SECOND ? a.v : a.k;
-      const char* xp = x.p + b * x.sb + kvh * x.sh + 16 * g4;
+  i16x8 kf[2][KST], vf[2][KST];
 #pragma unroll
-      for (int cb = 0; cb < NCB; ++cb) {
-        const int64_t j = min(w0 + 16 * cb + l16, a.m - 1);
+  for (int cb = 0; cb < 2; ++cb) {
+    const int64_t j = min(w0 + 16 * cb + (lane & 15), a.m - 1);
+    const char* kp = a.k.p + b * a.k.sb + kvh * a.k.sh + j * a.k.st + (lane >> 4) * 16;
+    const char* vp = a.v.p + b * a.v.sb + kvh * a.v.sh + j * a.v.st + (lane >> 4) * 16;
 #pragma unroll
-        for (int st = 0; st < KST; ++st) f[cb][st] = *reinterpret_cast<const i16x8*>(xp + j * x.st + 64 * st);
-      }
+    for (int st = 0; st < KST; ++st) {
+      kf[cb][st] = *reinterpret_cast<const i16x8*>(kp + 64 * st);
+      vf[cb][st] = *reinterpret_cast<const i16x8*>(vp + 64 * st);
     }
-    float factor = 1.0f;
-    if constexpr (!BF16) {
-      float top = 0.0f;
-      const float* tops = a.tops + ((int64_t)b * a.heads + h0) * a.spans;
-      for (int64_t i = threadIdx.x; i < (int64_t)a.group * a.spans; i += 512) top = fmaxf(top, tops[i]);
+  }
+  float factor = 1.0f;
+  if constexpr (!BF16) {
+    float top = 0.0f;
+    const float* tops = a.tops + ((int64_t)b * a.heads + h0) * a.spans;
+    for (int64_t i = threadIdx.x; i < (int64_t)a.group * a.spans; i += 256) top = fmaxf(top, tops[i]);
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-      if (lane == 0) sh.top[wave] = top;
-      __syncthreads();
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if (lane == 0) top_part[wave] = top;
+    __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, sh.top[i]);
-      factor = uniform(grad_factor<BF16>(uniform(top)));
-    }
-    f32x4 acc[DB][NCB];
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, top_part[i]);
+    factor = uniform(grad_factor<BF16>(uniform(top)));
+  }
+  f32x4 gk[DB][2], gv[DB][2];
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+  for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int cb = 0; cb < NCB; ++cb) acc[db][cb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int cb = 0; cb < 2; ++cb) gk[db][cb] = gv[db][cb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    // The spans with a row that sees a key of the workgroup, of the split's (every
-    // splits-th, so that the splits of a causal mask are alike), head after head:
-    // bit i of `hit` is span at0 + i.
-    const int4* bounds = reinterpret_cast<const int4*>(a.bounds) + (int64_t)b * a.spans;
-    uint64_t hit = 0, seen = 0, whole = 0, all = 0;
-    int h = 0, at0 = -64;
-    auto next = [&]() FA_INLINE -> Item {
-      while (hit == 0) {
-        at0 += 64;
-        if (at0 >= a.spans) {
-          at0 = 0;
-          if (++h >= a.group) return Item{-1, 0, false, false, false};
-        }
-        const int s = at0 + lane;
-        int4 k = {kNoKey, 0, kNoKey, 0};
-        if (s < a.spans) k = bounds[s];
-        const bool mine = s - fast_div(s, a.by_splits) * a.splits == split;
-        hit = __ballot(mine && k.x < j0 + kAttnKeys && k.y > j0);
-        seen = __ballot(k.x < w0 + 16 * NCB && k.y > w0);
-        whole = __ballot(k.z <= w0 && k.w >= w0 + 16 * NCB);
-        all = __ballot(k.z <= j0 && k.w >= j0 + kAttnKeys);
+  // The spans with a row that sees a key of the workgroup, of the split's (every
+  // splits-th, so that the splits of a causal mask are alike), head after head, the
+  // last ones first: those are a causal mask's that all tiles of keys have, and are
+  // read from L2 by all but one.  Bit i of `hit` is span at0 + i.
+  const int spans = a.spans, group = a.group, last0 = (spans - 1) & ~63;
+  uint64_t hit = 0, seen = 0, whole = 0, all = 0;
+  int h = 0, at0 = last0 + 64;
+  auto next = [&]() FA_INLINE -> Span {
+    while (hit == 0) {
+      at0 -= 64;
+      if (at0 < 0) {
+        at0 = last0;
+        if (++h >= group) return Span{-1, 0};
       }
-      const int i = __builtin_ctzll(hit);
-      hit &= hit - 1;
-      return Item{h, at0 + i, (bool)((seen >> i) & 1), (bool)((whole >> i) & 1), (bool)((all >> i) & 1)};
-    };
+      const auto& x = late_args();
+      const int s = at0 + lane;
+      int4 k = {kNoKey, 0, kNoKey, 0};
+      if (s < spans) k = reinterpret_cast<const int4*>(x.bounds)[(int64_t)b * spans + s];
+      const bool mine = s - fast_div(s, FastDiv{x.by_splits.mul, x.by_splits.shift}) * x.splits == split;
+      hit = __ballot(mine && k.x < j0 + kAttnKeys && k.y > j0);
+      seen = __ballot(k.x < w0 + 32 && k.y > w0);
+      whole = __ballot(k.z <= w0 && k.w >= w0 + 32);
+      all = __ballot(k.z <= j0 && k.w >= j0 + kAttnKeys);
+    }
+    const int i = 63 - __builtin_clzll(hit);
+    hit ^= 1ull << i;
+    return Span{h, (uint32_t)(at0 + i) | (uint32_t)((seen >> i) & 1) << 29 | (uint32_t)((whole >> i) & 1) << 30 |
+                       (uint32_t)((all >> i) & 1) << 31};
+  };
 
-    // Staging: at D = 128 all waves copy 8 rows each, the first ones of Q, the others
-    // of go; at D = 64 four waves copy 16 rows.  Wave 0 brings the record.
-    const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(&sh));
-    const int sr = wave % WPT * (kSpan / WPT);  // this wave's first row
-    const bool stages = wave < 2 * WPT, of_go = wave >= WPT;
-    const Rows3& sx = of_go ? a.go : a.q;
-    const char* sp = sx.p + b * sx.sb + h0 * sx.sh;
-    const uint32_t sst = (uint32_t)sx.st, sto = (of_go ? TB : 0) + sr * ROWB;
-    const char* records = reinterpret_cast<const char*>(a.records + ((int64_t)b * a.heads + h0) * a.spans * kRecord);
-    auto issue = [&](const Item& x, int slot) FA_INLINE {
-      if (!stages) return;
-      const int r0 = min(x.span * kSpan + sr, a.n - 1), lim = a.n - 1 - r0;
-      const char* p = sp + x.head * sx.sh + r0 * sx.st;
-      const uint32_t dst = base + slot * SLOT + sto;
-      const int l = fresh(lane);
+  // Staging: waves 0 and 1 copy 16 rows of Q each, 2 and 3 of go; wave 0 the record.
+  // (The swizzle of row i + r is that of i, exclusive or that of r.)
+  const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(smem));
+  const bool of_go = wave >= 2;
+  const int sr = (wave & 1) * 16;  // this wave's first row
+  const Rows3& sx = of_go ? a.go : a.q;
+  const uint32_t sst = (uint32_t)sx.st, sto = (of_go ? TB : 0) + sr * ROWB;
+  const char* sp = sx.p + b * sx.sb + h0 * sx.sh + sr * (int64_t)sst;  // of the head to come
+  const char* records = reinterpret_cast<const char*>(a.records + ((int64_t)b * a.heads + h0) * spans * kRecord);
+  const int64_t head_step = sx.sh;
+  const int row_end = a.n - 1 - sr;
+  int staged_head = 0;
+  const uint32_t src_row = (lane / LPR) * sst, src_chunk = ((lane % LPR) ^ lds::TileBoth<D>::swz(lane / LPR)) * 16;
+  auto issue = [&](const Span& x, uint32_t slot) FA_INLINE {
+    if (x.head != staged_head) {
+      staged_head = x.head;
+      sp += head_step;
+      records += (int64_t)spans * (kRecord * 4);
+    }
+    const int row = x.at() * kSpan;  // (less sr)
+    const uint32_t dst = base + slot * SLOT + sto;
+    const char* from = sp + (int64_t)row * sst;
+    if (row + 15 <= row_end) {
 #pragma unroll
       for (int it = 0; it < NI; ++it) {
         poison_1k(dst + it * 1024);
-        const int r = it * (64 / LPR) + l / LPR, c = (l % LPR) ^ lds::TileBoth<D>::swz(sr + r);
-        dma_16b(min(r, lim) * sst + c * 16, p, dst + it * 1024);
+        dma_16b(src_row + it * RPI * sst + (src_chunk ^ (lds::TileBoth<D>::swz(it * RPI) * 16)), from, dst + it * 1024);
       }
-      if (wave == 0) {  // (1 KiB: the next record too, or what is behind the last one)
-        poison_1k(base + slot * SLOT + 2 * TB);
-        dma_16b(l * 16, records + ((int64_t)x.head * a.spans + x.span) * kRecord * 4, base + slot * SLOT + 2 * TB);
+    } else {  // rows past the last one re-read it
+      const int l = fresh(lane), back = max(0, row - row_end);
+#pragma unroll
+      for (int it = 0; it < NI; ++it) {
+        poison_1k(dst + it * 1024);
+        const int r = it * RPI + l / LPR, c = (l % LPR) ^ lds::TileBoth<D>::swz(r);
+        dma_16b(min(r, row_end - row + back) * sst + c * 16, from - (int64_t)back * sst, dst + it * 1024);
       }
-    };
-    // The copies of a span are there, `later`: but for those of one issued after it.
-    // If the span is not seen whole, this wave cleans the rows that it has copied.
-    const uint32_t spoiled_at = base + offsetof(Shared, spoiled);
-    auto finish = [&](const Item& x, int slot, bool later) FA_INLINE {
-      if (later && stages) {
-        if (wave == 0)
-          wait_vmcnt<NI + 1>();
-        else
-          wait_vmcnt<NI>();
-      } else {
-        wait_vmcnt<0>();
-      }
-      if (stages && x.head >= 0 && !x.all) {
-        const unsigned bad = clean_rows<D, BF16, kSpan / WPT>(base + slot * SLOT + sto);
-        if (lane < kSpan / WPT)
-          lds_write4(spoiled_at + (slot * 2 + (of_go ? 1 : 0)) * kSpan * 4 + (sr + lane) * 4,
-                     (bad >> lane) & 1 ? NAN : 0.0f);
-      }
-      __builtin_amdgcn_s_waitcnt(0xc07f);
-      __syncthreads();
-    };
-
-    Grads<CAP> grads;
-    const uint32_t row_at = base + (SECOND ? TB : 0), turned_at = base + (SECOND ? 0 : TB);
-    const uint32_t p_at = base + offsetof(Shared, p) + pair * 2 * PB;
-
-    // A span in `slot`, P in buffer pb.  (Scores become P in place: the accumulators
-    // leave few registers.)
-    auto step = [&](int row0, int slot, int pb, bool masked) FA_INLINE {
-      const int l = fresh(lane);  // (nothing below is worth a register across spans)
-      const int key0 = w0 + (l & 15);
-      u32x4 w[NCB];  // P or dS as packed pairs: words 0, 1 of rows 4 g4 .., 2, 3 of those 16 on
-      static_for<0, 2>([&](auto rb_c) FA_INLINE {
-        constexpr int rb = decltype(rb_c)::value;
-        f32x4 c[NCB];
-        row_product<D, BF16, NCB>(row_at + slot * SLOT + rb * 16 * ROWB + lds::TileBoth<D>::row_offset(l), f, c);
-        const uint32_t quad = base + slot * SLOT + 2 * TB + rb * 256 + (l >> 4) * 16;
-        const uint32_t p_quad = p_at + pb * PB + rb * 512 + l * 8;
-        f32x4 stat = lds_quad(quad + (SECOND ? 64 * kDelta : 64 * kLse));
-        // (two blocks at a time: all at once would take more registers than there are)
-        auto each = [&](auto&& fn) FA_INLINE {
-#pragma unroll
-          for (int cb = 0; cb < NCB; ++cb) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) c[cb][i] = fn(c[cb][i], cb, i);
-            if (cb % 2 == 1) __builtin_amdgcn_sched_barrier(0);
-          }
-        };
-        const int away = row0 + 16 * rb + 4 * (l >> 4) + a.m - a.n - key0;  // of key block 0
-        auto away_of = [&](int cb, int i) FA_INLINE { return (float)(away - 16 * cb) + (float)i; };
-        if constexpr (!SECOND) {
-          if (masked) {
-            const uint32_t bad = spoiled_at + slot * 2 * kSpan * 4 + rb * 64 + (l >> 4) * 16;
-            stat += lds_quad(bad) + lds_quad(bad + kSpan * 4);
-          }
-          if constexpr (CAP) each([&](float x, int, int) FA_INLINE { return grads.capped(x); });
-          if (grads.score.biased)
-            each([&](float x, int cb, int i) FA_INLINE { return grads.biased(x, away_of(cb, i)); });
-          each([&](float x, int, int i) FA_INLINE { return fmaf(x, grads.unit, -stat[i]); });
-        } else {
-          each([&](float x, int, int i) FA_INLINE { return x - stat[i]; });
-        }
-        if (masked) {  // P = 2^-inf; dS = P 0
-          const float none = SECOND ? 0.0f : -INFINITY;
-          const i32x4 lo = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kLo)) - key0;
-          each([&](float x, int cb, int i) FA_INLINE { return fresh(16 * cb >= lo[i] ? x : none); });
-          const i32x4 hi = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kHi)) - key0;
-          each([&](float x, int cb, int i) FA_INLINE { return 16 * cb < hi[i] ? x : none; });
-        }
-        static_for<0, NCB>([&](auto cb_c) FA_INLINE {
-          constexpr int cb = decltype(cb_c)::value;
-          f32x4 x;
-          if constexpr (SECOND) {
-            const u32x2 pw = lds_read8<cb * 1024>(p_quad);
-            float p[4];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) unpack2<BF16>(pw[j], p + 2 * j);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = (BF16 ? p[i] : p[i] * factor) * c[cb][i];
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = fast_exp2(c[cb][i]);
-          }
-          const u32x2 out = {pack2<BF16>(x[0], x[1]), pack2<BF16>(x[2], x[3])};
-          w[cb][2 * rb] = fresh((uint32_t)out[0]);
-          w[cb][2 * rb + 1] = fresh((uint32_t)out[1]);
-          if constexpr (!SECOND) {
-            u32x2 mate = out;
-            if constexpr (CAP) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                float u = c[cb][i] + stat[i];
-                if (grads.score.biased) u = fmaf(grads.slope, fabsf(away_of(cb, i)), u);
-                x[i] *= grads.slope_of(u);
-              }
-              mate = u32x2{pack2<BF16>(x[0], x[1]), pack2<BF16>(x[2], x[3])};
-            }
-            lds_write8<cb * 1024>(p_quad, mate);
-          }
-          if constexpr (CAP || cb % 2 == 1) __builtin_amdgcn_sched_barrier(0);
-        });
-        __builtin_amdgcn_sched_barrier(0);
-      });
-      i16x8 wf[NCB];
-#pragma unroll
-      for (int cb = 0; cb < NCB; ++cb) wf[cb] = __builtin_bit_cast(i16x8, w[cb]);
-      turned_product<D, BF16, NCB>(turned_at + slot * SLOT + lds::TileBoth<D>::turned_offset(fresh(lane)), wf, acc);
-    };
-
-    // Spans t + 1 and t + 2 are on their way while the first waves have t and the
-    // second ones t - 1.
-    Item before = {-1, 0, false, false, false}, now = next(), then = before;
-    int slot = 0, pb = 0, head = -1;
-    wait_vmcnt<0>();  // (what was loaded so far: no wait for it later, which would be one for copies too)
-    if (now.head >= 0) {
-      issue(now, 0);
-      then = next();
-      if (then.head >= 0) issue(then, 1);
-      finish(now, 0, then.head >= 0);
     }
-    while (now.head >= 0 || before.head >= 0) {
-      Item last = {-1, 0, false, false, false};
-      if (then.head >= 0) last = next();
-      if (last.head >= 0) issue(last, (slot + 2) % SLOTS);
-      const Item mine = SECOND ? before : now;
-      if (mine.head >= 0 && mine.seen) {
-        if (mine.head != head) {
-          head = mine.head;
-          grads.init(a, h0 + head);
-        }
-        step(mine.span * kSpan, SECOND ? (slot + SLOTS - 1) % SLOTS : slot, SECOND ? pb ^ 1 : pb, !mine.whole);
-      }
-      finish(then, (slot + 1) % SLOTS, last.head >= 0);
-      before = now;
-      now = then;
-      then = last;
-      slot = (slot + 1) % SLOTS;
-      pb ^= 1;
+    if (wave == 0) {  // (1 KiB: the next record too, or what is behind the last one)
+      poison_1k(base + slot * SLOT + 2 * TB);
+      dma_16b(fresh(lane) * 16, records + (int64_t)x.at() * (kRecord * 4), base + slot * SLOT + 2 * TB);
     }
+  };
+  // The copies of a span are there, `later`: but for those of one issued after it.
+  // If the span is not seen whole, this wave cleans the rows that it has copied.
+  const uint32_t spoiled_at = __builtin_amdgcn_readfirstlane(lds_addr(spoiled));
+  auto finish = [&](const Span& x, uint32_t slot, bool later) FA_INLINE {
+    if (!later)
+      wait_vmcnt<0>();
+    else if (wave == 0)
+      wait_vmcnt<NI + 1>();
+    else
+      wait_vmcnt<NI>();
+    if (x.is() && !x.all()) {
+      const unsigned bad = clean_rows<D, BF16, 16>(base + slot * SLOT + sto);
+      if (lane < 16)
+        lds_write4(spoiled_at + (slot * 2 + (of_go ? 1 : 0)) * kSpan * 4 + (sr + lane) * 4, (bad >> lane) & 1 ? NAN : 0.0f);
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    __syncthreads();
+  };
 
-    // (powers of two but for the scale)
-    const float out = SECOND ? a.scale * fast_exp2(-kShift<BF16>) / factor : fast_exp2(-kShift<BF16>);
+  Grads<CAP> grads;
+  // A span in `slot`.  (Scores become P in place, dS takes the place of go V^T: the
+  // accumulators leave few registers, none to keep addresses across spans.)
+  auto step = [&](int row0, uint32_t slot, bool masked) FA_INLINE {
     const int l = fresh(lane);
-    if (a.parts != nullptr) {
-      const int64_t rows = (int64_t)a.batch * a.kv_heads * a.m;
-      float* to = a.parts + ((int64_t)split * rows + (int64_t)unit * a.m) * 2 * D + (SECOND ? 0 : D) + 4 * (l >> 4);
-#pragma unroll
-      for (int cb = 0; cb < NCB; ++cb) {
-        const int j = w0 + 16 * cb + (l & 15);
-        if (j >= a.m) continue;
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-          *reinterpret_cast<f32x4*>(to + (int64_t)j * 2 * D + 16 * db) = acc[db][cb] * out;
+    const int key0 = w0 + (l & 15);
+    const uint32_t tile = base + slot * SLOT;
+    u32x4 pw[2], dw[2];  // P and dS as packed pairs: words 0, 1 of rows 4 (l / 16) .., 2, 3 of those 16 on
+    static_for<0, 2>([&](auto rb_c) FA_INLINE {
+      constexpr int rb = decltype(rb_c)::value;
+      const uint32_t rows = tile + rb * 16 * ROWB + lds::TileBoth<D>::row_offset(l);
+      const uint32_t quad = tile + 2 * TB + rb * 256 + (l >> 4) * 16;
+      f32x4 c[2], e[2];
+      row_product<D, BF16, 2>(rows, kf, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, c);
+      row_product<D, BF16, 2>(rows + TB, vf, lds_quad(quad + 64 * kDelta), e);
+      const int away = row0 + 16 * rb + 4 * (l >> 4) + a.m - a.n - key0;  // of key block 0
+      auto away_of = [&](int cb, int i) FA_INLINE { return (float)(away - 16 * cb) + (float)i; };
+      f32x4 lse = lds_quad(quad + 64 * kLse);
+      if (masked) {
+        const uint32_t bad = spoiled_at + slot * 2 * kSpan * 4 + rb * 64 + (l >> 4) * 16;
+        lse += lds_quad(bad) + lds_quad(bad + kSpan * 4);
       }
-      return;
-    }
-    const Rows3& y = SECOND ? a.gk : a.gv;
-    char* yp = y.p + b * y.sb + kvh * y.sh;
-    const float outs[2] = {out, out};
-    static_for<0, NCB / 2>([&](auto i_c) FA_INLINE {
-      constexpr int i = decltype(i_c)::value;
-      f32x4 part[DB][2];
+      if constexpr (CAP) {
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+        for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
-        for (int cb = 0; cb < 2; ++cb) part[db][cb] = acc[db][2 * i + cb];
-      write_rows<D, BF16>(sh.ring + wave * 32 * ROWB, part, outs, l, [&](int r) FA_INLINE -> char* {
-        const int j = w0 + 32 * i + r;
-        return j < a.m ? yp + j * y.st : nullptr;
-      });
+          for (int i = 0; i < 4; ++i) {
+            const float t = grads.score.half_tail(c[cb][i]);
+            c[cb][i] = fmaf(-grads.score.twice, t, grads.score.out);
+            e[cb][i] *= 4.0f * t * (1.0f - t);
+          }
+      }
+      if (grads.score.biased)
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) c[cb][i] = grads.biased(c[cb][i], away_of(cb, i));
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[cb][i] = fmaf(c[cb][i], grads.unit, -lse[i]);
+      if (masked) {  // P = 2^-inf; dS = P 0
+        const i32x4 lo = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kLo)) - key0;
+        const i32x4 hi = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kHi)) - key0;
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (16 * cb < lo[i] || 16 * cb >= hi[i]) {
+              c[cb][i] = -INFINITY;
+              e[cb][i] = 0.0f;
+            }
+      }
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          c[cb][i] = fast_exp2(c[cb][i]);
+          e[cb][i] *= BF16 ? c[cb][i] : c[cb][i] * factor;
+        }
+        // (kept: the compiler would pack at the end and hold all until then)
+        pw[cb][2 * rb] = fresh(pack2<BF16>(c[cb][0], c[cb][1]));
+        pw[cb][2 * rb + 1] = fresh(pack2<BF16>(c[cb][2], c[cb][3]));
+        dw[cb][2 * rb] = fresh(pack2<BF16>(e[cb][0], e[cb][1]));
+        dw[cb][2 * rb + 1] = fresh(pack2<BF16>(e[cb][2], e[cb][3]));
+      }
+      __builtin_amdgcn_sched_barrier(0);
     });
-  }
-};
+    const uint32_t turned = tile + lds::TileBoth<D>::turned_offset(fresh(lane));
+    const i16x8 pf[2] = {__builtin_bit_cast(i16x8, pw[0]), __builtin_bit_cast(i16x8, pw[1])};
+    const i16x8 df[2] = {__builtin_bit_cast(i16x8, dw[0]), __builtin_bit_cast(i16x8, dw[1])};
+    turned_product<D, BF16, 2>(turned + TB, pf, gv);
+    turned_product<D, BF16, 2>(turned, df, gk);
+  };
 
-template <int D, bool BF16, bool CAP>
-__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
-    fa_attn_dkv_kernel(const AttnArgs a) {
-  using W = DkvWave<D, BF16, CAP>;
-  static_assert(4 * 32 * 2 * D * 2 <= sizeof(typename W::Shared), "rows on their way out");
-  __shared__ __attribute__((aligned(1024))) typename W::Shared sh;
-  // Waves 0..3 and 4..7: the two of a pair share a SIMD unit, one's exponentials
-  // beside the other's products.  Both halves pass the same barriers.
-  if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 8) == 0)
-    W::template run<false>(a, sh);
-  else
-    W::template run<true>(a, sh);
+  // Two spans are on their way while one is computed.
+  Span now = next(), then = {-1, 0};
+  uint32_t slot = 0;
+  int head = -1;
+  wait_vmcnt<0>();  // (what was loaded so far: no wait for it later, which would be one for copies too)
+  if (now.is()) {
+    issue(now, 0);
+    then = next();
+    if (then.is()) issue(then, 1);
+    finish(now, 0, then.is());
+  }
+  while (now.is()) {
+    Span last = {-1, 0};
+    if (then.is()) last = next();
+    if (last.is()) issue(last, (slot + 2) % SLOTS);
+    if (now.seen()) {
+      if (now.head != head) {
+        head = now.head;
+        grads.init(a, h0 + head);
+      }
+      step(now.at() * kSpan, slot, !now.whole());
+    }
+    slot = (slot + 1) % SLOTS;
+    finish(then, slot, last.is());
+    now = then;
+    then = last;
+  }
+
+  // (powers of two but for the scale)
+  const auto& x = late_args();
+  const float fv[2] = {fast_exp2(-kShift<BF16>), fast_exp2(-kShift<BF16>)};
+  const float fk[2] = {x.scale * fv[0] / factor, x.scale * fv[0] / factor};
+  const int l = fresh(lane), m = x.m;
+  if (x.parts != nullptr) {
+    const int64_t rows = (int64_t)x.batch * x.kv_heads * m;
+    float* to = x.parts + ((int64_t)split * rows + (int64_t)unit * m) * 2 * D + 4 * (l >> 4);
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) {
+      const int j = w0 + 16 * cb + (l & 15);
+      if (j >= m) continue;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        *reinterpret_cast<f32x4*>(to + (int64_t)j * 2 * D + 16 * db) = gk[db][cb] * fk[0];
+        *reinterpret_cast<f32x4*>(to + (int64_t)j * 2 * D + D + 16 * db) = gv[db][cb] * fv[0];
+      }
+    }
+    return;
+  }
+  char* ot = smem + wave * 32 * ROWB;
+  char* kp = x.gk.p + b * x.gk.sb + kvh * x.gk.sh;
+  char* vp = x.gv.p + b * x.gv.sb + kvh * x.gv.sh;
+  const int64_t k_st = x.gk.st, v_st = x.gv.st;
+  write_rows<D, BF16>(ot, gk, fk, l, [&](int r) FA_INLINE -> char* { return w0 + r < m ? kp + (w0 + r) * k_st : nullptr; });
+  write_rows<D, BF16>(ot, gv, fv, l, [&](int r) FA_INLINE -> char* { return w0 + r < m ? vp + (w0 + r) * v_st : nullptr; });
 }
 
 // Adds the splits' parts in their order: 8 elements a thread.
@@ -575,7 +562,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int row0 = (a.tiles - 1 - back) * kAttnRows, wrow0 = row0 + 32 * wave;
 
   i16x8 qf[2][KST], gf[2][KST];
-  float lse[2], delta[2], factor[2];
+  float lse[2], delta[2], factor[2];  // (minus delta)
   RowKeys see[2];
   TileKeys keys;
 #pragma unroll
@@ -670,11 +657,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   // 32 keys from k0, in half `half` of the tile.
   auto step = [&](int k0, int off, int half, bool masked) FA_INLINE {
     const uint32_t rows = row_at + off + half * 32 * ROWB;
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
     f32x4 s[2][2], dp[2][2];
     static_for<0, 2>([&](auto kb_c) FA_INLINE {
       constexpr int kb = decltype(kb_c)::value;
-      row_product<D, BF16, 2>(rows + kb * 16 * ROWB, qf, s[kb]);
-      row_product<D, BF16, 2>(rows + TB + kb * 16 * ROWB, gf, dp[kb]);
+      row_product<D, BF16, 2>(rows + kb * 16 * ROWB, qf, zero, s[kb]);
+      row_product<D, BF16, 2>(rows + TB + kb * 16 * ROWB, gf, zero, dp[kb]);
     });
     i16x8 df[2];
 #pragma unroll
@@ -700,7 +688,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
           p *= grads.slope_of(u);
         }
         if constexpr (!BF16) p *= factor[rb];
-        return p * (dp[kb][rb][i] - delta[rb]);
+        return p * (dp[kb][rb][i] + delta[rb]);
       });
       if (masked)
         each([&](float x, int kb, int i) FA_INLINE {
@@ -741,10 +729,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 }
 
 template <class F>
-hipError_t launch(F* fn, int64_t grid, const AttnArgs& a, hipStream_t stream, int threads = 256) {
+hipError_t launch(F* fn, int64_t grid, const AttnArgs& a, hipStream_t stream) {
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
   void* kargs[] = {const_cast<AttnArgs*>(&a)};
-  return hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)grid), dim3(threads), kargs, 0, stream);
+  return hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)grid), dim3(256), kargs, 0, stream);
 }
 
 template <int D, bool BF16>
@@ -754,8 +742,8 @@ hipError_t launch_as(const AttnArgs& a, hipStream_t stream) {
   if (e != hipSuccess) return e;
   const bool cap = a.score.cap > 0.0f;
   const int64_t dkv = (int64_t)a.batch * a.kv_heads * a.key_tiles * a.splits;
-  e = cap ? launch(&fa_attn_dkv_kernel<D, BF16, true>, dkv, a, stream, 512)
-          : launch(&fa_attn_dkv_kernel<D, BF16, false>, dkv, a, stream, 512);
+  e = cap ? launch(&fa_attn_dkv_kernel<D, BF16, true>, dkv, a, stream)
+          : launch(&fa_attn_dkv_kernel<D, BF16, false>, dkv, a, stream);
   if (e != hipSuccess) return e;
   if (a.parts != nullptr) {
     const int64_t rows = (int64_t)a.batch * a.kv_heads * a.m;

@@ -41,7 +41,7 @@ struct AttnArgs {
 };
 
 constexpr int kAttnRows = 128;  // rows of a forward or dq workgroup
-constexpr int kAttnKeys = 256;  // keys of a dk, dv workgroup
+constexpr int kAttnKeys = 128;  // keys of a dk, dv workgroup
 constexpr int kSpan = 32;       // rows that it stages at a time
 
 struct AttnBwdPlan {
