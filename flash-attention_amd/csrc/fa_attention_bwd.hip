@@ -162,16 +162,9 @@ struct Grads {
     slope = uniform(score.biased ? a.score.slopes[h] * kLog2e : 0.0f);
     unit = uniform(CAP || score.biased ? 1.0f : a.scale_log2);
   }
-  // (scores q.k, capped and biased); away: from a score's row to its key.
-  __device__ __forceinline__ float capped(float x) const { return CAP ? score.cap(x) : x; }
+  // away: from a score's row to its key.
   __device__ __forceinline__ float biased(float x, float away) const {
     return fmaf(-slope, fabsf(away), CAP ? x : x * score.unit);
-  }
-  // P's factor 1 - tanh^2 from its exponent, plus lse, less the bias: the capped
-  // score.  A masked one's, -inf, and a NaN have 0.
-  __device__ __forceinline__ float slope_of(float x) const {
-    const float t = x * score.inverse;
-    return fmaxf(fmaf(-t, t, 1.0f), 0.0f);
   }
 };
 
@@ -187,9 +180,10 @@ __device__ __forceinline__ f32x4 lds_quad(uint32_t addr) {
 
 // c[cb] = init + sum over D of the 16 rows at LDS address `at` (a lane's offset in
 // it) times the 16 NCB columns held in f.
-template <int D, bool BF16, int NCB>
+// beside(i): vector work that goes between the products, in D / 32 parts.
+template <int D, bool BF16, int NCB, class Beside>
 __device__ __forceinline__ void row_product(uint32_t at, const i16x8 (&f)[NCB][D / 32], const f32x4& init,
-                                            f32x4 (&c)[NCB]) {
+                                            f32x4 (&c)[NCB], Beside&& beside) {
   constexpr int KST = D / 32, AHEAD = KST < 3 ? KST : 3;
   i16x8 x[AHEAD];
   auto read = [&](auto i_c) FA_INLINE {
@@ -203,6 +197,7 @@ __device__ __forceinline__ void row_product(uint32_t at, const i16x8 (&f)[NCB][D
 #pragma unroll
     for (int cb = 0; cb < NCB; ++cb) c[cb] = mfma16<BF16>(x[st % AHEAD], f[cb][st], st == 0 ? init : c[cb]);
     if constexpr (st + AHEAD < KST) read(std::integral_constant<int, st + AHEAD>{});
+    beside(i_c);
     __builtin_amdgcn_sched_barrier(0);
   });
 }
@@ -217,6 +212,10 @@ __device__ __forceinline__ void turned_product(uint32_t at, const i16x8 (&f)[NCB
     x[db % AHEAD] = ds_read_tr_pair<0, 16 * ROWB>(at ^ lds::TileBoth<D>::turned_block(db));
   };
   static_for<0, AHEAD>(read);
+  // The wave that is in these products goes first, so that the other wave's
+  // exponentials fill the gaps (dk, dv of 2 x 8192 tokens, 32 heads on 8, causal, us without
+  // and with: D = 128 2288 and 2214; D = 64 1652 and 1670).
+  if constexpr (D == 128) __builtin_amdgcn_s_setprio(1);
   __builtin_amdgcn_sched_barrier(0);
   static_for<0, DB>([&](auto i_c) FA_INLINE {
     constexpr int db = decltype(i_c)::value;
@@ -225,6 +224,7 @@ __device__ __forceinline__ void turned_product(uint32_t at, const i16x8 (&f)[NCB
     if constexpr (db + AHEAD < DB) read(std::integral_constant<int, db + AHEAD>{});
     __builtin_amdgcn_sched_barrier(0);
   });
+  if constexpr (D == 128) __builtin_amdgcn_s_setprio(0);
 }
 
 // ---- gradients of k and v ----
@@ -404,8 +404,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 1
       const uint32_t rows = tile + rb * 16 * ROWB + lds::TileBoth<D>::row_offset(l);
       const uint32_t quad = tile + 2 * TB + rb * 256 + (l >> 4) * 16;
       f32x4 c[2], e[2];
-      row_product<D, BF16, 2>(rows, kf, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, c);
-      row_product<D, BF16, 2>(rows + TB, vf, lds_quad(quad + 64 * kDelta), e);
+      const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+      row_product<D, BF16, 2>(rows, kf, zero, c, [](auto) FA_INLINE {});
       const int away = row0 + 16 * rb + 4 * (l >> 4) + a.m - a.n - key0;  // of key block 0
       auto away_of = [&](int cb, int i) FA_INLINE { return (float)(away - 16 * cb) + (float)i; };
       f32x4 lse = lds_quad(quad + 64 * kLse);
@@ -413,44 +413,55 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 1
         const uint32_t bad = spoiled_at + slot * 2 * kSpan * 4 + rb * 64 + (l >> 4) * 16;
         lse += lds_quad(bad) + lds_quad(bad + kSpan * 4);
       }
+      if (!CAP && grads.score.biased)
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) c[cb][i] = grads.biased(c[cb][i], away_of(cb, i));
+      // The exponentials, or the first ones of capped scores, beside go V^T.
+      row_product<D, BF16, 2>(rows + TB, vf, lds_quad(quad + 64 * kDelta), e, [&](auto i_c) FA_INLINE {
+        constexpr int PART = 8 / KST;
+#pragma unroll
+        for (int j = 0; j < PART; ++j) {
+          const int at = decltype(i_c)::value * PART + j;
+          const float x = c[at / 4][at % 4];
+          c[at / 4][at % 4] = CAP ? grads.score.half_tail(x) : fast_exp2(fmaf(x, grads.unit, -lse[at % 4]));
+        }
+      });
       if constexpr (CAP) {
 #pragma unroll
         for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float t = grads.score.half_tail(c[cb][i]);
+            const float t = c[cb][i];
             c[cb][i] = fmaf(-grads.score.twice, t, grads.score.out);
             e[cb][i] *= 4.0f * t * (1.0f - t);
           }
-      }
-      if (grads.score.biased)
+        if (grads.score.biased)
+#pragma unroll
+          for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[cb][i] = grads.biased(c[cb][i], away_of(cb, i));
 #pragma unroll
         for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) c[cb][i] = grads.biased(c[cb][i], away_of(cb, i));
+          for (int i = 0; i < 4; ++i) c[cb][i] = fast_exp2(c[cb][i] - lse[i]);
+      }
 #pragma unroll
       for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c[cb][i] = fmaf(c[cb][i], grads.unit, -lse[i]);
-      if (masked) {  // P = 2^-inf; dS = P 0
+        for (int i = 0; i < 4; ++i) e[cb][i] *= BF16 ? c[cb][i] : c[cb][i] * factor;
+      if (masked) {
         const i32x4 lo = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kLo)) - key0;
         const i32x4 hi = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kHi)) - key0;
 #pragma unroll
         for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (16 * cb < lo[i] || 16 * cb >= hi[i]) {
-              c[cb][i] = -INFINITY;
-              e[cb][i] = 0.0f;
-            }
+            if (16 * cb < lo[i] || 16 * cb >= hi[i]) c[cb][i] = e[cb][i] = 0.0f;
       }
 #pragma unroll
       for (int cb = 0; cb < 2; ++cb) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          c[cb][i] = fast_exp2(c[cb][i]);
-          e[cb][i] *= BF16 ? c[cb][i] : c[cb][i] * factor;
-        }
         // (kept: the compiler would pack at the end and hold all until then)
         pw[cb][2 * rb] = fresh(pack2<BF16>(c[cb][0], c[cb][1]));
         pw[cb][2 * rb + 1] = fresh(pack2<BF16>(c[cb][2], c[cb][3]));
@@ -659,36 +670,56 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     const uint32_t rows = row_at + off + half * 32 * ROWB;
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
     f32x4 s[2][2], dp[2][2];
-    static_for<0, 2>([&](auto kb_c) FA_INLINE {
-      constexpr int kb = decltype(kb_c)::value;
-      row_product<D, BF16, 2>(rows + kb * 16 * ROWB, qf, zero, s[kb]);
-      row_product<D, BF16, 2>(rows + TB + kb * 16 * ROWB, gf, zero, dp[kb]);
-    });
+    const int key0 = k0 + 4 * g4;
+    auto away_of = [&](int rb, int kb, int i) FA_INLINE {
+      return (float)(key0 + 16 * kb - (min(wrow0 + 16 * rb + l16, a.n - 1) + ahead)) + (float)i;
+    };
+    // The exponentials of a product, or the first ones of capped scores, beside the next.
+    auto none = [](auto) FA_INLINE {};
+    auto bias = [&](int kb) FA_INLINE {
+      if (!CAP && grads.score.biased)
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[kb][rb][i] = grads.biased(s[kb][rb][i], away_of(rb, kb, i));
+    };
+    auto part = [&](auto kb_c) FA_INLINE {
+      return [&](auto i_c) FA_INLINE {
+        constexpr int PART = 8 / KST, kb = decltype(kb_c)::value;
+#pragma unroll
+        for (int j = 0; j < PART; ++j) {
+          const int at = decltype(i_c)::value * PART + j;
+          const float x = s[kb][at / 4][at % 4];
+          s[kb][at / 4][at % 4] = CAP ? grads.score.half_tail(x) : fast_exp2(fmaf(x, grads.unit, -lse[at / 4]));
+        }
+      };
+    };
+    row_product<D, BF16, 2>(rows, qf, zero, s[0], none);
+    bias(0);
+    row_product<D, BF16, 2>(rows + 16 * ROWB, qf, zero, s[1], part(std::integral_constant<int, 0>{}));
+    bias(1);
+    row_product<D, BF16, 2>(rows + TB, gf, zero, dp[0], part(std::integral_constant<int, 1>{}));
+    row_product<D, BF16, 2>(rows + TB + 16 * ROWB, gf, zero, dp[1], none);
     i16x8 df[2];
 #pragma unroll
     for (int rb = 0; rb < 2; ++rb) {
-      const int key0 = k0 + 4 * g4;
-      const int pos = min(wrow0 + 16 * rb + l16, a.n - 1) + ahead;
-      auto away_of = [&](int kb, int i) FA_INLINE { return (float)(key0 + 16 * kb - pos) + (float)i; };
       auto each = [&](auto&& fn) FA_INLINE {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[kb][rb][i] = fn(s[kb][rb][i], kb, i);
       };
-      if constexpr (CAP) each([&](float x, int, int) FA_INLINE { return grads.capped(x); });
-      if (grads.score.biased)
-        each([&](float x, int kb, int i) FA_INLINE { return grads.biased(x, away_of(kb, i)); });
       each([&](float x, int kb, int i) FA_INLINE {
-        const float e = fmaf(x, grads.unit, -lse[rb]);
-        float p = fast_exp2(e);
+        float p = x;
         if constexpr (CAP) {
-          float u = e + lse[rb];
-          if (grads.score.biased) u = fmaf(grads.slope, fabsf(away_of(kb, i)), u);
-          p *= grads.slope_of(u);
+          const float c = fmaf(-grads.score.twice, x, grads.score.out);
+          dp[kb][rb][i] = (dp[kb][rb][i] + delta[rb]) * (4.0f * x * (1.0f - x));
+          p = fast_exp2((grads.score.biased ? grads.biased(c, away_of(rb, kb, i)) : c) - lse[rb]);
+        } else {
+          dp[kb][rb][i] += delta[rb];
         }
         if constexpr (!BF16) p *= factor[rb];
-        return p * (dp[kb][rb][i] + delta[rb]);
+        return p * dp[kb][rb][i];
       });
       if (masked)
         each([&](float x, int kb, int i) FA_INLINE {
