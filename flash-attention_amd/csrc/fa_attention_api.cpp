@@ -12,6 +12,35 @@
 
 namespace fa {
 
+namespace {
+constexpr int kXcds = 8;
+}
+
+GridOrder grid_order(int units, int places, int compute_units) {
+  GridOrder o = {};
+  o.units = units;
+  o.places = places;
+  o.xcd_cus = compute_units / kXcds;
+  o.per_xcd = units % kXcds == 0 ? units / kXcds : 0;
+  o.xcds = o.per_xcd == 0 && kXcds % units == 0 ? kXcds / units : 0;
+  // As many units at once as give each CU two workgroups, of those that divide an
+  // XCD's evenly.
+  o.unit_group = 1;
+  while (o.per_xcd > 0 && (o.per_xcd % o.unit_group != 0 ||
+                           (o.unit_group < o.per_xcd && (int64_t)o.unit_group * places < 2 * o.xcd_cus)))
+    ++o.unit_group;
+  o.turn = (int64_t)units * places > (int64_t)kXcds * o.xcd_cus;
+  o.by_group_places = make_fast_div((uint32_t)(o.unit_group * places));
+  o.by_unit_group = make_fast_div((uint32_t)o.unit_group);
+  o.by_units = make_fast_div((uint32_t)units);
+  return o;
+}
+
+int64_t grid_size(const GridOrder& o) {
+  if (o.xcds > 0) return (int64_t)kXcds * ((o.places + o.xcds - 1) / o.xcds);
+  return (int64_t)o.units * o.places;
+}
+
 AttnBwdPlan plan_attn_bwd(const AttnArgs& a, int head_dim, int compute_units) {
   AttnBwdPlan p = {};
   const int64_t bh = (int64_t)a.batch * a.heads;
@@ -69,7 +98,7 @@ Rows3 rows3(const void* p, const int64_t st[3]) {
   return Rows3{static_cast<char*>(const_cast<void*>(p)), 2 * st[0], 2 * st[1], 2 * st[2]};
 }
 
-AttnArgs attn_args(const fa_attn_params& p) {
+AttnArgs attn_args(const fa_attn_params& p, int compute_units) {
   AttnArgs a = {};
   a.q = rows3(p.q, p.q_stride);
   a.k = rows3(p.k, p.k_stride);
@@ -89,18 +118,21 @@ AttnArgs attn_args(const fa_attn_params& p) {
   a.scale_log2 = (float)(p.softmax_scale * kLog2e);
   a.score = score_args(p.score, p.softmax_scale);
   a.tiles = (p.seq_len + kAttnRows - 1) / kAttnRows;
-  a.by_unit = make_fast_div((uint32_t)(a.tiles * a.group));
   a.by_group = make_fast_div((uint32_t)a.group);
   a.by_kvh = make_fast_div((uint32_t)a.kv_heads);
+  a.rows = grid_order(a.batch * a.kv_heads, a.tiles * a.group, compute_units);
   a.spans = (p.seq_len + kSpan - 1) / kSpan;
   a.key_tiles = (p.keys + kAttnKeys - 1) / kAttnKeys;
   return a;
 }
 
-fa_status bwd_plan(const fa_attn_bwd_params& p, AttnBwdPlan* plan) {
+fa_status bwd_plan(const fa_attn_bwd_params& p, AttnArgs* args, AttnBwdPlan* plan) {
   int cus = 0;
   FA_TRY(current_compute_units(&cus));
-  *plan = plan_attn_bwd(attn_args(p.fwd), p.fwd.head_dim, cus);
+  *args = attn_args(p.fwd, cus);
+  *plan = plan_attn_bwd(*args, p.fwd.head_dim, cus);
+  args->splits = plan->splits;
+  args->cols = grid_order(args->batch * args->kv_heads, args->key_tiles * plan->splits, cus);
   return FA_OK;
 }
 
@@ -141,7 +173,9 @@ fa_status fa_attn_bwd_validate(const fa_attn_bwd_params* p) {
 
 fa_status fa_attn_fwd(const fa_attn_params* p, void* stream) {
   FA_TRY(fa_attn_fwd_validate(p));
-  return launched(launch_attn_fwd(attn_args(*p), p->head_dim, p->dtype == FA_DTYPE_BF16,
+  int cus = 0;
+  FA_TRY(current_compute_units(&cus));
+  return launched(launch_attn_fwd(attn_args(*p, cus), p->head_dim, p->dtype == FA_DTYPE_BF16,
                                   static_cast<hipStream_t>(stream)));
 }
 
@@ -149,18 +183,19 @@ fa_status fa_attn_bwd_workspace_size(const fa_attn_bwd_params* p, uint64_t* byte
   if (bytes == nullptr) return fail(FA_ERR_NULL, "bytes is NULL");
   *bytes = 0;
   FA_TRY(fa_attn_bwd_validate(p));
+  AttnArgs a;
   AttnBwdPlan plan;
-  FA_TRY(bwd_plan(*p, &plan));
+  FA_TRY(bwd_plan(*p, &a, &plan));
   *bytes = total(plan);
   return FA_OK;
 }
 
 fa_status fa_attn_bwd(const fa_attn_bwd_params* p, void* workspace, uint64_t workspace_bytes, void* stream) {
   FA_TRY(fa_attn_bwd_validate(p));
+  AttnArgs a;
   AttnBwdPlan plan;
-  FA_TRY(bwd_plan(*p, &plan));
+  FA_TRY(bwd_plan(*p, &a, &plan));
   FA_TRY(check_workspace(workspace, workspace_bytes, total(plan)));
-  AttnArgs a = attn_args(p->fwd);
   a.go = rows3(p->go, p->go_stride);
   a.gq = rows3(p->gq, p->gq_stride);
   a.gk = rows3(p->gk, p->gk_stride);
@@ -170,9 +205,7 @@ fa_status fa_attn_bwd(const fa_attn_bwd_params* p, void* workspace, uint64_t wor
   a.records = reinterpret_cast<float*>(ws);
   a.bounds = reinterpret_cast<int32_t*>(ws + plan.records);
   a.tops = reinterpret_cast<float*>(ws + plan.records + plan.bounds);
-  a.splits = plan.splits;
   a.parts = plan.parts > 0 ? reinterpret_cast<float*>(ws + plan.records + plan.bounds + plan.tops) : nullptr;
-  a.by_keys = make_fast_div((uint32_t)(a.key_tiles * a.splits));
   a.by_splits = make_fast_div((uint32_t)a.splits);
   return launched(launch_attn_bwd(a, p->fwd.head_dim, p->fwd.dtype == FA_DTYPE_BF16,
                                   static_cast<hipStream_t>(stream)));

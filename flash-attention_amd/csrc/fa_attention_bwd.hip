@@ -261,10 +261,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 1
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // As the forward pass, the first keys first: a causal mask's longest.
-  const int unit_blocks = a.key_tiles * a.splits;
-  const int at = xcd_remap(blockIdx.x, gridDim.x);
-  const int unit = fast_div(at, a.by_keys), within = at - unit * unit_blocks;
+  // The first keys first: a causal mask's longest.
+  int unit, within;
+  if (!unit_and_place(a.cols, unit, within)) return;
   const int tile = fast_div(within, a.by_splits), split = within - tile * a.splits;
   const int b = fast_div(unit, a.by_kvh), kvh = unit - b * a.kv_heads, h0 = kvh * a.group;
   const int j0 = tile * kAttnKeys, w0 = j0 + 32 * wave;
@@ -564,9 +563,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 
   const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int unit_blocks = a.tiles * a.group;
-  const int at = xcd_remap(blockIdx.x, gridDim.x);
-  const int unit = fast_div(at, a.by_unit), within = at - unit * unit_blocks;
+  int unit, within;
+  if (!unit_and_place(a.rows, unit, within)) return;
   const int back = fast_div(within, a.by_group);
   const int b = fast_div(unit, a.by_kvh), kvh = unit - b * a.kv_heads;
   const int h = kvh * a.group + within - back * a.group;
@@ -772,7 +770,7 @@ hipError_t launch_as(const AttnArgs& a, hipStream_t stream) {
                         a, stream);
   if (e != hipSuccess) return e;
   const bool cap = a.score.cap > 0.0f;
-  const int64_t dkv = (int64_t)a.batch * a.kv_heads * a.key_tiles * a.splits;
+  const int64_t dkv = grid_size(a.cols);
   e = cap ? launch(&fa_attn_dkv_kernel<D, BF16, true>, dkv, a, stream)
           : launch(&fa_attn_dkv_kernel<D, BF16, false>, dkv, a, stream);
   if (e != hipSuccess) return e;
@@ -781,7 +779,7 @@ hipError_t launch_as(const AttnArgs& a, hipStream_t stream) {
     e = launch(&fa_attn_join_kernel<D, BF16>, (rows * (2 * D / 8) + 255) / 256, a, stream);
     if (e != hipSuccess) return e;
   }
-  const int64_t dq = (int64_t)a.batch * a.heads * a.tiles;
+  const int64_t dq = grid_size(a.rows);
   return cap ? launch(&fa_attn_dq_kernel<D, BF16, true>, dq, a, stream)
              : launch(&fa_attn_dq_kernel<D, BF16, false>, dq, a, stream);
 }

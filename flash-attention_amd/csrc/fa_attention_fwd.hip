@@ -30,11 +30,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (threadIdx.x == 0) again = 0;  // ordered by the first barrier
-  // XCD x has the kv heads x, ... in a row, so that their keys stay in its L2; of
-  // each the last tiles first, which are the longest of a causal mask.
-  const int unit_blocks = a.tiles * a.group;
-  const int at = xcd_remap(blockIdx.x, gridDim.x);
-  const int unit = fast_div(at, a.by_unit), within = at - unit * unit_blocks;
+  int unit, within;  // (the last tiles first, which are the longest of a causal mask)
+  if (!unit_and_place(a.rows, unit, within)) return;
   const int back = fast_div(within, a.by_group);
   const int b = fast_div(unit, a.by_kvh), kvh = unit - b * a.kv_heads;
   const int h = kvh * a.group + within - back * a.group;
@@ -152,7 +149,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 
 template <int D, bool BF16>
 hipError_t launch_as(const AttnArgs& a, hipStream_t stream) {
-  const int64_t grid = (int64_t)a.batch * a.heads * a.tiles;
+  const int64_t grid = grid_size(a.rows);
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
   void* kargs[] = {const_cast<AttnArgs*>(&a)};
   return hipLaunchKernel(reinterpret_cast<const void*>(&fa_attn_fwd_kernel<D, BF16>), dim3((unsigned)grid),

@@ -16,6 +16,13 @@ struct Rows3 {
   int64_t sb, sh, st;  // batch, head, row
 };
 
+// Order of a grid: `places` workgroups of each unit (batch entry and kv head), the
+// longest of a causal mask first.
+struct GridOrder {
+  int32_t units, places, per_xcd, unit_group, xcds, xcd_cus, turn;
+  FastDiv by_group_places, by_unit_group, by_units;
+};
+
 struct AttnArgs {
   Rows3 q, k, v, o;
   float* lse;               // [batch, heads, n] contiguous
@@ -27,7 +34,8 @@ struct AttnArgs {
   float scale, scale_log2;
   ScoreArgs score;
   int32_t tiles;            // row tiles of a head (kAttnRows)
-  FastDiv by_unit, by_group, by_kvh;  // by_unit: tiles * group workgroups of a kv head
+  FastDiv by_group, by_kvh;
+  GridOrder rows;           // forward and dq: tiles * group places
   // backward
   Rows3 go, gq, gk, gv;     // gradients of o, q, k, v
   const float* glse;        // of lse; may be NULL
@@ -36,7 +44,8 @@ struct AttnArgs {
   float* tops;              // [batch, heads, spans]: largest |go|
   int32_t spans;            // spans of kSpan rows
   int32_t key_tiles, splits;
-  FastDiv by_keys, by_splits;  // by_keys: key tiles * splits workgroups of a kv head
+  FastDiv by_splits;
+  GridOrder cols;           // dk, dv: key_tiles * splits places
   float* parts;             // [splits][batch, kv_heads, m][2][D] gradients of k and v; NULL: one split
 };
 
@@ -48,6 +57,8 @@ struct AttnBwdPlan {
   int32_t splits;
   uint64_t records, bounds, tops, parts;  // bytes, each a multiple of 16
 };
+GridOrder grid_order(int units, int places, int compute_units);
+int64_t grid_size(const GridOrder& o);
 AttnBwdPlan plan_attn_bwd(const AttnArgs& a, int head_dim, int compute_units);
 
 hipError_t launch_attn_fwd(const AttnArgs& args, int head_dim, bool bf16, hipStream_t stream);

@@ -63,6 +63,33 @@ struct TileKeys {
   }
 };
 
+// Unit and place of a workgroup; false: none.  Workgroup w runs on XCD w % 8, in
+// order; the workgroups of a unit share its keys (or rows) through the XCD's L2, and the
+// longest ones of all units should start first:
+//  * a multiple of 8 units: whole units per XCD, as many of them interleaved as fill
+//    it;
+//  * 1, 2 or 4: 8 / units XCDs take turns with a unit's places;
+//  * else all units interleaved over all XCDs.
+// Workgroups k and k + xcd_cus of an XCD share a CU: `turn`, the first xcd_cus run
+// backwards, so that the longest of them has the shortest neighbour.
+__device__ __forceinline__ bool unit_and_place(const GridOrder& o, int& unit, int& place) {
+  const int xcd = blockIdx.x % kNumXcd;
+  int i = blockIdx.x / kNumXcd;
+  if (o.turn && i < o.xcd_cus) i = o.xcd_cus - 1 - i;
+  if (o.per_xcd > 0) {
+    const int grp = fast_div(i, o.by_group_places), w = i - grp * o.unit_group * o.places;
+    place = fast_div(w, o.by_unit_group);
+    unit = xcd * o.per_xcd + grp * o.unit_group + (w - place * o.unit_group);
+  } else if (o.xcds > 0) {
+    unit = xcd / o.xcds;
+    place = i * o.xcds + xcd % o.xcds;
+  } else {
+    place = fast_div(i * kNumXcd + xcd, o.by_units);
+    unit = i * kNumXcd + xcd - place * o.units;
+  }
+  return place < o.places;
+}
+
 // Staging of 16 rows of a tensor into LDS in the layout of lds::TileBoth.
 template <int D>
 struct RowStage {
