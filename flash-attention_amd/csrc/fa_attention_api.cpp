@@ -16,20 +16,20 @@ namespace {
 constexpr int kXcds = 8;
 }
 
-GridOrder grid_order(int units, int places, int compute_units) {
+GridOrder grid_order(int units, int places, int compute_units, int per_cu) {
   GridOrder o = {};
   o.units = units;
   o.places = places;
   o.xcd_cus = compute_units / kXcds;
   o.per_xcd = units % kXcds == 0 ? units / kXcds : 0;
   o.xcds = o.per_xcd == 0 && kXcds % units == 0 ? kXcds / units : 0;
-  // As many units at once as give each CU two workgroups, of those that divide an
+  // As many units at once as give each CU its workgroups, of those that divide an
   // XCD's evenly.
   o.unit_group = 1;
   while (o.per_xcd > 0 && (o.per_xcd % o.unit_group != 0 ||
-                           (o.unit_group < o.per_xcd && (int64_t)o.unit_group * places < 2 * o.xcd_cus)))
+                           (o.unit_group < o.per_xcd && (int64_t)o.unit_group * places < per_cu * o.xcd_cus)))
     ++o.unit_group;
-  o.turn = (int64_t)units * places > (int64_t)kXcds * o.xcd_cus;
+  o.turn = per_cu > 1 && (int64_t)units * places > (int64_t)kXcds * o.xcd_cus;
   o.by_group_places = make_fast_div((uint32_t)(o.unit_group * places));
   o.by_unit_group = make_fast_div((uint32_t)o.unit_group);
   o.by_units = make_fast_div((uint32_t)units);
@@ -49,8 +49,17 @@ AttnBwdPlan plan_attn_bwd(const AttnArgs& a, int head_dim, int compute_units) {
   p.bounds = (uint64_t)a.batch * a.spans * 16;
   p.tops = ((uint64_t)bh * a.spans * 4 + 15) / 16 * 16;
   const int64_t tiles = (int64_t)a.batch * a.kv_heads * a.key_tiles;
-  int64_t splits = (2 * (int64_t)compute_units + tiles - 1) / tiles;
-  splits = std::max<int64_t>(1, std::min<int64_t>(splits, a.spans / 4));
+  // Teams where a CU has one workgroup at most; or two of different lengths, which a
+  // team more evens out (D = 128, us with one and with teams: 16 causal heads of 4096 rows 206
+  // and 186, 32 heads without a mask of 2048 rows 142 and 172); or any number of lengths
+  // that only the device knows, the longest first (documents of 21 to 3960 rows in 16384, 32 heads
+  // on 8: 1190 and 970; of 2048 each: 650 and 775).
+  const bool ranked = a.ranges != nullptr && tiles > 2 * compute_units && a.key_tiles <= kMaxOrdered;
+  const bool uneven = a.ranges != nullptr || (a.causal && a.score.window == 0);
+  p.order = ranked ? ((uint64_t)a.batch * a.key_tiles * 4 + 15) / 16 * 16 : 0;
+  p.teams = ranked || tiles <= (uneven ? 2 : 1) * compute_units ? key_teams(head_dim) : 1;
+  int64_t splits = ((int64_t)compute_units + tiles - 1) / tiles;
+  splits = std::max<int64_t>(1, std::min<int64_t>(splits, a.spans / (4 * p.teams)));
   p.splits = (int32_t)splits;
   p.parts = splits > 1 ? (uint64_t)splits * a.batch * a.kv_heads * a.m * 2 * head_dim * 4 : 0;
   return p;
@@ -120,7 +129,12 @@ AttnArgs attn_args(const fa_attn_params& p, int compute_units) {
   a.tiles = (p.seq_len + kAttnRows - 1) / kAttnRows;
   a.by_group = make_fast_div((uint32_t)a.group);
   a.by_kvh = make_fast_div((uint32_t)a.kv_heads);
-  a.rows = grid_order(a.batch * a.kv_heads, a.tiles * a.group, compute_units);
+  const int64_t row_tiles = (int64_t)a.batch * a.heads * a.tiles;
+  // Two teams where a CU has one workgroup at most: 16 heads of 2048 rows, D = 128, us with
+  // one and two: forward 51 and 43, dq 70 and 60; with two workgroups a CU (2 x 2000 rows in
+  // documents) 66 and 68, 72 and 76.
+  a.row_teams = row_tiles <= compute_units ? 2 : 1;
+  a.rows = grid_order(a.batch * a.kv_heads, a.tiles * a.group, compute_units, a.row_teams == 1 ? 2 : 1);
   a.spans = (p.seq_len + kSpan - 1) / kSpan;
   a.key_tiles = (p.keys + kAttnKeys - 1) / kAttnKeys;
   return a;
@@ -132,11 +146,12 @@ fa_status bwd_plan(const fa_attn_bwd_params& p, AttnArgs* args, AttnBwdPlan* pla
   *args = attn_args(p.fwd, cus);
   *plan = plan_attn_bwd(*args, p.fwd.head_dim, cus);
   args->splits = plan->splits;
-  args->cols = grid_order(args->batch * args->kv_heads, args->key_tiles * plan->splits, cus);
+  args->cols = grid_order(args->batch * args->kv_heads, args->key_tiles * plan->splits, cus, plan->teams == 1 ? 2 : 1);
+  args->key_teams = plan->teams;
   return FA_OK;
 }
 
-uint64_t total(const AttnBwdPlan& p) { return p.records + p.bounds + p.tops + p.parts; }
+uint64_t total(const AttnBwdPlan& p) { return p.records + p.bounds + p.tops + p.parts + p.order; }
 
 }  // namespace
 }  // namespace fa
@@ -205,7 +220,9 @@ fa_status fa_attn_bwd(const fa_attn_bwd_params* p, void* workspace, uint64_t wor
   a.records = reinterpret_cast<float*>(ws);
   a.bounds = reinterpret_cast<int32_t*>(ws + plan.records);
   a.tops = reinterpret_cast<float*>(ws + plan.records + plan.bounds);
-  a.parts = plan.parts > 0 ? reinterpret_cast<float*>(ws + plan.records + plan.bounds + plan.tops) : nullptr;
+  ws += plan.records + plan.bounds + plan.tops;
+  a.parts = plan.parts > 0 ? reinterpret_cast<float*>(ws) : nullptr;
+  a.key_order = plan.order > 0 ? reinterpret_cast<int32_t*>(ws + plan.parts) : nullptr;
   a.by_splits = make_fast_div((uint32_t)a.splits);
   return launched(launch_attn_bwd(a, p->fwd.head_dim, p->fwd.dtype == FA_DTYPE_BF16,
                                   static_cast<hipStream_t>(stream)));

@@ -139,9 +139,55 @@ __global__ void __launch_bounds__(256) fa_attn_rows_kernel(const AttnArgs a) {
   if constexpr (!BF16) a.tops[bhs] = most;
 }
 
+// ---- the order of the tiles of keys ----
+
+// Ranks them by the spans of rows that see a key of them: one workgroup a batch entry.
+// Each span adds one where its keys begin and takes it off behind their end (sums of
+// integers: their order does not matter), and the running sum is the tiles' work.
+constexpr int kOrderThreads = 1024;
+__global__ void __launch_bounds__(kOrderThreads) fa_attn_order_kernel(const AttnArgs a) {
+  static_assert(kMaxOrdered == kOrderThreads, "a thread per tile");
+  __shared__ __attribute__((aligned(16))) int work[kMaxOrdered + 1];
+  __shared__ int sums[kOrderThreads / 64];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int4* bounds = reinterpret_cast<const int4*>(a.bounds) + (int64_t)b * a.spans;
+  work[tid] = 0;
+  if (tid == 0) work[kMaxOrdered] = 0;
+  __syncthreads();
+  for (int s = tid; s < a.spans; s += kOrderThreads) {
+    const int2 k = *reinterpret_cast<const int2*>(bounds + s);
+    if (k.x >= k.y) continue;
+    atomicAdd(&work[k.x / kAttnKeys], 1);
+    atomicAdd(&work[(k.y - 1) / kAttnKeys + 1], -1);
+  }
+  __syncthreads();
+  int mine = work[tid];
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int x = __shfl_up(mine, d);
+    if (lane >= d) mine += x;
+  }
+  if (lane == 63) sums[tid / 64] = mine;
+  __syncthreads();
+  for (int i = 0; i < tid / 64; ++i) mine += sums[i];
+  work[tid] = tid < a.key_tiles ? mine : -1;
+  __syncthreads();
+  // A tile's place: behind those with more work and the earlier ones with as much.
+  if (tid >= a.key_tiles) return;
+  int place = 0;
+#pragma unroll 4
+  for (int u = 0; u < a.key_tiles; u += 4) {
+    const int4 w = *reinterpret_cast<const int4*>(work + u);
+    place += (w.x > mine || (w.x == mine && u < tid)) + (w.y > mine || (w.y == mine && u + 1 < tid)) +
+             (w.z > mine || (w.z == mine && u + 2 < tid)) + (w.w > mine || (w.w == mine && u + 3 < tid));
+  }
+  a.key_order[(int64_t)b * a.key_tiles + place] = tid;
+}
+
 // ---- scores and their gradients, four at a time ----
 
 // A value that is the same in every lane, in a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ float uniform(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
 }
@@ -172,10 +218,6 @@ template <bool BF16>
 __device__ __forceinline__ i16x8 pack8(const f32x4& x, const f32x4& y) {
   return __builtin_bit_cast(i16x8, u32x4{pack2<BF16>(x[0], x[1]), pack2<BF16>(x[2], x[3]),
                                          pack2<BF16>(y[0], y[1]), pack2<BF16>(y[2], y[3])});
-}
-
-__device__ __forceinline__ f32x4 lds_quad(uint32_t addr) {
-  return __builtin_bit_cast(f32x4, lds_read16<0>(addr));
 }
 
 // c[cb] = init + sum over D of the 16 rows at LDS address `at` (a lane's offset in
@@ -227,6 +269,22 @@ __device__ __forceinline__ void turned_product(uint32_t at, const i16x8 (&f)[NCB
   if constexpr (D == 128) __builtin_amdgcn_s_setprio(0);
 }
 
+// A wave's sums at a lane's place in LDS, 1 KiB a register quad.
+template <int DB>
+__device__ __forceinline__ void put_sums(uint32_t at, const f32x4 (&x)[DB][2]) {
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) lds_write16(at + (2 * db + cb) * 1024, __builtin_bit_cast(u32x4, x[db][cb]));
+}
+template <int DB>
+__device__ __forceinline__ void add_sums(uint32_t at, f32x4 (&x)[DB][2]) {
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) x[db][cb] += lds_quad(at + (2 * db + cb) * 1024);
+}
+
 // ---- gradients of k and v ----
 
 // A span of rows of a head, below 0: none; `code`: the span, and whether the wave's
@@ -249,25 +307,149 @@ __device__ __forceinline__ const __attribute__((address_space(4))) AttnArgs& lat
   return *p;
 }
 
-template <int D, bool BF16, bool CAP>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 128 ? 2 : 3, D == 128 ? 2 : 3)))
+template <int D, bool BF16, bool CAP, int TEAMS>
+__global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_eu(D == 128 ? 2 : 3, D == 128 ? 2 : 3)))
     fa_attn_dkv_kernel(const AttnArgs a) {
   constexpr int ROWB = 2 * D, KST = D / 32, DB = D / 16;
   constexpr int TB = kSpan * ROWB, SLOT = 2 * TB + 1024, SLOTS = 4;  // bytes: Q, go, record
   constexpr int NI = 16 * ROWB / 1024, LPR = ROWB / 16, RPI = 64 / LPR;  // copies of 16 rows
-  __shared__ __attribute__((aligned(1024))) char smem[SLOTS * SLOT];
-  __shared__ float spoiled[SLOTS][2][kSpan];  // NaN for rows of Q, of go with an infinity or NaN, else 0
-  __shared__ float top_part[4];
+  constexpr int PART = 2 * DB * 1024;  // bytes of a wave's sums
+  constexpr int RINGS = TEAMS * SLOTS * SLOT, SUMS = (TEAMS - 1) * 2 * 4 * PART;
+  __shared__ __attribute__((aligned(1024))) char smem[RINGS > SUMS ? RINGS : SUMS];
+  __shared__ float spoiled[TEAMS][SLOTS][2][kSpan];  // NaN for rows of Q, of go with an infinity or NaN, else 0
+  __shared__ float top_part[4 * TEAMS];
 
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int team = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;  // of its team
   // The first keys first: a causal mask's longest.
   int unit, within;
   if (!unit_and_place(a.cols, unit, within)) return;
-  const int tile = fast_div(within, a.by_splits), split = within - tile * a.splits;
+  const int place = fast_div(within, a.by_splits), split = within - place * a.splits;
   const int b = fast_div(unit, a.by_kvh), kvh = unit - b * a.kv_heads, h0 = kvh * a.group;
+  const int tile = a.key_order != nullptr ? uniform(a.key_order[(int64_t)b * a.key_tiles + place]) : place;
   const int j0 = tile * kAttnKeys, w0 = j0 + 32 * wave;
 
+  f32x4 gk[DB][2], gv[DB][2];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) gk[db][cb] = gv[db][cb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  // The spans with a row that sees a key of the workgroup, of the split's (every
+  // splits-th, so that the splits of a causal mask are alike), head after head, the
+  // last ones first: those are a causal mask's that all tiles of keys have, and are
+  // read from L2 by all but one.  Bit i of `hit` is span at0 + i.  Each turn takes one for
+  // each team; `any`: there was one for the first.
+  const int spans = a.spans, group = a.group, last0 = (spans - 1) & ~63;
+  uint64_t hit = 0, seen = 0, whole = 0, all = 0;
+  int h = 0, at0 = last0 + 64;
+  auto next = [&](bool& any) FA_INLINE -> Span {
+    Span mine = {-1, 0};
+    any = false;
+#pragma unroll 1
+    for (int e = 0; e < TEAMS; ++e) {
+      while (hit == 0) {
+        at0 -= 64;
+        if (at0 < 0) {
+          if (h + 1 >= group) {
+            at0 = 0;  // (and none next time)
+            return mine;
+          }
+          ++h;
+          at0 = last0;
+        }
+        const auto& x = late_args();
+        const int s = at0 + lane_now();
+        int4 k = {kNoKey, 0, kNoKey, 0};
+        if (s < spans) k = reinterpret_cast<const int4*>(x.bounds)[(int64_t)b * spans + s];
+        const bool of_split = s - fast_div(s, FastDiv{x.by_splits.mul, x.by_splits.shift}) * x.splits == split;
+        hit = __ballot(of_split && k.x < j0 + kAttnKeys && k.y > j0);
+        seen = __ballot(k.x < w0 + 32 && k.y > w0);
+        whole = __ballot(k.z <= w0 && k.w >= w0 + 32);
+        all = __ballot(k.z <= j0 && k.w >= j0 + kAttnKeys);
+      }
+      const int i = 63 - __builtin_clzll(hit);
+      hit ^= 1ull << i;
+      any = true;
+      if (e == team)
+        mine = Span{h, (uint32_t)(at0 + i) | (uint32_t)((seen >> i) & 1) << 29 | (uint32_t)((whole >> i) & 1) << 30 |
+                           (uint32_t)((all >> i) & 1) << 31};
+    }
+    return mine;
+  };
+
+  // Staging: waves 0 and 1 copy 16 rows of Q each, 2 and 3 of go; wave 0 the record.
+  // (The swizzle of row i + r is that of i, exclusive or that of r.)
+  const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(smem)) + team * SLOTS * SLOT;
+  const bool of_go = wave >= 2;
+  const int sr = (wave & 1) * 16;  // this wave's first row
+  const Rows3& sx = of_go ? a.go : a.q;
+  const uint32_t sst = (uint32_t)sx.st, sto = (of_go ? TB : 0) + sr * ROWB;
+  const char* sp = sx.p + b * sx.sb + h0 * sx.sh + sr * (int64_t)sst;  // of the head to come
+  const char* records = reinterpret_cast<const char*>(a.records + ((int64_t)b * a.heads + h0) * spans * kRecord);
+  const int64_t head_step = sx.sh;
+  const int row_end = a.n - 1 - sr;
+  int staged_head = 0;
+  const uint32_t src_row = (lane / LPR) * sst, src_chunk = ((lane % LPR) ^ lds::TileBoth<D>::swz(lane / LPR)) * 16;
+  auto issue = [&](const Span& x, uint32_t slot) FA_INLINE {
+    for (; staged_head < x.head; ++staged_head) {
+      sp += head_step;
+      records += (int64_t)spans * (kRecord * 4);
+    }
+    const int row = x.at() * kSpan;  // (less sr)
+    const uint32_t dst = base + slot * SLOT + sto;
+    const char* from = sp + (int64_t)row * sst;
+    if (row + 15 <= row_end) {
+#pragma unroll
+      for (int it = 0; it < NI; ++it) {
+        poison_1k(dst + it * 1024);
+        dma_16b(src_row + it * RPI * sst + (src_chunk ^ (lds::TileBoth<D>::swz(it * RPI) * 16)), from, dst + it * 1024);
+      }
+    } else {  // rows past the last one re-read it
+      const int l = lane_now(), back = max(0, row - row_end);
+#pragma unroll
+      for (int it = 0; it < NI; ++it) {
+        poison_1k(dst + it * 1024);
+        const int r = it * RPI + l / LPR, c = (l % LPR) ^ lds::TileBoth<D>::swz(r);
+        dma_16b(min(r, row_end - row + back) * sst + c * 16, from - (int64_t)back * sst, dst + it * 1024);
+      }
+    }
+    if (wave == 0) {  // (1 KiB: the next record too, or what is behind the last one)
+      poison_1k(base + slot * SLOT + 2 * TB);
+      dma_16b(lane_now() * 16, records + (int64_t)x.at() * (kRecord * 4), base + slot * SLOT + 2 * TB);
+    }
+  };
+  // The copies of a span are there, `later`: but for those of one issued after it.
+  // If the span is not seen whole, this wave cleans the rows that it has copied.
+  const uint32_t spoiled_at = __builtin_amdgcn_readfirstlane(lds_addr(spoiled)) + team * SLOTS * 2 * kSpan * 4;
+  auto finish = [&](const Span& x, uint32_t slot, bool later) FA_INLINE {
+    if (!later)
+      wait_vmcnt<0>();
+    else if (wave == 0)
+      wait_vmcnt<NI + 1>();
+    else
+      wait_vmcnt<NI>();
+    if (x.is() && !x.all()) {
+      const unsigned bad = clean_rows<D, BF16, 16>(base + slot * SLOT + sto);
+      const int l = lane_now();
+      if (l < 16)
+        lds_write4(spoiled_at + (slot * 2 + (of_go ? 1 : 0)) * kSpan * 4 + (sr + l) * 4, (bad >> l) & 1 ? NAN : 0.0f);
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    __syncthreads();
+  };
+
+  // Two spans are on their way while one is computed.
+  bool now_any, then_any = false;
+  Span now = next(now_any), then = {-1, 0};
+  uint32_t slot = 0;
+  int head = -1;
+  if (now_any) {
+    if (now.is()) issue(now, 0);
+    then = next(then_any);
+    if (then.is()) issue(then, 1);
+  }
   i16x8 kf[2][KST], vf[2][KST];
 #pragma unroll
   for (int cb = 0; cb < 2; ++cb) {
@@ -284,117 +466,22 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 1
   if constexpr (!BF16) {
     float top = 0.0f;
     const float* tops = a.tops + ((int64_t)b * a.heads + h0) * a.spans;
-    for (int64_t i = threadIdx.x; i < (int64_t)a.group * a.spans; i += 256) top = fmaxf(top, tops[i]);
+    for (int64_t i = threadIdx.x; i < (int64_t)a.group * a.spans; i += 256 * TEAMS) top = fmaxf(top, tops[i]);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if (lane == 0) top_part[wave] = top;
+    if (lane == 0) top_part[threadIdx.x / 64] = top;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = fmaxf(top, top_part[i]);
+    for (int i = 0; i < 4 * TEAMS; ++i) top = fmaxf(top, top_part[i]);
     factor = uniform(grad_factor<BF16>(uniform(top)));
   }
-  f32x4 gk[DB][2], gv[DB][2];
-#pragma unroll
-  for (int db = 0; db < DB; ++db)
-#pragma unroll
-    for (int cb = 0; cb < 2; ++cb) gk[db][cb] = gv[db][cb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-  // The spans with a row that sees a key of the workgroup, of the split's (every
-  // splits-th, so that the splits of a causal mask are alike), head after head, the
-  // last ones first: those are a causal mask's that all tiles of keys have, and are
-  // read from L2 by all but one.  Bit i of `hit` is span at0 + i.
-  const int spans = a.spans, group = a.group, last0 = (spans - 1) & ~63;
-  uint64_t hit = 0, seen = 0, whole = 0, all = 0;
-  int h = 0, at0 = last0 + 64;
-  auto next = [&]() FA_INLINE -> Span {
-    while (hit == 0) {
-      at0 -= 64;
-      if (at0 < 0) {
-        at0 = last0;
-        if (++h >= group) return Span{-1, 0};
-      }
-      const auto& x = late_args();
-      const int s = at0 + lane;
-      int4 k = {kNoKey, 0, kNoKey, 0};
-      if (s < spans) k = reinterpret_cast<const int4*>(x.bounds)[(int64_t)b * spans + s];
-      const bool mine = s - fast_div(s, FastDiv{x.by_splits.mul, x.by_splits.shift}) * x.splits == split;
-      hit = __ballot(mine && k.x < j0 + kAttnKeys && k.y > j0);
-      seen = __ballot(k.x < w0 + 32 && k.y > w0);
-      whole = __ballot(k.z <= w0 && k.w >= w0 + 32);
-      all = __ballot(k.z <= j0 && k.w >= j0 + kAttnKeys);
-    }
-    const int i = 63 - __builtin_clzll(hit);
-    hit ^= 1ull << i;
-    return Span{h, (uint32_t)(at0 + i) | (uint32_t)((seen >> i) & 1) << 29 | (uint32_t)((whole >> i) & 1) << 30 |
-                       (uint32_t)((all >> i) & 1) << 31};
-  };
-
-  // Staging: waves 0 and 1 copy 16 rows of Q each, 2 and 3 of go; wave 0 the record.
-  // (The swizzle of row i + r is that of i, exclusive or that of r.)
-  const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(smem));
-  const bool of_go = wave >= 2;
-  const int sr = (wave & 1) * 16;  // this wave's first row
-  const Rows3& sx = of_go ? a.go : a.q;
-  const uint32_t sst = (uint32_t)sx.st, sto = (of_go ? TB : 0) + sr * ROWB;
-  const char* sp = sx.p + b * sx.sb + h0 * sx.sh + sr * (int64_t)sst;  // of the head to come
-  const char* records = reinterpret_cast<const char*>(a.records + ((int64_t)b * a.heads + h0) * spans * kRecord);
-  const int64_t head_step = sx.sh;
-  const int row_end = a.n - 1 - sr;
-  int staged_head = 0;
-  const uint32_t src_row = (lane / LPR) * sst, src_chunk = ((lane % LPR) ^ lds::TileBoth<D>::swz(lane / LPR)) * 16;
-  auto issue = [&](const Span& x, uint32_t slot) FA_INLINE {
-    if (x.head != staged_head) {
-      staged_head = x.head;
-      sp += head_step;
-      records += (int64_t)spans * (kRecord * 4);
-    }
-    const int row = x.at() * kSpan;  // (less sr)
-    const uint32_t dst = base + slot * SLOT + sto;
-    const char* from = sp + (int64_t)row * sst;
-    if (row + 15 <= row_end) {
-#pragma unroll
-      for (int it = 0; it < NI; ++it) {
-        poison_1k(dst + it * 1024);
-        dma_16b(src_row + it * RPI * sst + (src_chunk ^ (lds::TileBoth<D>::swz(it * RPI) * 16)), from, dst + it * 1024);
-      }
-    } else {  // rows past the last one re-read it
-      const int l = fresh(lane), back = max(0, row - row_end);
-#pragma unroll
-      for (int it = 0; it < NI; ++it) {
-        poison_1k(dst + it * 1024);
-        const int r = it * RPI + l / LPR, c = (l % LPR) ^ lds::TileBoth<D>::swz(r);
-        dma_16b(min(r, row_end - row + back) * sst + c * 16, from - (int64_t)back * sst, dst + it * 1024);
-      }
-    }
-    if (wave == 0) {  // (1 KiB: the next record too, or what is behind the last one)
-      poison_1k(base + slot * SLOT + 2 * TB);
-      dma_16b(fresh(lane) * 16, records + (int64_t)x.at() * (kRecord * 4), base + slot * SLOT + 2 * TB);
-    }
-  };
-  // The copies of a span are there, `later`: but for those of one issued after it.
-  // If the span is not seen whole, this wave cleans the rows that it has copied.
-  const uint32_t spoiled_at = __builtin_amdgcn_readfirstlane(lds_addr(spoiled));
-  auto finish = [&](const Span& x, uint32_t slot, bool later) FA_INLINE {
-    if (!later)
-      wait_vmcnt<0>();
-    else if (wave == 0)
-      wait_vmcnt<NI + 1>();
-    else
-      wait_vmcnt<NI>();
-    if (x.is() && !x.all()) {
-      const unsigned bad = clean_rows<D, BF16, 16>(base + slot * SLOT + sto);
-      if (lane < 16)
-        lds_write4(spoiled_at + (slot * 2 + (of_go ? 1 : 0)) * kSpan * 4 + (sr + lane) * 4, (bad >> lane) & 1 ? NAN : 0.0f);
-    }
-    __builtin_amdgcn_s_waitcnt(0xc07f);
-    __syncthreads();
-  };
+  finish(now, 0, false);  // (what was loaded so far: no wait for it later, which would be one for copies too)
 
   Grads<CAP> grads;
   // A span in `slot`.  (Scores become P in place, dS takes the place of go V^T: the
   // accumulators leave few registers, none to keep addresses across spans.)
   auto step = [&](int row0, uint32_t slot, bool masked) FA_INLINE {
-    const int l = fresh(lane);
+    const int l = lane_now();
     const int key0 = w0 + (l & 15);
     const uint32_t tile = base + slot * SLOT;
     u32x4 pw[2], dw[2];  // P and dS as packed pairs: words 0, 1 of rows 4 (l / 16) .., 2, 3 of those 16 on
@@ -469,29 +556,19 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 1
       }
       __builtin_amdgcn_sched_barrier(0);
     });
-    const uint32_t turned = tile + lds::TileBoth<D>::turned_offset(fresh(lane));
+    const uint32_t turned = tile + lds::TileBoth<D>::turned_offset(lane_now());
     const i16x8 pf[2] = {__builtin_bit_cast(i16x8, pw[0]), __builtin_bit_cast(i16x8, pw[1])};
     const i16x8 df[2] = {__builtin_bit_cast(i16x8, dw[0]), __builtin_bit_cast(i16x8, dw[1])};
     turned_product<D, BF16, 2>(turned + TB, pf, gv);
     turned_product<D, BF16, 2>(turned, df, gk);
   };
 
-  // Two spans are on their way while one is computed.
-  Span now = next(), then = {-1, 0};
-  uint32_t slot = 0;
-  int head = -1;
-  wait_vmcnt<0>();  // (what was loaded so far: no wait for it later, which would be one for copies too)
-  if (now.is()) {
-    issue(now, 0);
-    then = next();
-    if (then.is()) issue(then, 1);
-    finish(now, 0, then.is());
-  }
-  while (now.is()) {
+  while (now_any) {
     Span last = {-1, 0};
-    if (then.is()) last = next();
+    bool last_any = false;
+    if (then_any) last = next(last_any);
     if (last.is()) issue(last, (slot + 2) % SLOTS);
-    if (now.seen()) {
+    if (now.is() && now.seen()) {
       if (now.head != head) {
         head = now.head;
         grads.init(a, h0 + head);
@@ -502,13 +579,31 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 1
     finish(then, slot, last.is());
     now = then;
     then = last;
+    now_any = then_any;
+    then_any = last_any;
   }
+
+  // The first team takes all of gk, the second all of gv, by wave and lane.
+  if constexpr (TEAMS > 1) {
+    const uint32_t at = lds_addr(smem) + wave * PART + lane * 16;
+    if (team != 0) put_sums<DB>(at + (team - 1) * 4 * PART, gk);
+    if (team != 1) put_sums<DB>(at + (TEAMS - 1 + (team == 0 ? 0 : team - 1)) * 4 * PART, gv);
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    __syncthreads();
+    if (team > 1) return;
+#pragma unroll
+    for (int i = 0; i < TEAMS - 1; ++i) {
+      if (team == 0) add_sums<DB>(at + i * 4 * PART, gk);
+      if (team == 1) add_sums<DB>(at + (TEAMS - 1 + i) * 4 * PART, gv);
+    }
+  }
+  const bool has_k = TEAMS == 1 || team == 0, has_v = TEAMS == 1 || team == 1;
 
   // (powers of two but for the scale)
   const auto& x = late_args();
   const float fv[2] = {fast_exp2(-kShift<BF16>), fast_exp2(-kShift<BF16>)};
   const float fk[2] = {x.scale * fv[0] / factor, x.scale * fv[0] / factor};
-  const int l = fresh(lane), m = x.m;
+  const int l = lane_now(), m = x.m;
   if (x.parts != nullptr) {
     const int64_t rows = (int64_t)x.batch * x.kv_heads * m;
     float* to = x.parts + ((int64_t)split * rows + (int64_t)unit * m) * 2 * D + 4 * (l >> 4);
@@ -518,18 +613,19 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 1
       if (j >= m) continue;
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        *reinterpret_cast<f32x4*>(to + (int64_t)j * 2 * D + 16 * db) = gk[db][cb] * fk[0];
-        *reinterpret_cast<f32x4*>(to + (int64_t)j * 2 * D + D + 16 * db) = gv[db][cb] * fv[0];
+        if (has_k) *reinterpret_cast<f32x4*>(to + (int64_t)j * 2 * D + 16 * db) = gk[db][cb] * fk[0];
+        if (has_v) *reinterpret_cast<f32x4*>(to + (int64_t)j * 2 * D + D + 16 * db) = gv[db][cb] * fv[0];
       }
     }
     return;
   }
-  char* ot = smem + wave * 32 * ROWB;
+  // (of the sums, what this wave has read)
+  char* ot = smem + wave * PART + (TEAMS > 1 && team == 1 ? (TEAMS - 1) * 4 * PART : 0);
   char* kp = x.gk.p + b * x.gk.sb + kvh * x.gk.sh;
   char* vp = x.gv.p + b * x.gv.sb + kvh * x.gv.sh;
   const int64_t k_st = x.gk.st, v_st = x.gv.st;
-  write_rows<D, BF16>(ot, gk, fk, l, [&](int r) FA_INLINE -> char* { return w0 + r < m ? kp + (w0 + r) * k_st : nullptr; });
-  write_rows<D, BF16>(ot, gv, fv, l, [&](int r) FA_INLINE -> char* { return w0 + r < m ? vp + (w0 + r) * v_st : nullptr; });
+  if (has_k) write_rows<D, BF16>(ot, gk, fk, l, [&](int r) FA_INLINE -> char* { return w0 + r < m ? kp + (w0 + r) * k_st : nullptr; });
+  if (has_v) write_rows<D, BF16>(ot, gv, fv, l, [&](int r) FA_INLINE -> char* { return w0 + r < m ? vp + (w0 + r) * v_st : nullptr; });
 }
 
 // Adds the splits' parts in their order: 8 elements a thread.
@@ -554,15 +650,15 @@ __global__ void __launch_bounds__(256) fa_attn_join_kernel(const AttnArgs a) {
 
 // ---- gradients of q ----
 
-template <int D, bool BF16, bool CAP>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+template <int D, bool BF16, bool CAP, int TEAMS>
+__global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_eu(2, 2)))
     fa_attn_dq_kernel(const AttnArgs a) {
   constexpr int ROWB = 2 * D, TB = 64 * ROWB, KST = D / 32, DB = D / 16;
-  __shared__ __attribute__((aligned(1024))) char smem[4 * TB];  // K0 V0 K1 V1
-  __shared__ TileKeys part[4];
+  __shared__ __attribute__((aligned(1024))) char smem[TEAMS * 4 * TB];  // of each team K0 V0 K1 V1
 
   const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int team = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;  // of its team
   int unit, within;
   if (!unit_and_place(a.rows, unit, within)) return;
   const int back = fast_div(within, a.by_group);
@@ -570,10 +666,31 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int h = kvh * a.group + within - back * a.group;
   const int row0 = (a.tiles - 1 - back) * kAttnRows, wrow0 = row0 + 32 * wave;
 
+  TileKeys keys, all;  // of the wave's rows, of the workgroup's
+  tile_keys(a, b, row0, wave, keys, all);
+  const int c0 = all.lo, c1 = all.hi;
+  // (tile t TEAMS + team is the team's in turn t)
+  const int turns = c0 < c1 ? ((c1 - c0 + 63) / 64 + TEAMS - 1) / TEAMS : 0;
+  auto key_of = [&](int t) FA_INLINE { return c0 + 64 * (t * TEAMS + team); };
+  const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(smem)) + team * 4 * TB;
+  const char* kh = a.k.p + b * a.k.sb + kvh * a.k.sh;
+  const char* vh = a.v.p + b * a.v.sb + kvh * a.v.sh;
+  RowStage<D> stage_k;
+  RowStage<D> stage_v;
+  stage_k.init(lane, (uint32_t)a.k.st);
+  stage_v.init(lane, (uint32_t)a.v.st);
+  auto issue = [&](int t, int buf) FA_INLINE {
+    if (t >= turns || key_of(t) >= c1) return;
+    const int r0 = min(key_of(t) + 16 * wave, c1 - 1);
+    const uint32_t dst = base + buf * 2 * TB + wave * 16 * ROWB;
+    stage_k.copy(kh + r0 * a.k.st, dst, c1 - 1 - r0, (uint32_t)a.k.st);
+    stage_v.copy(vh + r0 * a.v.st, dst + TB, c1 - 1 - r0, (uint32_t)a.v.st);
+  };
+  issue(0, 0);
+  // (behind the first copies: one wait for all)
   i16x8 qf[2][KST], gf[2][KST];
   float lse[2], delta[2], factor[2];  // (minus delta)
   RowKeys see[2];
-  TileKeys keys;
 #pragma unroll
   for (int rb = 0; rb < 2; ++rb) {
     const int r = min(wrow0 + 16 * rb + l16, a.n - 1);
@@ -591,12 +708,6 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     delta[rb] = rec[16 * kDelta];
     see[rb].lo = __builtin_bit_cast(int, rec[16 * kLo]);
     see[rb].hi = __builtin_bit_cast(int, rec[16 * kHi]);
-    TileKeys t;
-    t.start(see[rb]);
-    if (rb == 0)
-      keys = t;
-    else
-      keys.add(t);
     factor[rb] = 1.0f;
     if constexpr (!BF16) {
       float top = 0.0f;
@@ -610,36 +721,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       factor[rb] = grad_factor<BF16>(WaveAttn<D, BF16, 4, 2>::red_max(top));
     }
   }
-  keys.reduce<16>();
-  if (lane == 0) part[wave] = keys;
-  __syncthreads();
-  TileKeys all = part[0];
-#pragma unroll
-  for (int i = 1; i < 4; ++i) all.add(part[i]);
-  keys.uniform();
-  all.uniform();
-
-  const int c0 = all.lo, c1 = all.hi;
-  const int n_tiles = c0 < c1 ? (c1 - c0 + 63) / 64 : 0;
-  const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(smem));
-  const char* kh = a.k.p + b * a.k.sb + kvh * a.k.sh;
-  const char* vh = a.v.p + b * a.v.sb + kvh * a.v.sh;
-  RowStage<D> stage_k;
-  RowStage<D> stage_v;
-  stage_k.init(lane, (uint32_t)a.k.st);
-  stage_v.init(lane, (uint32_t)a.v.st);
-  auto issue = [&](int t, int buf) FA_INLINE {
-    const int r0 = min(c0 + 64 * t + 16 * wave, c1 - 1);
-    const uint32_t dst = base + buf * 2 * TB + wave * 16 * ROWB;
-    stage_k.copy(kh + r0 * a.k.st, dst, c1 - 1 - r0, (uint32_t)a.k.st);
-    stage_v.copy(vh + r0 * a.v.st, dst + TB, c1 - 1 - r0, (uint32_t)a.v.st);
-  };
   // The staged keys of tile t are there: cleaned if some row does not see all of
   // them, with V's rows set to NaN for the ones that do.
   auto finish = [&](int t, int buf) FA_INLINE {
     __builtin_amdgcn_s_waitcnt(0);
-    const int k0 = c0 + 64 * t;
-    if (t < n_tiles && !(k0 >= all.all_lo && k0 + 64 <= all.all_hi)) {
+    const int k0 = key_of(t);
+    if (t < turns && k0 < c1 && !(k0 >= all.all_lo && k0 + 64 <= all.all_hi)) {
       const uint32_t rows = base + buf * 2 * TB + wave * 16 * ROWB;
       const unsigned bad = clean_rows<D, BF16, 16>(rows);
       if (__builtin_expect(bad != 0, false)) {
@@ -729,14 +816,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     turned_product<D, BF16, 2>(turned_at + off + half * 32 * ROWB, df, gq);
   };
 
-  if (n_tiles > 0) {
-    issue(0, 0);
-    finish(0, 0);
-  }
+  finish(0, 0);
   int buf = 0;
-  for (int t = 0; t < n_tiles; ++t, buf ^= 1) {
-    const int k0 = c0 + 64 * t;
-    if (t + 1 < n_tiles) issue(t + 1, buf ^ 1);
+  for (int t = 0; t < turns; ++t, buf ^= 1) {
+    const int k0 = key_of(t);
+    issue(t + 1, buf ^ 1);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int k = k0 + 32 * half;
@@ -748,40 +832,64 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     finish(t + 1, buf ^ 1);
   }
 
+  // The second team hands its sums to the first, by wave and lane.
+  constexpr int PART = 2 * DB * 1024;
+  if constexpr (TEAMS == 2) {
+    const uint32_t at = lds_addr(smem) + wave * PART + lane * 16;
+    if (team == 1) put_sums<DB>(at, gq);
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    __syncthreads();
+    if (team == 1) return;
+    add_sums<DB>(at, gq);
+  }
   float f[2];
 #pragma unroll
   for (int rb = 0; rb < 2; ++rb) f[rb] = a.scale * fast_exp2(-kShift<BF16>) / factor[rb];
   char* qh = a.gq.p + b * a.gq.sb + h * a.gq.sh;
-  write_rows<D, BF16>(smem + wave * 32 * ROWB, gq, f, lane, [&](int r) FA_INLINE -> char* {
+  write_rows<D, BF16>(smem + wave * PART, gq, f, lane, [&](int r) FA_INLINE -> char* {
     return wrow0 + r < a.n ? qh + (wrow0 + r) * a.gq.st : nullptr;
   });
 }
 
 template <class F>
-hipError_t launch(F* fn, int64_t grid, const AttnArgs& a, hipStream_t stream) {
+hipError_t launch(F* fn, int64_t grid, int threads, const AttnArgs& a, hipStream_t stream) {
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
   void* kargs[] = {const_cast<AttnArgs*>(&a)};
-  return hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)grid), dim3(256), kargs, 0, stream);
+  return hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)grid), dim3(threads), kargs, 0, stream);
+}
+
+template <int D, bool BF16, bool CAP>
+hipError_t launch_dkv(const AttnArgs& a, hipStream_t stream) {
+  constexpr int TEAMS = key_teams(D);
+  const int64_t grid = grid_size(a.cols);
+  return a.key_teams == 1 ? launch(&fa_attn_dkv_kernel<D, BF16, CAP, 1>, grid, 256, a, stream)
+                          : launch(&fa_attn_dkv_kernel<D, BF16, CAP, TEAMS>, grid, 256 * TEAMS, a, stream);
+}
+template <int D, bool BF16, bool CAP>
+hipError_t launch_dq(const AttnArgs& a, hipStream_t stream) {
+  const int64_t grid = grid_size(a.rows);
+  return a.row_teams == 1 ? launch(&fa_attn_dq_kernel<D, BF16, CAP, 1>, grid, 256, a, stream)
+                          : launch(&fa_attn_dq_kernel<D, BF16, CAP, 2>, grid, 512, a, stream);
 }
 
 template <int D, bool BF16>
 hipError_t launch_as(const AttnArgs& a, hipStream_t stream) {
   hipError_t e = launch(&fa_attn_rows_kernel<D, BF16>, (int64_t)a.batch * a.heads * ((a.n + kRowsBlock - 1) / kRowsBlock),
-                        a, stream);
+                        256, a, stream);
   if (e != hipSuccess) return e;
+  if (a.key_order != nullptr) {
+    e = launch(&fa_attn_order_kernel, a.batch, kOrderThreads, a, stream);
+    if (e != hipSuccess) return e;
+  }
   const bool cap = a.score.cap > 0.0f;
-  const int64_t dkv = grid_size(a.cols);
-  e = cap ? launch(&fa_attn_dkv_kernel<D, BF16, true>, dkv, a, stream)
-          : launch(&fa_attn_dkv_kernel<D, BF16, false>, dkv, a, stream);
+  e = cap ? launch_dkv<D, BF16, true>(a, stream) : launch_dkv<D, BF16, false>(a, stream);
   if (e != hipSuccess) return e;
   if (a.parts != nullptr) {
     const int64_t rows = (int64_t)a.batch * a.kv_heads * a.m;
-    e = launch(&fa_attn_join_kernel<D, BF16>, (rows * (2 * D / 8) + 255) / 256, a, stream);
+    e = launch(&fa_attn_join_kernel<D, BF16>, (rows * (2 * D / 8) + 255) / 256, 256, a, stream);
     if (e != hipSuccess) return e;
   }
-  const int64_t dq = grid_size(a.rows);
-  return cap ? launch(&fa_attn_dq_kernel<D, BF16, true>, dq, a, stream)
-             : launch(&fa_attn_dq_kernel<D, BF16, false>, dq, a, stream);
+  return cap ? launch_dq<D, BF16, true>(a, stream) : launch_dq<D, BF16, false>(a, stream);
 }
 
 }  // namespace

@@ -36,6 +36,7 @@ struct AttnArgs {
   int32_t tiles;            // row tiles of a head (kAttnRows)
   FastDiv by_group, by_kvh;
   GridOrder rows;           // forward and dq: tiles * group places
+  int32_t row_teams, key_teams;  // teams of four waves of their workgroups, of dk and dv's
   // backward
   Rows3 go, gq, gk, gv;     // gradients of o, q, k, v
   const float* glse;        // of lse; may be NULL
@@ -46,18 +47,23 @@ struct AttnArgs {
   int32_t key_tiles, splits;
   FastDiv by_splits;
   GridOrder cols;           // dk, dv: key_tiles * splits places
+  int32_t* key_order;       // [batch, key_tiles]: the tiles of keys, the longest first; NULL: as they lie
   float* parts;             // [splits][batch, kv_heads, m][2][D] gradients of k and v; NULL: one split
 };
 
 constexpr int kAttnRows = 128;  // rows of a forward or dq workgroup
 constexpr int kAttnKeys = 128;  // keys of a dk, dv workgroup
 constexpr int kSpan = 32;       // rows that it stages at a time
+constexpr int kMaxOrdered = 1024;  // tiles of keys that key_order ranks
+
+// Teams of a workgroup of few: as many as fill a CU.
+constexpr int key_teams(int head_dim) { return head_dim == 128 ? 2 : 3; }
 
 struct AttnBwdPlan {
-  int32_t splits;
-  uint64_t records, bounds, tops, parts;  // bytes, each a multiple of 16
+  int32_t teams, splits;
+  uint64_t records, bounds, tops, parts, order;  // bytes, each a multiple of 16
 };
-GridOrder grid_order(int units, int places, int compute_units);
+GridOrder grid_order(int units, int places, int compute_units, int per_cu);
 int64_t grid_size(const GridOrder& o);
 AttnBwdPlan plan_attn_bwd(const AttnArgs& a, int head_dim, int compute_units);
 

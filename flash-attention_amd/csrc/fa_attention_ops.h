@@ -22,19 +22,25 @@ constexpr int kNoKey = 0x7fffffff;
 struct RowKeys {
   int lo, hi;
 };
-__device__ __forceinline__ RowKeys row_keys(const AttnArgs& a, int b, int i) {
+// (hi at or below lo: none)
+__device__ __forceinline__ RowKeys limits(const AttnArgs& a, int i, RowKeys k) {
   const int p = i + a.m - a.n;
+  if (a.causal) k.hi = min(k.hi, p + 1);
+  if (a.score.window > 0) {
+    k.lo = max(k.lo, p - (a.score.window - 1));
+    if (!a.causal) k.hi = min(k.hi, p + a.score.window);
+  }
+  return k;
+}
+__device__ __forceinline__ RowKeys limits(const AttnArgs& a, int i) { return limits(a, i, {0, a.m}); }
+__device__ __forceinline__ RowKeys row_keys(const AttnArgs& a, int b, int i) {
   RowKeys k = {0, a.m};
   if (a.ranges != nullptr) {
     const int2 r = *reinterpret_cast<const int2*>(a.ranges + b * a.range_sb + 2 * (int64_t)i);
     k.lo = max(r.x, 0);
     k.hi = min(r.y, a.m);
   }
-  if (a.causal) k.hi = min(k.hi, p + 1);
-  if (a.score.window > 0) {
-    k.lo = max(k.lo, p - (a.score.window - 1));
-    if (!a.causal) k.hi = min(k.hi, p + a.score.window);
-  }
+  k = limits(a, i, k);
   if (k.lo >= k.hi) k = {kNoKey, 0};
   return k;
 }
@@ -55,13 +61,41 @@ struct TileKeys {
     for (int d = 1; d < WIDTH; d <<= 1)
       add({__shfl_xor(lo, d), __shfl_xor(hi, d), __shfl_xor(all_lo, d), __shfl_xor(all_hi, d)});
   }
-  __device__ __forceinline__ void uniform() {
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    hi = __builtin_amdgcn_readfirstlane(hi);
-    all_lo = __builtin_amdgcn_readfirstlane(all_lo);
-    all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+  __device__ __forceinline__ TileKeys of_lane(int l) const {
+    return {__builtin_amdgcn_readlane(lo, l), __builtin_amdgcn_readlane(hi, l), __builtin_amdgcn_readlane(all_lo, l),
+            __builtin_amdgcn_readlane(all_hi, l)};
   }
 };
+
+// Those of the rows from one with the limits x to one with y.  Without ranges no
+// row sees keys before an earlier row's first, nor past a later row's last; rows without
+// any come first, and end at or before key 0.
+__device__ __forceinline__ TileKeys between(const RowKeys& x, const RowKeys& y) {
+  return {x.lo, max(y.hi, 0), y.lo, x.hi};
+}
+
+// Those of the 128 rows from row0 on, `all`, and of the 32 of a wave, `own`.
+__device__ __forceinline__ void tile_keys(const AttnArgs& a, int b, int row0, int wave, TileKeys& own, TileKeys& all) {
+  const int lane = threadIdx.x & 63, end = a.n - 1;
+  TileKeys s, t;  // of the first 64 rows, of the others; lanes below 32 and from 32 on
+  if (a.ranges != nullptr) {
+    s.start(row_keys(a, b, min(row0 + lane, end)));
+    t.start(row_keys(a, b, min(row0 + 64 + lane, end)));
+    s.reduce<32>();
+    t.reduce<32>();
+  } else {
+    const int i = row0 + (lane & 32);
+    s = between(limits(a, min(i, end)), limits(a, min(i + 31, end)));
+    t = between(limits(a, min(i + 64, end)), limits(a, min(i + 95, end)));
+  }
+  all = s.of_lane(0);
+  all.add(s.of_lane(32));
+  all.add(t.of_lane(0));
+  all.add(t.of_lane(32));
+  const int at = wave % 2 * 32;
+  s = {wave < 2 ? s.lo : t.lo, wave < 2 ? s.hi : t.hi, wave < 2 ? s.all_lo : t.all_lo, wave < 2 ? s.all_hi : t.all_hi};
+  own = s.of_lane(at);
+}
 
 // Unit and place of a workgroup; false: none.  Workgroup w runs on XCD w % 8, in
 // order; the workgroups of a unit share its keys (or rows) through the XCD's L2, and the
@@ -88,6 +122,13 @@ __device__ __forceinline__ bool unit_and_place(const GridOrder& o, int& unit, in
     unit = i * kNumXcd + xcd - place * o.units;
   }
   return place < o.places;
+}
+
+// The lane, computed anew: a register less along the loop.
+__device__ __forceinline__ int lane_now() {
+  int l;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=&v"(l));
+  return l;
 }
 
 // Staging of 16 rows of a tensor into LDS in the layout of lds::TileBoth.
@@ -122,6 +163,9 @@ template <int OFF>
 __device__ __forceinline__ void lds_write8(uint32_t addr, u32x2 w) {
   *(__attribute__((address_space(3))) u32x2*)(uintptr_t)(addr + OFF) = w;
 }
+__device__ __forceinline__ f32x4 lds_quad(uint32_t addr) {
+  return __builtin_bit_cast(f32x4, lds_read16<0>(addr));
+}
 __device__ __forceinline__ void lds_write4(uint32_t addr, float x) {
   *(__attribute__((address_space(3))) float*)(uintptr_t)addr = x;
 }
@@ -137,7 +181,7 @@ template <int D, bool BF16, int ROWS>
 __device__ __forceinline__ unsigned clean_rows(uint32_t at) {
   constexpr int ROWB = 2 * D, NI = ROWS * ROWB / 1024, LPR = ROWB / 16;
   constexpr uint32_t E = BF16 ? 0x7F807F80u : 0x7C007C00u, L = BF16 ? 0x00800080u : 0x04000400u;
-  const int lane = threadIdx.x & 63;
+  const int lane = lane_now();
   unsigned rows = 0;
 #pragma unroll
   for (int it = 0; it < NI; ++it) {

@@ -116,7 +116,6 @@ inline ScoreArgs score_args(const fa_score_params& s, float scale) {
   if (s.softcap != 0.0f) {
     a.cap = (float)(s.softcap * kLog2e);
     a.cap_twice = 2.0f * a.cap;
-    a.cap_inverse = 1.0f / a.cap;
     a.cap_in = (float)(2.0 * scale * kLog2e / s.softcap);
   }
   a.unit = s.softcap != 0.0f ? 1.0f : (float)(scale * kLog2e);

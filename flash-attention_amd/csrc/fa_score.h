@@ -14,7 +14,7 @@ namespace fa {
 
 struct ScoreArgs {
   float cap;            // softcap * log2(e); 0: none
-  float cap_twice, cap_inverse;  // twice that, and its inverse
+  float cap_twice;      // twice that
   float cap_in;         // 2 softmax_scale log2(e) / softcap
   float unit;           // log2(e) softmax_scale, or 1 for capped scores: what the bias is added to
   const float* slopes;  // of each query head; NULL: no bias
@@ -27,7 +27,7 @@ namespace {
 // The scores of a wave, in units of log2 so that exp2 takes them as they are.
 struct Score {
   bool capped, biased;
-  float in, out, twice, inverse;  // capped
+  float in, out, twice;  // capped
   float unit;            // factor of the scores that the bias is added to
   __device__ __forceinline__ void init(const ScoreArgs& a) {
     capped = a.cap > 0.0f;
@@ -35,7 +35,6 @@ struct Score {
     in = a.cap_in;
     out = a.cap;
     twice = a.cap_twice;
-    inverse = a.cap_inverse;
     unit = a.unit;
   }
   // out tanh(x) with e^2x = 2^(in x): out - 2 out / (1 + e^2x).  Its error, about

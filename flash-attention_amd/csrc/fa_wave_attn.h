@@ -25,7 +25,8 @@ constexpr float kHeadroom = BF16 ? 4.0f : 1.0f;
 
 constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
 
-enum StepMode { kWhole, kMasked, kSafe };
+// kTrusting: kMasked, but for its look for infinities and NaN.
+enum StepMode { kWhole, kMasked, kTrusting, kSafe };
 
 // The state of a wave's RB blocks of 16 rows over tiles of 16 NKB keys, on
 // v_mfma_f32_16x16x32 with the layouts of fa_fwd16_kernel: S^T = K Q^T (lane
@@ -225,10 +226,8 @@ struct WaveAttn {
         for (int rb = 0; rb < RB; ++rb) ls[rb] = mfma16<BF16>(ones, pf[ch][rb], ls[rb]);
       return;
     }
-    if constexpr (MODE == kMasked) {
-      odd = odd || any_non_finite(v_tile);
-      static_for<0, VD>(read_v);
-    }
+    if constexpr (MODE == kMasked) odd = odd || any_non_finite(v_tile);
+    if constexpr (MODE == kMasked || MODE == kTrusting) static_for<0, VD>(read_v);
     // With two waves on a SIMD unit, the one in its products goes first: the
     // other's exponentials fill the gaps.  4096 tokens over 16384 keys, bf16, 32
     // heads on 8, us without and with: D = 128 causal 827 and 798, without the
@@ -259,6 +258,18 @@ struct WaveAttn {
       for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[kb][rb][i] = f(s[kb][rb][i], kb, rb, i);
+  }
+
+  // Whether some sum is NaN.  It stays so, once it is.
+  __device__ __forceinline__ bool any_nan() const {
+    bool nan = false;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) nan = nan || o[db][rb][i] != o[db][rb][i];
+    return __any(nan);
   }
 
   // Whether the V tile at LDS address v_tile holds an infinity or a NaN.

@@ -70,6 +70,15 @@ CASES = {
     "nothing-seen": (1, 2, 1, 100, 100, 64, "fp16", "bhnd", 1, dict(nothing=True)),
     "long": (1, 2, 1, 1500, 1500, 64, "fp16", "bhnd", 1, dict(causal=True)),
     "long-128": (1, 2, 2, 1100, 1100, 128, "bf16", "bhnd", 1, dict(docs=[700, 1100])),
+    # more workgroups than compute units, so without teams (with ranges: ranked by their work)
+    "many-full": (3, 100, 100, 90, 130, 64, "fp16", "bhnd", 1, {}),
+    "many-causal": (3, 180, 180, 140, 140, 128, "bf16", "bnhd", 1, dict(causal=True)),
+    "many-window": (2, 150, 150, 260, 260, 64, "bf16", "bhnd", 1, dict(window=50)),
+    "many-docs": (2, 150, 150, 300, 300, 128, "fp16", "bhnd", 1, dict(docs=[20, 200, 290])),
+    "many-ranges": (2, 320, 160, 300, 200, 64, "bf16", "bhnd", 1, dict(random=7)),
+    "many-cap": (2, 150, 150, 200, 330, 64, "bf16", "bhnd", 4, dict(softcap=12.0, slopes=0.001)),
+    "many-all-options": (2, 150, 150, 280, 280, 128, "fp16", "bhnd", 4,
+                         dict(causal=True, softcap=20.0, slopes=0.002, window=100)),
 }
 
 
@@ -173,15 +182,16 @@ def test_small_and_large_incoming_gradients_in_fp16(fa, D, factor):
             *reference((q, k, v, go), None, None, dict(causal=True)))
 
 
-@pytest.mark.parametrize("D,dtype", [(64, "fp16"), (128, "bf16")])
+@pytest.mark.parametrize("D,dtype,heads", [(64, "fp16", 4), (128, "bf16", 4), (64, "bf16", 90), (128, "bf16", 180)])
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
-def test_masked_rows_and_keys_may_hold_anything(fa, D, dtype, bad):
+def test_masked_rows_and_keys_may_hold_anything(fa, D, dtype, heads, bad):
     """A document of infinities or NaN in the middle, and garbage rows that see and are seen by nothing:
     the other documents' results keep every bit that they have with zeros in its place."""
-    print("case masked", D, dtype, bad, flush=True)
+    print("case masked", D, dtype, heads, bad, flush=True)
     g = torch.Generator().manual_seed(8)
     N, dt = 300, DT[dtype]
-    good = [rows(1, h, N, D, dt, g) for h in (4, 2, 2, 4)]
+    kv_heads = 2 if heads == 4 else heads
+    good = [rows(1, h, N, D, dt, g) for h in (heads, kv_heads, kv_heads, heads)]
     cu = torch.tensor([0, 70, 150, 280], dtype=torch.int32)  # rows 280 .. 299 belong to none
     ranges = fa.document_ranges(cu, N)
     mine = torch.zeros(N, dtype=torch.bool)
@@ -206,11 +216,11 @@ def test_masked_rows_and_keys_may_hold_anything(fa, D, dtype, bad):
         assert not bool(torch.isfinite(b[n][:, :, 76:150]).any()), n
 
 
-@pytest.mark.parametrize("D", [64, 128])
-def test_one_bad_key_reaches_the_rows_that_see_it(fa, D):
-    print("case bad key", D, flush=True)
+@pytest.mark.parametrize("D,H", [(64, 2), (128, 2), (64, 300), (128, 300)])
+def test_one_bad_key_reaches_the_rows_that_see_it(fa, D, H):
+    print("case bad key", D, H, flush=True)
     g = torch.Generator().manual_seed(18)
-    q, k, v, go = (rows(1, 2, 200, D, torch.bfloat16, g) for _ in range(4))
+    q, k, v, go = (rows(1, H, 200, D, torch.bfloat16, g) for _ in range(4))
     for x in (k, v):
         y = [t.clone() for t in (q, k, v, go)]
         y[1 if x is k else 2][0, 0, 120, 3] = math.nan
