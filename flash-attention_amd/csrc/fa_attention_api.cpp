@@ -95,6 +95,7 @@ fa_status check_attn(const fa_attn_params& p, bool backward) {
                   (long long)kMaxKeyStride);
   if (backward && p.lse == nullptr) return fail(FA_ERR_NULL, "lse is NULL");
   if (!aligned(p.lse, 4)) return fail(FA_ERR_STRIDE, "lse pointer is not 4-byte aligned");
+  if (!aligned(p.o_low, 16)) return fail(FA_ERR_STRIDE, "o_low pointer is not 16-byte aligned");
   if (!aligned(p.ranges, 8)) return fail(FA_ERR_STRIDE, "ranges pointer is not 8-byte aligned");
   if (p.range_stride < 0 || p.range_stride % 2 != 0)
     return fail(FA_ERR_STRIDE, "range_stride %lld is negative or odd", (long long)p.range_stride);
@@ -114,6 +115,7 @@ AttnArgs attn_args(const fa_attn_params& p, int compute_units) {
   a.v = rows3(p.v, p.v_stride);
   a.o = rows3(p.o, p.o_stride);
   a.lse = p.lse;
+  a.o_low = static_cast<char*>(p.o_low);
   a.ranges = p.ranges;
   a.range_sb = p.range_stride;
   a.batch = p.batch;

@@ -1,6 +1,6 @@
 // Gradients of attention with capped, biased and masked scores, on gfx950.
 //
-//   delta_i = go_i.o_i - glse_i;  dS = P (go_i.v_j - delta_i) (1 - (c / cap)^2)
+//   delta_i = go_i.(o_i + o_low_i) - glse_i;  dS = P (go_i.v_j - delta_i) (1 - (c / cap)^2)
 //   gv_j = sum_i P go_i;  gk_j = scale sum_i dS q_i;  gq_i = scale sum_j dS k_j
 //
 // P is computed again from the logsumexp.  Three kernels, no atomics: sums run in
@@ -52,23 +52,6 @@ __device__ __forceinline__ float grad_factor(float top) {
   return __builtin_bit_cast(float, (uint32_t)(127 - 12 - e) << 23);
 }
 
-template <bool BF16>
-__device__ __forceinline__ void unpack2(uint32_t u, float* f) {
-  if constexpr (BF16) {
-    f[0] = __builtin_bit_cast(float, u << 16);
-    f[1] = __builtin_bit_cast(float, u & 0xffff0000u);
-  } else {
-    const f16x2 x = __builtin_bit_cast(f16x2, u);
-    f[0] = (float)x[0];
-    f[1] = (float)x[1];
-  }
-}
-template <bool BF16>
-__device__ __forceinline__ void unpack8(u32x4 w, float* f) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) unpack2<BF16>(w[j], f + 2 * j);
-}
-
 // ---- rows ----
 
 // 64 rows of one head a workgroup, D / 8 lanes a row.  Bound by reading go and o.
@@ -90,6 +73,12 @@ __global__ void __launch_bounds__(256) fa_attn_rows_kernel(const AttnArgs a) {
     float g[8], o[8], sum = 0.0f, most = 0.0f;
     unpack8<BF16>(*reinterpret_cast<const u32x4*>(gh + i * a.go.st + at), g);
     unpack8<BF16>(*reinterpret_cast<const u32x4*>(oh + i * a.o.st + at), o);
+    if (a.o_low != nullptr) {
+      float low[8];
+      unpack8<BF16>(*reinterpret_cast<const u32x4*>(a.o_low + ((int64_t)bh * a.n + i) * 2 * D + at), low);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] += low[j];
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       sum = fmaf(g[j], o[j], sum);

@@ -163,9 +163,28 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
     lu[rb] = W::red_sum(w.lu[rb]);
   }
   char* oh = a.o.p + b * a.o.sb + h * a.o.sh;
-  write_rows<D, BF16>(smem + wave * (TEAMS == 1 ? 32 * ROWB : (D / 16 * 2 + 2) * 1024), w.o, inv, lane, [&](int r) FA_INLINE -> char* {
+  char* ot = smem + wave * (TEAMS == 1 ? 32 * ROWB : (D / 16 * 2 + 2) * 1024);
+  write_rows<D, BF16>(ot, w.o, inv, lane, [&](int r) FA_INLINE -> char* {
     return wrow0 + r < a.n ? oh + (wrow0 + r) * a.o.st : nullptr;
   });
+  if (a.o_low != nullptr) {  // (nothing of what is no number, or rounds to none)
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+      for (int db = 0; db < W::DB; ++db) {
+        const f32x4 x = w.o[db][rb] * inv[rb];
+        float r[4];
+        unpack2<BF16>(pack2<BF16>(x[0], x[1]), r);
+        unpack2<BF16>(pack2<BF16>(x[2], x[3]), r + 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w.o[db][rb][i] = fabsf(r[i]) < INFINITY ? x[i] - r[i] : 0.0f;
+      }
+    const float one[2] = {1.0f, 1.0f};
+    char* lh = a.o_low + ((int64_t)b * a.heads + h) * a.n * ROWB;
+    write_rows<D, BF16>(ot, w.o, one, lane, [&](int r) FA_INLINE -> char* {
+      return wrow0 + r < a.n ? lh + (int64_t)(wrow0 + r) * ROWB : nullptr;
+    });
+  }
   if (a.lse != nullptr && g4 < 2) {
     const int r = wrow0 + 16 * g4 + l16;
     const float m = g4 == 0 ? w.m[0] : w.m[1], sum = g4 == 0 ? w.ls[0][0] : w.ls[1][0];

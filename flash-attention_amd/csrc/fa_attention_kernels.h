@@ -26,6 +26,7 @@ struct GridOrder {
 struct AttnArgs {
   Rows3 q, k, v, o;
   float* lse;               // [batch, heads, n] contiguous
+  char* o_low;              // [batch, heads, n, head_dim] contiguous: what o's rounding left out; NULL: none
   const int32_t* ranges;    // pairs (first key, end) of each row; NULL: all keys
   int64_t range_sb;         // elements
   int32_t batch, heads, kv_heads, group;

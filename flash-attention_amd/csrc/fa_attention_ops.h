@@ -173,6 +173,23 @@ __device__ __forceinline__ void lds_write16(uint32_t addr, u32x4 w) {
   *(__attribute__((address_space(3))) u32x4*)(uintptr_t)addr = w;
 }
 
+template <bool BF16>
+__device__ __forceinline__ void unpack2(uint32_t u, float* f) {
+  if constexpr (BF16) {
+    f[0] = __builtin_bit_cast(float, u << 16);
+    f[1] = __builtin_bit_cast(float, u & 0xffff0000u);
+  } else {
+    const f16x2 x = __builtin_bit_cast(f16x2, u);
+    f[0] = (float)x[0];
+    f[1] = (float)x[1];
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ void unpack8(u32x4 w, float* f) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) unpack2<BF16>(w[j], f + 2 * j);
+}
+
 // A tile that some row or key does not see whole: 0 times an infinity or NaN of a
 // masked row would be NaN in the products that sum over these rows.  Clears the
 // infinities and NaN among the ROWS rows at LDS address `at`, which this wave has

@@ -50,23 +50,31 @@ fa_attn_params attn_params(const Tensor& q, const Tensor& k, const Tensor& v,
   return p;
 }
 
-std::pair<Tensor, Tensor> attn_forward(const Tensor& q, const Tensor& k, const Tensor& v,
+struct Forward {
+  Tensor o, lse, o_low;
+};
+
+// for_gradients: with lse and o_low.
+Forward attn_forward(const Tensor& q, const Tensor& k, const Tensor& v,
                                        const std::optional<Tensor>& ranges,
-                                       const std::optional<Tensor>& slopes, const Options& opt, bool with_lse) {
+                                       const std::optional<Tensor>& slopes, const Options& opt, bool with_lse,
+                     bool for_gradients) {
   fa_attn_params p = attn_params(q, k, v, ranges, slopes, opt);
   const c10::OptionalDeviceGuard guard(q.device());
-  Tensor o = new_like(q), lse;
-  if (with_lse) lse = new_tensor({q.size(0), q.size(1), q.size(2)}, torch::kFloat32, q);
+  Tensor o = new_like(q), lse, o_low;
+  if (with_lse || for_gradients) lse = new_tensor({q.size(0), q.size(1), q.size(2)}, torch::kFloat32, q);
   p.o = o.data_ptr();
-  p.lse = with_lse ? lse.data_ptr<float>() : nullptr;
+  p.lse = lse.defined() ? lse.data_ptr<float>() : nullptr;
+  if (for_gradients) o_low = new_tensor(q.sizes(), q.scalar_type(), q);
+  p.o_low = for_gradients ? o_low.data_ptr() : nullptr;
   set_strides(p.o_stride, o, 3);
   check_status(fa_attn_fwd(&p, stream_of(q)), "attention");
-  return {o, lse};
+  return {o, lse, o_low};
 }
 
-// glse may be undefined.
+// glse and o_low may be undefined.
 std::array<Tensor, 3> attn_backward(const Tensor& go, const Tensor& glse, const Tensor& q, const Tensor& k,
-                                    const Tensor& v, const Tensor& o, const Tensor& lse,
+                                    const Tensor& v, const Tensor& o, const Tensor& lse, const Tensor& o_low,
                                     const std::optional<Tensor>& ranges, const std::optional<Tensor>& slopes,
                                     const Options& opt) {
   fa_attn_bwd_params p{};
@@ -90,6 +98,7 @@ std::array<Tensor, 3> attn_backward(const Tensor& go, const Tensor& glse, const 
   Tensor gq = new_like(q), gk = new_like(k), gv = new_like(v);
   p.fwd.o = o.data_ptr();
   p.fwd.lse = lse.data_ptr<float>();
+  p.fwd.o_low = o_low.defined() ? o_low.data_ptr() : nullptr;
   set_strides(p.fwd.o_stride, o, 3);
   p.go = g.data_ptr();
   set_strides(p.go_stride, g, 3);
@@ -120,14 +129,14 @@ struct Attention : torch::autograd::Function<Attention> {
                                                 std::optional<int64_t> window, std::optional<double> softcap,
                                                 std::optional<double> scale) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const auto y = attn_forward(q, k, v, ranges, slopes, Options{causal, window, softcap, scale}, true);
+    const Forward y = attn_forward(q, k, v, ranges, slopes, Options{causal, window, softcap, scale}, true, true);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({q, k, v, y.first, y.second, ranges.value_or(Tensor()), slopes.value_or(Tensor())});
+    ctx->save_for_backward({q, k, v, y.o, y.lse, ranges.value_or(Tensor()), slopes.value_or(Tensor()), y.o_low});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["window"] = window;
     ctx->saved_data["softcap"] = softcap;
     ctx->saved_data["scale"] = scale;
-    return {y.first, y.second};
+    return {y.o, y.lse};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list g) {
@@ -141,7 +150,7 @@ struct Attention : torch::autograd::Function<Attention> {
                         ctx->saved_data["softcap"].toOptional<double>(),
                         ctx->saved_data["scale"].toOptional<double>()};
       const Tensor go = g[0].defined() ? g[0] : torch::zeros_like(s[3]);
-      d = attn_backward(go, g[1], s[0], s[1], s[2], s[3], s[4], optional_of(s[5]), optional_of(s[6]), opt);
+      d = attn_backward(go, g[1], s[0], s[1], s[2], s[3], s[4], s[7], optional_of(s[5]), optional_of(s[6]), opt);
     }
     out = once({d.begin(), d.end()}, "attention");
     out.resize(9);
@@ -164,8 +173,10 @@ pybind11::object attention(const Tensor& q, const Tensor& k, const Tensor& v, st
     o = y[0];
     lse = y[1];
   } else {
-    std::tie(o, lse) =
-        attn_forward(q, k, v, ranges, slopes, Options{causal, window, softcap, softmax_scale}, return_lse);
+    const Forward y =
+        attn_forward(q, k, v, ranges, slopes, Options{causal, window, softcap, softmax_scale}, return_lse, false);
+    o = y.o;
+    lse = y.lse;
   }
   if (return_lse) return pybind11::make_tuple(o, lse);
   return pybind11::cast(o);
@@ -178,7 +189,7 @@ pybind11::tuple attention_backward(const Tensor& go, const Tensor& q, const Tens
                                    std::optional<Tensor> glse) {
   check_no_tangent("attention_backward", {&go, &q, &k, &v, &o, &lse});
   at::NoGradGuard no_grad;
-  const auto d = attn_backward(go, glse.value_or(Tensor()), q, k, v, o, lse, ranges, slopes,
+  const auto d = attn_backward(go, glse.value_or(Tensor()), q, k, v, o, lse, Tensor(), ranges, slopes,
                                Options{causal, window, softcap, softmax_scale});
   return pybind11::make_tuple(d[0], d[1], d[2]);
 }

@@ -46,6 +46,9 @@ typedef struct {
   const void* v;
   void* o;                /* like q */
   float* lse;             /* [batch, heads, seq_len] contiguous, natural log; may be NULL in fa_attn_fwd */
+  void* o_low;            /* [batch, heads, seq_len, head_dim] contiguous, 16-byte aligned: what the rounding
+                             of o left out, rounded likewise; fa_attn_bwd takes delta from both.  NULL: none,
+                             at the price of delta's exactness where few keys have most of the weight */
   int64_t q_stride[3];    /* batch, head, row; multiples of 8 elements */
   int64_t k_stride[3];
   int64_t v_stride[3];
@@ -60,13 +63,13 @@ typedef struct {
   fa_score_params score;
 } fa_attn_params;
 
-/* Gradients of fa_attn_fwd:  delta_i = go_i.o_i - glse_i,
+/* Gradients of fa_attn_fwd:  delta_i = go_i.(o_i + o_low_i) - glse_i,
  *   dx_ij = P_ij (go_i.v_j - delta_i),  P = exp(x - lse),
  *   dz = dx (1 - (c / softcap)^2),  gv_j = sum_i P go_i,
  *   gk_j = softmax_scale sum_i dz q_i,  gq_i = softmax_scale sum_j dz k_j,
  * those of k and v summed over the query heads that read them.  Sums run in a fixed
- * order (no atomics).  fwd: as given to fa_attn_fwd, o and lse as it wrote them
- * (read only).  Rows and keys that do not see each other contribute nothing to each
+ * order (no atomics).  fwd: as given to fa_attn_fwd, o, lse and o_low as it wrote
+ * them (read only).  Rows and keys that do not see each other contribute nothing to each
  * other, whatever they hold; the results of rows and keys that see an infinity or
  * a NaN are infinities or NaN. */
 typedef struct {

@@ -13,7 +13,7 @@ _p, _i32, _i64, _f = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_f
 
 Score = _struct("Score", [("softcap", _f), ("window", _i32), ("slopes", _p)])
 Attn = _struct("Attn", [
-    ("q", _p), ("k", _p), ("v", _p), ("o", _p), ("lse", _p), ("q_stride", _i64 * 3), ("k_stride", _i64 * 3),
+    ("q", _p), ("k", _p), ("v", _p), ("o", _p), ("lse", _p), ("o_low", _p), ("q_stride", _i64 * 3), ("k_stride", _i64 * 3),
     ("v_stride", _i64 * 3), ("o_stride", _i64 * 3), ("ranges", _p), ("range_stride", _i64), ("batch", _i32),
     ("heads", _i32), ("kv_heads", _i32), ("seq_len", _i32), ("keys", _i32), ("head_dim", _i32), ("dtype", _i32),
     ("causal", _i32), ("softmax_scale", _f), ("score", Score)])

@@ -88,7 +88,7 @@ def test_valid_and_null(lib, name):
 def test_valid_edges(lib):
     """What the header allows at its limits."""
     for field, value in [("ranges", None), ("range_stride", 0), ("score.slopes", None), ("score.window", 0),
-                         ("score.window", 2 ** 31 - 1), ("score.softcap", 0.0), ("score.softcap", 1000.0), ("lse", None),
+                         ("score.window", 2 ** 31 - 1), ("score.softcap", 0.0), ("score.softcap", 1000.0), ("lse", None), ("o_low", None),
                          ("keys", 2 ** 22), ("k_stride", (0, 0, 0)), ("seq_len", 1), ("kv_heads", 4)]:
         s = make("fa_attn_fwd")[0]
         put(s, field, value)
@@ -108,7 +108,7 @@ ATTN_BAD = [
     ("q", None, A.FA_ERR_NULL), ("k", PTR + 8, A.FA_ERR_STRIDE), ("v", None, A.FA_ERR_NULL), ("o", None, A.FA_ERR_NULL),
     ("q_stride[0]", -64, A.FA_ERR_STRIDE), ("k_stride[2]", 68, A.FA_ERR_STRIDE),
     ("v_stride[2]", 2 ** 24 + 8, A.FA_ERR_UNSUPPORTED), ("q_stride[2]", 2 ** 24 + 8, A.FA_ERR_UNSUPPORTED),
-    ("lse", PTR + 2, A.FA_ERR_STRIDE), ("ranges", PTR + 4, A.FA_ERR_STRIDE), ("range_stride", 3, A.FA_ERR_STRIDE),
+    ("lse", PTR + 2, A.FA_ERR_STRIDE), ("o_low", PTR + 8, A.FA_ERR_STRIDE), ("ranges", PTR + 4, A.FA_ERR_STRIDE), ("range_stride", 3, A.FA_ERR_STRIDE),
     ("range_stride", -2, A.FA_ERR_STRIDE), ("causal", 2, A.FA_ERR_ARG), ("softmax_scale", 0.0, A.FA_ERR_ARG),
     ("softmax_scale", math.nan, A.FA_ERR_ARG), ("softmax_scale", 2e38, A.FA_ERR_ARG),
     ("softmax_scale", 1.5e-38, A.FA_OK),

@@ -233,6 +233,36 @@ def test_one_bad_key_reaches_the_rows_that_see_it(fa, D, H):
         assert bool(torch.isnan(got["o"][0, 0, 120:]).any(-1).all())
 
 
+@pytest.mark.parametrize("name", ["causal", "any-ranges-128", "all-options", "many-window"])
+def test_attention_backward(fa, name):
+    """By itself, from the o that attention returned."""
+    print("case backward", name, flush=True)
+    tensors, ranges, slopes, opt = setup(fa, name)
+    q, k, v, go = (dev(x) for x in tensors)
+    rest = dict(key_ranges=None if ranges is None else ranges.to(DEV), slopes=None if slopes is None else slopes.to(DEV), **opt)
+    o, lse = fa.attention(q, k, v, return_lse=True, **rest)
+    got = dict(zip(("gq", "gk", "gv"), fa.attention_backward(go, q, k, v, o, lse, **rest)), o=o, lse=lse)
+    compare(got, *reference(tensors, ranges, slopes, opt))
+
+
+def test_gradients_of_sharp_rows_take_what_rounding_left_of_o(fa):
+    """Where few keys have most of the weight, go.v - delta cancels, and the rounding of o that
+    attention_backward is given weighs as much as all others: without it the root mean square error is smaller."""
+    print("case sharp", flush=True)
+    g = torch.Generator().manual_seed(44)
+    q, go = (rows(1, 2, 500, 128, torch.bfloat16, g, scale=s) for s in (4.0, 1.0))
+    k, v = (rows(1, 2, 500, 128, torch.bfloat16, g) for _ in range(2))
+    opt = dict(causal=True, softcap=50.0)
+    got = call(fa, (q, k, v, go), None, None, opt)
+    val, _ = reference((q, k, v, go), None, None, opt)
+    x = [dev(t) for t in (q, k, v)]
+    o, lse = fa.attention(*x, return_lse=True, **opt)
+    plain = dict(zip(("gq", "gk"), fa.attention_backward(dev(go), *x, o, lse, **opt)))
+    for n in plain:
+        off = [float((y[n].cpu().double() - val[n]).norm()) for y in (got, plain)]
+        assert off[0] < off[1], (n, off)
+
+
 def test_gradients_with_expanded_and_odd_strides(fa):
     """sum().backward() hands in an expanded gradient; k and v of one head may be broadcast."""
     g = torch.Generator(device=DEV).manual_seed(2)
@@ -242,9 +272,8 @@ def test_gradients_with_expanded_and_odd_strides(fa):
     fa.attention(q, k, k, causal=True).sum().backward()
     a, b = q.grad.clone(), kv.grad.clone()
     ones = torch.ones(2, 4, 90, 64, device=DEV).half()
-    kc = k.detach().contiguous().requires_grad_()
-    o, lse = fa.attention(q.detach(), kc, kc.detach(), causal=True, return_lse=True)
-    dq, dk, dv = fa.attention_backward(ones, q.detach(), kc.detach(), kc.detach(), o.detach(), lse.detach(), causal=True)
+    kc, vc = (k.detach().clone().requires_grad_() for _ in range(2))
+    dq, dk, dv = torch.autograd.grad(fa.attention(q, kc, vc, causal=True), (q, kc, vc), ones)
     assert torch.equal(a, dq)
     want = (dk.float() + dv.float()).sum(0, keepdim=True)
     assert float((b.float() - want).abs().max()) <= 4 * 2.0 ** -11 * float(want.abs().max())
@@ -306,6 +335,9 @@ def test_autograd_in_a_graph(fa):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(got, want))
+    x = [t.detach() for t in (q, k, v)]
+    o, lse = fa.attention(*x, causal=True, return_lse=True)
+    want = fa.attention_backward(go, *x, o, lse, causal=True)
     alive = fa.attention(q, k, v, causal=True)  # holds the leaves' accumulators
     other = torch.cuda.CUDAGraph()
     with torch.cuda.graph(other):
