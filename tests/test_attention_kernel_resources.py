@@ -22,7 +22,8 @@ WANT = {
     "fa_attention_bwd.hip": [(r"fa_attn_rows_kernel", 256, 4), (r"fa_attn_order_kernel", 1024, 1),
                              (r"fa_attn_dkv_kernelILi128.*ELi1EEE", 256, 2), (r"fa_attn_dkv_kernelILi128.*ELi2EEE", 512, 1),
                              (r"fa_attn_dkv_kernelILi64.*ELi1EEE", 256, 3), (r"fa_attn_dkv_kernelILi64.*ELi3EEE", 768, 1),
-                             (r"fa_attn_dq_kernel.*ELi1EEE", 256, 2), (r"fa_attn_dq_kernel.*ELi2EEE", 512, 1),
+                             (r"fa_attn_dq_kernelILi128.*ELi1EEE", 256, 2), (r"fa_attn_dq_kernelILi64.*ELi1EEE", 256, 3),
+                             (r"fa_attn_dq_kernel.*ELi2EEE", 512, 1),
                              (r"fa_attn_join_kernel", 256, 4)],
     "fa_paged_scored.hip": [(r"fa_paged_chunk_kernel", 256, 2), (r"fa_paged_decode_kernelILi\d+ELb\dELi\dELi2E", 128, 2),
                             (r"fa_paged_decode_kernelILi\d+ELb\dELi\dELi4E", 256, 1), (r"fa_paged_merge_kernel", 256, 4)],
