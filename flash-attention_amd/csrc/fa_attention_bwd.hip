@@ -40,7 +40,10 @@ template <bool BF16>
 constexpr float kShift = BF16 ? 0.0f : 12.0f;  // log2 of P's factor
 
 // The record of a span, [2][4 fields][16 rows] floats: for each 16 rows
-enum RecordField { kLse, kDelta, kLo, kHi };  // (lse in log2, less kShift; minus delta)
+enum RecordField { kLse, kDelta, kLo, kHi };  // (lse in log2, less kShift and the cap; minus delta)
+// dS is made with a quarter of capped scores' derivative, 1 - tanh^2 = 4 tail (1 - tail).
+template <bool CAP>
+constexpr float kQuarters = CAP ? 4.0f : 1.0f;
 constexpr int kRecord = kSpan * 4;
 
 // 2^-(e + 12) for a largest |go| in [2^e, 2^(e + 1)): dS's factor.  1 for bf16.
@@ -103,7 +106,7 @@ __global__ void __launch_bounds__(256) fa_attn_rows_kernel(const AttnArgs a) {
     k = row_keys(a, b, i);
     if (k.hi > 0) {
       const int64_t at = (int64_t)bh * a.n + i;
-      lse = a.lse[at] * kLog2e - kShift<BF16>;
+      lse = a.lse[at] * kLog2e - kShift<BF16> - a.score.cap;  // (the cap that scores leave out)
       d = (a.glse != nullptr ? a.glse[at] : 0.0f) - delta[r];
       most = top[r];
     }
@@ -462,7 +465,7 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4 * TEAMS; ++i) top = fmaxf(top, top_part[i]);
-    factor = uniform(grad_factor<BF16>(uniform(top)));
+    factor = uniform(kQuarters<CAP> * grad_factor<BF16>(uniform(top)));
   }
   finish(now, 0, false);  // (what was loaded so far: no wait for it later, which would be one for copies too)
 
@@ -500,7 +503,7 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
         for (int j = 0; j < PART; ++j) {
           const int at = decltype(i_c)::value * PART + j;
           const float x = c[at / 4][at % 4];
-          c[at / 4][at % 4] = CAP ? grads.score.half_tail(x) : fast_exp2(fmaf(x, grads.unit, -lse[at % 4]));
+          c[at / 4][at % 4] = CAP ? grads.score.tail(x) : fast_exp2(fmaf(x, grads.unit, -lse[at % 4]));
         }
       });
       if constexpr (CAP) {
@@ -509,8 +512,8 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float t = c[cb][i];
-            c[cb][i] = fmaf(-grads.score.twice, t, grads.score.out);
-            e[cb][i] *= 4.0f * t * (1.0f - t);
+            e[cb][i] *= fmaf(-t, t, t);
+            c[cb][i] = fmaf(-grads.score.twice, t, -lse[i]);
           }
         if (grads.score.biased)
 #pragma unroll
@@ -520,7 +523,7 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
 #pragma unroll
         for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) c[cb][i] = fast_exp2(c[cb][i] - lse[i]);
+          for (int i = 0; i < 4; ++i) c[cb][i] = fast_exp2(c[cb][i]);
       }
 #pragma unroll
       for (int cb = 0; cb < 2; ++cb)
@@ -591,7 +594,7 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
   // (powers of two but for the scale)
   const auto& x = late_args();
   const float fv[2] = {fast_exp2(-kShift<BF16>), fast_exp2(-kShift<BF16>)};
-  const float fk[2] = {x.scale * fv[0] / factor, x.scale * fv[0] / factor};
+  const float scale = kQuarters<CAP> * x.scale * fv[0] / factor, fk[2] = {scale, scale};
   const int l = lane_now(), m = x.m;
   if (x.parts != nullptr) {
     const int64_t rows = (int64_t)x.batch * x.kv_heads * m;
@@ -710,7 +713,7 @@ __global__ void __launch_bounds__(256 * TEAMS)
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(f[j]));
       }
-      factor[rb] = grad_factor<BF16>(WaveAttn<D, BF16, 4, 2>::red_max(top));
+      factor[rb] = kQuarters<CAP> * grad_factor<BF16>(WaveAttn<D, BF16, 4, 2>::red_max(top));
     }
   }
   // The staged keys of tile t are there: cleaned if some row does not see all of
@@ -767,7 +770,7 @@ __global__ void __launch_bounds__(256 * TEAMS)
         for (int j = 0; j < PART; ++j) {
           const int at = decltype(i_c)::value * PART + j;
           const float x = s[kb][at / 4][at % 4];
-          s[kb][at / 4][at % 4] = CAP ? grads.score.half_tail(x) : fast_exp2(fmaf(x, grads.unit, -lse[at / 4]));
+          s[kb][at / 4][at % 4] = CAP ? grads.score.tail(x) : fast_exp2(fmaf(x, grads.unit, -lse[at / 4]));
         }
       };
     };
@@ -789,9 +792,9 @@ __global__ void __launch_bounds__(256 * TEAMS)
       each([&](float x, int kb, int i) FA_INLINE {
         float p = x;
         if constexpr (CAP) {
-          const float c = fmaf(-grads.score.twice, x, grads.score.out);
-          dp[kb][rb][i] = (dp[kb][rb][i] + delta[rb]) * (4.0f * x * (1.0f - x));
-          p = fast_exp2((grads.score.biased ? grads.biased(c, away_of(rb, kb, i)) : c) - lse[rb]);
+          const float c = fmaf(-grads.score.twice, x, -lse[rb]);
+          dp[kb][rb][i] = (dp[kb][rb][i] + delta[rb]) * fmaf(-x, x, x);
+          p = fast_exp2(grads.score.biased ? grads.biased(c, away_of(rb, kb, i)) : c);
         } else {
           dp[kb][rb][i] += delta[rb];
         }
@@ -836,7 +839,7 @@ __global__ void __launch_bounds__(256 * TEAMS)
   }
   float f[2];
 #pragma unroll
-  for (int rb = 0; rb < 2; ++rb) f[rb] = a.scale * fast_exp2(-kShift<BF16>) / factor[rb];
+  for (int rb = 0; rb < 2; ++rb) f[rb] = kQuarters<CAP> * a.scale * fast_exp2(-kShift<BF16>) / factor[rb];
   char* qh = a.gq.p + b * a.gq.sb + h * a.gq.sh;
   write_rows<D, BF16>(smem + wave * PART, gq, f, lane, [&](int r) FA_INLINE -> char* {
     return wrow0 + r < a.n ? qh + (wrow0 + r) * a.gq.st : nullptr;

@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
     const float m = g4 == 0 ? w.m[0] : w.m[1], sum = g4 == 0 ? w.ls[0][0] : w.ls[1][0];
     const float l = g4 == 0 ? lu[0] : lu[1];
     if (r < a.n)
-      a.lse[((int64_t)b * a.heads + h) * a.n + r] = sum == 0.0f ? -INFINITY : (m * w.c + __log2f(l)) * kLn2;
+      a.lse[((int64_t)b * a.heads + h) * a.n + r] = sum == 0.0f ? -INFINITY : w.log2_sum(m, l) * kLn2;
   }
 }
 

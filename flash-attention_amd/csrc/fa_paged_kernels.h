@@ -260,13 +260,13 @@ __global__ void __launch_bounds__(64 * NW) fa_paged_decode_kernel(const PagedFwd
       *reinterpret_cast<u32x2*>(a.o + t * a.o_st + h * a.o_sh + d * 2) =
           u32x2{pack2<BF16>(acc[0], acc[1]), pack2<BF16>(acc[2], acc[3])};
       if (a.lse != nullptr && d == 0)
-        a.lse[t * a.heads + h] = none ? -INFINITY : (mm * w.c + __log2f(lu)) * kLn2;
+        a.lse[t * a.heads + h] = none ? -INFINITY : w.log2_sum(mm, lu) * kLn2;
     } else {
       const int64_t wr = (((int64_t)b * a.kv_heads + kvh) * a.splits + split) * BM + r;
       *reinterpret_cast<f32x4*>(a.ws_o + wr * D + d) = acc;
       if (d == 0) {
-        a.ws_e[wr * 2] = none ? -INFINITY : mm * w.c + __log2f(lr);
-        a.ws_e[wr * 2 + 1] = none ? -INFINITY : mm * w.c + __log2f(lu);
+        a.ws_e[wr * 2] = none ? -INFINITY : w.log2_sum(mm, lr);
+        a.ws_e[wr * 2 + 1] = none ? -INFINITY : w.log2_sum(mm, lu);
       }
     }
   }
@@ -482,8 +482,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
         *reinterpret_cast<f32x4*>(a.ws_o + (wr0 + r) * D + 16 * db + 4 * g4) = w.o[db][rb] * inv[rb];
       if (g4 == 0) {
         const bool none = w.ls[rb][0] == 0.0f;
-        a.ws_e[(wr0 + r) * 2] = none ? -INFINITY : w.m[rb] * w.c + __log2f(w.ls[rb][0]);
-        a.ws_e[(wr0 + r) * 2 + 1] = none ? -INFINITY : w.m[rb] * w.c + __log2f(lu[rb]);
+        a.ws_e[(wr0 + r) * 2] = none ? -INFINITY : w.log2_sum(w.m[rb], w.ls[rb][0]);
+        a.ws_e[(wr0 + r) * 2 + 1] = none ? -INFINITY : w.log2_sum(w.m[rb], lu[rb]);
       }
     }
     return;
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     if (r < n_rows) {
       const int i = fast_div(r, a.by_group), h = kvh * a.group + r - i * a.group;
       a.lse[(int64_t)(s.q0 + i) * a.heads + h] =
-          sum == 0.0f ? -INFINITY : (m * w.c + __log2f(l)) * kLn2;
+          sum == 0.0f ? -INFINITY : w.log2_sum(m, l) * kLn2;
     }
   }
 }

@@ -16,7 +16,7 @@ struct ScoreArgs {
   float cap;            // softcap * log2(e); 0: none
   float cap_twice;      // twice that
   float cap_in;         // 2 softmax_scale log2(e) / softcap
-  float unit;           // log2(e) softmax_scale, or 1 for capped scores: what the bias is added to
+  float unit;           // log2(e) softmax_scale, or cap_twice: factor of what the bias is added to
   const float* slopes;  // of each query head; NULL: no bias
   int32_t window;       // keys at a distance below it are seen; 0: all
 };
@@ -25,10 +25,14 @@ struct ScoreArgs {
 namespace {
 
 // The scores of a wave, in units of log2 so that exp2 takes them as they are.
+//   cap tanh(x) = cap - 2 cap tail,  tail = (1 - tanh(x)) / 2 = 1 / (1 + e^2x)
+// The first cap is the same for all keys: it is left out and added to the logsumexp.
+// The error, about 1.2e-7 cap, is that of 1 + e^2x: of no weight for scores up to some hundreds.
+// Two instructions beside two of a quarter of the rate.
 struct Score {
   bool capped, biased;
-  float in, out, twice;  // capped
-  float unit;            // factor of the scores that the bias is added to
+  float in, out, twice;  // capped: e^2x = 2^(in z), the cap, 2 caps
+  float unit;
   __device__ __forceinline__ void init(const ScoreArgs& a) {
     capped = a.cap > 0.0f;
     biased = a.slopes != nullptr;
@@ -37,16 +41,14 @@ struct Score {
     twice = a.cap_twice;
     unit = a.unit;
   }
-  // out tanh(x) with e^2x = 2^(in x): out - 2 out / (1 + e^2x).  Its error, about
-  // 1.2e-7 out, is that of 1 + e^2x: of no weight for scores up to some hundreds.
-  // Three instructions beside two of a quarter of the rate.
-  __device__ __forceinline__ float cap(float x) const {
-    return fmaf(-twice, half_tail(x), out);
+  __device__ __forceinline__ float tail(float z) const {
+    return __builtin_amdgcn_rcpf(1.0f + dev::fast_exp2(z * in));
   }
-  // (1 - tanh(x)) / 2
-  __device__ __forceinline__ float half_tail(float x) const {
-    return __builtin_amdgcn_rcpf(1.0f + dev::fast_exp2(x * in));
+  __device__ __forceinline__ float minus_tail(float z) const {
+    return __builtin_amdgcn_rcpf(-(1.0f + dev::fast_exp2(z * in)));
   }
+  // What the scores are less than those of the formula.
+  __device__ __forceinline__ float left_out() const { return capped ? out : 0.0f; }
 };
 
 }  // namespace

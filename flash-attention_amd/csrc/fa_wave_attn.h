@@ -75,11 +75,17 @@ struct WaveAttn {
     }
   }
 
-  // (in front of init's use of c: scores that are capped or biased have their
-  // factor already)
+  // Behind init.  (Biased scores have their factor already.)
   __device__ __forceinline__ void init_score(const ScoreArgs& a) {
     score.init(a);
-    if (score.capped || score.biased) c = 1.0f;
+    if (score.capped) c = score.twice;
+    if (score.biased) c = 1.0f;
+  }
+
+  // log2 of the sum of exponentials, from the offset and the sum by it.
+  __device__ __forceinline__ float log2_sum(float offset, float sum) const {
+    const float x = offset * c + __log2f(sum);
+    return SCORED ? x + score.left_out() : x;
   }
 
   static __device__ __forceinline__ float red_max(float x) {
@@ -135,7 +141,7 @@ struct WaveAttn {
 
     if constexpr (SCORED) {
       if (score.capped)
-        each(s, [&](float x, int, int, int) FA_INLINE { return score.cap(x); });
+        each(s, [&](float x, int, int, int) FA_INLINE { return score.minus_tail(x); });
       if (score.biased) {
         float at[RB];  // the lane's first key as seen from its row
 #pragma unroll
