@@ -789,15 +789,20 @@ __global__ void __launch_bounds__(256 * TEAMS)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[kb][rb][i] = fn(s[kb][rb][i], kb, i);
       };
+      if constexpr (CAP) {
+        each([&](float x, int kb, int i) FA_INLINE {
+          dp[kb][rb][i] = (dp[kb][rb][i] + delta[rb]) * fmaf(-x, x, x);
+          return fmaf(-grads.score.twice, x, -lse[rb]);
+        });
+        if (grads.score.biased)
+          each([&](float x, int kb, int i) FA_INLINE { return grads.biased(x, away_of(rb, kb, i)); });
+      }
       each([&](float x, int kb, int i) FA_INLINE {
         float p = x;
-        if constexpr (CAP) {
-          const float c = fmaf(-grads.score.twice, x, -lse[rb]);
-          dp[kb][rb][i] = (dp[kb][rb][i] + delta[rb]) * fmaf(-x, x, x);
-          p = fast_exp2(grads.score.biased ? grads.biased(c, away_of(rb, kb, i)) : c);
-        } else {
+        if constexpr (CAP)
+          p = fast_exp2(x);
+        else
           dp[kb][rb][i] += delta[rb];
-        }
         if constexpr (!BF16) p *= factor[rb];
         return p * dp[kb][rb][i];
       });
