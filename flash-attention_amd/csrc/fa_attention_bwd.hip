@@ -3,17 +3,25 @@
 //   delta_i = go_i.(o_i + o_low_i) - glse_i;  dS = P (go_i.v_j - delta_i) (1 - (c / cap)^2)
 //   gv_j = sum_i P go_i;  gk_j = scale sum_i dS q_i;  gq_i = scale sum_j dS k_j
 //
-// P is computed again from the logsumexp.  Three kernels, no atomics: sums run in
-// a fixed order, at the price of computing scores and go.v twice (7 products of
-// the size of q.k in place of 5):
+// P is computed again from the logsumexp.  No atomics on results: sums run in a fixed
+// order, at the price of computing scores and go.v twice (7 products of the size of
+// q.k in place of 5):
 //  * fa_attn_rows_kernel: delta, the keys that each row sees, and, for every span
 //    of 32 rows, their limits.
+//  * fa_attn_order_kernel, with key ranges: which tiles of keys have most rows.
 //  * fa_attn_dkv_kernel: 128 keys of a kv head, four waves of 32, whose K and V
 //    stay in registers; passes over the spans of 32 rows that see any of them, of all query
 //    heads of the group, staged through a ring.  S = Q K^T and go V^T come out with
 //    lanes along the keys, as P and dS have to go into gv^T += go^T P and
-//    gk^T += Q^T dS.
+//    gk^T += Q^T dS.  Few keys and many rows are split over workgroups, whose parts
+//    fa_attn_join_kernel adds.
 //  * fa_attn_dq_kernel: 128 rows of a head, as the forward pass.
+// Where workgroups are few, teams of four waves share one's spans or tiles (plan_attn_bwd).
+//
+// 2 x 8192 causal tokens, 32 heads on 8, D = 128, bf16, us: rows 47 (75 with o_low, 5.3 TB/s), dk and
+// dv 2170 (1010 TFLOP/s of their four products), dq 1480 (1120 of three); a matrix product
+// of 8192^3 reaches 1245.  The matrix cores are busy 49 and 55 % of the cycles, at 1.9 GHz (the power
+// limit); capped scores add vector work, 2430 and 1790.  D = 64, fp16: 1540 and 930, vector units.
 //
 // Rounding: P and dS are rounded to the input type for the matrix cores (as P of
 // the forward pass); all sums are fp32.  fp16 has few exponents: P is scaled by
