@@ -23,12 +23,14 @@ GridOrder grid_order(int units, int places, int compute_units, int per_cu) {
   o.xcd_cus = compute_units / kXcds;
   o.per_xcd = units % kXcds == 0 ? units / kXcds : 0;
   o.xcds = o.per_xcd == 0 && kXcds % units == 0 ? kXcds / units : 0;
-  // As many units at once as give each CU its workgroups, of those that divide an
-  // XCD's evenly.
-  o.unit_group = 1;
-  while (o.per_xcd > 0 && (o.per_xcd % o.unit_group != 0 ||
-                           (o.unit_group < o.per_xcd && (int64_t)o.unit_group * places < per_cu * o.xcd_cus)))
-    ++o.unit_group;
+  // The fewest units at once that give each CU its workgroups, of those that divide an
+  // XCD's evenly; all of them if none does.
+  o.unit_group = std::max(o.per_xcd, 1);
+  for (int g = 1; g < o.per_xcd && g <= per_cu * o.xcd_cus; ++g)
+    if (o.per_xcd % g == 0 && (int64_t)g * places >= per_cu * o.xcd_cus) {
+      o.unit_group = g;
+      break;
+    }
   o.turn = per_cu > 1 && (int64_t)units * places > (int64_t)kXcds * o.xcd_cus;
   o.by_group_places = make_fast_div((uint32_t)(o.unit_group * places));
   o.by_unit_group = make_fast_div((uint32_t)o.unit_group);

@@ -43,8 +43,9 @@ def attention(
     sees no key has o = 0, lse = -inf and no gradients; keys that a row does not see contribute
     nothing to it, whatever they hold.
 
-    Differentiable once in q, k and v, through o and lse; slopes get no gradient.  The same call
-    gives the same bits, gradients included.  In a graph capture a backward pass through leaves that
+    Differentiable once in q, k and v, through o and lse; slopes get no gradient.  Besides its
+    arguments and results a graph holds one more tensor like o, what rounding left out of it.  The
+    same call gives the same bits, gradients included.  In a graph capture a backward pass through leaves that
     an older autograd graph still holds is refused; ``attention_backward`` can always be captured.
     """
     return _EXT.attention(q, k, v, key_ranges, causal, window, softcap, slopes, softmax_scale, return_lse)
@@ -67,7 +68,8 @@ def attention_backward(
     dlse: torch.Tensor | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The gradients ``(dq, dk, dv)`` of ``attention`` for o's gradient ``do`` (and lse's, ``dlse``), without
-    autograd; ``o`` and ``lse`` as it returned them for the same arguments."""
+    autograd; ``o`` and ``lse`` as it returned them for the same arguments.  With the rounded o alone dq
+    and dk are up to a third less exact than autograd's where few keys have most of the weight."""
     return _EXT.attention_backward(do, q, k, v, o, lse, key_ranges, causal, window, softcap, slopes,
                                    softmax_scale, dlse)
 
