@@ -202,15 +202,15 @@ __device__ __forceinline__ T fresh(T x) {
 template <bool CAP>
 struct Grads {
   Score score;
-  float slope, unit;  // unit: of the score that the exponent takes
+  float slope, unit;  // slope: in units of what it is added to; unit: the factor of products
   __device__ __forceinline__ void init(const AttnArgs& a, int h) {
     score.init(a.score);
-    slope = uniform(score.biased ? a.score.slopes[h] * kLog2e : 0.0f);
-    unit = uniform(CAP || score.biased ? 1.0f : a.scale_log2);
+    slope = uniform(score.biased ? a.score.slopes[h] * (CAP ? kLog2e : a.score.slope_unit) : 0.0f);
+    unit = uniform(a.scale_log2);
   }
   // away: from a score's row to its key.
   __device__ __forceinline__ float biased(float x, float away) const {
-    return fmaf(-slope, fabsf(away), CAP ? x : x * score.unit);
+    return fmaf(-slope, fabsf(away), x);
   }
 };
 

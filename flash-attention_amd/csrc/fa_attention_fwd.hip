@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
   w.init(base, base + 2 * TB, a.scale_log2);
   w.init_score(a.score);
   const int l16 = w.l16, g4 = w.g4;
-  const float slope = w.score.biased ? a.score.slopes[h] * kLog2e : 0.0f;
+  const float slope = w.score.biased ? a.score.slopes[h] * a.score.slope_unit : 0.0f;
   TileKeys keys, all;  // of the wave's rows, of the workgroup's
   tile_keys(a, b, row0, wave, keys, all);
   const int c0 = all.lo, c1 = all.hi;  // (no key: kNoKey and 0)

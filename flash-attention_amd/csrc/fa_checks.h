@@ -118,7 +118,7 @@ inline ScoreArgs score_args(const fa_score_params& s, float scale) {
     a.cap_twice = 2.0f * a.cap;
     a.cap_in = (float)(2.0 * scale * kLog2e / s.softcap);
   }
-  a.unit = s.softcap != 0.0f ? a.cap_twice : (float)(scale * kLog2e);
+  a.slope_unit = (float)(s.softcap != 0.0f ? kLog2e / a.cap_twice : 1.0 / scale);
   a.slopes = s.slopes;
   a.window = s.window < (1 << 30) ? s.window : 0;
   return a;

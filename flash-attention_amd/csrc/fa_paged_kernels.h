@@ -70,7 +70,7 @@ template <class W>
 __device__ __forceinline__ void set_row(const PagedFwdArgs& a, const Seq& s, int i, int h, W& w, int rb) {
   w.first[rb] = first_key<true>(a, s, i);
   w.pos[rb] = s.first + i;
-  w.slope[rb] = a.score.slopes != nullptr ? a.score.slopes[h] * kLog2e : 0.0f;
+  w.slope[rb] = a.score.slopes != nullptr ? a.score.slopes[h] * a.score.slope_unit : 0.0f;
 }
 
 // ---- few rows: decode ----

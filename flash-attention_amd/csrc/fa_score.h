@@ -16,7 +16,8 @@ struct ScoreArgs {
   float cap;            // softcap * log2(e); 0: none
   float cap_twice;      // twice that
   float cap_in;         // 2 softmax_scale log2(e) / softcap
-  float unit;           // log2(e) softmax_scale, or cap_twice: factor of what the bias is added to
+  float slope_unit;     // of the scores as products, or tails, that the bias is added to: log2(e) over
+                        // their factor, log2(e) softmax_scale or cap_twice
   const float* slopes;  // of each query head; NULL: no bias
   int32_t window;       // keys at a distance below it are seen; 0: all
 };
@@ -24,7 +25,7 @@ struct ScoreArgs {
 #if defined(__HIPCC__)
 namespace {
 
-// The scores of a wave, in units of log2 so that exp2 takes them as they are.
+// The scores of a wave, to a factor: times log2(e) softmax_scale, or 2 caps in units of log2.
 //   cap tanh(x) = cap - 2 cap tail,  tail = (1 - tanh(x)) / 2 = 1 / (1 + e^2x)
 // The first cap is the same for all keys: it is left out and added to the logsumexp.
 // The error, about 1.2e-7 cap, is that of 1 + e^2x: of no weight for scores up to some hundreds.
@@ -32,14 +33,12 @@ namespace {
 struct Score {
   bool capped, biased;
   float in, out, twice;  // capped: e^2x = 2^(in z), the cap, 2 caps
-  float unit;
   __device__ __forceinline__ void init(const ScoreArgs& a) {
     capped = a.cap > 0.0f;
     biased = a.slopes != nullptr;
     in = a.cap_in;
     out = a.cap;
     twice = a.cap_twice;
-    unit = a.unit;
   }
   __device__ __forceinline__ float tail(float z) const {
     return __builtin_amdgcn_rcpf(1.0f + dev::fast_exp2(z * in));

@@ -48,7 +48,7 @@ struct WaveAttn {
   // SCORED
   int first[RB];            // first key this lane's row sees
   int pos[RB];              // the row's place among the keys
-  float slope[RB];          // slope of its bias in units of log2
+  float slope[RB];          // slope of its bias, in units of the scores
   Score score;
 
   __device__ __forceinline__ void init(uint32_t k_lds, uint32_t v_lds, float scale_log2) {
@@ -75,11 +75,10 @@ struct WaveAttn {
     }
   }
 
-  // Behind init.  (Biased scores have their factor already.)
+  // Behind init.
   __device__ __forceinline__ void init_score(const ScoreArgs& a) {
     score.init(a);
     if (score.capped) c = score.twice;
-    if (score.biased) c = 1.0f;
   }
 
   // log2 of the sum of exponentials, from the offset and the sum by it.
@@ -147,7 +146,7 @@ struct WaveAttn {
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) at[rb] = (float)(kt0 + 4 * g4 - pos[rb]);
         each(s, [&](float x, int kb, int rb, int i) FA_INLINE {
-          return fmaf(-slope[rb], fabsf(at[rb] + (float)(16 * kb + i)), x * score.unit);
+          return fmaf(-slope[rb], fabsf(at[rb] + (float)(16 * kb + i)), x);
         });
       }
     }

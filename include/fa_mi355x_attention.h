@@ -33,7 +33,7 @@ extern "C" {
 typedef struct {
   float softcap;       /* 0: none; else from 0.001 to 1000 (its error is about 1e-7 of it) */
   int32_t window;      /* 0: none */
-  const float* slopes; /* [heads], device memory; NULL: none */
+  const float* slopes; /* [heads], device memory; slopes over softmax_scale are finite; NULL: none */
 } fa_score_params;
 
 /* o_i = sum_j exp(x_ij - lse_i) v_j,  lse_i = ln sum_j exp(x_ij), over the keys
