@@ -54,14 +54,20 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
   tile_keys(a, b, row0, wave, keys, all);
   const int c0 = all.lo, c1 = all.hi;  // (no key: kNoKey and 0)
   const int n_tiles = c0 < c1 ? (c1 - c0 + 63) / 64 : 0;
-  const int turns = (n_tiles + TEAMS - 1) / TEAMS;  // tile t TEAMS + team is the team's in turn t
-  auto key_of = [&](int t) FA_INLINE { return c0 + 64 * (t * TEAMS + team); };
+  // Tile t TEAMS + team is the team's in turn t.  With a bias by distance the last one comes
+  // first: a causal row's scores grow towards it, and its offset would be raised tile by tile
+  // (us, 2 x 8192 causal rows, 32 heads on 8, D = 128: 1380 and 1095; a window of 1024 without a
+  // bias, 16384 rows, 16 heads: 184 from the first, 190 from the last).
+  const int turns = (n_tiles + TEAMS - 1) / TEAMS;
+  const bool down = w.score.biased;
+  const int first_key = down ? c0 + 64 * (n_tiles - 1) : c0, tile_step = down ? -64 : 64;
+  auto key_of = [&](int t) FA_INLINE { return first_key + tile_step * (t * TEAMS + team); };
   const char* kh = a.k.p + b * a.k.sb + kvh * a.k.sh;
   const char* vh = a.v.p + b * a.v.sb + kvh * a.v.sh;
   GroupStage<D> stage;
   stage.init(lane, (uint32_t)a.k.st, (uint32_t)a.v.st);
   auto issue = [&](int t, int buf) FA_INLINE {
-    if (t >= turns || key_of(t) >= c1) return;
+    if (t * TEAMS + team >= n_tiles) return;
     const int r0 = min(key_of(t) + 16 * wave, c1 - 1);
     const uint32_t dst = base + buf * TB + wave * 16 * ROWB;
     stage.copy(kh + r0 * a.k.st, vh + r0 * a.v.st, dst, dst + 2 * TB, c1 - 1 - r0, (uint32_t)a.k.st,
@@ -104,8 +110,8 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
   const int whole0 = keys.all_lo <= c0 ? 0 : (int)min((uint32_t)n_tiles, ((uint32_t)(keys.all_lo - c0) + 63) / 64);
   const int whole1 = min(n_tiles, max(keys.all_hi - c0, 0) / 64);
   auto turns_to = [&](int tiles) FA_INLINE { return (max(tiles - team, 0) + TEAMS - 1) / TEAMS; };
-  const int turn1 = turns_to(whole1);
-  masked(turns_to(whole0));
+  const int turn1 = turns_to(down ? n_tiles - whole0 : whole1);
+  masked(turns_to(down ? n_tiles - whole1 : whole0));
   for (; t < turn1; ++t, buf ^= 1) {
     issue(t + 1, buf ^ 1);
     w.template step<0, kWhole>(key_of(t), 15u, buf * TB);

@@ -203,7 +203,13 @@ struct WaveAttn {
         for (int kb = 0; kb < NKB; ++kb)
           mx = max3(mx, max3(s[kb][rb][0], s[kb][rb][1], s[kb][rb][2]), s[kb][rb][3]);
         mx = red_max(mx);
-        const bool grow = mx > m[rb];
+        bool grow = mx > m[rb];
+        if constexpr (SCORED) {
+          // (only a row's own sums: no bit of it goes by the rows beside it)
+          const int own = !(tsum[rb] < kSumLimit);
+          const int pair = own | __shfl_xor(own, 16);
+          grow = grow && (pair | __shfl_xor(pair, 32)) != 0;
+        }
         const float m_new = grow ? mx + kHeadroom<BF16> / c : m[rb];
         const float alpha = fast_exp2(grow ? (m[rb] - m_new) * c : 0.0f);
         m[rb] = m_new;

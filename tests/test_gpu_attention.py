@@ -388,6 +388,21 @@ def test_what_autograd_is_owed(fa):
         o.sum().backward()
 
 
+@pytest.mark.parametrize("H", [2, 150])
+@pytest.mark.parametrize("D,opt", [(64, {}), (128, dict(softcap=30.0)), (64, dict(window=150)), (128, dict(biased=True))])
+def test_no_bit_of_a_row_goes_by_other_rows(fa, H, D, opt):
+    """The rows beside it have scores that raise their offsets again and again."""
+    print("case alone", H, D, opt, flush=True)
+    g = torch.Generator(device=DEV).manual_seed(31)
+    q, k, v = (torch.randn(1, H, 300, D, generator=g, device=DEV).half() for _ in range(3))
+    opt = dict(opt)
+    if opt.pop("biased", False):
+        opt["slopes"] = torch.rand(H, generator=g, device=DEV) * 0.2
+    loud = q * torch.where(torch.arange(300, device=DEV) % 3 == 0, 1.0, 40.0).half()[:, None]
+    a, b = (fa.attention(x, k, v, return_lse=True, **opt) for x in (q, loud))
+    assert torch.equal(a[0][:, :, ::3], b[0][:, :, ::3]) and torch.equal(a[1][:, :, ::3], b[1][:, :, ::3])
+
+
 def test_splits_of_the_rows_and_long_keys(fa):
     """Few keys and many rows are split over workgroups whose parts are joined in order."""
     print("case splits", flush=True)
