@@ -388,6 +388,59 @@ def test_what_autograd_is_owed(fa):
         o.sum().backward()
 
 
+@pytest.mark.parametrize("D,dt", [(64, torch.float16), (128, torch.bfloat16)])
+def test_offsets_past_32_bits(fa, D, dt):
+    """Rows 8 MiB apart: the last ones of each tensor are 5 GiB behind the first."""
+    print("case far", D, flush=True)
+    g = torch.Generator(device=DEV).manual_seed(33)
+    N, apart = 700, 1 << 22
+
+    def far():
+        x = torch.empty(N * apart, dtype=dt, device=DEV).as_strided((1, 1, N, D), (N * apart, N * apart, apart, 1))
+        return x.copy_(torch.randn(1, 1, N, D, generator=g, device=DEV).to(dt))
+
+    q, k, v, go = (far() for _ in range(4))
+    near = [x.contiguous() for x in (q, k, v, go)]
+    assert q.stride(2) == apart and near[0].stride(2) == D
+    got = []
+    for a, b, c, d in ((q, k, v, go), near):
+        o, lse = fa.attention(a, b, c, causal=True, return_lse=True)
+        got.append((o, lse, *fa.attention_backward(d, a, b, c, o, lse, causal=True)))
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+
+
+def test_other_documents_in_a_replayed_graph(fa):
+    """Enough tiles that they are ranked by their work, whose order then changes between replays."""
+    print("case documents in a graph", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(34)
+    B, H, N, D = 2, 40, 1000, 64
+    q, k, v, go = (torch.randn(B, H, N, D, generator=g, device=DEV).half() for _ in range(4))
+    ends = [[0, 100, 1000], [0, 900, 950, 1000], [0, 333, 700, 990]]
+    ranges = [fa.document_ranges(torch.tensor(e, device=DEV), N) for e in ends]
+
+    def step(r):
+        o, lse = fa.attention(q, k, v, r, return_lse=True)
+        return (o, lse, *fa.attention_backward(go, q, k, v, o, lse, r))
+
+    want = [step(r) for r in ranges]
+    r = ranges[0].clone()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(r)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(r)
+    for i in (1, 2, 0, 1):
+        r.copy_(ranges[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want[i])), i
+        step(ranges[i])
+
+
 @pytest.mark.parametrize("H", [2, 150])
 @pytest.mark.parametrize("D,opt", [(64, {}), (128, dict(softcap=30.0)), (64, dict(window=150)), (128, dict(biased=True))])
 def test_no_bit_of_a_row_goes_by_other_rows(fa, H, D, opt):
