@@ -35,6 +35,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "fa_cache_kernels.h"
 #include "fa_device_ops.h"
@@ -360,11 +361,23 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const char* kbase = a.k + kvh * a.k_sh;
   const char* vbase = a.v + kvh * a.v_sh;
   const int last = c1 - 1;
-  PageIds ids;
+  // With a bias by distance from the last tile to the first: a causal row's scores
+  // grow towards it, and the first of them would be raised over tile by tile (4096 tokens
+  // over 16384 keys, 32 heads on 8, D = 128, bf16, us: 1280 and 868).
+  const bool down = SCORED && w.score.biased;
+  auto key_of = [&](int t) FA_INLINE { return c0 + 64 * (down ? n_tiles - 1 - t : t); };
+  std::conditional_t<SCORED, PageIdsBoth, PageIds> ids;
+  auto start_ids = [&]() FA_INLINE {
+    const int32_t* row = a.pt.table + b * a.pt.table_stride;
+    if constexpr (SCORED)
+      ids.start(a.pt, row, c0, n_tiles, down);
+    else
+      ids.start(a.pt, row, c0);
+  };
   // Stages this wave's 16-key group of tile t; returns which of the tile's four
   // groups have a page.
   auto issue = [&](int t, int buf) FA_INLINE -> unsigned {
-    const int key = c0 + 64 * t;
+    const int key = key_of(t);
     ids.reach(key);
     const int r0 = min(key + 16 * wave, last & ~15);
     const int64_t page = ids.page(r0);
@@ -377,7 +390,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   };
   unsigned present = 0, present_next = 0;
   if (n_tiles > 0) {
-    ids.start(a.pt, a.pt.table + b * a.pt.table_stride, c0);
+    start_ids();
     present = issue(0, 0);
   }
   const char* qh = a.q + s.q0 * a.q_st + (int64_t)kvh * a.group * a.q_sh;
@@ -414,19 +427,20 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   // rest: masked tiles are the last ones, or lie on absent pages.  Every wave
   // passes one barrier per tile, whichever loop it is in.
   auto whole = [&](int t) FA_INLINE {
-    return c0 + 64 * t + 64 <= full_end && (!SCORED || c0 + 64 * t >= full_start) && present == 15u;
+    return key_of(t) + 64 <= full_end && (!SCORED || key_of(t) >= full_start) && present == 15u;
   };
   int t = 0, buf = 0;
   // (a window's masked tiles are the first ones too)
-  for (; SCORED && t < n_tiles && !whole(t) && c0 + 64 * t < full_start; ++t, buf ^= 1) {
+  auto before_whole = [&](int t) FA_INLINE { return down ? key_of(t) + 64 > full_end : key_of(t) < full_start; };
+  auto seen = [&](int t) FA_INLINE { return key_of(t) < wave_end && (!SCORED || key_of(t) + 64 > wave_start); };
+  for (; SCORED && t < n_tiles && !whole(t) && before_whole(t); ++t, buf ^= 1) {
     stage_next(t, buf);
-    if (c0 + 64 * t < wave_end && c0 + 64 * t + 64 > wave_start)
-      w.template step<0, kMasked>(c0 + 64 * t, present, buf * TB, base + (2 + buf) * TB);
+    if (seen(t)) w.template step<0, kMasked>(key_of(t), present, buf * TB, base + (2 + buf) * TB);
     end_tile();
   }
   for (; SCORED && t < n_tiles && whole(t); ++t, buf ^= 1) {
     stage_next(t, buf);
-    w.template step<0, kWhole>(c0 + 64 * t, present, buf * TB);
+    w.template step<0, kWhole>(key_of(t), present, buf * TB);
     end_tile();
   }
   for (; !SCORED && t < n_tiles && whole(t); ++t) {
@@ -443,8 +457,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   }
   for (; t < n_tiles; ++t, buf ^= 1) {
     stage_next(t, buf);
-    if (c0 + 64 * t < wave_end)
-      w.template step<0, kMasked>(c0 + 64 * t, present, buf * TB, base + (2 + buf) * TB);
+    if (seen(t)) w.template step<0, kMasked>(key_of(t), present, buf * TB, base + (2 + buf) * TB);
     end_tile();
   }
   // Infinities or NaN in a masked tile of some wave: all start again (the
@@ -453,14 +466,14 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   __syncthreads();
   if (__builtin_expect(__builtin_amdgcn_readfirstlane(again) != 0, false)) {
     w.reset();
-    ids.start(a.pt, a.pt.table + b * a.pt.table_stride, c0);
+    start_ids();
     present = issue(0, 0);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     buf = 0;
     for (t = 0; t < n_tiles; ++t, buf ^= 1) {
       stage_next(t, buf);
-      if (c0 + 64 * t < wave_end) w.template step<0, kSafe>(c0 + 64 * t, present, buf * TB);
+      if (seen(t)) w.template step<0, kSafe>(key_of(t), present, buf * TB);
       end_tile();
     }
   }

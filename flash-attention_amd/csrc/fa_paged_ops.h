@@ -131,6 +131,32 @@ struct PageIds {
   }
 };
 
+// The same in either direction.
+struct PageIdsBoth : PageIds {
+  int step;  // 1024, or -1024
+  __device__ __forceinline__ int load_at(int key0) const {
+    return row[max(min(key0 + 16 * (int)(threadIdx.x & 63), limit), 0) >> shift];
+  }
+  // Of keys c0 .. c0 + 64 tiles - 1, tile by tile from the first, or `down` from the last.
+  __device__ __forceinline__ void start(const PageTable& pt, const int32_t* r, int c0, int tiles, bool down) {
+    row = r;
+    limit = max(pt.max_kv - 1, 0);
+    shift = pt.page_shift;
+    step = down ? -1024 : 1024;
+    const int key0 = down ? c0 + (tiles - 1) / 16 * 1024 : c0;
+    base = key0 - step;
+    pages = (uint32_t)pt.num_pages;
+    next = load_at(key0);
+  }
+  __device__ __forceinline__ void reach(int key) {
+    if ((uint32_t)(key - base) < 1024) return;
+    base += step;
+    cur = next;
+    there = __ballot((uint32_t)cur < pages);
+    next = load_at(base + step);
+  }
+};
+
 // Row tiles of the chunk kernel, the longest first: sequence and tile of the
 // n-th one, and how many there are.
 //
