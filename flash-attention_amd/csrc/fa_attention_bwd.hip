@@ -30,7 +30,8 @@
 //
 // Masked keys and rows contribute nothing whatever they hold: their P and dS are
 // 0, and infinities and NaN among the staged rows of a tile that is not seen
-// whole are cleared (clean_rows); rows and keys that do see one get NaN.
+// whole are cleared (clean_rows); rows and keys that do see one get NaN, also those
+// of a wave whose own part of the tile is seen whole.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -478,9 +479,10 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
   finish(now, 0, false);  // (what was loaded so far: no wait for it later, which would be one for copies too)
 
   Grads<CAP> grads;
-  // A span in `slot`.  (Scores become P in place, dS takes the place of go V^T: the
+  // A span in `slot`; `masked`: some row does not see all of the wave's keys, `cleaned`: of
+  // the workgroup's (finish).  (Scores become P in place, dS takes the place of go V^T: the
   // accumulators leave few registers, none to keep addresses across spans.)
-  auto step = [&](int row0, uint32_t slot, bool masked) FA_INLINE {
+  auto step = [&](int row0, uint32_t slot, bool masked, bool cleaned) FA_INLINE {
     const int l = lane_now();
     const int key0 = w0 + (l & 15);
     const uint32_t tile = base + slot * SLOT;
@@ -495,7 +497,7 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
       const int away = row0 + 16 * rb + 4 * (l >> 4) + a.m - a.n - key0;  // of key block 0
       auto away_of = [&](int cb, int i) FA_INLINE { return (float)(away - 16 * cb) + (float)i; };
       f32x4 lse = lds_quad(quad + 64 * kLse);
-      if (masked) {
+      if (cleaned) {
         const uint32_t bad = spoiled_at + slot * 2 * kSpan * 4 + rb * 64 + (l >> 4) * 16;
         lse += lds_quad(bad) + lds_quad(bad + kSpan * 4);
       }
@@ -573,7 +575,7 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
         head = now.head;
         grads.init(a, h0 + head);
       }
-      step(now.at() * kSpan, slot, !now.whole());
+      step(now.at() * kSpan, slot, !now.whole(), !now.all());
     }
     slot = (slot + 1) % SLOTS;
     finish(then, slot, last.is());
