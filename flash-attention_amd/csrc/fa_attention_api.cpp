@@ -43,13 +43,12 @@ int64_t grid_size(const GridOrder& o) {
   return (int64_t)o.units * o.places;
 }
 
-AttnBwdPlan plan_attn_bwd(const AttnArgs& a, int head_dim, int compute_units) {
+AttnBwdPlan plan_attn_bwd(const AttnArgs& a, int head_dim, bool bf16, int compute_units) {
   AttnBwdPlan p = {};
   const int64_t bh = (int64_t)a.batch * a.heads;
-  // (a record is staged with the 512 bytes behind it)
-  p.records = (uint64_t)bh * a.spans * kSpan * 16 + 512;
+  // (1 KiB from a record's start is staged, at most 512 bytes behind it)
+  p.records = (uint64_t)bh * a.spans * record_floats(bf16) * 4 + 512;
   p.bounds = (uint64_t)a.batch * a.spans * 16;
-  p.tops = ((uint64_t)bh * a.spans * 4 + 15) / 16 * 16;
   const int64_t tiles = (int64_t)a.batch * a.kv_heads * a.key_tiles;
   // Teams where a CU has one workgroup at most; or two of different lengths, which a
   // team more evens out (D = 128, us with one and with teams: 16 causal heads of 4096 rows 206
@@ -148,14 +147,14 @@ fa_status bwd_plan(const fa_attn_bwd_params& p, AttnArgs* args, AttnBwdPlan* pla
   int cus = 0;
   FA_TRY(current_compute_units(&cus));
   *args = attn_args(p.fwd, cus);
-  *plan = plan_attn_bwd(*args, p.fwd.head_dim, cus);
+  *plan = plan_attn_bwd(*args, p.fwd.head_dim, p.fwd.dtype == FA_DTYPE_BF16, cus);
   args->splits = plan->splits;
   args->cols = grid_order(args->batch * args->kv_heads, args->key_tiles * plan->splits, cus, plan->teams == 1 ? 2 : 1);
   args->key_teams = plan->teams;
   return FA_OK;
 }
 
-uint64_t total(const AttnBwdPlan& p) { return p.records + p.bounds + p.tops + p.parts + p.order; }
+uint64_t total(const AttnBwdPlan& p) { return p.records + p.bounds + p.parts + p.order; }
 
 }  // namespace
 }  // namespace fa
@@ -223,8 +222,7 @@ fa_status fa_attn_bwd(const fa_attn_bwd_params* p, void* workspace, uint64_t wor
   char* ws = static_cast<char*>(workspace);
   a.records = reinterpret_cast<float*>(ws);
   a.bounds = reinterpret_cast<int32_t*>(ws + plan.records);
-  a.tops = reinterpret_cast<float*>(ws + plan.records + plan.bounds);
-  ws += plan.records + plan.bounds + plan.tops;
+  ws += plan.records + plan.bounds;
   a.parts = plan.parts > 0 ? reinterpret_cast<float*>(ws) : nullptr;
   a.key_order = plan.order > 0 ? reinterpret_cast<int32_t*>(ws + plan.parts) : nullptr;
   a.by_splits = make_fast_div((uint32_t)a.splits);

@@ -26,7 +26,9 @@
 // Rounding: P and dS are rounded to the input type for the matrix cores (as P of
 // the forward pass); all sums are fp32.  fp16 has few exponents: P is scaled by
 // 2^12, so that it keeps its 11 bits down to 2^-26, and dS by a power of two that brings
-// the largest |go| (of the rows of a dk, dv workgroup; of a dq row) to 2^-12 .. 2^-11.
+// the largest |go| to 2^-12 .. 2^-11: of a dq row, and of the rows so far that see a key.  (Of all
+// rows of the head: a row that does not see a key, of another document or before it, would
+// decide what is left of that key's sums.)
 //
 // Masked keys and rows contribute nothing whatever they hold: their P and dS are
 // 0, and infinities and NaN among the staged rows of a tile that is not seen
@@ -50,10 +52,16 @@ constexpr float kShift = BF16 ? 0.0f : 12.0f;  // log2 of P's factor
 
 // The record of a span, [2][4 fields][16 rows] floats: for each 16 rows
 enum RecordField { kLse, kDelta, kLo, kHi };  // (lse in log2, less kShift and the cap; minus delta)
+// fp16: then the largest |go| of each row that is finite, and of all of them.
+constexpr int kRowTops = 4 * kSpan, kSpanTop = kRowTops + kSpan;
+template <bool BF16>
+constexpr int kRecord = record_floats(BF16);
 // dS is made with a quarter of capped scores' derivative, 1 - tanh^2 = 4 tail (1 - tail).
 template <bool CAP>
 constexpr float kQuarters = CAP ? 4.0f : 1.0f;
-constexpr int kRecord = kSpan * 4;
+// Such a factor's product with the largest |go| is below this.
+template <bool CAP>
+constexpr float kFactorMost = 0x1p-11f * kQuarters<CAP>;
 
 // 2^-(e + 12) for a largest |go| in [2^e, 2^(e + 1)): dS's factor.  1 for bf16.
 template <bool BF16>
@@ -123,13 +131,16 @@ __global__ void __launch_bounds__(256) fa_attn_rows_kernel(const AttnArgs a) {
   TileKeys t;
   t.start(k);
   t.reduce<kSpan>();
+  // (infinities: the results of the keys that see them are no numbers, whatever the factor)
+  float all = most = most < INFINITY ? most : 0.0f;
   if constexpr (!BF16) {
 #pragma unroll
-    for (int w = 1; w < kSpan; w <<= 1) most = fmaxf(most, __shfl_xor(most, w));
+    for (int w = 1; w < kSpan; w <<= 1) all = fmaxf(all, __shfl_xor(all, w));
   }
   if (span >= a.spans) return;
-  const int64_t bhs = (int64_t)bh * a.spans + span;
-  float* rec = a.records + bhs * kRecord + (r % kSpan >> 4) * 64 + (r & 15);
+  float* record = a.records + ((int64_t)bh * a.spans + span) * kRecord<BF16>;
+  if constexpr (!BF16) record[kRowTops + r % kSpan] = most;
+  float* rec = record + (r % kSpan >> 4) * 64 + (r & 15);
   rec[16 * kLse] = lse;
   rec[16 * kDelta] = d;
   rec[16 * kLo] = __builtin_bit_cast(float, k.lo);
@@ -137,7 +148,7 @@ __global__ void __launch_bounds__(256) fa_attn_rows_kernel(const AttnArgs a) {
   if (r % kSpan != 0) return;
   if (h == 0)
     reinterpret_cast<int4*>(a.bounds)[(int64_t)b * a.spans + span] = int4{t.lo, t.hi, t.all_lo, t.all_hi};
-  if constexpr (!BF16) a.tops[bhs] = most;
+  if constexpr (!BF16) record[kSpanTop] = all;
 }
 
 // ---- the order of the tiles of keys ----
@@ -317,8 +328,11 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
   constexpr int PART = 2 * DB * 1024;  // bytes of a wave's sums
   constexpr int RINGS = TEAMS * SLOTS * SLOT, SUMS = (TEAMS - 1) * 2 * 4 * PART;
   __shared__ __attribute__((aligned(1024))) char smem[RINGS > SUMS ? RINGS : SUMS];
-  __shared__ float spoiled[TEAMS][SLOTS][2][kSpan];  // NaN for rows of Q, of go with an infinity or NaN, else 0
-  __shared__ float top_part[4 * TEAMS];
+  __shared__ __attribute__((aligned(16))) struct {
+    float spoiled[SLOTS][2][kSpan];  // NaN for rows of Q, of go with an infinity or NaN, else 0
+    // of a wave's keys: dS's factor, by the largest |go| so far of the rows that see one; the largest of them
+    float factor[BF16 ? 0 : 4][32], largest[BF16 ? 0 : 4];
+  } aside[TEAMS];
 
   const int lane = threadIdx.x & 63;
   const int team = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
@@ -388,7 +402,7 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
   const Rows3& sx = of_go ? a.go : a.q;
   const uint32_t sst = (uint32_t)sx.st, sto = (of_go ? TB : 0) + sr * ROWB;
   const char* sp = sx.p + b * sx.sb + h0 * sx.sh + sr * (int64_t)sst;  // of the head to come
-  const char* records = reinterpret_cast<const char*>(a.records + ((int64_t)b * a.heads + h0) * spans * kRecord);
+  const char* records = reinterpret_cast<const char*>(a.records + ((int64_t)b * a.heads + h0) * spans * kRecord<BF16>);
   const int64_t head_step = sx.sh;
   const int row_end = a.n - 1 - sr;
   int staged_head = 0;
@@ -396,7 +410,7 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
   auto issue = [&](const Span& x, uint32_t slot) FA_INLINE {
     for (; staged_head < x.head; ++staged_head) {
       sp += head_step;
-      records += (int64_t)spans * (kRecord * 4);
+      records += (int64_t)spans * (kRecord<BF16> * 4);
     }
     const int row = x.at() * kSpan;  // (less sr)
     const uint32_t dst = base + slot * SLOT + sto;
@@ -418,12 +432,12 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
     }
     if (wave == 0) {  // (1 KiB: the next record too, or what is behind the last one)
       poison_1k(base + slot * SLOT + 2 * TB);
-      dma_16b(lane_now() * 16, records + (int64_t)x.at() * (kRecord * 4), base + slot * SLOT + 2 * TB);
+      dma_16b(lane_now() * 16, records + (int64_t)x.at() * (kRecord<BF16> * 4), base + slot * SLOT + 2 * TB);
     }
   };
   // The copies of a span are there, `later`: but for those of one issued after it.
   // If the span is not seen whole, this wave cleans the rows that it has copied.
-  const uint32_t spoiled_at = __builtin_amdgcn_readfirstlane(lds_addr(spoiled)) + team * SLOTS * 2 * kSpan * 4;
+  const uint32_t spoiled_at = __builtin_amdgcn_readfirstlane(lds_addr(aside)) + team * (int)sizeof(aside[0]);
   auto finish = [&](const Span& x, uint32_t slot, bool later) FA_INLINE {
     if (!later)
       wait_vmcnt<0>();
@@ -463,22 +477,52 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
       vf[cb][st] = *reinterpret_cast<const i16x8*>(vp + 64 * st);
     }
   }
-  float factor = 1.0f;
+  // (each wave its own keys', in its order: no barrier)
+  auto factor_at = [&](int l) FA_INLINE { return spoiled_at + SLOTS * 2 * kSpan * 4 + (w0 & 96) * 4 + l * 4; };
+  auto largest_at = [&]() FA_INLINE { return spoiled_at + (SLOTS * 2 * kSpan + 4 * 32) * 4 + (w0 & 96) / 8; };
   if constexpr (!BF16) {
-    float top = 0.0f;
-    const float* tops = a.tops + ((int64_t)b * a.heads + h0) * a.spans;
-    for (int64_t i = threadIdx.x; i < (int64_t)a.group * a.spans; i += 256 * TEAMS) top = fmaxf(top, tops[i]);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if (lane == 0) top_part[threadIdx.x / 64] = top;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4 * TEAMS; ++i) top = fmaxf(top, top_part[i]);
-    factor = uniform(kQuarters<CAP> * grad_factor<BF16>(uniform(top)));
+    constexpr float first = kFactorMost<CAP> * 0x1p23f;  // (no |go| but 0 is below 2^-24)
+    lds_write4(lane < 32 ? factor_at(lane) : largest_at(), first);
   }
   finish(now, 0, false);  // (what was loaded so far: no wait for it later, which would be one for copies too)
 
   Grads<CAP> grads;
+  // fp16: new factors of dS where rows that see a key have a larger |go| than those before, also for
+  // what its sum holds.
+  auto fit = [&](uint32_t record, bool masked) FA_INLINE {
+    const int l = lane_now(), key0 = w0 + (l & 15);
+    const uint32_t at = factor_at(l & 15);
+    float largest = 0.0f;
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) {
+      float top = lds_read4(record + 4 * kSpanTop);
+      if (masked) {
+        top = 0.0f;
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+          const uint32_t quad = record + rb * 256 + (l >> 4) * 16;
+          const i32x4 lo = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kLo)) - key0;
+          const i32x4 hi = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kHi)) - key0;
+          const f32x4 of_row = lds_quad(record + 4 * kRowTops + rb * 64 + (l >> 4) * 16);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, 16 * cb >= lo[i] && 16 * cb < hi[i] ? of_row[i] : 0.0f);
+        }
+        top = fmaxf(top, from_lane(top, lane_now() ^ 16));
+        top = fmaxf(top, from_lane(top, lane_now() ^ 32));
+      }
+      const float factor = lds_read4(at + 64 * cb);
+      const float to = top * factor >= kFactorMost<CAP> ? kQuarters<CAP> * grad_factor<BF16>(top) : factor;
+      // (their ratio: powers of two)
+      const float change = __builtin_bit_cast(float, __builtin_bit_cast(int, to) - __builtin_bit_cast(int, factor) + 0x3f800000);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) gk[db][cb] *= change;
+      lds_write4(at + 64 * cb, to);
+      largest = fmaxf(largest, to);
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) largest = fmaxf(largest, from_lane(largest, lane_now() ^ d));
+    lds_write4(largest_at(), largest);
+  };
   // A span in `slot`; `masked`: some row does not see all of the wave's keys, `cleaned`: of
   // the workgroup's (finish).  (Scores become P in place, dS takes the place of go V^T: the
   // accumulators leave few registers, none to keep addresses across spans.)
@@ -487,6 +531,11 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
     const int key0 = w0 + (l & 15);
     const uint32_t tile = base + slot * SLOT;
     u32x4 pw[2], dw[2];  // P and dS as packed pairs: words 0, 1 of rows 4 (l / 16) .., 2, 3 of those 16 on
+    float top = 0.0f, largest = 0.0f;  // (read ahead of the first product)
+    if constexpr (!BF16) {
+      top = lds_read4(tile + 2 * TB + 4 * kSpanTop);
+      largest = lds_read4(largest_at());
+    }
     static_for<0, 2>([&](auto rb_c) FA_INLINE {
       constexpr int rb = decltype(rb_c)::value;
       const uint32_t rows = tile + rb * 16 * ROWB + lds::TileBoth<D>::row_offset(l);
@@ -494,6 +543,8 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
       f32x4 c[2], e[2];
       const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
       row_product<D, BF16, 2>(rows, kf, zero, c, [](auto) FA_INLINE {});
+      if constexpr (!BF16 && rb == 0)
+        if (__any(top * largest >= kFactorMost<CAP>)) fit(tile + 2 * TB, masked);
       const int away = row0 + 16 * rb + 4 * (l >> 4) + a.m - a.n - key0;  // of key block 0
       auto away_of = [&](int cb, int i) FA_INLINE { return (float)(away - 16 * cb) + (float)i; };
       f32x4 lse = lds_quad(quad + 64 * kLse);
@@ -507,8 +558,16 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
 #pragma unroll
           for (int i = 0; i < 4; ++i) c[cb][i] = grads.biased(c[cb][i], away_of(cb, i));
       // The exponentials, or the first ones of capped scores, beside go V^T.
+      float factor[2];  // (read late: registers)
+      auto read_factor = [&]() FA_INLINE {
+        if constexpr (BF16) return;
+        const uint32_t at = factor_at(lane_now() & 15);
+        factor[0] = lds_read4(at);
+        factor[1] = lds_read4(at + 64);
+      };
       row_product<D, BF16, 2>(rows + TB, vf, lds_quad(quad + 64 * kDelta), e, [&](auto i_c) FA_INLINE {
         constexpr int PART = 8 / KST;
+        if constexpr (!CAP && decltype(i_c)::value == KST - 1) read_factor();
 #pragma unroll
         for (int j = 0; j < PART; ++j) {
           const int at = decltype(i_c)::value * PART + j;
@@ -530,6 +589,7 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
           for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
             for (int i = 0; i < 4; ++i) c[cb][i] = grads.biased(c[cb][i], away_of(cb, i));
+        read_factor();
 #pragma unroll
         for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
@@ -538,7 +598,7 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
 #pragma unroll
       for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[cb][i] *= BF16 ? c[cb][i] : c[cb][i] * factor;
+        for (int i = 0; i < 4; ++i) e[cb][i] *= BF16 ? c[cb][i] : c[cb][i] * factor[cb];
       if (masked) {
         const i32x4 lo = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kLo)) - key0;
         const i32x4 hi = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kHi)) - key0;
@@ -585,6 +645,16 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
     then_any = last_any;
   }
 
+  // (powers of two but for the scale)
+  if constexpr (!BF16) {
+    const uint32_t at = factor_at(lane_now() & 15);
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) {
+      const float back = 1.0f / lds_read4(at + cb * 64);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) gk[db][cb] *= back;
+    }
+  }
   // The first team takes all of gk, the second all of gv, by wave and lane.
   if constexpr (TEAMS > 1) {
     const uint32_t at = lds_addr(smem) + wave * PART + lane * 16;
@@ -601,10 +671,9 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
   }
   const bool has_k = TEAMS == 1 || team == 0, has_v = TEAMS == 1 || team == 1;
 
-  // (powers of two but for the scale)
   const auto& x = late_args();
   const float fv[2] = {fast_exp2(-kShift<BF16>), fast_exp2(-kShift<BF16>)};
-  const float scale = kQuarters<CAP> * x.scale * fv[0] / factor, fk[2] = {scale, scale};
+  const float scale = kQuarters<CAP> * x.scale * fv[0], fk[2] = {scale, scale};
   const int l = lane_now(), m = x.m;
   if (x.parts != nullptr) {
     const int64_t rows = (int64_t)x.batch * x.kv_heads * m;
@@ -707,7 +776,7 @@ __global__ void __launch_bounds__(256 * TEAMS)
       qf[rb][st] = *reinterpret_cast<const i16x8*>(qp + 64 * st);
       gf[rb][st] = *reinterpret_cast<const i16x8*>(gp + 64 * st);
     }
-    const float* rec = a.records + (((int64_t)b * a.heads + h) * a.spans + r / kSpan) * kRecord +
+    const float* rec = a.records + (((int64_t)b * a.heads + h) * a.spans + r / kSpan) * kRecord<BF16> +
                        r % kSpan / 16 * 64 + r % 16;
     lse[rb] = rec[16 * kLse];
     delta[rb] = rec[16 * kDelta];

@@ -41,9 +41,8 @@ struct AttnArgs {
   // backward
   Rows3 go, gq, gk, gv;     // gradients of o, q, k, v
   const float* glse;        // of lse; may be NULL
-  float* records;           // [batch, heads, spans][2][4][16], see fa_attention_bwd.hip
+  float* records;           // [batch, heads, spans][record_floats], see fa_attention_bwd.hip
   int32_t* bounds;          // [batch, spans][4]: limits of a span's rows
-  float* tops;              // [batch, heads, spans]: largest |go|
   int32_t spans;            // spans of kSpan rows
   int32_t key_tiles, splits;
   FastDiv by_splits;
@@ -60,13 +59,16 @@ constexpr int kMaxOrdered = 1024;  // tiles of keys that key_order ranks
 // Teams of a workgroup of few: as many as fill a CU.
 constexpr int key_teams(int head_dim) { return head_dim == 128 ? 2 : 3; }
 
+// Of the record of a span: four of each row, and with fp16 one more, one of all and filling.
+constexpr int record_floats(bool bf16) { return bf16 ? 4 * kSpan : 5 * kSpan + 4; }
+
 struct AttnBwdPlan {
   int32_t teams, splits;
-  uint64_t records, bounds, tops, parts, order;  // bytes, each a multiple of 16
+  uint64_t records, bounds, parts, order;  // bytes, each a multiple of 16
 };
 GridOrder grid_order(int units, int places, int compute_units, int per_cu);
 int64_t grid_size(const GridOrder& o);
-AttnBwdPlan plan_attn_bwd(const AttnArgs& a, int head_dim, int compute_units);
+AttnBwdPlan plan_attn_bwd(const AttnArgs& a, int head_dim, bool bf16, int compute_units);
 
 hipError_t launch_attn_fwd(const AttnArgs& args, int head_dim, bool bf16, hipStream_t stream);
 hipError_t launch_attn_bwd(const AttnArgs& args, int head_dim, bool bf16, hipStream_t stream);

@@ -131,6 +131,11 @@ __device__ __forceinline__ int lane_now() {
   return l;
 }
 
+// x of lane l.  (__shfl_xor keeps the lane in a register.)
+__device__ __forceinline__ float from_lane(float x, int l) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(4 * l, __builtin_bit_cast(int, x)));
+}
+
 // Staging of 16 rows of a tensor into LDS in the layout of lds::TileBoth.
 template <int D>
 struct RowStage {
@@ -165,6 +170,9 @@ __device__ __forceinline__ void lds_write8(uint32_t addr, u32x2 w) {
 }
 __device__ __forceinline__ f32x4 lds_quad(uint32_t addr) {
   return __builtin_bit_cast(f32x4, lds_read16<0>(addr));
+}
+__device__ __forceinline__ float lds_read4(uint32_t addr) {
+  return *(__attribute__((address_space(3))) const float*)(uintptr_t)addr;
 }
 __device__ __forceinline__ void lds_write4(uint32_t addr, float x) {
   *(__attribute__((address_space(3))) float*)(uintptr_t)addr = x;
