@@ -25,10 +25,15 @@
 //
 // Rounding: P and dS are rounded to the input type for the matrix cores (as P of
 // the forward pass); all sums are fp32.  fp16 has few exponents: P is scaled by
-// 2^12, so that it keeps its 11 bits down to 2^-26, and dS by a power of two that brings
-// the largest |go| to 2^-12 .. 2^-11: of a dq row, and of the rows so far that see a key.  (Of all
-// rows of the head: a row that does not see a key, of another document or before it, would
-// decide what is left of that key's sums.)
+// 2^12, so that it keeps its 11 bits down to 2^-26, and dS by a power of two, by what bounds it:
+//   |dS_ij| <= |go_i| |v_j| + |delta_i|   (P and the derivative are at most 1; |.|: 2-norms)
+//  * dk: a key's rows so far that see it; the bound goes to 2^12 .. 2^13 and may grow to 2^15
+//    before the factor and the sum so far are lowered.  (Of all rows of the head: a row that does
+//    not see the key, of another document or before it, would decide what is left of its sums.)
+//  * dq: a row's bound for |v| up to 64, at 2^12 .. 2^13 too.  Should a sum be no number all the
+//    same, the rows start again with that for the largest |v| that there is, 2^20.  (The largest
+//    dS is then above 2: what is lost is below 2^-26 of it.)
+// What dS loses to the type's least step, 2^-25, is below 2^-37 of the bound.
 //
 // Masked keys and rows contribute nothing whatever they hold: their P and dS are
 // 0, and infinities and NaN among the staged rows of a tile that is not seen
@@ -52,24 +57,22 @@ constexpr float kShift = BF16 ? 0.0f : 12.0f;  // log2 of P's factor
 
 // The record of a span, [2][4 fields][16 rows] floats: for each 16 rows
 enum RecordField { kLse, kDelta, kLo, kHi };  // (lse in log2, less kShift and the cap; minus delta)
-// fp16: then the largest |go| of each row that is finite, and of all of them.
-constexpr int kRowTops = 4 * kSpan, kSpanTop = kRowTops + kSpan;
+// fp16: then |go| of each row, and the largest |go| and |delta| of all; 0 in place of infinities and NaN,
+// for whose rows and keys no factor helps.
+constexpr int kRowNorms = 4 * kSpan, kSpanMost = kRowNorms + kSpan;
 template <bool BF16>
 constexpr int kRecord = record_floats(BF16);
 // dS is made with a quarter of capped scores' derivative, 1 - tanh^2 = 4 tail (1 - tail).
 template <bool CAP>
 constexpr float kQuarters = CAP ? 4.0f : 1.0f;
-// Such a factor's product with the largest |go| is below this.
+// The largest product of a factor (which holds these, and P's 2^-12) with the bound of dS.
 template <bool CAP>
-constexpr float kFactorMost = 0x1p-11f * kQuarters<CAP>;
-
-// 2^-(e + 12) for a largest |go| in [2^e, 2^(e + 1)): dS's factor.  1 for bf16.
-template <bool BF16>
-__device__ __forceinline__ float grad_factor(float top) {
-  if constexpr (BF16) return 1.0f;
-  const int e = (int)((__builtin_bit_cast(uint32_t, top) >> 23) & 255) - 127;
-  if (e < -24 || e > 15) return 1.0f;  // 0, or no number
-  return __builtin_bit_cast(float, (uint32_t)(127 - 12 - e) << 23);
+constexpr float kBoundMost = 8.0f * kQuarters<CAP>;
+// dS's factor for a bound in [2^e, 2^(e + 1)).
+template <bool CAP>
+__device__ __forceinline__ float grad_factor(float bound) {
+  const int e = (int)((__builtin_bit_cast(uint32_t, bound) >> 23) & 255) - 127;
+  return kQuarters<CAP> * __builtin_bit_cast(float, (uint32_t)(127 - min(max(e, -60), 100)) << 23);
 }
 
 // ---- rows ----
@@ -79,7 +82,7 @@ constexpr int kRowsBlock = 64;
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) fa_attn_rows_kernel(const AttnArgs a) {
   constexpr int LPR = D / 8, RPP = 256 / LPR;  // rows of a pass
-  __shared__ float delta[kRowsBlock], top[kRowsBlock];
+  __shared__ float delta[kRowsBlock], squares[kRowsBlock];
   const int blocks = (a.n + kRowsBlock - 1) / kRowsBlock;
   const int bh = blockIdx.x / blocks, block = blockIdx.x - bh * blocks;
   const int b = bh / a.heads, h = bh - b * a.heads;
@@ -90,7 +93,7 @@ __global__ void __launch_bounds__(256) fa_attn_rows_kernel(const AttnArgs a) {
     const int r = r0 + (int)threadIdx.x / LPR;
     const int64_t i = min(block * kRowsBlock + r, a.n - 1);
     const int at = (int)threadIdx.x % LPR * 16;
-    float g[8], o[8], sum = 0.0f, most = 0.0f;
+    float g[8], o[8], sum = 0.0f, square = 0.0f;
     unpack8<BF16>(*reinterpret_cast<const u32x4*>(gh + i * a.go.st + at), g);
     unpack8<BF16>(*reinterpret_cast<const u32x4*>(oh + i * a.o.st + at), o);
     if (a.o_low != nullptr) {
@@ -102,44 +105,46 @@ __global__ void __launch_bounds__(256) fa_attn_rows_kernel(const AttnArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       sum = fmaf(g[j], o[j], sum);
-      most = fmaxf(most, fabsf(g[j]));
+      if constexpr (!BF16) square = fmaf(g[j], g[j], square);
     }
 #pragma unroll
     for (int d = 1; d < LPR; d <<= 1) {
       sum += __shfl_xor(sum, d);
-      most = fmaxf(most, __shfl_xor(most, d));
+      if constexpr (!BF16) square += __shfl_xor(square, d);
     }
     if (threadIdx.x % LPR == 0) {
       delta[r] = sum;
-      top[r] = most;
+      squares[r] = square;
     }
   }
   __syncthreads();
   if (threadIdx.x >= kRowsBlock) return;
   const int r = threadIdx.x, i = block * kRowsBlock + r, span = i / kSpan;
   RowKeys k = {kNoKey, 0};
-  float lse = INFINITY, d = 0.0f, most = 0.0f;  // P = 0
+  float lse = INFINITY, d = 0.0f, norm = 0.0f;  // P = 0
   if (i < a.n) {
     k = row_keys(a, b, i);
     if (k.hi > 0) {
       const int64_t at = (int64_t)bh * a.n + i;
       lse = a.lse[at] * kLog2e - kShift<BF16> - a.score.cap;  // (the cap that scores leave out)
       d = (a.glse != nullptr ? a.glse[at] : 0.0f) - delta[r];
-      most = top[r];
+      norm = sqrtf(squares[r]);
     }
   }
   TileKeys t;
   t.start(k);
   t.reduce<kSpan>();
-  // (infinities: the results of the keys that see them are no numbers, whatever the factor)
-  float all = most = most < INFINITY ? most : 0.0f;
+  float most[2] = {norm < INFINITY ? norm : 0.0f, fabsf(d) < INFINITY ? fabsf(d) : 0.0f};
+  norm = most[0];
   if constexpr (!BF16) {
 #pragma unroll
-    for (int w = 1; w < kSpan; w <<= 1) all = fmaxf(all, __shfl_xor(all, w));
+    for (int w = 1; w < kSpan; w <<= 1)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) most[i] = fmaxf(most[i], __shfl_xor(most[i], w));
   }
   if (span >= a.spans) return;
   float* record = a.records + ((int64_t)bh * a.spans + span) * kRecord<BF16>;
-  if constexpr (!BF16) record[kRowTops + r % kSpan] = most;
+  if constexpr (!BF16) record[kRowNorms + r % kSpan] = norm;
   float* rec = record + (r % kSpan >> 4) * 64 + (r & 15);
   rec[16 * kLse] = lse;
   rec[16 * kDelta] = d;
@@ -148,7 +153,7 @@ __global__ void __launch_bounds__(256) fa_attn_rows_kernel(const AttnArgs a) {
   if (r % kSpan != 0) return;
   if (h == 0)
     reinterpret_cast<int4*>(a.bounds)[(int64_t)b * a.spans + span] = int4{t.lo, t.hi, t.all_lo, t.all_hi};
-  if constexpr (!BF16) record[kSpanTop] = all;
+  if constexpr (!BF16) *reinterpret_cast<float2*>(record + kSpanMost) = float2{most[0], most[1]};
 }
 
 // ---- the order of the tiles of keys ----
@@ -330,8 +335,8 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
   __shared__ __attribute__((aligned(1024))) char smem[RINGS > SUMS ? RINGS : SUMS];
   __shared__ __attribute__((aligned(16))) struct {
     float spoiled[SLOTS][2][kSpan];  // NaN for rows of Q, of go with an infinity or NaN, else 0
-    // of a wave's keys: dS's factor, by the largest |go| so far of the rows that see one; the largest of them
-    float factor[BF16 ? 0 : 4][32], largest[BF16 ? 0 : 4];
+    // of a wave's keys: dS's factors, |v|; the largest of their products, of the factors
+    float factor[BF16 ? 0 : 4][2][32], largest[BF16 ? 0 : 4][2];
   } aside[TEAMS];
 
   const int lane = threadIdx.x & 63;
@@ -478,50 +483,78 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
     }
   }
   // (each wave its own keys', in its order: no barrier)
-  auto factor_at = [&](int l) FA_INLINE { return spoiled_at + SLOTS * 2 * kSpan * 4 + (w0 & 96) * 4 + l * 4; };
-  auto largest_at = [&]() FA_INLINE { return spoiled_at + (SLOTS * 2 * kSpan + 4 * 32) * 4 + (w0 & 96) / 8; };
+  auto factor_at = [&](int l) FA_INLINE { return spoiled_at + SLOTS * 2 * kSpan * 4 + (w0 & 96) * 8 + l * 4; };
+  auto largest_at = [&]() FA_INLINE { return spoiled_at + (SLOTS * 2 * kSpan + 4 * 64) * 4 + (w0 & 96) / 4; };
   if constexpr (!BF16) {
-    constexpr float first = kFactorMost<CAP> * 0x1p23f;  // (no |go| but 0 is below 2^-24)
-    lds_write4(lane < 32 ? factor_at(lane) : largest_at(), first);
+    // (more than any bound above 2^-57 takes)
+    constexpr float first = kBoundMost<CAP> * 0x1p57f;
+    if (lane < 32) lds_write4(factor_at(lane), first);
+    lds_write8<0>(largest_at(), u32x2{__builtin_bit_cast(uint32_t, first), __builtin_bit_cast(uint32_t, first)});
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) {
+      float square = 0.0f;
+#pragma unroll
+      for (int st = 0; st < KST; ++st) {
+        const u32x4 x = __builtin_bit_cast(u32x4, vf[cb][st]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const auto pair = __builtin_bit_cast(f16x2, x[j]);
+          square = __builtin_amdgcn_fdot2(pair, pair, square, false);
+        }
+      }
+      square += from_lane(square, lane ^ 16);
+      square += from_lane(square, lane ^ 32);
+      if (lane < 16) lds_write4(factor_at(32 + 16 * cb + lane), square < INFINITY ? sqrtf(square) : 0.0f);
+    }
   }
   finish(now, 0, false);  // (what was loaded so far: no wait for it later, which would be one for copies too)
 
   Grads<CAP> grads;
-  // fp16: new factors of dS where rows that see a key have a larger |go| than those before, also for
-  // what its sum holds.
+  // fp16: new factors of dS, also for what its sum holds, where rows that see a key take its bound
+  // further than those before.  (The look at each span costs 5 % of dk and dv at D = 64, 2 % at 128; one at
+  // 64 spans where their limits are read costs as much.)
   auto fit = [&](uint32_t record, bool masked) FA_INLINE {
     const int l = lane_now(), key0 = w0 + (l & 15);
     const uint32_t at = factor_at(l & 15);
-    float largest = 0.0f;
+    float largest[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int cb = 0; cb < 2; ++cb) {
-      float top = lds_read4(record + 4 * kSpanTop);
+      const float v = lds_read4(at + 128 + 64 * cb);
+      float bound = 0.0f;
       if (masked) {
-        top = 0.0f;
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb) {
           const uint32_t quad = record + rb * 256 + (l >> 4) * 16;
           const i32x4 lo = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kLo)) - key0;
           const i32x4 hi = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kHi)) - key0;
-          const f32x4 of_row = lds_quad(record + 4 * kRowTops + rb * 64 + (l >> 4) * 16);
+          const f32x4 go = lds_quad(record + 4 * kRowNorms + rb * 64 + (l >> 4) * 16), delta = lds_quad(quad + 64 * kDelta);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, 16 * cb >= lo[i] && 16 * cb < hi[i] ? of_row[i] : 0.0f);
+          for (int i = 0; i < 4; ++i)
+            bound = fmaxf(bound, 16 * cb >= lo[i] && 16 * cb < hi[i] ? fmaf(go[i], v, fabsf(delta[i])) : 0.0f);
         }
-        top = fmaxf(top, from_lane(top, lane_now() ^ 16));
-        top = fmaxf(top, from_lane(top, lane_now() ^ 32));
+        bound = fmaxf(bound, from_lane(bound, lane_now() ^ 16));
+        bound = fmaxf(bound, from_lane(bound, lane_now() ^ 32));
+      } else {
+        bound = fmaf(lds_read4(record + 4 * kSpanMost), v, lds_read4(record + 4 * kSpanMost + 4));
       }
       const float factor = lds_read4(at + 64 * cb);
-      const float to = top * factor >= kFactorMost<CAP> ? kQuarters<CAP> * grad_factor<BF16>(top) : factor;
-      // (their ratio: powers of two)
-      const float change = __builtin_bit_cast(float, __builtin_bit_cast(int, to) - __builtin_bit_cast(int, factor) + 0x3f800000);
+      const float to = bound * factor > kBoundMost<CAP> ? grad_factor<CAP>(bound) : factor;
+      // (their ratio: powers of two; 0 if it is less than there is)
+      const float change =
+          __builtin_bit_cast(float, max(__builtin_bit_cast(int, to) - __builtin_bit_cast(int, factor) + 0x3f800000, 0));
 #pragma unroll
       for (int db = 0; db < DB; ++db) gk[db][cb] *= change;
       lds_write4(at + 64 * cb, to);
-      largest = fmaxf(largest, to);
+      largest[0] = fmaxf(largest[0], v * to);
+      largest[1] = fmaxf(largest[1], to);
     }
 #pragma unroll
-    for (int d = 1; d < 16; d <<= 1) largest = fmaxf(largest, from_lane(largest, lane_now() ^ d));
-    lds_write4(largest_at(), largest);
+    for (int i = 0; i < 2; ++i) {
+      static_for<0, 4>([&](auto d_c) FA_INLINE {
+        largest[i] = fmaxf(largest[i], turned_row<1 << decltype(d_c)::value>(largest[i]));
+      });
+      lds_write4(largest_at() + 4 * i, largest[i]);
+    }
   };
   // A span in `slot`; `masked`: some row does not see all of the wave's keys, `cleaned`: of
   // the workgroup's (finish).  (Scores become P in place, dS takes the place of go V^T: the
@@ -531,10 +564,10 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
     const int key0 = w0 + (l & 15);
     const uint32_t tile = base + slot * SLOT;
     u32x4 pw[2], dw[2];  // P and dS as packed pairs: words 0, 1 of rows 4 (l / 16) .., 2, 3 of those 16 on
-    float top = 0.0f, largest = 0.0f;  // (read ahead of the first product)
+    u32x2 most, largest;  // (read ahead of the first product)
     if constexpr (!BF16) {
-      top = lds_read4(tile + 2 * TB + 4 * kSpanTop);
-      largest = lds_read4(largest_at());
+      most = lds_read8<4 * kSpanMost>(tile + 2 * TB);
+      largest = lds_read8<0>(largest_at());
     }
     static_for<0, 2>([&](auto rb_c) FA_INLINE {
       constexpr int rb = decltype(rb_c)::value;
@@ -543,8 +576,11 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
       f32x4 c[2], e[2];
       const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
       row_product<D, BF16, 2>(rows, kf, zero, c, [](auto) FA_INLINE {});
-      if constexpr (!BF16 && rb == 0)
-        if (__any(top * largest >= kFactorMost<CAP>)) fit(tile + 2 * TB, masked);
+      if constexpr (!BF16 && rb == 0) {
+        auto f = [](uint32_t x) FA_INLINE { return __builtin_bit_cast(float, x); };
+        if (__builtin_expect(__any(fmaf(f(most[0]), f(largest[0]), f(most[1]) * f(largest[1])) > kBoundMost<CAP>), false))
+          fit(tile + 2 * TB, masked);
+      }
       const int away = row0 + 16 * rb + 4 * (l >> 4) + a.m - a.n - key0;  // of key block 0
       auto away_of = [&](int cb, int i) FA_INLINE { return (float)(away - 16 * cb) + (float)i; };
       f32x4 lse = lds_quad(quad + 64 * kLse);
@@ -657,7 +693,7 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
   }
   // The first team takes all of gk, the second all of gv, by wave and lane.
   if constexpr (TEAMS > 1) {
-    const uint32_t at = lds_addr(smem) + wave * PART + lane * 16;
+    const uint32_t at = lds_addr(smem) + wave * PART + lane_now() * 16;
     if (team != 0) put_sums<DB>(at + (team - 1) * 4 * PART, gk);
     if (team != 1) put_sums<DB>(at + (TEAMS - 1 + (team == 0 ? 0 : team - 1)) * 4 * PART, gv);
     __builtin_amdgcn_s_waitcnt(0xc07f);
@@ -729,6 +765,9 @@ __global__ void __launch_bounds__(256 * TEAMS)
     fa_attn_dq_kernel(const AttnArgs a) {
   constexpr int ROWB = 2 * D, TB = 64 * ROWB, KST = D / 32, DB = D / 16;
   __shared__ __attribute__((aligned(1024))) char smem[TEAMS * 4 * TB];  // of each team K0 V0 K1 V1
+  // fp16: some row's sum is no number, which rows', the rows' factors then
+  __shared__ int again, odd[BF16 ? 1 : kAttnRows];
+  __shared__ float least[BF16 ? 1 : kAttnRows];
 
   const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = lane >> 4;
   const int team = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
@@ -761,6 +800,10 @@ __global__ void __launch_bounds__(256 * TEAMS)
     stage_v.copy(vh + r0 * a.v.st, dst + TB, c1 - 1 - r0, (uint32_t)a.v.st);
   };
   issue(0, 0);
+  if constexpr (!BF16) {  // (ordered by the first barrier)
+    if (threadIdx.x == 0) again = 0;
+    if (threadIdx.x < kAttnRows) odd[threadIdx.x] = 0;
+  }
   // (behind the first copies: one wait for all)
   i16x8 qf[2][KST], gf[2][KST];
   float lse[2], delta[2], factor[2];  // (minus delta)
@@ -776,23 +819,17 @@ __global__ void __launch_bounds__(256 * TEAMS)
       qf[rb][st] = *reinterpret_cast<const i16x8*>(qp + 64 * st);
       gf[rb][st] = *reinterpret_cast<const i16x8*>(gp + 64 * st);
     }
-    const float* rec = a.records + (((int64_t)b * a.heads + h) * a.spans + r / kSpan) * kRecord<BF16> +
-                       r % kSpan / 16 * 64 + r % 16;
+    const float* record = a.records + (((int64_t)b * a.heads + h) * a.spans + r / kSpan) * kRecord<BF16>;
+    const float* rec = record + r % kSpan / 16 * 64 + r % 16;
     lse[rb] = rec[16 * kLse];
     delta[rb] = rec[16 * kDelta];
     see[rb].lo = __builtin_bit_cast(int, rec[16 * kLo]);
     see[rb].hi = __builtin_bit_cast(int, rec[16 * kHi]);
     factor[rb] = 1.0f;
     if constexpr (!BF16) {
-      float top = 0.0f;
-#pragma unroll
-      for (int st = 0; st < KST; ++st) {
-        float f[8];
-        unpack8<BF16>(__builtin_bit_cast(u32x4, gf[rb][st]), f);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(f[j]));
-      }
-      factor[rb] = kQuarters<CAP> * grad_factor<BF16>(WaveAttn<D, BF16, 4, 2>::red_max(top));
+      const float norm = record[kRowNorms + r % kSpan];
+      factor[rb] = grad_factor<CAP>(fmaf(norm, 0x1p6f, fabsf(delta[rb])));
+      least[32 * wave + 16 * rb + l16] = grad_factor<CAP>(fmaf(norm, 0x1p20f, fabsf(delta[rb])));
     }
   }
   // The staged keys of tile t are there: cleaned if some row does not see all of
@@ -805,8 +842,9 @@ __global__ void __launch_bounds__(256 * TEAMS)
       const unsigned bad = clean_rows<D, BF16, 16>(rows);
       if (__builtin_expect(bad != 0, false)) {
         constexpr int LPR = ROWB / 16;
-        for (int r = lane / LPR; r < 16; r += 64 / LPR)
-          if ((bad >> r) & 1) lds_write16(rows + TB + r * ROWB + lane % LPR * 16, u32x4{~0u, ~0u, ~0u, ~0u});
+        const int l = lane_now();
+        for (int r = l / LPR; r < 16; r += 64 / LPR)
+          if ((bad >> r) & 1) lds_write16(rows + TB + r * ROWB + l % LPR * 16, u32x4{~0u, ~0u, ~0u, ~0u});
       }
       __builtin_amdgcn_s_waitcnt(0);
     }
@@ -814,10 +852,6 @@ __global__ void __launch_bounds__(256 * TEAMS)
   };
 
   f32x4 gq[DB][2];
-#pragma unroll
-  for (int db = 0; db < DB; ++db)
-#pragma unroll
-    for (int rb = 0; rb < 2; ++rb) gq[db][rb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   const uint32_t row_at = base + lds::TileBoth<D>::row_offset(lane);
   const uint32_t turned_at = base + lds::TileBoth<D>::turned_offset(lane);
   Grads<CAP> grads;
@@ -895,26 +929,52 @@ __global__ void __launch_bounds__(256 * TEAMS)
     turned_product<D, BF16, 2>(turned_at + off + half * 32 * ROWB, df, gq);
   };
 
-  finish(0, 0);
-  int buf = 0;
-  for (int t = 0; t < turns; ++t, buf ^= 1) {
-    const int k0 = key_of(t);
-    issue(t + 1, buf ^ 1);
+#pragma unroll 1
+  for (bool last = BF16;;) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int k = k0 + 32 * half;
-      if (k >= keys.all_lo && k + 32 <= keys.all_hi)
-        step(k, buf * 2 * TB, half, false);
-      else if (k < keys.hi && k + 32 > keys.lo)
-        step(k, buf * 2 * TB, half, true);
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb) gq[db][rb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    finish(0, 0);
+    int buf = 0;
+    for (int t = 0; t < turns; ++t, buf ^= 1) {
+      const int k0 = key_of(t);
+      issue(t + 1, buf ^ 1);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int k = k0 + 32 * half;
+        if (k >= keys.all_lo && k + 32 <= keys.all_hi)
+          step(k, buf * 2 * TB, half, false);
+        else if (k < keys.hi && k + 32 > keys.lo)
+          step(k, buf * 2 * TB, half, true);
+      }
+      finish(t + 1, buf ^ 1);
     }
-    finish(t + 1, buf ^ 1);
+    if (last) break;
+    // (all start again: the staging is shared, and teams have the same factors)
+    last = true;
+    const int at = 32 * wave + (lane_now() & 15);
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) {
+      bool no = false;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) no = no || !(fabsf(gq[db][rb][i]) < INFINITY);
+      if (no) again = odd[at + 16 * rb] = 1;
+    }
+    __syncthreads();
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(again) == 0, true)) break;
+    issue(0, 0);
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb)
+      if (odd[at + 16 * rb] != 0) factor[rb] = least[at + 16 * rb];
   }
 
   // The second team hands its sums to the first, by wave and lane.
   constexpr int PART = 2 * DB * 1024;
   if constexpr (TEAMS == 2) {
-    const uint32_t at = lds_addr(smem) + wave * PART + lane * 16;
+    const uint32_t at = lds_addr(smem) + wave * PART + lane_now() * 16;
     if (team == 1) put_sums<DB>(at, gq);
     __builtin_amdgcn_s_waitcnt(0xc07f);
     __syncthreads();
@@ -925,7 +985,7 @@ __global__ void __launch_bounds__(256 * TEAMS)
 #pragma unroll
   for (int rb = 0; rb < 2; ++rb) f[rb] = kQuarters<CAP> * a.scale * fast_exp2(-kShift<BF16>) / factor[rb];
   char* qh = a.gq.p + b * a.gq.sb + h * a.gq.sh;
-  write_rows<D, BF16>(smem + wave * PART, gq, f, lane, [&](int r) FA_INLINE -> char* {
+  write_rows<D, BF16>(smem + wave * PART, gq, f, lane_now(), [&](int r) FA_INLINE -> char* {
     return wrow0 + r < a.n ? qh + (wrow0 + r) * a.gq.st : nullptr;
   });
 }

@@ -136,6 +136,13 @@ __device__ __forceinline__ float from_lane(float x, int l) {
   return __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(4 * l, __builtin_bit_cast(int, x)));
 }
 
+// x of the lane that is N ahead in the same 16 (DPP row_ror), around their end.
+template <int N>
+__device__ __forceinline__ float turned_row(float x) {
+  const int w = __builtin_bit_cast(int, x);
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(w, w, 0x120 + N, 0xf, 0xf, false));
+}
+
 // Staging of 16 rows of a tensor into LDS in the layout of lds::TileBoth.
 template <int D>
 struct RowStage {
