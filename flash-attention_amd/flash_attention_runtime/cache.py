@@ -71,10 +71,17 @@ def paged_forward(
     seen nor read, and ``slopes`` (fp32 [H] on the GPU) times the distance is taken off.
 
     Returns ``o`` like q, or ``(o, lse)`` with the natural-log logsumexp, fp32
-    [T, H].  A row without visible keys has o = 0 and lse = -inf.
+    [T, H], of these scores: ``paged_key_weights`` takes that of plain ones only.  A row
+    without visible keys has o = 0 and lse = -inf.
     """
-    return _EXT.paged_forward(q, k_cache, v_cache, block_table, cu_seqlens, seq_lens, out, max_q,
-                              max_kv, causal, softmax_scale, return_lse, softcap, window, slopes)
+    res = _EXT.paged_forward(q, k_cache, v_cache, block_table, cu_seqlens, seq_lens, out, max_q,
+                             max_kv, causal, softmax_scale, return_lse, softcap, window, slopes)
+    if return_lse and (softcap is not None or slopes is not None or window is not None):
+        # (plain scores where a window leaves all keys; a token without a place lies before the first)
+        keys = block_table.shape[1] * k_cache.shape[2] if max_kv is None else max_kv
+        if softcap is not None or slopes is not None or window < keys + (0 if causal else q.shape[0]):
+            res[1].scores = "capped, biased or windowed"
+    return res
 
 
 def paged_key_weights(
@@ -95,9 +102,13 @@ def paged_key_weights(
     attention weight each key receives from the new tokens: the sum over the
     query heads of its kv head and the tokens that see it of
     ``exp(scale q.k - lse)``.  ``q``, ``lse`` and the limits as given to and
-    returned by ``paged_forward``.  The new tokens' own keys are set, not added
+    returned by ``paged_forward`` without ``softcap``, ``window`` and ``slopes``: there are no weights
+    of such scores.  The ``lse`` that it returned with them is refused; nothing tells a copy or
+    a part of it from another tensor.  The new tokens' own keys are set, not added
     to, so a reused page needs no clearing.  A page must belong to one sequence of
     the call only (sequences that share a prefix need weights of their own).  Returns ``key_weights``."""
+    if getattr(lse, "scores", None) is not None:
+        raise RuntimeError(f"paged_key_weights has plain scores only: this lse is of {lse.scores} ones")
     _EXT.paged_key_weights(q, lse, k_cache, block_table, cu_seqlens, seq_lens, key_weights, max_q,
                            max_kv, causal, softmax_scale)
     return key_weights

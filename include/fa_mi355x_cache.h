@@ -93,7 +93,8 @@ typedef struct {
 typedef struct {
   fa_paged_cache cache;   /* v unused */
   const void* q;          /* [tokens, heads, head_dim] */
-  const float* lse;       /* [tokens, heads] contiguous, as fa_paged_fwd writes it */
+  const float* lse;       /* [tokens, heads] contiguous, as fa_paged_fwd writes it (not fa_paged_fwd_scored:
+                             the weights are those of plain scores) */
   float* key_weights;     /* [num_pages, kv_heads, page_size], unit key stride */
   int64_t q_stride[2];    /* token, head */
   int64_t w_stride[2];    /* page, kv head */
