@@ -85,6 +85,10 @@ def document_ranges(
     ``cu_seqlens[d + 1]`` (ascending, on any device; the result is on the same).  A token sees the tokens
     of its document up to itself (all of them with ``causal=False``), and the first ``prefix_lens[d]`` ones.
     Tokens outside the documents see nothing.  Computed once per batch, for all layers."""
+    if cu_seqlens.dim() != 1:
+        raise RuntimeError("cu_seqlens must have one dimension")
+    if prefix_lens is not None and prefix_lens.shape != (max(cu_seqlens.shape[0] - 1, 0),):
+        raise RuntimeError("prefix_lens must have one entry per document")
     cu = cu_seqlens.to(torch.int64)
     i = torch.arange(n, device=cu.device)
     if cu.shape[0] < 2:
