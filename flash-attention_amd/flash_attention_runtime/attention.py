@@ -87,7 +87,7 @@ def document_ranges(
     Tokens outside the documents see nothing.  Computed once per batch, for all layers."""
     if cu_seqlens.dim() != 1:
         raise RuntimeError("cu_seqlens must have one dimension")
-    if prefix_lens is not None and prefix_lens.shape != (max(cu_seqlens.shape[0] - 1, 0),):
+    if prefix_lens is not None and (prefix_lens.dim() != 1 or prefix_lens.shape[0] < cu_seqlens.shape[0] - 1):
         raise RuntimeError("prefix_lens must have one entry per document")
     cu = cu_seqlens.to(torch.int64)
     i = torch.arange(n, device=cu.device)
