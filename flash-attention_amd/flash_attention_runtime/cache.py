@@ -30,6 +30,7 @@ carries forward-mode tangents on: inputs that ask for them are refused.
 """
 from __future__ import annotations
 
+import operator
 from collections.abc import Sequence
 
 import torch
@@ -143,7 +144,8 @@ def paged_evict(
 
 
 def _axes(axes) -> bytes | None:
-    return axes if axes is None or isinstance(axes, bytes) else bytes(axes)
+    # (bytes(axes) would be an array's memory, and a number's many zeros)
+    return axes if axes is None or isinstance(axes, bytes) else bytes(operator.index(a) for a in axes)
 
 
 def paged_store(

@@ -24,3 +24,20 @@ def test_cu_seqlens_has_one_dimension(fa, cu):
 def test_no_documents(fa):
     for cu in ([], [0]):
         assert fa.document_ranges(torch.tensor(cu, dtype=torch.int32), 2).tolist() == [[0, 0], [0, 0]]
+
+
+def test_axes_are_read_one_by_one(fa):
+    """Integers of any sequence, an entry each: never the bytes of an array's memory, nor a number of zeros."""
+    import numpy as np
+
+    from flash_attention_runtime import cache
+
+    want = bytes([0, 2, 1, 3, 0, 1, 2, 3])
+    for axes in (list(want), tuple(want), want, bytearray(want), torch.tensor(list(want)),
+                 *(np.array(list(want), dtype=t) for t in (np.int64, np.int32, np.uint8))):
+        assert cache._axes(axes) == want, type(axes)
+    assert cache._axes(None) is None
+    for bad, error in ((8, TypeError), ("0213", TypeError), ([0.5] * 8, TypeError), ([-1] * 8, ValueError),
+                       ([256] * 8, ValueError)):
+        with pytest.raises(error):
+            cache._axes(bad)
