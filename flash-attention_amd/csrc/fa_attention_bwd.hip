@@ -486,9 +486,9 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
   auto factor_at = [&](int l) FA_INLINE { return spoiled_at + SLOTS * 2 * kSpan * 4 + (w0 & 96) * 8 + l * 4; };
   auto largest_at = [&]() FA_INLINE { return spoiled_at + (SLOTS * 2 * kSpan + 4 * 64) * 4 + (w0 & 96) / 4; };
   if constexpr (!BF16) {
-    // (more than any bound above 2^-57 takes)
+    // (more than any bound above 2^-57 takes; behind the last key one that every bound fits)
     constexpr float first = kBoundMost<CAP> * 0x1p57f;
-    if (lane < 32) lds_write4(factor_at(lane), first);
+    if (lane < 32) lds_write4(factor_at(lane), w0 + lane < a.m ? first : 0x1p-60f);
     lds_write8<0>(largest_at(), u32x2{__builtin_bit_cast(uint32_t, first), __builtin_bit_cast(uint32_t, first)});
 #pragma unroll
     for (int cb = 0; cb < 2; ++cb) {
