@@ -511,41 +511,53 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
 
   Grads<CAP> grads;
   // fp16: new factors of dS, also for what its sum holds, where rows that see a key take its bound
-  // further than those before.  (The look at each span costs 5 % of dk and dv at D = 64, 2 % at 128; one at
-  // 64 spans where their limits are read costs as much.)
+  // further than those before.  (2 x 8192 causal rows, 32 heads on 8, us without any look and with one at each
+  // span: D = 64 1362 and 1445, D = 128 1997 and 2077; one at 64 spans where their limits are read costs
+  // as much.)
   auto fit = [&](uint32_t record, bool masked) FA_INLINE {
     const int l = lane_now(), key0 = w0 + (l & 15);
     const uint32_t at = factor_at(l & 15);
-    float largest[2] = {0.0f, 0.0f};
+    const float v[2] = {lds_read4(at + 128), lds_read4(at + 192)};
+    float bound[2] = {0.0f, 0.0f}, largest[2] = {0.0f, 0.0f};
+    if (masked) {
 #pragma unroll
-    for (int cb = 0; cb < 2; ++cb) {
-      const float v = lds_read4(at + 128 + 64 * cb);
-      float bound = 0.0f;
-      if (masked) {
+      for (int rb = 0; rb < 2; ++rb) {
+        const uint32_t quad = record + rb * 256 + (l >> 4) * 16;
+        const i32x4 lo = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kLo)) - key0;
+        const i32x4 hi = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kHi)) - key0;
+        const f32x4 go = lds_quad(record + 4 * kRowNorms + rb * 64 + (l >> 4) * 16), delta = lds_quad(quad + 64 * kDelta);
 #pragma unroll
-        for (int rb = 0; rb < 2; ++rb) {
-          const uint32_t quad = record + rb * 256 + (l >> 4) * 16;
-          const i32x4 lo = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kLo)) - key0;
-          const i32x4 hi = __builtin_bit_cast(i32x4, lds_quad(quad + 64 * kHi)) - key0;
-          const f32x4 go = lds_quad(record + 4 * kRowNorms + rb * 64 + (l >> 4) * 16), delta = lds_quad(quad + 64 * kDelta);
+        for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            bound = fmaxf(bound, 16 * cb >= lo[i] && 16 * cb < hi[i] ? fmaf(go[i], v, fabsf(delta[i])) : 0.0f);
-        }
-        bound = fmaxf(bound, from_lane(bound, lane_now() ^ 16));
-        bound = fmaxf(bound, from_lane(bound, lane_now() ^ 32));
-      } else {
-        bound = fmaf(lds_read4(record + 4 * kSpanMost), v, lds_read4(record + 4 * kSpanMost + 4));
+            bound[cb] =
+                fmaxf(bound[cb], 16 * cb >= lo[i] && 16 * cb < hi[i] ? fmaf(go[i], v[cb], fabsf(delta[i])) : 0.0f);
       }
-      const float factor = lds_read4(at + 64 * cb);
-      const float to = bound * factor > kBoundMost<CAP> ? grad_factor<CAP>(bound) : factor;
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb) {
+        bound[cb] = fmaxf(bound[cb], from_lane(bound[cb], lane_now() ^ 16));
+        bound[cb] = fmaxf(bound[cb], from_lane(bound[cb], lane_now() ^ 32));
+      }
+    } else {
+      const u32x2 most = lds_read8<4 * kSpanMost>(record);
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb)
+        bound[cb] = fmaf(__builtin_bit_cast(float, most[0]), v[cb], __builtin_bit_cast(float, most[1]));
+    }
+    const float factors[2] = {lds_read4(at), lds_read4(at + 64)};
+    // (that keys which no row has seen yet have the first factor made it look)
+    if (!__any(bound[0] * factors[0] > kBoundMost<CAP> || bound[1] * factors[1] > kBoundMost<CAP>)) return;
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) {
+      const float factor = factors[cb];
+      const float to = bound[cb] * factor > kBoundMost<CAP> ? grad_factor<CAP>(bound[cb]) : factor;
       // (their ratio: powers of two; 0 if it is less than there is)
       const float change =
           __builtin_bit_cast(float, max(__builtin_bit_cast(int, to) - __builtin_bit_cast(int, factor) + 0x3f800000, 0));
 #pragma unroll
       for (int db = 0; db < DB; ++db) gk[db][cb] *= change;
       lds_write4(at + 64 * cb, to);
-      largest[0] = fmaxf(largest[0], v * to);
+      largest[0] = fmaxf(largest[0], v[cb] * to);
       largest[1] = fmaxf(largest[1], to);
     }
 #pragma unroll
