@@ -498,7 +498,8 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
         const u32x4 x = __builtin_bit_cast(u32x4, vf[cb][st]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const auto pair = __builtin_bit_cast(f16x2, x[j]);
+          const uint32_t word = x[j];  // (bit_cast of an element itself takes the first one)
+          const auto pair = __builtin_bit_cast(f16x2, word);
           square = __builtin_amdgcn_fdot2(pair, pair, square, false);
         }
       }
@@ -539,10 +540,9 @@ __global__ void __launch_bounds__(256 * TEAMS) __attribute__((amdgpu_waves_per_e
         bound[cb] = fmaxf(bound[cb], from_lane(bound[cb], lane_now() ^ 32));
       }
     } else {
-      const u32x2 most = lds_read8<4 * kSpanMost>(record);
+      const float go = lds_read4(record + 4 * kSpanMost), delta = lds_read4(record + 4 * kSpanMost + 4);
 #pragma unroll
-      for (int cb = 0; cb < 2; ++cb)
-        bound[cb] = fmaf(__builtin_bit_cast(float, most[0]), v[cb], __builtin_bit_cast(float, most[1]));
+      for (int cb = 0; cb < 2; ++cb) bound[cb] = fmaf(go, v[cb], delta);
     }
     const float factors[2] = {lds_read4(at), lds_read4(at + 64)};
     // (that keys which no row has seen yet have the first factor made it look)

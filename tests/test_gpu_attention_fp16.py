@@ -113,7 +113,7 @@ def lost(tensors, see, opt, glse, scale):
 
 def check_against_64_bits(fa, tensors, opt, glse=None):
     D, n = tensors[0].shape[3], tensors[0].shape[2]
-    see, scale = A.visible(n, n, causal=True), 1 / math.sqrt(D)
+    see, scale = A.visible(n, n, causal=True, window=opt.get("window")), 1 / math.sqrt(D)
     got = call(fa, tensors, None, None, dict(opt, causal=True), glse)
     val, tol = A.attend(*tensors[:3], see, scale=scale, cap=opt.get("softcap"), go=tensors[3], glse=glse)
     more = lost(tensors, see, opt, glse, scale)
@@ -170,3 +170,17 @@ def test_no_bit_goes_by_rows_that_start_again(fa, D, H, KH):
             assert torch.equal(a[n][:, :, inside(i)], b[n][:, :, inside(i)]), (n, i)
     # (in 64 bits the loud document's dq is up to 2.2e3, its dk up to 3.7e5, past what fp16 holds)
     assert bool(torch.isfinite(b["gq"]).all()) and not bool(torch.isnan(b["gk"]).any())
+
+
+@pytest.mark.parametrize("D,H,KH", [(64, 2, 1), (128, 4, 2)])
+@pytest.mark.parametrize("dims", [[0], [1], [2], [3], [5], [6, 15], [60], [63]])
+def test_values_and_gradients_in_a_few_dims(fa, D, H, KH, dims):
+    """One or two dims of v and go hold nearly all of their norms, as outlier channels do; rows see two keys of
+    about the same weight and of opposite v there, so that go.o cancels and dS is half of |go| |v|."""
+    print("case dims", D, H, dims, flush=True)
+    tensors = inputs(D, H, KH, 89)
+    sign = 1.0 - 2.0 * (torch.arange(N) % 2)
+    tensors[2][..., dims] = (20000.0 * sign[:, None]).to(HALF)
+    tensors[3][..., dims] = 4.0
+    tensors[0], tensors[1] = ((x.float() * 0.01).to(HALF) for x in tensors[:2])
+    check_against_64_bits(fa, tensors, dict(window=2))
