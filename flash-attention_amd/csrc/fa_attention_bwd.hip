@@ -21,7 +21,8 @@
 // 2 x 8192 causal tokens, 32 heads on 8, D = 128, bf16, us: rows 47 (75 with o_low, 5.3 TB/s), dk and
 // dv 2170 (1010 TFLOP/s of their four products), dq 1480 (1120 of three); a matrix product
 // of 8192^3 reaches 1245.  The matrix cores are busy 49 and 55 % of the cycles, at 1.9 GHz (the power
-// limit); capped scores add vector work, 2430 and 1790.  D = 64, fp16: 1540 and 930, vector units.
+// limit); capped scores add vector work, 2430 and 1790.  fp16, on a box that takes 1930 and 1357 for these:
+// 2135 and 1466; D = 64 1460 and 820, vector units (the look at dS's factors is 85 of each dk, dv).
 //
 // Rounding: P and dS are rounded to the input type for the matrix cores (as P of
 // the forward pass); all sums are fp32.  fp16 has few exponents: P is scaled by

@@ -46,7 +46,8 @@ def attention(
     Differentiable once in q, k and v, through o and lse; slopes get no gradient.  Besides its
     arguments and results a graph holds one more tensor like o, what rounding left out of it.  The
     same call gives the same bits, gradients included.  In a graph capture a backward pass through leaves that
-    an older autograd graph still holds is refused; ``attention_backward`` can always be captured.
+    an older autograd graph still holds is refused (of q, k and v that are leaves themselves: what made others
+    of them is not looked at); ``attention_backward`` can always be captured.
     """
     return _EXT.attention(q, k, v, key_ranges, causal, window, softcap, slopes, softmax_scale, return_lse)
 

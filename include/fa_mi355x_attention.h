@@ -17,7 +17,8 @@
  *   c = softcap tanh(z / softcap)              (softcap 0: c = z)
  *   x = c - slopes[head] |p - j|               (slopes NULL: x = c)
  * Row i sees the keys j of its range that, with causal, are j <= p and, with a
- * window, are at |p - j| < window.
+ * window, are at |p - j| < window.  Distances are fp32: whole numbers to 2^24, beyond
+ * that to 24 bits.
  */
 #ifndef FA_MI355X_ATTENTION_H
 #define FA_MI355X_ATTENTION_H
@@ -70,8 +71,8 @@ typedef struct {
  * those of k and v summed over the query heads that read them.  Sums run in a fixed
  * order (no atomics).  fwd: as given to fa_attn_fwd, o, lse and o_low as it wrote
  * them (read only).  Rows and keys that do not see each other contribute nothing to each
- * other, whatever they hold; the results of rows and keys that see an infinity or
- * a NaN are infinities or NaN. */
+ * other, whatever they hold.  A result that takes in an infinity or a NaN of a row or
+ * key that it sees is one of them; so may be the others of that row or key. */
 typedef struct {
   fa_attn_params fwd;
   const void* go;         /* like q */
