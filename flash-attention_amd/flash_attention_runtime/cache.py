@@ -81,7 +81,7 @@ def paged_forward(
         # (plain scores where a window leaves all keys; a token without a place lies before the first)
         keys = block_table.shape[1] * k_cache.shape[2] if max_kv is None else max_kv
         if softcap is not None or slopes is not None or window < keys + (0 if causal else q.shape[0]):
-            res[1].scores = "capped, biased or windowed"
+            res[1]._fa_scores = "capped, biased or windowed"
     return res
 
 
@@ -108,8 +108,8 @@ def paged_key_weights(
     a part of it from another tensor.  The new tokens' own keys are set, not added
     to, so a reused page needs no clearing.  A page must belong to one sequence of
     the call only (sequences that share a prefix need weights of their own).  Returns ``key_weights``."""
-    if getattr(lse, "scores", None) is not None:
-        raise RuntimeError(f"paged_key_weights has plain scores only: this lse is of {lse.scores} ones")
+    if getattr(lse, "_fa_scores", None) is not None:
+        raise RuntimeError(f"paged_key_weights has plain scores only: this lse is of {lse._fa_scores} ones")
     _EXT.paged_key_weights(q, lse, k_cache, block_table, cu_seqlens, seq_lens, key_weights, max_q,
                            max_kv, causal, softmax_scale)
     return key_weights

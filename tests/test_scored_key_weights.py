@@ -8,7 +8,7 @@ import torch
 
 def test_a_marked_logsumexp_is_refused_before_anything_is_read(fa):
     lse = torch.zeros(3, 2)
-    lse.scores = "capped, biased or windowed"
+    lse._fa_scores = "capped, biased or windowed"
     with pytest.raises(RuntimeError, match="plain scores only"):
         fa.paged_key_weights(None, lse, None, None, None, None, None, max_q=1)
 
